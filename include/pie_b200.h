@@ -280,6 +280,61 @@ int pie_sample(int32_t* tokens, const void* logits, int rows, int vocab, int ld,
                int min_tokens_to_keep, int top_k, void* rng_state, const float* uniforms, float* logprobs_out,
                int32_t* positions_to_advance, int32_t* seq_out, int seq_ld, void* stream);
 
+/* ---- ragged steps: every request brings another number of new tokens ------------------------------------------------------
+ * The reference declares the descriptor of such a step (BatchDetails, CORE/include/engine/batch_details.hpp:10-90) and no kernel that
+ * reads it.  Lengths, page ids and plan are DEVICE memory, so that a captured step runs again on other lengths; the host knows the
+ * dimensions below, which are upper bounds: rows behind the last request's belong to nobody.
+ *   requests <= 4096, rows >= 1, logit_rows >= 1 (rows whose logits are wanted), blocks (of a row of the block table), pages (of the pools, 64 tokens each),
+ *   Hq / Hkv <= 128.
+ * pie_step_plan_build fills a plan of pie_step_plan_words() 32-bit words, 16-byte aligned, whose parts begin at the words that pie_step_plan_offsets gives:
+ *   0 row_starts [requests + 1]   first row of each request          1 contexts [requests]          tokens it has in the cache
+ *   2 sequences [rows]            request of each row; -1            3 positions [rows]             in its request; 0
+ *   4 slots [rows]                page * 64 + place in it; -1        5 block_table [requests, blocks]   page ids; 0 behind them
+ *   6 logit_starts [requests + 1]                                    7 logit_rows [logit_rows]      each request's last 1 + drafted rows; 0
+ *   8 draft_tokens [logit_rows]   token of the next row; -1          9 status [192]                 PIE_STEP_* of what did not fit
+ * (-1 and 0 behind the last, and draft_tokens -1 at a request's last row; a request without new tokens has no rows), and behind them the attention's
+ * schedule.  draft_lengths: NULL, or how many of a request's new tokens are drafted ones, 0 .. new - 1.  pages: the requests' page ids one behind the
+ * other, ceil((cached + new) / 64) each (page_stride 0, n_page_ids of them), or a table whose rows are page_stride apart (n_page_ids: columns).
+ * A request whose lengths are negative, exceed the step or its table's row is taken as one without tokens; rows and logit rows that do not fit are cut
+ * off; a page id outside the pools gives slots of -1 and page 0.  Each sets its bit in a status word; nothing is read or written out of bounds.           */
+typedef struct pie_step_dims {
+  int requests, rows, logit_rows, blocks, pages, Hq, Hkv;
+} pie_step_dims;
+enum { PIE_STEP_LENGTH = 1, PIE_STEP_ROWS = 2, PIE_STEP_PAGES = 4, PIE_STEP_PAGE_ID = 8, PIE_STEP_DRAFT = 16, PIE_STEP_LOGITS = 32 };
+#define PIE_STEP_STATUS_WORDS 192
+size_t pie_step_plan_words(const pie_step_dims* dims);
+int pie_step_plan_offsets(const pie_step_dims* dims, long long* offsets_host /* [10] */);
+int pie_step_plan_build(int32_t* plan, const pie_step_dims* dims, const int32_t* token_ids, const int32_t* input_lengths, const int32_t* context_lengths,
+                        const int32_t* draft_lengths, const int32_t* pages, long long n_page_ids, long long page_stride, void* stream);
+
+/* Rotation of q and k (pie_rope with dims == D, halves paired, scale 1 and freqs, at each row's own position) and the write of k and v to the rows' slots, bit
+ * for bit pie_rope_kv_append.  Rows of head h at p + row * stride_l + h * stride_h (elements, multiples of 8, 16-byte aligned; stride_b is not looked at).  q_out [rows, Hq, D].
+ * Pools [pages, 64, Hkv, D] with tok_stride and head_stride of kv_host (page_table is not looked at).  Rows whose slot is outside the pools are not written;
+ * rest: their rows of q_out are set to zero (1) or left as they are (0). */
+int pie_rope_kv_slots(void* q_out, void* kpool, void* vpool, const pie_kv_layout* kv_host, const pie_head_rows* q, const pie_head_rows* k, const pie_head_rows* v,
+                      const int32_t* positions, const int32_t* slots, const float* freqs, int rows, int pages, int Hq, int Hkv, int D, int rest, void* stream);
+
+/* Causal attention of every request's new tokens over its pages, which hold them already: row t of out [rows, Hq * D] is
+ * softmax(scale q_t . K[0 .. position t]) V of its request.  scale > 0.  q as above.  rest: rows behind the last request's are set to zero (1) or left as they are (0).
+ * Workspace: pie_chunk_attn_workspace_bytes() bytes, ZEROED ONCE at allocation (counters are left at zero), for launches that come one after the other. */
+size_t pie_chunk_attn_workspace_bytes(const pie_step_dims* dims, int D);
+int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const void* vpool, const pie_kv_layout* kv_host, const int32_t* plan,
+                   const pie_step_dims* dims, int D, float scale, int rest, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Drafted tokens against the target's probabilities.  Request s has the rows logit_starts[s] .. logit_starts[s + 1] - 1 of logits (bf16 [rows, ld >= vocab]); row r
+ * judges draft_tokens[r], the last one none.  p = softmax(logits / temp); q = softmax(draft_logits / temp) (laid out as logits), or with draft_logits NULL all of it on
+ * the drafted token.  In order, a token x is accepted while uniforms[r] q(x) < p(x).  Behind the accepted ones comes one more: at the first refusal the one of largest
+ * w_v / -log(noise[s, v]), w = max(p - q, 0) (p where that is nowhere positive), and with all accepted of w = p; the lowest index where two are largest.  temp 0: greedy, a token
+ * is accepted if it is the first largest logit, which is what comes behind; p = softmax(logits) is for the log-probabilities alone, and uniforms and noise are not read.
+ * tokens int32 [requests, max_draft + 1]: accepted ones, that one, -1; counts int32 [requests]: how many; logprobs f32 [requests, max_draft + 1]: log p of
+ * each, 0 behind them.  A request without rows gets none; of one with more than max_draft + 1 the first max_draft + 1 count (max_draft <= 127).  A drafted token
+ * outside the vocabulary is refused.  -inf logits are tokens that cannot be; a row with a NaN, +inf or nothing else has no distribution: it refuses its
+ * token, and what comes behind is token 0 (temp 0: NaN is passed over).  Workspace: as pie_chunk_attn's. */
+size_t pie_verify_workspace_bytes(int requests, int rows, int vocab);
+int pie_verify_draft(int32_t* tokens, int32_t* counts, float* logprobs, const void* logits, const void* draft_logits, long long ld, const int32_t* draft_tokens,
+                     const int32_t* logit_starts, int requests, int rows, int vocab, int max_draft, float temp, const float* uniforms, const float* noise,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- (e) tensor-parallel exchange steps, one-shot over NVLink peer memory ----------------------------------------
  * Replace the collectives of MLX's sharded linears at decode sizes: `all_sum` after a row-split matrix
  * (QuantizedShardedToAllLinear, MLX/python/mlx/nn/layers/distributed.py:459-566) and the gather of vocabulary-split

@@ -44,6 +44,12 @@ class HeadRows(C.Structure):
     _fields_ = [("p", C.c_void_p), ("stride_b", C.c_longlong), ("stride_h", C.c_longlong), ("stride_l", C.c_longlong)]
 
 
+class StepDims(C.Structure):
+    """pie_step_dims"""
+    _fields_ = [("requests", C.c_int), ("rows", C.c_int), ("logit_rows", C.c_int), ("blocks", C.c_int), ("pages", C.c_int), ("Hq", C.c_int),
+                ("Hkv", C.c_int)]
+
+
 class TpPeers(C.Structure):
     """pie_tp_peers"""
     _fields_ = [("base", C.c_void_p * 8), ("rank", C.c_int), ("world", C.c_int), ("max_elems", C.c_int),
@@ -151,6 +157,15 @@ SIGNATURES = {
     "pie_page_allocator_stress": (_ll, [_vp, _i, _i]),
     "pie_debug_stamps": (_i, [_vp, _sz]),
     "pie_sample": (_i, [_vp, _vp, _i, _i, _i, _f, _f, _f, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    "pie_step_plan_words": (_sz, [C.POINTER(StepDims)]),
+    "pie_step_plan_offsets": (_i, [C.POINTER(StepDims), C.POINTER(_ll)]),
+    "pie_step_plan_build": (_i, [_vp, C.POINTER(StepDims), _vp, _vp, _vp, _vp, _vp, _ll, _ll, _vp]),
+    "pie_rope_kv_slots": (_i, [_vp, _vp, _vp, C.POINTER(KvLayout), C.POINTER(HeadRows), C.POINTER(HeadRows), C.POINTER(HeadRows), _vp, _vp, _vp, _i, _i,
+                               _i, _i, _i, _i, _vp]),
+    "pie_chunk_attn_workspace_bytes": (_sz, [C.POINTER(StepDims), _i]),
+    "pie_chunk_attn": (_i, [_vp, C.POINTER(HeadRows), _vp, _vp, C.POINTER(KvLayout), _vp, C.POINTER(StepDims), _i, _f, _i, _vp, _sz, _vp]),
+    "pie_verify_workspace_bytes": (_sz, [_i, _i, _i]),
+    "pie_verify_draft": (_i, [_vp, _vp, _vp, _vp, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp, _vp, _sz, _vp]),
     "pie_decode_step_plan_bytes": (_sz, [_i]),
     "pie_decode_step_pick_splits": (_i, [_i, _i, _i, _i]),
     "pie_decode_step_attn_ws_bytes": (_sz, [_i, _i, _i, _i]),

@@ -17,7 +17,7 @@ import warnings
 import torch
 
 from . import _lib
-from ._lib import EPI_RESADD, EPI_SILUMUL, EPI_STORE, HeadRows, KvLayout, KvqCache, QmvSeg
+from ._lib import EPI_RESADD, EPI_SILUMUL, EPI_STORE, HeadRows, KvLayout, KvqCache, QmvSeg, StepDims
 
 _BF16 = torch.bfloat16
 
@@ -624,6 +624,164 @@ def sample(logits, temp: float, top_p: float = 0.0, min_p: float = 0.0, min_toke
                                       _p(positions_to_advance), _p(seq_out), 0 if seq_out is None else seq_out.shape[1],
                                       _stream()), "sample")
     return (out, logprobs_out) if return_logprobs else out
+
+
+def _one_device(what: str, *tensors):
+    """The device of an operator's tensors, which is made the current one for its launches."""
+    device = tensors[0].device
+    if device.type != "cuda" or any(t is not None and t.device != device for t in tensors):
+        raise ValueError(f"[{what}] all tensors must be on one CUDA device, but they are on {[str(t.device) for t in tensors if t is not None]}")
+    return torch.cuda.device(device)
+
+
+def _head_rows(x) -> tuple:
+    """Rows [rows, heads, D] as a kernel reads them, 16 bytes at a time: (tensor to be held until the launch is queued, HeadRows)."""
+    if x.stride(2) != 1 or (x.stride(0) | x.stride(1)) % 8 or x.stride(0) < 0 or x.stride(1) < 0 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x, HeadRows(x.data_ptr(), 0, x.stride(1), x.stride(0))
+
+
+def _slot_pools(what: str, k_pool, v_pool) -> KvLayout:
+    """Strides of two page pools [pages, 64, n_kv, D] whose slots lie one behind the other."""
+    for t in (k_pool, v_pool):
+        if t.dim() != 4 or t.shape[1] != 64 or t.dtype != _BF16:
+            raise ValueError(f"[{what}] pools must be bfloat16 [pages, 64, n_kv, D], but one is {t.dtype} {tuple(t.shape)}")
+        if t.stride(3) != 1 or t.stride(0) != 64 * t.stride(1) or (t.stride(1) | t.stride(2)) % 8 or t.stride(1) <= 0 or t.stride(2) < 0 or t.data_ptr() % 16:
+            raise ValueError(f"[{what}] pools must lie page behind page with 16-byte aligned heads, but one has strides {tuple(t.stride())}")
+    if k_pool.shape != v_pool.shape or k_pool.stride() != v_pool.stride():
+        raise ValueError(f"[{what}] keys' and values' pools must share one layout")
+    lay = KvLayout()
+    lay.batch_stride, lay.head_stride, lay.tok_stride = 0, k_pool.stride(2), k_pool.stride(1)
+    lay.page_table, lay.pt_stride, lay.page_size = None, 0, 64
+    return lay
+
+
+def _step_ints(what: str, name: str, t, shape=None):
+    if t.dtype != torch.int32 or not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"[{what}] {name} must be contiguous int32{'' if shape is None else ' ' + str(list(shape))}, but is {t.dtype} {list(t.shape)}")
+
+
+def _check_out(what: str, out, shape):
+    if out is None:
+        return
+    if out.dtype != _BF16 or tuple(out.shape) != tuple(shape) or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"[{what}] out must be contiguous bfloat16 {list(shape)}, but is {out.dtype} {list(out.shape)}")
+
+
+def _fresh(out, shape, device):
+    """(where the result goes, 1 where rows that belong to nobody are to be zeroed in it: a given tensor keeps what it has there)."""
+    return (torch.empty(shape, dtype=_BF16, device=device), 1) if out is None else (out, 0)
+
+
+def rope_kv_slots(queries, keys, values, freqs, positions, slots, k_pool, v_pool, out=None):
+    """A ragged step's rows into its cache: queries [T, Hq, D] and keys [T, Hkv, D] rotated at each row's own position (the arithmetic of ``rope`` with
+    freqs, bit for bit), keys and values [T, Hkv, D] written to the rows' slots of pools [pages, 64, Hkv, D] (slot = page * 64 + place in it).  Rows may lie
+    anywhere, as a projection wrote them.  positions, slots: int32 [T].  Returns the rotated queries, [T, Hq, D] contiguous.  A row whose slot is outside
+    the pools (-1: it belongs to nobody) writes nothing to them; its queries are zero, or with ``out`` given what that held.  No two rows may share a slot."""
+    what = "rope_kv_slots"
+    if queries.dim() != 3 or keys.dim() != 3 or values.shape != keys.shape or keys.shape[0] != queries.shape[0] or keys.shape[2] != queries.shape[2]:
+        raise ValueError(f"[{what}] queries [T, Hq, D], keys and values [T, Hkv, D] expected, but they are {tuple(queries.shape)}, {tuple(keys.shape)} and "
+                         f"{tuple(values.shape)}")
+    T, Hq, D = queries.shape
+    Hkv = keys.shape[1]
+    if D not in (64, 128):
+        raise ValueError(f"[{what}] head size {D} is not built here (64 or 128)")
+    if any(t.dtype != _BF16 for t in (queries, keys, values)):
+        raise ValueError(f"[{what}] only bfloat16 is built here")
+    if freqs.dtype != torch.float32 or tuple(freqs.shape) != (D // 2,) or not freqs.is_contiguous():
+        raise ValueError(f"[{what}] freqs must be contiguous float32 [{D // 2}], but is {freqs.dtype} {list(freqs.shape)}")
+    _step_ints(what, "positions", positions, (T,))
+    _step_ints(what, "slots", slots, (T,))
+    lay = _slot_pools(what, k_pool, v_pool)
+    if k_pool.shape[2:] != (Hkv, D):
+        raise ValueError(f"[{what}] pools of {tuple(k_pool.shape[2:])} heads and features do not hold keys of {(Hkv, D)}")
+    _check_out(what, out, (T, Hq, D))
+    with _one_device(what, queries, keys, values, freqs, positions, slots, k_pool, v_pool, *(() if out is None else (out,))):
+        out, rest = _fresh(out, (T, Hq, D), queries.device)
+        held = [_head_rows(t) for t in (queries, keys, values)]
+        _lib.check(_lib.load().pie_rope_kv_slots(_p(out), _p(k_pool), _p(v_pool), C.byref(lay), *(C.byref(r) for _, r in held), _p(positions), _p(slots), _p(freqs),
+                                                 T, k_pool.shape[0], Hq, Hkv, D, rest, _stream()), what)
+    return out
+
+
+def chunk_attention(q, k_pool, v_pool, plan, scale: float, out=None):
+    """Causal attention of a ragged step: row t of q [T, Hq, D] (rows may lie anywhere) attends to the keys 0 .. position of its own request, which the pools
+    [pages, 64, Hkv, D] hold already (rope_kv_slots).  plan: the step's ragged.StepPlan, built for these numbers of heads and pages.  Returns [T, Hq * D].
+    Rows that belong to nobody are zero, or with ``out`` given what that held."""
+    what = "chunk_attention"
+    if q.dim() != 3 or q.dtype != _BF16:
+        raise ValueError(f"[{what}] queries must be bfloat16 [T, Hq, D], but are {q.dtype} {tuple(q.shape)}")
+    T, Hq, D = q.shape
+    lay = _slot_pools(what, k_pool, v_pool)
+    d = plan.dims
+    if D not in (64, 128):
+        raise ValueError(f"[{what}] head size {D} is not built here (64 or 128)")
+    if (T, Hq) != (d.rows, d.Hq) or tuple(k_pool.shape) != (d.pages, 64, d.Hkv, D):
+        raise ValueError(f"[{what}] the plan is for {d.rows} rows of {d.Hq} heads over {d.pages} pages of {d.Hkv} heads, but queries are {tuple(q.shape)} and pools "
+                         f"{tuple(k_pool.shape)}")
+    if not scale > 0:
+        raise ValueError(f"[{what}] scale must be positive, but is {scale}")
+    _check_out(what, out, (T, Hq * D))
+    with _one_device(what, q, k_pool, v_pool, plan.words, *(() if out is None else (out,))):
+        out, rest = _fresh(out, (T, Hq * D), q.device)
+        held, rows = _head_rows(q)
+        L = _lib.load()
+        ws = workspaces.get("chunk", L.pie_chunk_attn_workspace_bytes(C.byref(d), D), q.device)
+        _lib.check(L.pie_chunk_attn(_p(out), C.byref(rows), _p(k_pool), _p(v_pool), C.byref(lay), _p(plan.words), C.byref(d), D, float(scale), rest, _p(ws),
+                                    ws.numel(), _stream()), what)
+    return out
+
+
+def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: float = 0.0, uniforms=None, noise=None, draft_logits=None):
+    """Drafted tokens against the target's probabilities, and the token behind the accepted ones.  Request s has rows logit_starts[s] .. logit_starts[s + 1] - 1
+    of logits (bf16 [R, vocab]): row r judges draft_tokens[r] (int32 [R]), a request's last row none (StepPlan has both arrays).
+
+    p = softmax(logits / temp); q = softmax(draft_logits / temp) (bf16 [R, vocab]), or all of it on the drafted token where the drafter has no probabilities
+    (draft_logits None).  In order, token x is accepted while uniforms[r] * q(x) < p(x) (f32 [R], in [0, 1)).  Behind the accepted ones comes one more, drawn by
+    noise[s] (f32 [requests, vocab], in (0, 1)): the v of largest w_v / -log(noise[s, v]), w = max(p - q, 0) at a refusal, p with all accepted -- so that the
+    tokens are distributed as the target's own.  temp 0: greedy; a token is accepted if it is the first largest logit.  Filters (top-p, ...) are logits of -inf.
+
+    Returns (tokens int32 [requests, max_draft + 1], padded by -1; counts int32 [requests], 1 + accepted (0: a request without rows); log-probabilities f32
+    [requests, max_draft + 1] of the tokens under p, padded by 0).  max_draft: at most 127; further drafts of a request are not looked at."""
+    what = "verify_draft"
+    for name, t in (("logits", logits), ("draft_logits", draft_logits)):
+        if t is not None and (t.dim() != 2 or t.dtype != _BF16 or t.shape != logits.shape or t.numel() == 0):
+            raise ValueError(f"[{what}] {name} must be bfloat16 [R, vocab], but is {t.dtype} {tuple(t.shape)}")
+    R, vocab = logits.shape
+    _step_ints(what, "draft_tokens", draft_tokens, (R,))
+    _step_ints(what, "logit_starts", logit_starts)
+    S = logit_starts.numel() - 1
+    if logit_starts.dim() != 1 or S < 1 or S > 65535 or R > 65535:
+        raise ValueError(f"[{what}] {S} requests of {R} rows: 1 to 65535 of either")
+    if not isinstance(max_draft, int) or not 0 <= max_draft <= 127:
+        raise ValueError(f"[{what}] max_draft must be an integer from 0 to 127, but is {max_draft}")
+    if not 0 <= temp < float("inf"):
+        raise ValueError(f"[{what}] temp must be at least 0, but is {temp}")
+    if temp > 0:
+        for name, t, shape in (("uniforms", uniforms, (R,)), ("noise", noise, (S, vocab))):
+            if t is None or t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"[{what}] {name} must be contiguous float32 {list(shape)} where temp is not 0")
+    elif draft_logits is not None:
+        raise ValueError(f"[{what}] a greedy draft has no probabilities: draft_logits is for temp > 0")
+    else:
+        uniforms = noise = None
+    given = [t for t in (logits, draft_tokens, logit_starts, uniforms, noise, draft_logits) if t is not None]
+    with _one_device(what, *given):
+        logits = logits if logits.stride(1) == 1 and logits.stride(0) >= vocab else logits.contiguous()
+        if draft_logits is not None and draft_logits.stride() != logits.stride():
+            logits, draft_logits = logits.contiguous(), draft_logits.contiguous()
+        dev = logits.device
+        tokens = torch.empty((S, max_draft + 1), dtype=torch.int32, device=dev)
+        counts = torch.empty((S,), dtype=torch.int32, device=dev)
+        logprobs = torch.empty((S, max_draft + 1), dtype=torch.float32, device=dev)
+        L = _lib.load()
+        # (keyed by the size of the counters' region, which has to be zero at a launch)
+        ws = workspaces.get(("verify", (S * 4 + 255) // 256), L.pie_verify_workspace_bytes(S, R, vocab), dev)
+        _lib.check(L.pie_verify_draft(_p(tokens), _p(counts), _p(logprobs), _p(logits), _p(draft_logits), logits.stride(0), _p(draft_tokens), _p(logit_starts), S, R,
+                                      vocab, max_draft, float(temp), _p(uniforms), _p(noise), _p(ws), ws.numel(), _stream()), what)
+    return tokens, counts, logprobs
 
 
 _VOID = ("a bounded wait inside a tensor-core pipeline expired: results since the last check that passed are void "

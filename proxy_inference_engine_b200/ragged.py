@@ -15,10 +15,14 @@ it yet (its scheduler is a skeleton); here ``ragged_step`` runs it:
   appended before any of its queries attends.
 
 Same arithmetic as the per-sequence path (Model.__call__ over a PagedKVCache); tests/test_gpu_ragged.py compares the two.
+
+``StepPlan`` is the descriptor built on the device from lengths that live there: rows, slots and block table in one launch, one attention launch a layer that
+reads a request's keys once for all its new tokens, and drafted tokens among them (``speculative_step``).
 """
 from __future__ import annotations
 
 import ctypes as C
+import math
 from dataclasses import dataclass, field
 
 import torch
@@ -144,11 +148,124 @@ class BatchDetails:
         return self.consolidated_block_table[seq_of_token].contiguous()
 
 
+@dataclass
+class StepPlan:
+    """A ragged step described on the device: BatchDetails for callers whose requests' lengths live there -- after drafted tokens were verified, or in a captured
+    step that runs again on other lengths.  One launch fills it; nothing is read back.  All int32, views of ``words``:
+
+        row_starts [S + 1], contexts [S]     first row of each request, tokens it has in the cache
+        sequences, positions, slots [T]      each row's request, position in it, and place in the pools (page * 64 + place in the page); -1, 0, -1 for rows behind the last
+        block_table [S, max_blocks]          page ids, 0 behind a request's own
+        logit_starts [S + 1], logit_rows [R] rows whose logits are wanted: each request's last 1 + drafted ones; 0 behind the last
+        draft_tokens [R]                     the token each of them judges (verify_draft); -1 at a request's last
+    """
+    token_ids: torch.Tensor
+    words: torch.Tensor
+    dims: _lib.StepDims
+    row_starts: torch.Tensor
+    contexts: torch.Tensor
+    sequences: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    block_table: torch.Tensor
+    logit_starts: torch.Tensor
+    logit_rows: torch.Tensor
+    draft_tokens: torch.Tensor
+    status: torch.Tensor
+
+    FAULTS = {1: "a length is negative, or a request is longer than the step or its row of the block table", 2: "the requests have more tokens than token_ids",
+              4: "the requests need more pages than there are page ids", 8: "a page id is outside the pools", 16: "a request's drafted tokens are not fewer than its new ones",
+              32: "the requests have more logit rows than num_logits"}
+
+    @classmethod
+    def build(cls, token_ids, input_lengths, context_lengths, pages, *, num_pages: int, max_blocks: int, num_heads: int, num_kv_heads: int, draft_lengths=None,
+              num_logits: int | None = None) -> "StepPlan":
+        """token_ids int32 [T]: the requests' new tokens one behind the other; what is left of T belongs to nobody (ids of padding have to be tokens all the same).
+        input_lengths, context_lengths int32 [S]: new tokens (0: the request sits this step out) and tokens in the cache.  pages: int32 page ids, ceil((cached + new) / 64) of
+        each request one behind the other, or a table [S, columns] of them.  num_pages: of the pools.  max_blocks: columns of the plan's own block table.
+        draft_lengths int32 [S]: how many of a request's new tokens are drafted ones (fewer than its new ones).  num_logits: logit rows to make room for (default: S, none drafted).
+        Lengths that do not fit one another cannot be seen from here: check() tells, and until then nothing is read or written out of bounds."""
+        what = "StepPlan"
+        ops._step_ints(what, "token_ids", token_ids)
+        S = input_lengths.numel()
+        ops._step_ints(what, "input_lengths", input_lengths, (S,))
+        ops._step_ints(what, "context_lengths", context_lengths, (S,))
+        if draft_lengths is not None:
+            ops._step_ints(what, "draft_lengths", draft_lengths, (S,))
+        if pages.dtype != torch.int32 or pages.dim() not in (1, 2) or (pages.dim() == 2 and pages.shape[0] != S):
+            raise ValueError(f"[{what}] pages must be int32, a list or a table of {S} rows, but is {pages.dtype} {list(pages.shape)}")
+        if pages.stride(-1) != 1 or (pages.dim() == 2 and pages.stride(0) < 1):
+            pages = pages.contiguous()
+        dims = _lib.StepDims(S, token_ids.numel(), S if num_logits is None else int(num_logits), int(max_blocks), int(num_pages), int(num_heads), int(num_kv_heads))
+        L = _lib.load()
+        n = L.pie_step_plan_words(C.byref(dims))
+        if token_ids.dim() != 1 or n == 0:
+            raise ValueError(f"[{what}] not built here: {dims.requests} requests (1 to 4096), {dims.rows} rows, {dims.logit_rows} logit rows, {dims.blocks} blocks, "
+                             f"{dims.pages} pages, {dims.Hq} query heads on {dims.Hkv}")
+        given = [t for t in (token_ids, input_lengths, context_lengths, pages, draft_lengths) if t is not None]
+        with ops._one_device(what, *given):
+            words = torch.empty(n, dtype=torch.int32, device=token_ids.device)
+            stride = 0 if pages.dim() == 1 else pages.stride(0)
+            _lib.check(L.pie_step_plan_build(_p(words), C.byref(dims), _p(token_ids), _p(input_lengths), _p(context_lengths), _p(draft_lengths), _p(pages),
+                                             pages.shape[-1], stride, _stream()), what)
+        at = (C.c_longlong * 10)()
+        _lib.check(L.pie_step_plan_offsets(C.byref(dims), at), what)
+        T, R = dims.rows, dims.logit_rows
+        part = lambda i, *shape: words[at[i]:at[i] + math.prod(shape)].view(shape)
+        return cls(token_ids, words, dims, part(0, S + 1), part(1, S), part(2, T), part(3, T), part(4, T), part(5, S, dims.blocks), part(6, S + 1), part(7, R),
+                   part(8, R), part(9, 192))
+
+    def check(self) -> None:
+        """Waits for the plan and raises ValueError for lengths and page ids that do not fit."""
+        bits = 0
+        for word in self.status.tolist():
+            bits |= word
+        if bits:
+            raise ValueError("StepPlan: " + "; ".join(text for bit, text in self.FAULTS.items() if bits & bit))
+
+
+def _planned_step(model, plan: StepPlan, pools, all_logits: bool) -> torch.Tensor:
+    """ragged_step over a StepPlan: the rows' projections as there, keys and values through the slot map, attention of all rows in one launch a layer."""
+    a, T = model.args, plan.dims.rows
+    at0 = model.layers[0].self_attn
+    Hq, Hkv, D = at0.num_heads, at0.n_kv_heads, at0.head_dim
+    if getattr(at0.rope, "traditional", False) or getattr(getattr(model, "tp", None), "on", False):
+        raise ValueError("[ragged_step] a StepPlan is for one GPU's whole model with rotation by halves")
+    if len(pools) != len(model.layers):
+        raise ValueError(f"[ragged_step] {len(pools)} pools for {len(model.layers)} layers")
+    h = model.model.embed_tokens(plan.token_ids[None])
+    for ly, (kp, vp) in zip(model.layers, pools):
+        if isinstance(kp, (tuple, list)):
+            raise ValueError("[ragged_step] a StepPlan's attention reads bfloat16 pools; 8-bit pools are for BatchDetails")
+        at = ly.self_attn
+        x = ly.input_layernorm(h)
+        q = ops.rope_kv_slots(at.q_proj(x).view(T, Hq, D), at.k_proj(x).view(T, Hkv, D), at.v_proj(x).view(T, Hkv, D), at.rope._freqs, plan.positions, plan.slots, kp, vp)
+        o = ops.chunk_attention(q, kp, vp, plan, at.scale)
+        h = ops.add(h, at.o_proj(o[None]))
+        h = ops.add(h, ly.mlp(ly.post_attention_layernorm(h)))
+    if not all_logits:
+        h = h.index_select(1, plan.logit_rows)
+    w, s, b = model.head_slices()
+    qz = a.quantization
+    return ops.quantized_matmul(model.model.norm(h), w, s, b, transpose=True, group_size=qz["group_size"], bits=qz["bits"])[0]
+
+
+def speculative_step(model, plan: StepPlan, pools, *, max_draft: int, temp: float = 0.0, uniforms=None, noise=None, draft_logits=None):
+    """One step of drafting decode: ragged_step over a plan whose requests bring their last token and some drafted ones (draft_lengths), then verify_draft.
+    Returns its (tokens, counts, logprobs).  A request then has context + new - drafted + counts - 1 tokens in the cache -- what lies behind them there is
+    written over -- and its last token, tokens[s, counts[s] - 1], is the next step's first."""
+    logits = ragged_step(model, plan, pools)
+    return ops.verify_draft(logits, plan.draft_tokens, plan.logit_starts, max_draft=max_draft, temp=temp, uniforms=uniforms, noise=noise, draft_logits=draft_logits)
+
+
 def ragged_step(model, batch: BatchDetails, pools, all_logits: bool = False) -> torch.Tensor:
     """One forward step of ``model`` over ``batch``.  pools: per layer (k_pool, v_pool) bf16 [n_pages, 64, n_kv, D] --
     the pools the block table's page ids index -- or, for the 8-bit KV cache of cache.PagedQuantizedKVCache, per layer
     ((k_quants, k_scales, k_biases), (v_quants, v_scales, v_biases)) [n_pages, n_kv, 64, .].
-    Returns logits [num_sequences, vocab] of each sequence's last token (all_logits: [total_tokens, vocab])."""
+    Returns logits [num_sequences, vocab] of each sequence's last token (all_logits: [total_tokens, vocab]).
+    ``batch`` may be a StepPlan (bfloat16 pools): logits [num_logits, vocab] of its logit rows."""
+    if isinstance(batch, StepPlan):
+        return _planned_step(model, batch, pools, all_logits)
     batch.validate()
     L = _lib.load()
     a = model.args

@@ -1,0 +1,461 @@
+"""The operators of a ragged step beside its plan: rotation and cache write through the slot map, attention of every request's new tokens over its pages, drafted tokens
+against the target's probabilities -- each against 64 bits, and all of them together."""
+import random
+
+import pytest
+import torch
+
+import step_oracle as O
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+gen = lambda seed: torch.Generator(device="cuda").manual_seed(seed)
+randn = lambda g, *s, std=1.0: (std * torch.randn(s, generator=g, device="cuda")).to(BF)
+FREQS = lambda D: 500000.0 ** (torch.arange(0, D, 2, dtype=torch.float32, device="cuda") / D)
+
+
+# ---------------------------------------------------------------------------------------------------- rotation and cache write
+@pytest.mark.parametrize("D,Hq,Hkv,T,fused", [(64, 4, 2, 1, False), (128, 32, 8, 33, True), (64, 32, 8, 1030, True), (128, 5, 1, 7, False), (128, 64, 8, 1024, False)])
+def test_rope_kv_slots(D, Hq, Hkv, T, fused):
+    from proxy_inference_engine_b200 import ops
+    g, n_pages = gen(T + D), T // 64 + 3
+    if fused:
+        q, k, v = (t.view(T, -1, D) for t in randn(g, T, (Hq + 2 * Hkv) * D).split([Hq * D, Hkv * D, Hkv * D], 1))
+    else:
+        q, k, v = randn(g, T, Hq, D), randn(g, T, Hkv, D), randn(g, T, Hkv, D)
+    kp, vp = randn(g, n_pages, 64, Hkv, D), randn(g, n_pages, 64, Hkv, D)
+    positions = torch.randint(0, 131072, (T,), generator=g, device="cuda").to(torch.int32)
+    slots = torch.randperm(n_pages * 64, generator=g, device="cuda")[:T].to(torch.int32)
+    positions[0], slots[T // 2] = 0, n_pages * 64 - 1 if (n_pages * 64 - 1) not in slots.tolist() else slots[T // 2]
+    dead = [T - 1] if T > 2 else []
+    if dead:
+        slots[T - 1] = -1
+        if T > 20:
+            slots[11], dead = n_pages * 64, dead + [11]
+    live = [t for t in range(T) if t not in dead]
+    was_k, was_v = kp.clone(), vp.clone()
+    got = ops.rope_kv_slots(q, k, v, FREQS(D), positions, slots, kp, vp)
+    # half a step of bf16, and 3e-6 of sine and cosine (2 pi in two pieces, the approximation unit) and two fp32 products on either feature
+    near = lambda got, x, want: bool(((got.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 4e-6 * x.cpu().double().abs().sum(-1, keepdim=True)).all())
+    assert near(got[live], q[live], O.rope(q, positions, FREQS(D))[live]) and not got[dead].any()
+    at = slots[live].long()
+    assert near(kp.view(-1, Hkv, D)[at], k[live], O.rope(k, positions, FREQS(D))[live]) and torch.equal(vp.view(-1, Hkv, D)[at], v[live])
+    rest = torch.ones(n_pages * 64, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    for pool, was in ((kp, was_k), (vp, was_v)):
+        assert torch.equal(pool.view(-1, Hkv, D)[rest], was.view(-1, Hkv, D)[rest])
+    out = torch.full_like(got, 7.0)
+    assert ops.rope_kv_slots(q, k, v, FREQS(D), positions, slots, kp, vp, out=out) is out
+    assert torch.equal(out[live], got[live]) and bool((out[dead] == 7.0).all())
+
+
+def test_rope_kv_slots_is_rope_kv_append():
+    """Bit for bit, through a table of pages of one row each."""
+    import ctypes as C
+    from proxy_inference_engine_b200 import _lib, ops
+    g, T, Hq, Hkv, D = gen(5), 37, 8, 2, 128
+    qkv = randn(g, T, (Hq + 2 * Hkv) * D)
+    positions = torch.randint(0, 4096, (T,), generator=g, device="cuda").to(torch.int32)
+    table = torch.randint(0, 1, (T, 64), device="cuda", dtype=torch.int32)
+    pages = torch.randperm(64, generator=g, device="cuda")[:T].to(torch.int32)
+    table[torch.arange(T), (positions // 64).long()] = pages
+    pools = [torch.zeros((64, 64, Hkv, D), dtype=BF, device="cuda") for _ in range(4)]
+    q = torch.empty((T, Hq, D), dtype=BF, device="cuda")
+    lay = ops.kv_layout(pools[0], table, 64)
+    _lib.check(_lib.load().pie_rope_kv_append(q.data_ptr(), qkv.data_ptr(), pools[0].data_ptr(), pools[1].data_ptr(), C.byref(lay), positions.data_ptr(), FREQS(D).data_ptr(), T,
+                                              Hq, Hkv, D, ops._stream()), "rope_kv_append")
+    parts = (t.view(T, -1, D) for t in qkv.split([Hq * D, Hkv * D, Hkv * D], 1))
+    got = ops.rope_kv_slots(*parts, FREQS(D), positions, pages * 64 + positions % 64, pools[2], pools[3])
+    assert torch.equal(got, q) and torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
+
+
+# ---------------------------------------------------------------------------------------------------- attention
+def attention_case(new, cached, Hq, Hkv, D, seed=0, pad=0, std=2.0, strided=False):
+    """A plan and random queries over pools whose unused places hold NaN."""
+    from proxy_inference_engine_b200.ragged import StepPlan
+    rng, g = random.Random(seed), gen(seed)
+    counts = [O.need(n, c) for n, c in zip(new, cached)]
+    n_pages, T = sum(counts) + 2, sum(new) + pad
+    order = rng.sample(range(n_pages), sum(counts))
+    tables = [[order.pop() for _ in range(k)] for k in counts]
+    plan = StepPlan.build(ints([0] * T), ints(new), ints(cached), ints([p for t in tables for p in t]), num_pages=n_pages, max_blocks=max(1, *counts), num_heads=Hq,
+                          num_kv_heads=Hkv)
+    k, v = randn(g, n_pages, 64, Hkv, D), randn(g, n_pages, 64, Hkv, D)
+    used = torch.zeros(n_pages * 64, dtype=torch.bool)
+    for n, c, t in zip(new, cached, tables):
+        for i, p in enumerate(t):
+            used[p * 64:p * 64 + max(0, min(64, n + c - 64 * i))] = True
+    k.view(-1, Hkv, D)[~used.cuda()] = torch.nan
+    v.view(-1, Hkv, D)[~used.cuda()] = torch.nan
+    q = randn(g, T, Hq + (3 if strided else 0), D, std=std)[:, :Hq]
+    return plan, q, k, v, tables
+
+
+def attention_holds(got, q, k, v, new, cached, tables, scale):
+    """A weight in [0, 1] is rounded to bf16 at most once (2^-8 of it), the result once; scores are sums of D products in fp32 (2^-24 D of the sum of
+    |q k| scale, up to 2^-13 here, and so for the weights and for their sum), exponentials are off by a few 2^-22."""
+    want, weight = O.attention(q, k, v, new, cached, tables, scale)
+    T = sum(new)
+    got = got.view(got.shape[0], *q.shape[1:]).cpu().double()
+    off = (got[:T] - want[:T]).abs() - (2.0 ** -8 * want[:T].abs() + (2.0 ** -8 + 2.0 ** -12) * weight[:T])
+    assert bool((off <= 0).all()), float(off.max())     # (a NaN is not below)
+
+
+SHAPES = [
+    ([1], [0]), ([1], [63]), ([1], [64]), ([1], [127]), ([1], [128]), ([2], [255]), ([5], [700]), ([64], [0]), ([65], [0]), ([33], [100]), ([130], [0]), ([300], [77]),
+    ([1, 1, 1, 1], [0, 1, 300, 5000]), ([0, 3, 0, 70, 1, 0], [5, 60, 0, 1, 128, 0]), ([1, 6, 200, 1], [1000, 63, 300, 0]), ([700, 2], [513, 9000]),
+]
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 2, 64), (8, 2, 128), (32, 8, 128)])
+@pytest.mark.parametrize("new,cached", SHAPES)
+def test_chunk_attention(new, cached, Hq, Hkv, D):
+    from proxy_inference_engine_b200 import ops
+    plan, q, k, v, tables = attention_case(new, cached, Hq, Hkv, D, seed=len(new) + sum(new), strided=len(new) % 2 == 1)
+    plan.check()
+    got = ops.chunk_attention(q, k, v, plan, D ** -0.5)
+    attention_holds(got, q, k, v, new, cached, tables, D ** -0.5)
+    assert torch.equal(got, ops.chunk_attention(q, k, v, plan, D ** -0.5))      # whichever CTA comes last
+    ops.check_pipeline()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(1, 1, 64), (3, 1, 128), (24, 8, 64), (64, 8, 128), (7, 1, 64), (40, 1, 128), (128, 1, 64), (16, 16, 128)])
+def test_chunk_attention_of_other_heads(Hq, Hkv, D):
+    from proxy_inference_engine_b200 import ops
+    new, cached = [1, 45, 9, 4], [900, 30, 250, 2000]
+    plan, q, k, v, tables = attention_case(new, cached, Hq, Hkv, D, seed=Hq)
+    attention_holds(ops.chunk_attention(q, k, v, plan, D ** -0.5), q, k, v, new, cached, tables, D ** -0.5)
+    ops.check_pipeline()
+
+
+@pytest.mark.parametrize("std", [0.0, 30.0])
+def test_chunk_attention_of_flat_and_of_steep_scores(std):
+    """All keys alike, and one key that takes all: the running maximum moves by hundreds."""
+    from proxy_inference_engine_b200 import ops
+    new, cached = [3, 140], [1000, 600]
+    plan, q, k, v, tables = attention_case(new, cached, 8, 2, 128, seed=9, std=std)
+    want, weight = O.attention(q, k, v, new, cached, tables, 128 ** -0.5)
+    got = ops.chunk_attention(q, k, v, plan, 128 ** -0.5).view(want.shape).cpu().double()
+    # scores of up to 30 * 4 * 128^0.5 = 1400: 1400 * 128 * 2^-24 = 0.011 in the exponent at the worst, on either side of a quotient
+    assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + (0.022 if std else 2.0 ** -12)) * weight).all())
+    ops.check_pipeline()
+
+
+def test_rows_that_belong_to_nobody():
+    from proxy_inference_engine_b200 import ops
+    new, cached = [2, 0, 150], [70, 3, 0]
+    plan, q, k, v, tables = attention_case(new, cached, 8, 2, 64, seed=4, pad=70)
+    got = ops.chunk_attention(q, k, v, plan, 0.125)
+    attention_holds(got, q, k, v, new, cached, tables, 0.125)
+    assert not got[152:].any()
+    out = torch.full((222, 512), 3.0, dtype=BF, device="cuda")
+    assert ops.chunk_attention(q, k, v, plan, 0.125, out=out) is out
+    assert torch.equal(out[:152], got[:152]) and bool((out[152:] == 3.0).all())
+    nobody, q, k, v, _ = attention_case([0, 0], [5, 70], 8, 2, 64, pad=9)
+    assert not ops.chunk_attention(q, k, v, nobody, 0.125).any()
+
+
+def test_a_page_shared_by_two_requests():
+    from proxy_inference_engine_b200 import ops
+    from proxy_inference_engine_b200.ragged import StepPlan
+    g = gen(8)
+    k, v, q = randn(g, 5, 64, 2, 64), randn(g, 5, 64, 2, 64), randn(g, 21, 4, 64)
+    tables, new, cached = [[2, 0], [2, 4]], [1, 20], [100, 64]
+    plan = StepPlan.build(ints([0] * 21), ints(new), ints(cached), ints(tables), num_pages=5, max_blocks=2, num_heads=4, num_kv_heads=2)
+    attention_holds(ops.chunk_attention(q, k, v, plan, 0.2), q, k, v, new, cached, tables, 0.2)
+
+
+def test_pools_inside_larger_ones():
+    """Keys and values beside each other in one allocation, heads apart."""
+    from proxy_inference_engine_b200 import ops
+    new, cached = [3, 90], [300, 40]
+    plan, q, k, v, tables = attention_case(new, cached, 8, 2, 128, seed=6)
+    both = torch.full((k.shape[0], 64, 5, 128), torch.nan, dtype=BF, device="cuda")
+    both[:, :, 0:2], both[:, :, 2:4] = k, v
+    assert torch.equal(ops.chunk_attention(q, both[:, :, 0:2], both[:, :, 2:4], plan, 0.1), ops.chunk_attention(q, k, v, plan, 0.1))
+
+
+def test_attention_on_two_streams_at_once():
+    from proxy_inference_engine_b200 import ops
+    cases = [attention_case([4, 1], [6000, 3000], 8, 2, 128, seed=s) for s in (1, 2)]
+    want = [ops.chunk_attention(q, k, v, plan, 0.1) for plan, q, k, v, _ in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(20):
+        for i, (stream, (plan, q, k, v, _)) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(stream):
+                got[i].append(ops.chunk_attention(q, k, v, plan, 0.1))
+    torch.cuda.synchronize()
+    for mine, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in mine)
+
+
+# ---------------------------------------------------------------------------------------------------- verification
+def verify_case(drafted, V, temp, model, seed=0, ld=None):
+    g = gen(seed)
+    starts = [0]
+    for k in drafted:
+        starts.append(starts[-1] + (k + 1 if k >= 0 else 0))      # -1: a request without rows
+    R = max(1, starts[-1])
+    logits = 2.5 * torch.randn((R, V), generator=g, device="cuda")
+    logits.scatter_add_(1, torch.randint(0, V, (R, 1), generator=g, device="cuda"), 12 * torch.rand((R, 1), generator=g, device="cuda"))
+    guess = (logits + 0.8 * torch.randn((R, V), generator=g, device="cuda")).to(BF) if model else None
+    tokens = (guess.float() / temp).softmax(1).multinomial(1, generator=g)[:, 0] if model else torch.where(
+        torch.rand(R, generator=g, device="cuda") < 0.8, logits.argmax(1), torch.randint(0, V, (R,), generator=g, device="cuda"))
+    logits = logits.to(BF)
+    if ld:
+        wide = [None if t is None else torch.full((R, ld), 99.0, dtype=BF, device="cuda") for t in (logits, guess)]
+        wide[0][:, :V] = logits
+        if model:
+            wide[1][:, :V] = guess
+        logits, guess = wide[0][:, :V], None if guess is None else wide[1][:, :V]
+    return dict(logits=logits, draft_tokens=tokens.to(torch.int32), logit_starts=ints(starts), temp=temp, draft_logits=guess,
+                uniforms=torch.rand(R, generator=g, device="cuda") if temp else None, noise=torch.rand((len(drafted), V), generator=g, device="cuda") if temp else None), starts
+
+
+def verified(kw, starts, most):
+    from proxy_inference_engine_b200 import ops
+    tokens, counts, logprobs = ops.verify_draft(kw["logits"], kw["draft_tokens"], kw["logit_starts"], max_draft=most, temp=kw["temp"], uniforms=kw["uniforms"], noise=kw["noise"],
+                                                draft_logits=kw["draft_logits"])
+    want = O.verify(kw["logits"], kw["draft_tokens"], starts, most, kw["temp"], kw["uniforms"], kw["noise"], kw["draft_logits"])
+    tokens, counts, logprobs = tokens.tolist(), counts.tolist(), logprobs.tolist()
+    # a logarithm of a sum of exponentials that are each off by 2^-21 or so, of arguments rounded in fp32, and a difference
+    off = 4e-6 + 2.0 ** -22 * float(kw["logits"].float().nan_to_num(0, 0, 0).abs().max()) / (kw["temp"] or 1.0)
+    surely = 0
+    for t, c, lp, (wt, wlp, sure) in zip(tokens, counts, logprobs, want):
+        assert t[c:] == [-1] * (most + 1 - c) and lp[c:] == [0.0] * (most + 1 - c)
+        if sure:
+            surely += 1
+            assert t[:c] == wt and all(abs(a - b) <= off for a, b in zip(lp, wlp))
+    assert surely >= 0.9 * len(want)
+    return counts
+
+
+@pytest.mark.parametrize("V,ld", [(640, None), (50257, None), (128256, None), (1001, 1016), (8, None), (1, None)])
+@pytest.mark.parametrize("temp,model", [(0.0, False), (0.7, False), (1.0, True), (0.3, True)])
+def test_verify_draft(V, ld, temp, model):
+    drafted = [4, 0, 7, -1, 1, 2, 5, 7, 3]
+    kw, starts = verify_case(drafted, V, temp, model, seed=V, ld=ld)
+    counts = verified(kw, starts, 7)
+    assert counts[3] == 0 and all(1 <= c <= k + 1 for c, k in zip(counts, drafted) if k >= 0)
+    verified(kw, starts, 2)      # further drafts are not looked at
+
+
+@pytest.mark.parametrize("S,K", [(1, 4), (1, 127), (300, 1), (64, 5)])
+def test_verify_of_few_and_of_many(S, K):
+    rng = random.Random(S)
+    kw, starts = verify_case([K if S == 1 else rng.randint(0, K) for _ in range(S)], 4001, 0.9, True, seed=S)
+    if S == 1 and K == 127:      # all of them accepted but the last: a draw below every quotient
+        kw["uniforms"].zero_()
+        kw["uniforms"][126] = 1.0 - 2.0 ** -24
+    verified(kw, starts, K)
+
+
+def test_the_same_draft_is_always_accepted():
+    kw, starts = verify_case([5] * 8, 3001, 1.0, True, seed=3)
+    kw["draft_logits"] = kw["logits"].clone()
+    kw["uniforms"].fill_(1.0 - 2.0 ** -24)
+    # q(x) u < p(x) with q = p in the same bits
+    from proxy_inference_engine_b200 import ops
+    counts = ops.verify_draft(kw["logits"], kw["draft_tokens"], kw["logit_starts"], max_draft=5, temp=1.0, uniforms=kw["uniforms"], noise=kw["noise"],
+                              draft_logits=kw["draft_logits"])[1]
+    assert counts.tolist() == [6] * 8
+
+
+def test_ties_go_to_the_first():
+    from proxy_inference_engine_b200 import ops
+    logits = torch.zeros((4, 5000), dtype=BF, device="cuda")
+    logits[:, 3000] = logits[:, 777] = 2.0
+    logits[1, 10], logits[2] = -0.0, -torch.inf
+    logits[2, 9], logits[2, 5], logits[3], logits[3, 40] = 0.0, -0.0, -1.0, -0.0
+    got = ops.verify_draft(logits, ints([777, 777, 5, 0]), ints([0, 4]), max_draft=3)
+    assert got[0].tolist() == [[777, 777, 5, 40]] and got[1].tolist() == [4]
+
+
+def test_filters_and_rows_without_a_distribution():
+    from proxy_inference_engine_b200 import ops
+    V, inf = 3000, float("inf")
+    kw, starts = verify_case([2] * 6, V, 0.8, True, seed=12)
+    for t in (kw["logits"], kw["draft_logits"]):
+        keep = torch.rand(t.shape, generator=gen(5), device="cuda") < 0.01
+        keep[:, 17] = True
+        t[~keep] = -inf                                       # a filter's work: the drafted token may be one that cannot be
+    verified(kw, starts, 2)
+    kw["logits"][0, 5], kw["logits"][3, 6], kw["logits"][6], kw["draft_logits"][9, 3] = float("nan"), inf, -inf, float("nan")
+    kw["logits"][12:15] = -inf
+    kw["logits"][12:15, 17] = 1.0                              # all of it on one token
+    kw["draft_tokens"][12:15] = 17
+    tokens, counts, logprobs = ops.verify_draft(kw["logits"], kw["draft_tokens"], kw["logit_starts"], max_draft=2, temp=0.8, uniforms=kw["uniforms"], noise=kw["noise"],
+                                                draft_logits=kw["draft_logits"])
+    tokens = tokens.tolist()
+    assert counts.tolist()[:4] == [1, 1, 1, 1] and [t[0] for t in tokens[:3]] == [0, 0, 0] and tokens[4] == [17, 17, 17]
+    assert all(0 <= x < V for x in tokens[3][:1]) and float(kw["logits"][9, tokens[3][0]]) > -inf
+    assert torch.isnan(logprobs[0, 0]) and logprobs[4].tolist() == [0.0, 0.0, 0.0]
+    greedy = torch.full((2, 64), -inf, dtype=BF, device="cuda")
+    greedy[0, 3], greedy[0, 7] = float("nan"), 2.0
+    assert ops.verify_draft(greedy, ints([7, 0]), ints([0, 2]), max_draft=1)[0].tolist() == [[7, 0]]
+
+
+def test_tokens_outside_the_vocabulary_and_starts_outside_the_rows():
+    from proxy_inference_engine_b200 import ops
+    kw, starts = verify_case([2, 2, 2], 900, 0.8, False, seed=2)
+    kw["draft_tokens"][0], kw["draft_tokens"][3], kw["uniforms"][:] = -1, 900, 0.0
+    got = ops.verify_draft(kw["logits"], kw["draft_tokens"], kw["logit_starts"], max_draft=2, temp=0.8, uniforms=kw["uniforms"], noise=kw["noise"])
+    assert got[1].tolist()[:2] == [1, 1] and got[1].tolist()[2] >= 1
+    for bad in ([-5, 2, 100, 7], [9, 3, 3, 9], [0, 1 << 30, -(1 << 30), 2]):
+        tokens, counts, _ = ops.verify_draft(kw["logits"], kw["draft_tokens"], ints(bad), max_draft=2, temp=0.8, uniforms=kw["uniforms"], noise=kw["noise"])
+        assert all(0 <= c <= 3 for c in counts.tolist())
+
+
+def test_draws_follow_the_target():
+    """Drafts from q, verified against p: the first token behind them is distributed as p.  4000 draws of 6 tokens: five standard deviations."""
+    from proxy_inference_engine_b200 import ops
+    S, V, g = 4000, 6, gen(77)
+    p, q = torch.tensor([2.0, 1.0, 0.0, 0.5, -1.0, 1.5], device="cuda"), torch.tensor([0.0, 2.0, 1.0, 0.5, 0.0, -2.0], device="cuda")
+    logits, guess = p.to(BF).expand(2 * S, V).contiguous(), q.to(BF).expand(2 * S, V).contiguous()
+    drafted = guess[0].float().softmax(0).multinomial(2 * S, replacement=True, generator=g).to(torch.int32)
+    for draft_logits, given in ((guess, drafted), (None, torch.full_like(drafted, 1))):
+        tokens, counts, _ = ops.verify_draft(logits, given, torch.arange(0, 2 * S + 1, 2, device="cuda", dtype=torch.int32), max_draft=1, temp=1.0,
+                                             uniforms=torch.rand(2 * S, generator=g, device="cuda"), noise=torch.rand((S, V), generator=g, device="cuda"), draft_logits=draft_logits)
+        want = p.double().softmax(0).cpu()
+        seen = torch.bincount(tokens[:, 0].long().cpu(), minlength=V).double() / S
+        assert bool(((seen - want).abs() <= 5 * (want * (1 - want) / S).sqrt()).all())
+        assert set(counts.tolist()) == {1, 2}
+
+
+# ---------------------------------------------------------------------------------------------------- together
+def _model(head_dim=64, n_pages=40, seed=5):
+    from parity_util import tiny_args
+    from proxy_inference_engine_b200.checkpoint import build_model, random_weights
+    args = tiny_args(bits=4, head_dim=head_dim)
+    w = random_weights(args, seed=seed, device="cuda", gen_device="cpu")
+    mk = lambda: [tuple(torch.full((n_pages, 64, args.num_key_value_heads, args.head_dim), torch.nan, dtype=BF, device="cuda") for _ in range(2))
+                  for _ in range(args.num_hidden_layers)]
+    return args, w, build_model(args, w), mk
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_a_planned_step_is_the_ragged_step(head_dim):
+    """The same logits as BatchDetails', whose rows each have a decode attention of their own, and as the oracle's."""
+    import numpy as np
+    from parity_util import make_oracle, rel_l2
+    from proxy_inference_engine_b200.ragged import BatchDetails, StepPlan, ragged_step
+    args, w, model, mk = _model(head_dim)
+    rng = np.random.default_rng(0)
+    seq = {s: rng.integers(0, args.vocab_size, n).tolist() for s, n in ((7, 70), (11, 101), (12, 84))}
+    pages = {7: [3, 9], 11: [1, 0], 12: [30, 5]}
+    old, new = mk(), mk()
+    for k, v in old:
+        k.zero_(), v.zero_()
+    steps = [[(11, 0, 100), (12, 0, 64)], [(7, 0, 70), (11, 100, 101), (12, 64, 84)]]
+    for step in steps:
+        batch = BatchDetails.build([(s, seq[s][a:b], a, pages[s]) for s, a, b in step])
+        want = ragged_step(model, batch, old, all_logits=True).float().cpu().numpy()
+        plan = StepPlan.build(ints([t for s, a, b in step for t in seq[s][a:b]]), ints([b - a for s, a, b in step]), ints([a for s, a, b in step]),
+                              ints([p for s, a, b in step for p in pages[s][:O.need(b - a, a)]]), num_pages=40, max_blocks=2, num_heads=args.num_attention_heads,
+                              num_kv_heads=args.num_key_value_heads)
+        plan.check()
+        got = ragged_step(model, plan, new, all_logits=True).float().cpu().numpy()
+        assert rel_l2(got, want) < 1e-2
+        last = ragged_step(model, plan, new).float().cpu().numpy()
+        assert last.shape[0] == len(step) and rel_l2(last, got[batch.last_token_rows().tolist()]) < 5e-3
+    o = make_oracle(args, w)
+    for row, (s, _, _) in zip(last, steps[-1]):
+        lo = o(np.asarray([seq[s]], np.int32), o.make_cache(), last_only=True)[0, -1]
+        assert rel_l2(row, lo) < 2e-2
+
+
+def test_drafting_gives_the_text_that_decoding_gives():
+    """Greedy speculative steps with good, bad and no drafts, lengths kept on the device: every token is the first largest logit of the 64-token-page cache's own
+    model, or one that the model cannot tell from it (other row counts round other sums)."""
+    import numpy as np
+    from parity_util import make_oracle
+    from proxy_inference_engine_b200.ragged import StepPlan, speculative_step
+    args, w, model, mk = _model(64)
+    pools, rng, S, K = mk(), random.Random(3), 3, 4
+    prompts = [[rng.randrange(args.vocab_size) for _ in range(n)] for n in (61, 5, 130)]
+    table = ints([[i * 8 + j for j in range(8)] for i in range(S)])
+    plan_of = lambda ids, new, cached, drafted, R: StepPlan.build(ids, new, cached, table, num_pages=40, max_blocks=8, num_heads=args.num_attention_heads,
+                                                                  num_kv_heads=args.num_key_value_heads, draft_lengths=drafted, num_logits=R)
+    new, cached = ints([len(p) for p in prompts]), ints([0] * S)
+    tokens, counts, _ = speculative_step(model, plan_of(ints(sum(prompts, [])), new, cached, None, S), pools, max_draft=0)
+    cached, text = cached + new, [p + [t] for p, t in zip(prompts, tokens[:, 0].tolist())]
+    o = make_oracle(args, w)
+    truth = [list(t) for t in text]
+    accepted = 0
+    for step in range(6):
+        drafts = []
+        for s in range(S):      # the oracle's own continuation as a draft, spoilt at some place
+            ids, mine = list(text[s]), []
+            for _ in range((step + s) % (K + 1)):
+                lo = o(np.asarray([ids], np.int32), o.make_cache(), last_only=True)[0, -1]
+                mine.append(int(lo.argmax()))
+                ids.append(mine[-1])
+            if mine and rng.random() < 0.5:
+                mine[rng.randrange(len(mine))] = rng.randrange(args.vocab_size)
+            drafts.append(mine)
+        ids = [t for s in range(S) for t in [text[s][-1]] + drafts[s]]
+        drafted = ints([len(d) for d in drafts])
+        plan = plan_of(ints(ids + [0] * 3), drafted + 1, cached, drafted, len(ids))
+        tokens, counts, _ = speculative_step(model, plan, pools, max_draft=K)
+        cached = cached + counts                                    # context + new - drafted + counts - 1
+        plan.check()
+        for s, (t, c) in enumerate(zip(tokens.tolist(), counts.tolist())):
+            accepted += c - 1
+            assert 1 <= c <= len(drafts[s]) + 1 and t[:c - 1] == drafts[s][:c - 1]
+            text[s] += t[:c]
+    assert accepted > 5
+    for s in range(S):
+        lo = o(np.asarray([text[s][:-1]], np.int32), o.make_cache())[0]
+        for i in range(len(prompts[s]), len(text[s])):
+            row = lo[i - 1]
+            assert text[s][i] == int(row.argmax()) or row.max() - row[text[s][i]] < 2e-2 * np.abs(row).max()
+
+
+def test_a_captured_step_runs_again_on_other_lengths():
+    from proxy_inference_engine_b200.ragged import StepPlan, speculative_step
+    args, w, model, mk = _model(128)
+    pools, S, T, V = mk(), 2, 12, args.vocab_size
+    g = gen(1)
+    for k, v in pools:
+        k.copy_(randn(g, *k.shape, std=0.5)), v.copy_(randn(g, *v.shape))
+    ids, new, cached, drafted = ints([0] * T), ints([1, 1]), ints([10, 10]), ints([0, 0])
+    table, uniforms, noise = ints([[3, 4, 5, 6], [7, 8, 9, 10]]), torch.rand(T, generator=g, device="cuda"), torch.rand((S, V), generator=g, device="cuda")
+
+    def step():
+        plan = StepPlan.build(ids, new, cached, table, num_pages=40, max_blocks=4, num_heads=args.num_attention_heads, num_kv_heads=args.num_key_value_heads, draft_lengths=drafted,
+                              num_logits=T)
+        return speculative_step(model, plan, pools, max_draft=4, temp=0.9, uniforms=uniforms, noise=noise)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    kept = [(k.clone(), v.clone()) for k, v in pools]
+    restore = lambda: [t.copy_(t0) for pair, pair0 in zip(pools, kept) for t, t0 in zip(pair, pair0)]
+    for lens, ctx, dr in (([3, 5], [60, 100], [2, 4]), ([0, 1], [7, 200], [0, 0]), ([5, 1], [130, 0], [4, 0])):
+        for t, x in ((new, lens), (cached, ctx), (drafted, dr), (ids, [(7 * i + sum(ctx)) % V for i in range(T)])):
+            t.copy_(ints(x))
+        restore()
+        graph.replay()
+        got = [t.clone() for t in out]
+        restore()
+        want = step()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def test_a_planned_step_refuses():
+    from proxy_inference_engine_b200.ragged import StepPlan, ragged_step
+    args, w, model, mk = _model(64)
+    plan = StepPlan.build(ints([1]), ints([1]), ints([0]), ints([0]), num_pages=40, max_blocks=1, num_heads=args.num_attention_heads, num_kv_heads=args.num_key_value_heads)
+    pools = mk()
+    with pytest.raises(ValueError, match="8-bit"):
+        ragged_step(model, plan, [((k,), (v,)) for k, v in pools])
+    with pytest.raises(ValueError, match="pools for"):
+        ragged_step(model, plan, pools[:1])
+    model.layers[0].self_attn.rope.traditional = True
+    with pytest.raises(ValueError, match="by halves"):
+        ragged_step(model, plan, pools)
