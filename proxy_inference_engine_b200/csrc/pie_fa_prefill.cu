@@ -491,3 +491,5 @@ cudaError_t fa_prefill_pipeline_post(unsigned int* host, cudaStream_t st) { retu
 cudaError_t fa_prefill_pipeline_clear() { return gemm_error_clear(); }
 
 }  // namespace pie
+
+#include "pie_chunk_attn.cuh"
