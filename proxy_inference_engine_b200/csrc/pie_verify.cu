@@ -4,6 +4,8 @@
 // Two launches.  verify_stats_kernel reads every row of logits once: maximum and sum of exponentials (greedy: and the first largest) of slices, in 32 bits.
 // verify_emit_kernel: each CTA of a request joins its rows' slices, finds how many drafted tokens are accepted, and takes a slice of the vocabulary of the one row behind
 // them; the last CTA to finish joins the slices' best.  All of it is bound by HBM: a row of 128256 logits is 257 KB.
+#include <algorithm>
+
 #include "pie_internal.h"
 #include "pie_ptx.cuh"
 
@@ -45,58 +47,153 @@ __device__ __forceinline__ unsigned long long ver_block_max(unsigned long long v
   __syncthreads();
   return v;
 }
-// (m, s) <- the maximum and the sum of exponentials of two parts
-__device__ __forceinline__ void ver_join(float& m, float& s, float m2, float s2) {
+// (m, s) <- the maximum and the sum of exp2(c (x - maximum)) of two parts
+__device__ __forceinline__ void ver_join(float& m, float& s, float m2, float s2, float c) {
   const float mx = fmaxf(m, m2);
-  s = (s == 0.f ? 0.f : s * __expf(m - mx)) + (s2 == 0.f ? 0.f : s2 * __expf(m2 - mx));
+  s = (s == 0.f ? 0.f : s * exp2f((m - mx) * c)) + (s2 == 0.f ? 0.f : s2 * exp2f((m2 - mx) * c));
   m = mx;
 }
-// elements [lo, hi) of slice i of n
-__device__ __forceinline__ void ver_slice(int vocab, int i, int n, int& lo, int& hi) {
-  const int per = ((vocab + n - 1) / n + 7) / 8 * 8;
-  lo = min(i * per, vocab);
-  hi = min(lo + per, vocab);
+// A row is read 16 bytes (8 logits) at a time from its first 16-byte boundary on; what lies in front of that and behind the last whole 8 is few single ones.
+struct VerRow {
+  const uint16_t* x;
+  int head, vectors, tail;   // logits in front, 8 at a time, first one behind
+};
+__device__ __forceinline__ VerRow ver_row(const uint16_t* x, int vocab) {
+  VerRow r;
+  r.x = x;
+  r.head = min((int)((8 - ((reinterpret_cast<uintptr_t>(x) >> 1) & 7)) & 7), vocab);
+  r.vectors = (vocab - r.head) / 8;
+  r.tail = r.head + 8 * r.vectors;
+  return r;
+}
+// vectors [lo, hi) of slice i of n
+__device__ __forceinline__ void ver_slice(int vectors, int i, int n, int& lo, int& hi) {
+  const int per = (vectors + n - 1) / n;
+  lo = min(i * per, vectors);
+  hi = min(lo + per, vectors);
+}
+__device__ __forceinline__ uint4 ver_load(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ uint32_t ver_max2(uint32_t a, uint32_t b) {   // of two pairs of bf16; a number before a NaN
+  uint32_t d;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ float ver_exp2(float x) {   // results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
+// A thread's part of a row: maximum x and sum of exp2(c x + off), off = -c maximum rounded -- one fused multiply-add an exponential, and what the rounding does to all
+// of them alike (2^-24 of c x, more than a sum may be off by) is taken back at the end.  32 logits a turn; their maximum is taken in pairs of bf16, and moves the sum
+// once a turn.  Greedy: where it moves is where the first largest lies so far.
+struct VerSum {
+  float m = -INFINITY, off = 0.f, s = 0.f;
+  int index = -1;
+  __device__ __forceinline__ void move(float mx, float c) {
+    const float to = -mx * c;
+    s = m == -INFINITY ? s : s * ver_exp2(to - off);        // (a NaN in s stays one)
+    m = mx;
+    off = to;
+  }
+  __device__ __forceinline__ void one(float x, int i, float c) {
+    x += 0.f;                                                // (-0 is 0)
+    if (x > m) { move(x, c); index = i; }
+    if (index < 0 && x == x) index = i;
+    s += x == -INFINITY ? 0.f : ver_exp2(fmaf(x, c, off));
+  }
+  __device__ __forceinline__ float sum(float c) const { return m == -INFINITY ? s : s * ver_exp2(-fmaf(m, c, off)); }   // of exp2(c (x - m))
+};
+
+constexpr int kVerTurn = 4;   // vectors a thread has in flight
 __global__ void __launch_bounds__(kVerThreads) verify_stats_kernel(const __grid_constant__ VerArgs a) {
   __shared__ float sm[kVerThreads / 32][2];
   __shared__ unsigned long long km[kVerThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
-  const uint16_t* x = (which ? a.guess : a.logits) + (size_t)r * a.ld;
+  const VerRow row = ver_row((which ? a.guess : a.logits) + (size_t)r * a.ld, a.vocab);
+  const float c = a.itemp * 1.4426950408889634f;
+  VerSum sum;
+  if (blockIdx.x == 0 && tid < row.head) sum.one(bf16lo((uint32_t)__ldg(row.x + tid)), tid, c);
   int lo, hi;
-  ver_slice(a.vocab, blockIdx.x, a.splits, lo, hi);
-  float m = -INFINITY, s = 0.f;
-  unsigned long long key = 0;
-  for (int i = lo + tid; i < hi; i += kVerThreads) {
-    const float v = bf16lo((uint32_t)__ldg(x + i)) + 0.f;   // (-0 is 0)
-    if (a.greedy && v == v) key = ver_max(key, ver_key(v, i));
-    const float t = v * a.itemp;
-    if (t > m) { s = s * __expf(m - t) + 1.f; m = t; }
-    else if (t != -INFINITY) s += __expf(t - m);   // (a NaN ends up in the sum)
+  ver_slice(row.vectors, blockIdx.x, a.splits, lo, hi);
+  for (int v0 = lo + tid; v0 < hi; v0 += kVerTurn * kVerThreads) {
+    uint4 x[kVerTurn];
+#pragma unroll
+    for (int t = 0; t < kVerTurn; ++t) {
+      const int v = v0 + t * kVerThreads;
+      x[t] = v < hi ? ver_load(row.x + row.head + 8 * (size_t)v) : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);   // -inf
+    }
+    uint32_t m2 = x[0].x;
+#pragma unroll
+    for (int t = 0; t < kVerTurn; ++t) m2 = ver_max2(ver_max2(m2, ver_max2(x[t].x, x[t].y)), ver_max2(x[t].z, x[t].w));
+    const float mx = fmaxf(bf16lo(m2), bf16hi(m2)) + 0.f;
+    if (mx > sum.m || (a.greedy && sum.index < 0)) {
+      if (mx > sum.m) { sum.move(mx, c); sum.index = -1; }
+      if (a.greedy) {   // the first of this turn that is the largest so far
+#pragma unroll
+        for (int t = 0; t < kVerTurn; ++t) {
+          const uint32_t w[4] = {x[t].x, x[t].y, x[t].z, x[t].w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float f = (e & 1 ? bf16hi(w[e / 2]) : bf16lo(w[e / 2])) + 0.f;
+            if (sum.index < 0 && f == sum.m && v0 + t * kVerThreads < hi) sum.index = row.head + 8 * (v0 + t * kVerThreads) + e;
+          }
+        }
+      }
+    }
+    const float off = sum.off;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int t = 0; t < kVerTurn; ++t) {
+      const uint32_t w[4] = {x[t].x, x[t].y, x[t].z, x[t].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s0 += ver_exp2(fmaf(bf16lo(w[e]), c, off));
+        s1 += ver_exp2(fmaf(bf16hi(w[e]), c, off));
+      }
+    }
+    sum.s += s0 + s1;
   }
+  if ((int)blockIdx.x == a.splits - 1 && tid < a.vocab - row.tail) sum.one(bf16lo((uint32_t)__ldg(row.x + row.tail + tid)), row.tail + tid, c);
+  float m = sum.m, s = sum.sum(c);
+  unsigned long long key = a.greedy && sum.index >= 0 ? ver_key(m, sum.index) : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    ver_join(m, s, m2, s2);
+    ver_join(m, s, m2, s2, c);
   }
   if ((tid & 31) == 0) { sm[tid >> 5][0] = m; sm[tid >> 5][1] = s; }
   if (a.greedy) key = ver_block_max(key, km); else __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < kVerThreads / 32; ++w) ver_join(m, s, sm[w][0], sm[w][1]);
+    for (int w = 1; w < kVerThreads / 32; ++w) ver_join(m, s, sm[w][0], sm[w][1], c);
     *reinterpret_cast<float4*>(a.stats + (((size_t)r * 2 + which) * a.splits + blockIdx.x) * 4) =
         make_float4(m, s, __uint_as_float((uint32_t)(key >> 32)), __int_as_float(key ? ver_index(key) : 0));
   }
 }
 
+// The race: of weights w and draws u, the largest w / -log(u), held as the pair (w, E = -log(u)) of the best so far, so that a comparison is two products.  As
+// 1 - u <= E, most lose without a logarithm.  (E is taken by logf: near u = 1, where the winners lie, it is good to its last place, and the approximation unit's is not.)
+struct VerRace {
+  float w = 0.f, e = 1.f;
+  int index = -1;
+  __device__ __forceinline__ void run(float wi, float u, int i) {
+    if (wi * e * 1.000001f > w * (1.f - u)) {   // (false for a NaN weight and for a weight of 0; at the start true for any other)
+      const float ei = fmaxf(-logf(fmaxf(u, 1.17549435e-38f)), 0.f);   // (a draw of 0 is the smallest there is: a token that is alone wins with it)
+      if (wi > 0.f && wi * e > w * ei) { w = wi; e = ei; index = i; }
+    }
+  }
+};
+
 __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_constant__ VerArgs a) {
-  __shared__ float lse[2][kVerMaxDraft + 1];
+  __shared__ float2 dist[2][kVerMaxDraft + 1];   // of p and q of each row: maximum, sum of exp2(c (x - maximum))
   __shared__ int top[kVerMaxDraft + 1], ok[kVerMaxDraft + 1], s_accepted, s_last;
   __shared__ unsigned long long km[kVerThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float c = a.itemp * 1.4426950408889634f;
   const int r0 = max(0, min(__ldg(a.starts + s), a.rows)), r1 = max(r0, min(__ldg(a.starts + s + 1), a.rows));
   const int n = min(r1 - r0, a.most + 1);   // rows that count
   int32_t* const tokens = a.tokens + (size_t)s * (a.most + 1);
@@ -112,7 +209,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
   for (int j = warp; j < n; j += kVerThreads / 32) {
     const int r = r0 + j, x = __ldg(a.draft + r);
     const bool last = j == n - 1, real = x >= 0 && x < a.vocab;
-    float l[2] = {0.f, 0.f};
+    float2 d[2] = {{0.f, 1.f}, {0.f, 1.f}};
     unsigned long long key = 0;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -120,26 +217,26 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
       float m = -INFINITY, sum = 0.f;
       for (int i = lane; i < a.splits; i += 32) {
         const float4 p = __ldcg(reinterpret_cast<const float4*>(a.stats + (((size_t)r * 2 + which) * a.splits + i) * 4));
-        ver_join(m, sum, p.x, p.y);
+        ver_join(m, sum, p.x, p.y, c);
         if (!which) key = ver_max(key, ((unsigned long long)__float_as_uint(p.z) << 32) | (uint32_t)~__float_as_int(p.w));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
-        ver_join(m, sum, m2, s2);
+        ver_join(m, sum, m2, s2, c);
         key = ver_max(key, __shfl_xor_sync(0xffffffffu, key, o));
       }
-      l[which] = m + logf(sum);
+      d[which] = make_float2(m, sum);
     }
     if (lane == 0) {
-      lse[0][j] = l[0];
-      lse[1][j] = l[1];
+      dist[0][j] = d[0];
+      dist[1][j] = d[1];
       top[j] = key >> 32 ? ver_index(key) : 0;
       bool yes = !last && real;
       if (yes && a.greedy) yes = top[j] == x;
       else if (yes) {
-        const float p = expf(bf16lo((uint32_t)a.logits[(size_t)r * a.ld + x]) * a.itemp - l[0]);
-        const float q = a.guess ? expf(bf16lo((uint32_t)a.guess[(size_t)r * a.ld + x]) * a.itemp - l[1]) : 1.f;
+        const float p = expf((bf16lo((uint32_t)a.logits[(size_t)r * a.ld + x]) - d[0].x) * a.itemp) / d[0].y;
+        const float q = a.guess ? expf((bf16lo((uint32_t)a.guess[(size_t)r * a.ld + x]) - d[1].x) * a.itemp) / d[1].y : 1.f;
         yes = a.uniforms[r] * q < p;
       }
       ok[j] = yes;
@@ -162,22 +259,45 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
     const uint16_t* const g = refused && a.guess ? a.guess + (size_t)r * a.ld : nullptr;
     const int out = refused && !a.guess ? __ldg(a.draft + r) : -1;   // the token that was refused
     const float* const u = a.noise + (size_t)s * a.vocab;
-    const float lp = lse[0][k], lq = lse[1][k];
-    auto race = [&](int lo, int hi, bool whole) {
-      unsigned long long key = 0;
-      for (int i = lo + tid; i < hi; i += kVerThreads) {
-        float w = expf(bf16lo((uint32_t)__ldg(x + i)) * a.itemp - lp);
-        if (!whole) {
-          if (g) w -= expf(bf16lo((uint32_t)__ldg(g + i)) * a.itemp - lq);
-          if (i == out) w = 0.f;
+    // p = kp exp2(c x + op), as in the first launch
+    const float2 dp = dist[0][k], dq = dist[1][k];
+    const float op = -dp.x * c, oq = -dq.x * c, kp = exp2f(-fmaf(dp.x, c, op)) / dp.y, kq = exp2f(-fmaf(dq.x, c, oq)) / dq.y;
+    const VerRow row = ver_row(x, a.vocab);
+    const bool flat = !(reinterpret_cast<uintptr_t>(u + row.head) & 15);   // the draws can be read 16 bytes at a time as well
+    // slice i of n; whole: of the target's own weights
+    auto race = [&](int i, int n, bool whole) {
+      const uint16_t* const q = whole ? nullptr : g;
+      const int not_this = whole ? -1 : out;
+      VerRace best;
+      auto run = [&](float xi, float qi, float ui, int at) {
+        float w = __fmul_rn(ver_exp2(fmaf(xi, c, op)), kp);
+        if (q) w = __fsub_rn(w, __fmul_rn(ver_exp2(fmaf(qi, c, oq)), kq));   // (no fused form: p = q leaves nothing)
+        best.run(at == not_this ? 0.f : w, ui, at);
+      };
+      auto single = [&](int at) { run(bf16lo((uint32_t)__ldg(x + at)), q ? bf16lo((uint32_t)__ldg(q + at)) : 0.f, __ldg(u + at), at); };
+      if (i == 0 && tid < row.head) single(tid);
+      int lo, hi;
+      ver_slice(row.vectors, i, n, lo, hi);
+#pragma unroll 2
+      for (int v = lo + tid; v < hi; v += kVerThreads) {
+        const int at = row.head + 8 * v;
+        const uint4 xv = ver_load(x + at), qv = q ? ver_load(q + at) : make_uint4(0, 0, 0, 0);
+        float ui[8];
+        if (flat) {
+          *reinterpret_cast<float4*>(ui) = __ldg(reinterpret_cast<const float4*>(u + at));
+          *reinterpret_cast<float4*>(ui + 4) = __ldg(reinterpret_cast<const float4*>(u + at + 4));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ui[e] = __ldg(u + at + e);
         }
-        if (w > 0.f) key = ver_max(key, ver_key(w / -logf(__ldg(u + i)), i));
+        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, qw[4] = {qv.x, qv.y, qv.z, qv.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) run(e & 1 ? bf16hi(xw[e / 2]) : bf16lo(xw[e / 2]), e & 1 ? bf16hi(qw[e / 2]) : bf16lo(qw[e / 2]), ui[e], at + e);
       }
-      return ver_block_max(key, km);
+      if (i == n - 1 && tid < a.vocab - row.tail) single(row.tail + tid);
+      return ver_block_max(best.index >= 0 ? ver_key(best.w / best.e, best.index) : 0, km);
     };
-    int lo, hi;
-    ver_slice(a.vocab, blockIdx.x, a.emit_splits, lo, hi);
-    unsigned long long key = race(lo, hi, false);
+    unsigned long long key = race(blockIdx.x, a.emit_splits, false);
     if (a.emit_splits > 1) {
       if (tid == 0) {
         __stcg(a.best + (size_t)s * a.emit_splits + blockIdx.x, key);
@@ -192,7 +312,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
       for (int i = tid; i < a.emit_splits; i += kVerThreads) key = ver_max(key, __ldcg(a.best + (size_t)s * a.emit_splits + i));
       key = ver_block_max(key, km);
     }
-    if (key == 0 && refused) key = race(0, a.vocab, true);
+    if (key == 0 && refused) key = race(0, 1, true);
     token = key ? ver_index(key) : 0;
   }
   for (int j = tid; j <= a.most; j += kVerThreads) {
@@ -200,7 +320,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
     float lp = 0.f;
     if (j <= k) {
       t = j < k ? __ldg(a.draft + r0 + j) : token;
-      lp = bf16lo((uint32_t)a.logits[(size_t)(r0 + j) * a.ld + t]) * a.itemp - lse[0][j];
+      lp = (bf16lo((uint32_t)a.logits[(size_t)(r0 + j) * a.ld + t]) - dist[0][j].x) * a.itemp - logf(dist[0][j].y);
     }
     tokens[j] = t;
     logprobs[j] = lp;
@@ -211,13 +331,13 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
 struct VerPlan { int splits, emit_splits; size_t stats, best, bytes; };
 static VerPlan ver_plan(int requests, int rows, int vocab) {
   VerPlan p;
-  // slices of at least 4096 tokens, as many as give the device two rounds of CTAs
-  auto pick = [&](int units) {
-    const int most = (vocab + 4095) / 4096, want = (4 * 148 + units - 1) / units;
-    return want < 1 ? 1 : want > most ? (most < kVerMaxSplits ? most : kVerMaxSplits) : want < kVerMaxSplits ? want : kVerMaxSplits;
+  // as many slices of a row as give every SM eight CTAs, each a turn of its threads at least
+  auto pick = [&](int units, int least) {
+    const int most = (vocab + least - 1) / least, want = (8 * 148 + units - 1) / units;
+    return std::max(1, std::min(std::min(want, most), kVerMaxSplits));
   };
-  p.splits = pick(rows);
-  p.emit_splits = pick(requests);
+  p.splits = pick(rows, 8 * kVerTurn * kVerThreads);
+  p.emit_splits = pick(requests, 8 * kVerThreads);
   const size_t counts = ((size_t)requests * 4 + 255) & ~(size_t)255;
   p.stats = counts;
   p.best = p.stats + (size_t)rows * 2 * p.splits * 16;
@@ -245,7 +365,7 @@ int pie_verify_draft(int32_t* tokens, int32_t* counts, float* logprobs, const vo
   if (temp > 0.f ? !uniforms || !noise : draft_logits != nullptr) return temp > 0.f ? PIE_ENULL : PIE_EINVAL_SHAPE;
   const VerPlan p = ver_plan(requests, rows, vocab);
   if (!workspace || workspace_bytes < p.bytes) return PIE_EWORKSPACE;
-  if (reinterpret_cast<uintptr_t>(workspace) & 15) return PIE_EALIGN;
+  if ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(draft_logits)) & 15) return PIE_EALIGN;
   VerArgs a;
   a.tokens = tokens; a.counts = counts; a.logprobs = logprobs;
   a.logits = (const uint16_t*)logits; a.guess = (const uint16_t*)draft_logits; a.ld = ld;

@@ -769,9 +769,13 @@ def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: fl
         uniforms = noise = None
     given = [t for t in (logits, draft_tokens, logit_starts, uniforms, noise, draft_logits) if t is not None]
     with _one_device(what, *given):
-        logits = logits if logits.stride(1) == 1 and logits.stride(0) >= vocab else logits.contiguous()
-        if draft_logits is not None and draft_logits.stride() != logits.stride():
-            logits, draft_logits = logits.contiguous(), draft_logits.contiguous()
+        def aligned(t):
+            t = t.contiguous()
+            return t if t.data_ptr() % 16 == 0 else t.clone()
+        if logits.stride(1) != 1 or logits.stride(0) < vocab or logits.data_ptr() % 16:
+            logits = aligned(logits)
+        if draft_logits is not None and (draft_logits.stride() != logits.stride() or draft_logits.data_ptr() % 16):
+            logits, draft_logits = aligned(logits), aligned(draft_logits)
         dev = logits.device
         tokens = torch.empty((S, max_draft + 1), dtype=torch.int32, device=dev)
         counts = torch.empty((S,), dtype=torch.int32, device=dev)
