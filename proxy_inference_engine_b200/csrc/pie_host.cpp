@@ -1,5 +1,6 @@
 // The host side of calls of few rows, natively: nn.fused_rows (a norm, matrices of one input, and what follows them), the two launches of a
-// feed-forward, and a decode step's attention (rotation and cache write, attention).  Each looks the layers and the activations over and makes the
+// feed-forward, a decode step's attention (rotation and cache write, attention), and the operators of a ragged step (its plan, rotation and cache write,
+// attention, verification of drafts).  Each looks the layers and the activations over and makes the
 // launches.  From Python a launch spends 13 of its 19 us on attributes, checks, argument tables and conversions, and a decode layer makes
 // eight.  Launches are programmatic dependents of whatever is before them on the stream and only ask L2 for weights ahead of their wait; the
 // second of a native call reads them ahead of it: the first does not write them, and starts its dependents behind its own wait for all before it.  One row of a 1B feed-forward, whose kernels take 9 us: 39 us
@@ -23,7 +24,9 @@ namespace {
 
 #define PIE_FUNCTIONS(X)                                                                                                                \
   X(pie_qmv_fused) X(pie_qmv_workspace_bytes) X(pie_qmt) X(pie_qmt_scratch_bytes) X(pie_rope_kv_rows) X(pie_rope_kvq_rows)                \
-  X(pie_decode_attn) X(pie_decode_attn_pick_splits_for) X(pie_decode_attn_q8) X(pie_decode_attn_q8_pick_splits) X(pie_decode_attn_workspace_bytes)
+  X(pie_decode_attn) X(pie_decode_attn_pick_splits_for) X(pie_decode_attn_q8) X(pie_decode_attn_q8_pick_splits) X(pie_decode_attn_workspace_bytes) \
+  X(pie_step_plan_words) X(pie_step_plan_offsets) X(pie_step_plan_build) X(pie_rope_kv_slots) X(pie_chunk_attn) X(pie_chunk_attn_workspace_bytes)     \
+  X(pie_verify_draft) X(pie_verify_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
   PIE_FUNCTIONS(X)
@@ -316,6 +319,225 @@ PyObject* attend_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------------- a ragged step
+// Tensors of one call: plain ones, all on the current device (which is not asked for where there may be none)
+bool on_gpu(PyObject* v) {
+  const at::Tensor* t = tensor_of(v);
+  return t && t->is_cuda();
+}
+bool here(const at::Tensor* t, int device) { return t && plain(*t) && t->get_device() == device; }
+bool ints(const at::Tensor* t, int device, int64_t n) {
+  return here(t, device) && t->scalar_type() == at::kInt && t->dim() == 1 && t->is_contiguous() && (n < 0 || t->size(0) == n) && t->size(0) <= INT32_MAX;
+}
+// rows [rows, heads, D] that a kernel reads 16 bytes at a time
+bool head_rows(const at::Tensor* t, int device, pie_head_rows& r) {
+  if (!here(t, device) || t->scalar_type() != at::kBFloat16 || t->dim() != 3 || t->stride(2) != 1 || t->size(0) < 1 || t->size(0) > INT32_MAX || t->size(1) < 1 ||
+      t->size(1) > 65535)
+    return false;
+  for (int i = 0; i < 2; ++i)
+    if (t->stride(i) % 8 || t->stride(i) < 0 || (t->stride(i) == 0 && t->size(i) > 1)) return false;
+  r = {t->const_data_ptr(), 0, t->stride(1), t->stride(0)};
+  return aligned(r.p, 16);
+}
+bool slot_pools(const at::Tensor* k, const at::Tensor* v, int device, pie_kv_layout& lay) {
+  if (!here(k, device) || !here(v, device) || k->scalar_type() != at::kBFloat16 || v->scalar_type() != at::kBFloat16 || k->dim() != 4 || k->sizes() != v->sizes() ||
+      k->strides() != v->strides() || k->size(1) != 64 || k->size(0) < 1 || k->size(0) > INT32_MAX / 64 || k->size(2) < 1 || k->size(2) > 65535 || k->stride(3) != 1 ||
+      k->stride(0) != 64 * k->stride(1) || k->stride(1) <= 0 || k->stride(2) <= 0 || (k->stride(1) | k->stride(2)) % 8)
+    return false;
+  lay = {0, k->stride(2), k->stride(1), nullptr, 0, 64};
+  return aligned(k->const_data_ptr(), 16) && aligned(v->const_data_ptr(), 16);
+}
+// where the result goes: a fresh tensor, or the one that is given
+bool result(PyObject* given, at::IntArrayRef shape, const at::Tensor& like, int device, at::Tensor& out, bool& fresh) {
+  fresh = given == Py_None;
+  if (fresh) {
+    out = at::empty(shape, like.options());
+    return plain(out);
+  }
+  const at::Tensor* t = tensor_of(given);
+  if (!here(t, device) || t->scalar_type() != at::kBFloat16 || t->sizes() != shape || !t->is_contiguous() || !aligned(t->const_data_ptr(), 16)) return false;
+  out = *t;
+  return true;
+}
+
+// step_plan(token_ids, input_lengths, context_lengths, pages, draft_lengths or None, dims) -> (words, its ten parts), or None
+PyObject* step_plan(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !bound || !on_gpu(args[0])) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const at::Tensor *ids = tensor_of(args[0]), *input = tensor_of(args[1]), *context = tensor_of(args[2]), *pages = tensor_of(args[3]),
+                   *draft = args[4] == Py_None ? nullptr : tensor_of(args[4]);
+  Py_buffer view;
+  pie_step_dims d;
+  if (PyObject_GetBuffer(args[5], &view, PyBUF_SIMPLE) < 0) { PyErr_Clear(); Py_RETURN_NONE; }
+  const bool whole = view.len == sizeof(d);
+  if (whole) memcpy(&d, view.buf, sizeof(d));
+  PyBuffer_Release(&view);
+  if (!whole || !ints(ids, device, d.rows) || !ints(input, device, d.requests) || !ints(context, device, d.requests) ||
+      (args[4] != Py_None && !ints(draft, device, d.requests)))
+    Py_RETURN_NONE;
+  if (!here(pages, device) || pages->scalar_type() != at::kInt || pages->dim() < 1 || pages->dim() > 2 || pages->stride(-1) != 1 ||
+      (pages->dim() == 2 && (pages->size(0) != d.requests || pages->stride(0) < 1)))
+    Py_RETURN_NONE;
+  const size_t size = lib.pie_step_plan_words(&d);
+  long long at[10];
+  if (!size || lib.pie_step_plan_offsets(&d, at) != PIE_OK) Py_RETURN_NONE;
+  const at::Tensor words = at::empty({(int64_t)size}, ids->options());
+  if (!plain(words)) Py_RETURN_NONE;
+  void* const stream = c10::cuda::getCurrentCUDAStream().stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = lib.pie_step_plan_build((int32_t*)words.data_ptr(), &d, (const int32_t*)ids->const_data_ptr(), (const int32_t*)input->const_data_ptr(),
+                                   (const int32_t*)context->const_data_ptr(), draft ? (const int32_t*)draft->const_data_ptr() : nullptr,
+                                   (const int32_t*)pages->const_data_ptr(), pages->size(-1), pages->dim() == 1 ? 0 : pages->stride(0), stream);
+  Py_END_ALLOW_THREADS
+  if (status != PIE_OK) Py_RETURN_NONE;
+  const int64_t S = d.requests, T = d.rows, R = d.logit_rows, sizes[10] = {S + 1, S, T, T, T, S, S + 1, R, R, PIE_STEP_STATUS_WORDS};
+  THPObjectPtr all(PyTuple_New(11));
+  if (!all) return nullptr;
+  for (int i = 0; i < 10; ++i) {
+    at::Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(words.storage()), words.key_set(), words.dtype());
+    c10::TensorImpl* const impl = part.unsafeGetTensorImpl();
+    impl->set_storage_offset(at[i]);
+    const int64_t shape[2] = {sizes[i], d.blocks}, strides[2] = {i == 5 ? d.blocks : 1, 1};
+    impl->set_sizes_and_strides(at::IntArrayRef(shape, i == 5 ? 2 : 1), at::IntArrayRef(strides, i == 5 ? 2 : 1));
+    PyObject* const v = THPVariable_Wrap(std::move(part));
+    if (!v) return nullptr;
+    PyTuple_SET_ITEM(all.get(), i + 1, v);
+  }
+  PyObject* const w = THPVariable_Wrap(words);
+  if (!w) return nullptr;
+  PyTuple_SET_ITEM(all.get(), 0, w);
+  return all.release();
+  END_HANDLE_TH_ERRORS
+}
+
+// rope_kv_slots(queries, keys, values, freqs, positions, slots, k_pool, v_pool, out or None) -> rotated queries, or None
+PyObject* rope_kv_slots(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !bound || !on_gpu(args[0])) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const at::Tensor* t[8];
+  for (int i = 0; i < 8; ++i) t[i] = tensor_of(args[i]);
+  pie_head_rows rows[3];
+  pie_kv_layout lay;
+  for (int i = 0; i < 3; ++i)
+    if (!head_rows(t[i], device, rows[i])) Py_RETURN_NONE;
+  const int64_t T = t[0]->size(0), Hq = t[0]->size(1), D = t[0]->size(2), Hkv = t[1]->size(1);
+  if ((D != 64 && D != 128) || t[1]->size(0) != T || t[1]->size(2) != D || t[1]->sizes() != t[2]->sizes() || !here(t[3], device) || t[3]->scalar_type() != at::kFloat ||
+      t[3]->dim() != 1 || t[3]->size(0) != D / 2 || !t[3]->is_contiguous() || !ints(t[4], device, T) || !ints(t[5], device, T) ||
+      !slot_pools(t[6], t[7], device, lay) || t[6]->size(2) != Hkv || t[6]->size(3) != D)
+    Py_RETURN_NONE;
+  at::Tensor out;
+  bool fresh;
+  if (!result(args[8], {T, Hq, D}, *t[0], device, out, fresh)) Py_RETURN_NONE;
+  void* const stream = c10::cuda::getCurrentCUDAStream().stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = lib.pie_rope_kv_slots(out.data_ptr(), t[6]->data_ptr(), t[7]->data_ptr(), &lay, &rows[0], &rows[1], &rows[2], (const int32_t*)t[4]->const_data_ptr(),
+                                 (const int32_t*)t[5]->const_data_ptr(), (const float*)t[3]->const_data_ptr(), (int)T, (int)t[6]->size(0), (int)Hq, (int)Hkv, (int)D,
+                                 fresh, stream);
+  Py_END_ALLOW_THREADS
+  if (status != PIE_OK) Py_RETURN_NONE;
+  if (!fresh) return Py_NewRef(args[8]);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// chunk_attention(q, k_pool, v_pool, plan's words, plan's dims, scale, out or None, workspace) -> [T, Hq D], or None.  workspace(key, bytes, device)
+PyObject* chunk_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || !bound || !on_gpu(args[0]) || !PyFloat_CheckExact(args[5])) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const at::Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *v = tensor_of(args[2]), *words = tensor_of(args[3]);
+  pie_head_rows rows;
+  pie_kv_layout lay;
+  pie_step_dims d;
+  Py_buffer view;
+  if (PyObject_GetBuffer(args[4], &view, PyBUF_SIMPLE) < 0) { PyErr_Clear(); Py_RETURN_NONE; }
+  const bool whole = view.len == sizeof(d);
+  if (whole) memcpy(&d, view.buf, sizeof(d));
+  PyBuffer_Release(&view);
+  if (!whole || !head_rows(q, device, rows) || !slot_pools(k, v, device, lay) || !ints(words, device, -1) || q->size(0) != d.rows || q->size(1) != d.Hq ||
+      k->size(0) != d.pages || k->size(2) != d.Hkv || q->size(2) != k->size(3) || (size_t)words->size(0) != lib.pie_step_plan_words(&d))
+    Py_RETURN_NONE;
+  const int64_t T = q->size(0), D = q->size(2);
+  const size_t need = lib.pie_chunk_attn_workspace_bytes(&d, (int)D);
+  if (!need) Py_RETURN_NONE;
+  THPObjectPtr dev(PyObject_GetAttr(args[0], s_device));
+  if (!dev) return nullptr;
+  at::Tensor ws, out;
+  if (const Answer a = buffer(Py_BuildValue("(snO)", "chunk", (Py_ssize_t)need, dev.get()), args[7], ws)) {
+    if (a == FAILED) return nullptr;
+    Py_RETURN_NONE;
+  }
+  bool fresh;
+  if (!result(args[6], {T, (int64_t)d.Hq * D}, *q, device, out, fresh)) Py_RETURN_NONE;
+  const float scale = (float)PyFloat_AS_DOUBLE(args[5]);
+  void* const stream = c10::cuda::getCurrentCUDAStream().stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = lib.pie_chunk_attn(out.data_ptr(), &rows, k->const_data_ptr(), v->const_data_ptr(), &lay, (const int32_t*)words->const_data_ptr(), &d, (int)D, scale, fresh,
+                              ws.data_ptr(), (size_t)ws.numel(), stream);
+  Py_END_ALLOW_THREADS
+  if (status != PIE_OK) Py_RETURN_NONE;
+  if (!fresh) return Py_NewRef(args[6]);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// verify_draft(logits, draft_tokens, logit_starts, max_draft, temp, uniforms, noise, draft_logits (or None each), workspace) -> (tokens, counts, logprobs), or None
+PyObject* verify_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  long most;
+  if (n != 9 || !bound || !on_gpu(args[0]) || !int_of(args[3], most) || most < 0 || most > 127 || !PyFloat_CheckExact(args[4])) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const double temp = PyFloat_AS_DOUBLE(args[4]);
+  const at::Tensor *x = tensor_of(args[0]), *draft = tensor_of(args[1]), *starts = tensor_of(args[2]), *u = nullptr, *noise = nullptr, *g = nullptr;
+  auto logits = [&](const at::Tensor* t) {
+    return here(t, device) && t->scalar_type() == at::kBFloat16 && t->dim() == 2 && t->stride(1) == 1 && t->size(1) >= 1 && t->size(1) <= INT32_MAX &&
+           t->stride(0) >= t->size(1) && aligned(t->const_data_ptr(), 16);
+  };
+  if (!logits(x) || x->size(0) < 1 || x->size(0) > 65535 || !ints(draft, device, x->size(0)) || !ints(starts, device, -1) || starts->size(0) < 2 ||
+      starts->size(0) > 65536)
+    Py_RETURN_NONE;
+  const int64_t R = x->size(0), V = x->size(1), S = starts->size(0) - 1;
+  if (temp > 0) {
+    u = tensor_of(args[5]);
+    noise = tensor_of(args[6]);
+    if (!here(u, device) || !here(noise, device) || u->scalar_type() != at::kFloat || noise->scalar_type() != at::kFloat || u->dim() != 1 || u->size(0) != R ||
+        noise->dim() != 2 || noise->size(0) != S || noise->size(1) != V || !u->is_contiguous() || !noise->is_contiguous())
+      Py_RETURN_NONE;
+  }
+  if (args[7] != Py_None) {
+    g = tensor_of(args[7]);
+    if (!logits(g) || g->sizes() != x->sizes() || g->strides() != x->strides()) Py_RETURN_NONE;
+  }
+  THPObjectPtr dev(PyObject_GetAttr(args[0], s_device));
+  if (!dev) return nullptr;
+  at::Tensor ws;
+  const size_t need = lib.pie_verify_workspace_bytes((int)S, (int)R, (int)V);
+  if (const Answer a = buffer(Py_BuildValue("((sn)nO)", "verify", (Py_ssize_t)((S * 4 + 255) / 256), (Py_ssize_t)need, dev.get()), args[8], ws)) {
+    if (a == FAILED) return nullptr;
+    Py_RETURN_NONE;
+  }
+  at::Tensor tokens = at::empty({S, most + 1}, draft->options()), counts = at::empty({S}, draft->options()),
+             logprobs = at::empty({S, most + 1}, x->options().dtype(at::kFloat));
+  if (!plain(tokens)) Py_RETURN_NONE;
+  void* const stream = c10::cuda::getCurrentCUDAStream().stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = lib.pie_verify_draft((int32_t*)tokens.data_ptr(), (int32_t*)counts.data_ptr(), (float*)logprobs.data_ptr(), x->const_data_ptr(), g ? g->const_data_ptr() : nullptr,
+                                x->stride(0), (const int32_t*)draft->const_data_ptr(), (const int32_t*)starts->const_data_ptr(), (int)S, (int)R, (int)V, (int)most,
+                                (float)temp, u ? (const float*)u->const_data_ptr() : nullptr, noise ? (const float*)noise->const_data_ptr() : nullptr, ws.data_ptr(),
+                                (size_t)ws.numel(), stream);
+  Py_END_ALLOW_THREADS
+  if (status != PIE_OK) Py_RETURN_NONE;
+  THPObjectPtr a(THPVariable_Wrap(std::move(tokens))), b(THPVariable_Wrap(std::move(counts))), c(THPVariable_Wrap(std::move(logprobs)));
+  return a && b && c ? PyTuple_Pack(3, a.get(), b.get(), c.get()) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address in the loaded library})
 PyObject* bind(PyObject*, PyObject* args) {
   PyObject* table;
@@ -336,6 +558,10 @@ PyObject* bind(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {{"fused_rows", (PyCFunction)(void (*)(void))fused_rows, METH_FASTCALL, "nn.fused_rows, or None"},
                          {"mlp_rows", (PyCFunction)(void (*)(void))mlp_rows, METH_FASTCALL, "a feed-forward of few rows, or None"},
                          {"attend_rows", (PyCFunction)(void (*)(void))attend_rows, METH_FASTCALL, "a decode step's attention, or None"},
+                         {"step_plan", (PyCFunction)(void (*)(void))step_plan, METH_FASTCALL, "a ragged step's plan, or None"},
+                         {"rope_kv_slots", (PyCFunction)(void (*)(void))rope_kv_slots, METH_FASTCALL, "ops.rope_kv_slots, or None"},
+                         {"chunk_attention", (PyCFunction)(void (*)(void))chunk_attention, METH_FASTCALL, "ops.chunk_attention, or None"},
+                         {"verify_draft", (PyCFunction)(void (*)(void))verify_draft, METH_FASTCALL, "ops.verify_draft, or None"},
                          {"bind", bind, METH_VARARGS, "addresses of the library's functions"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pie_host", nullptr, -1, methods};

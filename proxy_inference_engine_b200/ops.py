@@ -263,7 +263,7 @@ def attention_workspace(units: int, nbytes: int, device) -> torch.Tensor:
 
 class _NoHost:
     """Where csrc/pie_host.cpp's module was not built, or for another torch or interpreter: None to every call."""
-    mlp_rows = attend_rows = staticmethod(lambda *args: None)
+    mlp_rows = attend_rows = step_plan = rope_kv_slots = chunk_attention = verify_draft = staticmethod(lambda *args: None)
 
 
 @functools.cache
@@ -279,7 +279,7 @@ def native_fused_rows():
         host = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(host)
         host.bind({name: C.cast(getattr(L, name), C.c_void_p).value for name in host.functions})
-        host.fused_rows, host.mlp_rows, host.attend_rows
+        host.fused_rows, host.mlp_rows, host.attend_rows, host.step_plan, host.rope_kv_slots, host.chunk_attention, host.verify_draft
     except (ImportError, OSError, AttributeError, KeyError, TypeError) as e:   # (one of an earlier build has other functions, or another bind)
         warnings.warn(f"{path} does not load ({e}): build it again with make -C {_lib.CSRC}.  Calls of few rows take the Python form meanwhile.")
         return lambda *args: None
@@ -287,7 +287,7 @@ def native_fused_rows():
 
 
 def native_host():
-    """The module native_fused_rows() is of: several launches of few rows (mlp_rows, attend_rows), with the same None."""
+    """The module native_fused_rows() is of: several launches of few rows (mlp_rows, attend_rows) and the operators of a ragged step, with the same None."""
     return getattr(native_fused_rows(), "__self__", _NoHost)
 
 
@@ -636,7 +636,7 @@ def _one_device(what: str, *tensors):
 
 def _head_rows(x) -> tuple:
     """Rows [rows, heads, D] as a kernel reads them, 16 bytes at a time: (tensor to be held until the launch is queued, HeadRows)."""
-    if x.stride(2) != 1 or (x.stride(0) | x.stride(1)) % 8 or x.stride(0) < 0 or x.stride(1) < 0 or x.data_ptr() % 16:
+    if x.stride(2) != 1 or (x.stride(0) | x.stride(1)) % 8 or any(st < 0 or (st == 0 and n > 1) for st, n in zip(x.stride(), x.shape)) or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
@@ -648,7 +648,7 @@ def _slot_pools(what: str, k_pool, v_pool) -> KvLayout:
     for t in (k_pool, v_pool):
         if t.dim() != 4 or t.shape[1] != 64 or t.dtype != _BF16:
             raise ValueError(f"[{what}] pools must be bfloat16 [pages, 64, n_kv, D], but one is {t.dtype} {tuple(t.shape)}")
-        if t.stride(3) != 1 or t.stride(0) != 64 * t.stride(1) or (t.stride(1) | t.stride(2)) % 8 or t.stride(1) <= 0 or t.stride(2) < 0 or t.data_ptr() % 16:
+        if t.stride(3) != 1 or t.stride(0) != 64 * t.stride(1) or (t.stride(1) | t.stride(2)) % 8 or t.stride(1) <= 0 or t.stride(2) <= 0 or t.data_ptr() % 16:
             raise ValueError(f"[{what}] pools must lie page behind page with 16-byte aligned heads, but one has strides {tuple(t.stride())}")
     if k_pool.shape != v_pool.shape or k_pool.stride() != v_pool.stride():
         raise ValueError(f"[{what}] keys' and values' pools must share one layout")
@@ -680,6 +680,9 @@ def rope_kv_slots(queries, keys, values, freqs, positions, slots, k_pool, v_pool
     freqs, bit for bit), keys and values [T, Hkv, D] written to the rows' slots of pools [pages, 64, Hkv, D] (slot = page * 64 + place in it).  Rows may lie
     anywhere, as a projection wrote them.  positions, slots: int32 [T].  Returns the rotated queries, [T, Hq, D] contiguous.  A row whose slot is outside
     the pools (-1: it belongs to nobody) writes nothing to them; its queries are zero, or with ``out`` given what that held.  No two rows may share a slot."""
+    got = native_host().rope_kv_slots(queries, keys, values, freqs, positions, slots, k_pool, v_pool, out)
+    if got is not None:
+        return got
     what = "rope_kv_slots"
     if queries.dim() != 3 or keys.dim() != 3 or values.shape != keys.shape or keys.shape[0] != queries.shape[0] or keys.shape[2] != queries.shape[2]:
         raise ValueError(f"[{what}] queries [T, Hq, D], keys and values [T, Hkv, D] expected, but they are {tuple(queries.shape)}, {tuple(keys.shape)} and "
@@ -710,6 +713,9 @@ def chunk_attention(q, k_pool, v_pool, plan, scale: float, out=None):
     """Causal attention of a ragged step: row t of q [T, Hq, D] (rows may lie anywhere) attends to the keys 0 .. position of its own request, which the pools
     [pages, 64, Hkv, D] hold already (rope_kv_slots).  plan: the step's ragged.StepPlan, built for these numbers of heads and pages.  Returns [T, Hq * D].
     Rows that belong to nobody are zero, or with ``out`` given what that held."""
+    got = native_host().chunk_attention(q, k_pool, v_pool, plan.words, plan.dims, float(scale), out, workspaces.get)
+    if got is not None:
+        return got
     what = "chunk_attention"
     if q.dim() != 3 or q.dtype != _BF16:
         raise ValueError(f"[{what}] queries must be bfloat16 [T, Hq, D], but are {q.dtype} {tuple(q.shape)}")
@@ -745,6 +751,9 @@ def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: fl
 
     Returns (tokens int32 [requests, max_draft + 1], padded by -1; counts int32 [requests], 1 + accepted (0: a request without rows); log-probabilities f32
     [requests, max_draft + 1] of the tokens under p, padded by 0).  max_draft: at most 127; further drafts of a request are not looked at."""
+    got = native_host().verify_draft(logits, draft_tokens, logit_starts, max_draft, float(temp), uniforms, noise, draft_logits, workspaces.get)
+    if got is not None:
+        return got
     what = "verify_draft"
     for name, t in (("logits", logits), ("draft_logits", draft_logits)):
         if t is not None and (t.dim() != 2 or t.dtype != _BF16 or t.shape != logits.shape or t.numel() == 0):

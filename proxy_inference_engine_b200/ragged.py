@@ -185,9 +185,13 @@ class StepPlan:
         each request one behind the other, or a table [S, columns] of them.  num_pages: of the pools.  max_blocks: columns of the plan's own block table.
         draft_lengths int32 [S]: how many of a request's new tokens are drafted ones (fewer than its new ones).  num_logits: logit rows to make room for (default: S, none drafted).
         Lengths that do not fit one another cannot be seen from here: check() tells, and until then nothing is read or written out of bounds."""
+        S = input_lengths.numel()
+        dims = _lib.StepDims(S, token_ids.numel(), S if num_logits is None else int(num_logits), int(max_blocks), int(num_pages), int(num_heads), int(num_kv_heads))
+        got = ops.native_host().step_plan(token_ids, input_lengths, context_lengths, pages, draft_lengths, dims)
+        if got is not None:
+            return cls(token_ids, got[0], dims, *got[1:])
         what = "StepPlan"
         ops._step_ints(what, "token_ids", token_ids)
-        S = input_lengths.numel()
         ops._step_ints(what, "input_lengths", input_lengths, (S,))
         ops._step_ints(what, "context_lengths", context_lengths, (S,))
         if draft_lengths is not None:
@@ -196,7 +200,6 @@ class StepPlan:
             raise ValueError(f"[{what}] pages must be int32, a list or a table of {S} rows, but is {pages.dtype} {list(pages.shape)}")
         if pages.stride(-1) != 1 or (pages.dim() == 2 and pages.stride(0) < 1):
             pages = pages.contiguous()
-        dims = _lib.StepDims(S, token_ids.numel(), S if num_logits is None else int(num_logits), int(max_blocks), int(num_pages), int(num_heads), int(num_kv_heads))
         L = _lib.load()
         n = L.pie_step_plan_words(C.byref(dims))
         if token_ids.dim() != 1 or n == 0:
@@ -205,7 +208,7 @@ class StepPlan:
         given = [t for t in (token_ids, input_lengths, context_lengths, pages, draft_lengths) if t is not None]
         with ops._one_device(what, *given):
             words = torch.empty(n, dtype=torch.int32, device=token_ids.device)
-            stride = 0 if pages.dim() == 1 else pages.stride(0)
+            stride = 0 if pages.dim() == 1 else max(1, pages.stride(0))
             _lib.check(L.pie_step_plan_build(_p(words), C.byref(dims), _p(token_ids), _p(input_lengths), _p(context_lengths), _p(draft_lengths), _p(pages),
                                              pages.shape[-1], stride, _stream()), what)
         at = (C.c_longlong * 10)()

@@ -447,6 +447,46 @@ def test_a_captured_step_runs_again_on_other_lengths():
             assert torch.equal(a, b)
 
 
+def test_the_native_host_form_is_the_python_one(monkeypatch):
+    """The same bits, for tensors that the native form takes and for those it leaves: views, other strides, odd addresses."""
+    from proxy_inference_engine_b200 import ops
+    from proxy_inference_engine_b200.ragged import StepPlan
+    assert ops.native_host() is not ops._NoHost
+    g, Hq, Hkv, D, V = gen(2), 8, 2, 64, 1000
+    lens = [ints([3, 0, 70]), ints([60, 5, 0]), ints([2, 0, 0])]
+    ids, pages, wide = ints(list(range(73))), ints([4, 2, 3, 0, 1]), ints([[4, 2, 9, 9], [3, 9, 9, 9], [0, 1, 9, 9]])
+    pool = lambda: (randn(gen(3), 6, 64, Hkv, D), randn(gen(4), 6, 64, Hkv, D))
+    rows = randn(g, 73, Hq + 2 * Hkv, D)
+    odd = torch.empty(73 * Hq * D + 1, dtype=BF, device="cuda")[1:].view(73, Hq, D)
+    odd.copy_(rows[:, :Hq])
+    logits, u, noise = randn(g, 6, V + 8), torch.rand(6, generator=g, device="cuda"), torch.rand((2, V), generator=g, device="cuda")
+    guess, drafts, starts = randn(g, 6, V + 8), ints([5, 6, 7, 8, 9, 10]), ints([0, 2, 6])
+    plain_q = rows[:, :Hq].contiguous()
+
+    def everything():
+        got = []
+        for table in (pages, wide, wide[:, :2], wide.t().contiguous().t()):
+            plan = StepPlan.build(ids, *lens[:2], table, num_pages=10, max_blocks=3, num_heads=Hq, num_kv_heads=Hkv, draft_lengths=lens[2], num_logits=5)
+            got += [getattr(plan, n) for n in ("row_starts", "contexts", "sequences", "positions", "slots", "block_table", "logit_starts", "logit_rows", "draft_tokens")]
+            plan = StepPlan.build(ids, *lens[:2], table, num_pages=6, max_blocks=3, num_heads=Hq, num_kv_heads=Hkv)
+            for q in (plain_q, rows[:, :Hq], odd, rows[:, :1].expand(73, Hq, D)):
+                k_pool, v_pool = pool()
+                turned = ops.rope_kv_slots(q, rows[:, Hq:Hq + Hkv], rows[:, Hq + Hkv:], FREQS(D), plan.positions, plan.slots, k_pool, v_pool)
+                got += [turned, k_pool, v_pool, ops.chunk_attention(q, k_pool, v_pool, plan, 0.2), ops.chunk_attention(q, k_pool, v_pool, plan, 0.2, out=torch.ones_like(turned).view(73, -1))]
+        for x, q in ((logits[:, :V], guess[:, :V]), (logits[:, :V].contiguous(), guess[:, :V].contiguous()), (logits[:, :V].contiguous(), guess[:, :V]), (logits[:, 3:V + 3], None),
+                     (logits[:, :V], None)):
+            got += ops.verify_draft(x, drafts, starts, max_draft=3, temp=0.7, uniforms=u, noise=noise, draft_logits=q)
+            got += ops.verify_draft(x, drafts, starts, max_draft=1)
+        return got
+
+    native = everything()
+    monkeypatch.setattr(ops, "native_host", lambda: ops._NoHost)
+    python = everything()
+    assert len(native) == len(python)
+    for i, (a, b) in enumerate(zip(native, python)):
+        assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride() and torch.equal(a.view(torch.int16) if a.dtype == BF else a, b.view(torch.int16) if b.dtype == BF else b), i
+
+
 def test_a_planned_step_refuses():
     from proxy_inference_engine_b200.ragged import StepPlan, ragged_step
     args, w, model, mk = _model(64)
