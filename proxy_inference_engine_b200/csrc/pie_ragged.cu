@@ -35,6 +35,7 @@ constexpr int kPlanThreads = 512;
 constexpr int kCostPair = 2, kCostTile = 1;   // a key of an item with rows in both query tiles, in one
 constexpr int kCostItem = 256;                // queries in, results out
 constexpr long long kCostShare = 512;         // least share worth a CTA
+constexpr int kCutPair = 4, kCutTile = 2;     // least key tiles of a piece: what it costs to leave a piece's results and to add them up
 
 __device__ __forceinline__ long long warp_scan(long long v, int lane) {
 #pragma unroll
@@ -221,11 +222,13 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     const int n = row[s + 1] - row[s], tokens = min(span, n - q * span), keys = ctx[s] + q * span + tokens;
     const int weight = tokens > a.l.tile_tokens ? kCostPair : kCostTile, tiles = (keys + kStepTile - 1) / kStepTile;
     const long long x = head * W1 + cost[s] + cost_before(q, ctx[s], span), end = x + (long long)weight * keys + kCostItem;
-    auto tile = [&](int c) {   // first key tile of CTA c's share
+    const int least = weight == kCostPair ? kCutPair : kCutTile;
+    auto tile = [&](int c) {   // first key tile of CTA c's share.  A cut that would leave little on one side of it is not made.
       const long long past = c * share - x;
       if (past <= 0) return 0;
       const long long per = (long long)weight * kStepTile, k = (past + per - 1) / per;
-      return k < tiles ? (int)k : tiles;
+      if (k < least) return 2 * k <= tiles || tiles >= 2 * least ? 0 : tiles;
+      return tiles - k < least ? tiles : (int)k;
     };
     const int c0 = (int)(x / share), c1 = (int)((end - 1) / share);
     int mine = 0, opens = c0;

@@ -66,9 +66,10 @@ __device__ __forceinline__ VerRow ver_row(const uint16_t* x, int vocab) {
   r.tail = r.head + 8 * r.vectors;
   return r;
 }
-// vectors [lo, hi) of slice i of n
+// vectors [lo, hi) of slice i of n, whole turns of the CTA
+constexpr int kVerTurn = 4;   // vectors a thread takes at a time
 __device__ __forceinline__ void ver_slice(int vectors, int i, int n, int& lo, int& hi) {
-  const int per = (vectors + n - 1) / n;
+  const int per = (vectors + n * kVerTurn * kVerThreads - 1) / (n * kVerTurn * kVerThreads) * (kVerTurn * kVerThreads);
   lo = min(i * per, vectors);
   hi = min(lo + per, vectors);
 }
@@ -84,6 +85,10 @@ __device__ __forceinline__ float ver_exp2(float x) {   // results below 2^-126 a
   return y;
 }
 
+__device__ __forceinline__ float ver_warp_max(float x) {   // of numbers, by integers in their order
+  const int i = __float_as_int(x), v = __reduce_max_sync(0xffffffffu, i ^ ((i >> 31) & 0x7fffffff));
+  return __int_as_float(v ^ ((v >> 31) & 0x7fffffff));
+}
 // A thread's part of a row: maximum x and sum of exp2(c x + off), off = -c maximum rounded -- one fused multiply-add an exponential, and what the rounding does to all
 // of them alike (2^-24 of c x, more than a sum may be off by) is taken back at the end.  32 logits a turn; their maximum is taken in pairs of bf16, and moves the sum
 // once a turn.  Greedy: where it moves is where the first largest lies so far.
@@ -105,90 +110,108 @@ struct VerSum {
   __device__ __forceinline__ float sum(float c) const { return m == -INFINITY ? s : s * ver_exp2(-fmaf(m, c, off)); }   // of exp2(c (x - m))
 };
 
-constexpr int kVerTurn = 4;   // vectors a thread has in flight
+// two fp32 operations an instruction
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 v2_pack(float a, float b) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void v2_unpack(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 v2_fma(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 v2_add(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 __global__ void __launch_bounds__(kVerThreads) verify_stats_kernel(const __grid_constant__ VerArgs a) {
   __shared__ float sm[kVerThreads / 32][2];
   __shared__ unsigned long long km[kVerThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
+  if (which) {   // a request's last row judges no token: its draft's logits are not read
+    bool last = false;
+    for (int i = tid; i < a.requests; i += kVerThreads) last = last || __ldg(a.starts + i + 1) == r + 1;
+    if (__syncthreads_or(last)) return;
+  }
   const VerRow row = ver_row((which ? a.guess : a.logits) + (size_t)r * a.ld, a.vocab);
   const float c = a.itemp * 1.4426950408889634f;
   VerSum sum;
   if (blockIdx.x == 0 && tid < row.head) sum.one(bf16lo((uint32_t)__ldg(row.x + tid)), tid, c);
   int lo, hi;
   ver_slice(row.vectors, blockIdx.x, a.splits, lo, hi);
-  for (int v0 = lo + tid; v0 < hi; v0 += kVerTurn * kVerThreads) {
-    uint4 x[kVerTurn];
+  uint4 x[kVerTurn];
+  auto load = [&](int v0) {
 #pragma unroll
     for (int t = 0; t < kVerTurn; ++t) {
       const int v = v0 + t * kVerThreads;
       x[t] = v < hi ? ver_load(row.x + row.head + 8 * (size_t)v) : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);   // -inf
     }
-    uint32_t m2 = x[0].x;
+  };
+  load(lo + tid);
+  for (int v0 = lo + tid; v0 < hi; v0 += kVerTurn * kVerThreads) {
+    uint32_t w[kVerTurn][4];
 #pragma unroll
-    for (int t = 0; t < kVerTurn; ++t) m2 = ver_max2(ver_max2(m2, ver_max2(x[t].x, x[t].y)), ver_max2(x[t].z, x[t].w));
+    for (int t = 0; t < kVerTurn; ++t) { w[t][0] = x[t].x; w[t][1] = x[t].y; w[t][2] = x[t].z; w[t][3] = x[t].w; }
+    load(v0 + kVerTurn * kVerThreads);
+    uint32_t m2 = w[0][0];
+#pragma unroll
+    for (int t = 0; t < kVerTurn; ++t) m2 = ver_max2(ver_max2(m2, ver_max2(w[t][0], w[t][1])), ver_max2(w[t][2], w[t][3]));
     const float mx = fmaxf(bf16lo(m2), bf16hi(m2)) + 0.f;
     if (mx > sum.m || (a.greedy && sum.index < 0)) {
       if (mx > sum.m) { sum.move(mx, c); sum.index = -1; }
       if (a.greedy) {   // the first of this turn that is the largest so far
 #pragma unroll
-        for (int t = 0; t < kVerTurn; ++t) {
-          const uint32_t w[4] = {x[t].x, x[t].y, x[t].z, x[t].w};
+        for (int t = 0; t < kVerTurn; ++t)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float f = (e & 1 ? bf16hi(w[e / 2]) : bf16lo(w[e / 2])) + 0.f;
+            const float f = (e & 1 ? bf16hi(w[t][e / 2]) : bf16lo(w[t][e / 2])) + 0.f;
             if (sum.index < 0 && f == sum.m && v0 + t * kVerThreads < hi) sum.index = row.head + 8 * (v0 + t * kVerThreads) + e;
           }
-        }
       }
     }
-    const float off = sum.off;
-    float s0 = 0.f, s1 = 0.f;
+    const f32x2 c2 = v2_pack(c, c), off2 = v2_pack(sum.off, sum.off);
+    f32x2 s01 = v2_pack(0.f, 0.f), s23 = s01;
 #pragma unroll
-    for (int t = 0; t < kVerTurn; ++t) {
-      const uint32_t w[4] = {x[t].x, x[t].y, x[t].z, x[t].w};
+    for (int t = 0; t < kVerTurn; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s0 += ver_exp2(fmaf(bf16lo(w[e]), c, off));
-        s1 += ver_exp2(fmaf(bf16hi(w[e]), c, off));
+        float y0, y1;
+        v2_unpack(v2_fma(v2_pack(bf16lo(w[t][e]), bf16hi(w[t][e])), c2, off2), y0, y1);
+        const f32x2 y = v2_pack(ver_exp2(y0), ver_exp2(y1));
+        if (e & 1) s23 = v2_add(s23, y);
+        else s01 = v2_add(s01, y);
       }
-    }
+    float s0, s1;
+    v2_unpack(v2_add(s01, s23), s0, s1);
     sum.s += s0 + s1;
   }
   if ((int)blockIdx.x == a.splits - 1 && tid < a.vocab - row.tail) sum.one(bf16lo((uint32_t)__ldg(row.x + row.tail + tid)), row.tail + tid, c);
-  float m = sum.m, s = sum.sum(c);
-  unsigned long long key = a.greedy && sum.index >= 0 ? ver_key(m, sum.index) : 0;
+  const unsigned long long mine = a.greedy && sum.index >= 0 ? ver_key(sum.m, sum.index) : 0;
+  const float m = ver_warp_max(sum.m), part = sum.sum(c);
+  float s = part == 0.f ? 0.f : part * exp2f((sum.m - m) * c);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    ver_join(m, s, m2, s2, c);
-  }
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((tid & 31) == 0) { sm[tid >> 5][0] = m; sm[tid >> 5][1] = s; }
-  if (a.greedy) key = ver_block_max(key, km); else __syncthreads();
+  unsigned long long key = 0;
+  if (a.greedy) key = ver_block_max(mine, km); else __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < kVerThreads / 32; ++w) ver_join(m, s, sm[w][0], sm[w][1], c);
+    float mb = m, sb = s;
+    for (int w = 1; w < kVerThreads / 32; ++w) ver_join(mb, sb, sm[w][0], sm[w][1], c);
     *reinterpret_cast<float4*>(a.stats + (((size_t)r * 2 + which) * a.splits + blockIdx.x) * 4) =
-        make_float4(m, s, __uint_as_float((uint32_t)(key >> 32)), __int_as_float(key ? ver_index(key) : 0));
+        make_float4(mb, sb, __uint_as_float((uint32_t)(key >> 32)), __int_as_float(key ? ver_index(key) : 0));
   }
 }
 
-// The race: of weights w and draws u, the largest w / -log(u), held as the pair (w, E = -log(u)) of the best so far, so that a comparison is two products.  As
-// 1 - u <= E, most lose without a logarithm.  (E is taken by logf: near u = 1, where the winners lie, it is good to its last place, and the approximation unit's is not.)
-struct VerRace {
-  float w = 0.f, e = 1.f;
-  int index = -1;
-  __device__ __forceinline__ void run(float wi, float u, int i) {
-    if (wi * e * 1.000001f > w * (1.f - u)) {   // (false for a NaN weight and for a weight of 0; at the start true for any other)
-      const float ei = fmaxf(-logf(fmaxf(u, 1.17549435e-38f)), 0.f);   // (a draw of 0 is the smallest there is: a token that is alone wins with it)
-      if (wi > 0.f && wi * e > w * ei) { w = wi; e = ei; index = i; }
-    }
-  }
-};
-
 __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_constant__ VerArgs a) {
   __shared__ float2 dist[2][kVerMaxDraft + 1];   // of p and q of each row: maximum, sum of exp2(c (x - maximum))
-  __shared__ int top[kVerMaxDraft + 1], ok[kVerMaxDraft + 1], s_accepted, s_last;
+  __shared__ int top[kVerMaxDraft + 1], ok[kVerMaxDraft + 1], s_accepted, s_last, s_best;
   __shared__ unsigned long long km[kVerThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
@@ -264,38 +287,75 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
     const float op = -dp.x * c, oq = -dq.x * c, kp = exp2f(-fmaf(dp.x, c, op)) / dp.y, kq = exp2f(-fmaf(dq.x, c, oq)) / dq.y;
     const VerRow row = ver_row(x, a.vocab);
     const bool flat = !(reinterpret_cast<uintptr_t>(u + row.head) & 15);   // the draws can be read 16 bytes at a time as well
-    // slice i of n; whole: of the target's own weights
+    // The race: of weights w and draws u, the largest w / E, E = -log(u), over turns i, i + n, ... of the row; whole: of the target's own weights.
+    // 1 - u <= E <= (1 - u) / u, so with b = w / (1 - u) a token's score lies between b u and b, which near u = 1, where the winners lie, is as good as equal: a thread keeps
+    // the b of its 32 tokens, the CTA the largest b u, and logarithms are taken of the one or two whose b is not below that.  (E by logf: near u = 1 it is good to its last
+    // place, and the approximation unit's is not.  A logarithm for each token, 64 requests: 36 us.)
     auto race = [&](int i, int n, bool whole) {
       const uint16_t* const q = whole ? nullptr : g;
       const int not_this = whole ? -1 : out;
-      VerRace best;
-      auto run = [&](float xi, float qi, float ui, int at) {
+      unsigned long long key = 0;
+      auto weight = [&](float xi, float qi) {
         float w = __fmul_rn(ver_exp2(fmaf(xi, c, op)), kp);
         if (q) w = __fsub_rn(w, __fmul_rn(ver_exp2(fmaf(qi, c, oq)), kq));   // (no fused form: p = q leaves nothing)
-        best.run(at == not_this ? 0.f : w, ui, at);
+        return w;
       };
-      auto single = [&](int at) { run(bf16lo((uint32_t)__ldg(x + at)), q ? bf16lo((uint32_t)__ldg(q + at)) : 0.f, __ldg(u + at), at); };
-      if (i == 0 && tid < row.head) single(tid);
-      int lo, hi;
-      ver_slice(row.vectors, i, n, lo, hi);
-#pragma unroll 2
-      for (int v = lo + tid; v < hi; v += kVerThreads) {
-        const int at = row.head + 8 * v;
-        const uint4 xv = ver_load(x + at), qv = q ? ver_load(q + at) : make_uint4(0, 0, 0, 0);
-        float ui[8];
-        if (flat) {
-          *reinterpret_cast<float4*>(ui) = __ldg(reinterpret_cast<const float4*>(u + at));
-          *reinterpret_cast<float4*>(ui + 4) = __ldg(reinterpret_cast<const float4*>(u + at + 4));
-        } else {
+      auto run = [&](int at) {   // exactly
+        const float w = at == not_this ? 0.f : weight(bf16lo((uint32_t)__ldg(x + at)), q ? bf16lo((uint32_t)__ldg(q + at)) : 0.f);
+        const float e = fmaxf(-logf(fmaxf(__ldg(u + at), 1.17549435e-38f)), 0.f);   // (a draw of 0 is the smallest there is: a token that is alone wins with it)
+        if (w > 0.f) key = ver_max(key, ver_key(w / e, at));
+      };
+      const int ends = row.head + a.vocab - row.tail;   // (at most 14)
+      if (i == 0 && tid < ends) run(tid < row.head ? tid : row.tail + tid - row.head);
+      for (int v0 = i * kVerTurn * kVerThreads; v0 < row.vectors; v0 += n * kVerTurn * kVerThreads) {
+        float bound[8 * kVerTurn], least = 0.f, most = 0.f;   // of a token without weight (or with a NaN): 0, as of one that is not there
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ui[e] = __ldg(u + at + e);
+        for (int t = 0; t < kVerTurn; ++t) {
+          const int v = v0 + t * kVerThreads + tid, at = row.head + 8 * v;
+          if (v >= row.vectors) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bound[8 * t + e] = 0.f;
+            continue;
+          }
+          const uint4 xv = ver_load(x + at), qv = q ? ver_load(q + at) : make_uint4(0, 0, 0, 0);
+          float ui[8];
+          if (flat) {
+            *reinterpret_cast<float4*>(ui) = __ldg(reinterpret_cast<const float4*>(u + at));
+            *reinterpret_cast<float4*>(ui + 4) = __ldg(reinterpret_cast<const float4*>(u + at + 4));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ui[e] = __ldg(u + at + e);
+          }
+          const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, qw[4] = {qv.x, qv.y, qv.z, qv.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float r;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f - ui[e]));   // (a draw of 1: infinite, and looked at)
+            float b = fmaxf(weight(e & 1 ? bf16hi(xw[e / 2]) : bf16lo(xw[e / 2]), e & 1 ? bf16hi(qw[e / 2]) : bf16lo(qw[e / 2])), 0.f) * r;
+            if (at + e == not_this) b = 0.f;
+            bound[8 * t + e] = b;
+            least = fmaxf(least, b * ui[e]);
+            most = fmaxf(most, b);
+          }
         }
-        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, qw[4] = {qv.x, qv.y, qv.z, qv.w};
+        if (tid == 0) s_best = 0;
+        __syncthreads();
+        const int mine = __reduce_max_sync(0xffffffffu, __float_as_int(least));   // (none is negative: in the order of their bits)
+        if (lane == 0) atomicMax(&s_best, mine);
+        __syncthreads();
+        const float bar = __int_as_float(s_best) * 0.99999f;
+        if (most >= bar && most > 0.f) {
+          unsigned left = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) run(e & 1 ? bf16hi(xw[e / 2]) : bf16lo(xw[e / 2]), e & 1 ? bf16hi(qw[e / 2]) : bf16lo(qw[e / 2]), ui[e], at + e);
+          for (int e = 0; e < 8 * kVerTurn; ++e) left |= (unsigned)(bound[e] >= bar && bound[e] > 0.f) << e;
+          for (; left; left &= left - 1) {
+            const int e = __ffs(left) - 1;
+            run(row.head + 8 * (v0 + (e / 8) * kVerThreads + tid) + e % 8);
+          }
+        }
+        __syncthreads();
       }
-      if (i == n - 1 && tid < a.vocab - row.tail) single(row.tail + tid);
-      return ver_block_max(best.index >= 0 ? ver_key(best.w / best.e, best.index) : 0, km);
+      return ver_block_max(key, km);
     };
     unsigned long long key = race(blockIdx.x, a.emit_splits, false);
     if (a.emit_splits > 1) {
@@ -331,13 +391,15 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
 struct VerPlan { int splits, emit_splits; size_t stats, best, bytes; };
 static VerPlan ver_plan(int requests, int rows, int vocab) {
   VerPlan p;
-  // as many slices of a row as give every SM eight CTAs, each a turn of its threads at least
-  auto pick = [&](int units, int least) {
-    const int most = (vocab + least - 1) / least, want = (8 * 148 + units - 1) / units;
-    return std::max(1, std::min(std::min(want, most), kVerMaxSplits));
+  // as many slices of a row as give every SM some CTAs, all of the same power of two of turns but the last
+  auto pick = [&](int units, int want) {
+    const int turns = (vocab / 8 + kVerTurn * kVerThreads - 1) / (kVerTurn * kVerThreads), most = std::max(1, turns * units / (want * 148));
+    int per = 1;
+    while (2 * per <= most || (turns + per - 1) / per > kVerMaxSplits) per *= 2;
+    return std::max(1, (turns + per - 1) / per);
   };
-  p.splits = pick(rows, 8 * kVerTurn * kVerThreads);
-  p.emit_splits = pick(requests, 8 * kVerThreads);
+  p.splits = pick(rows, 4);
+  p.emit_splits = pick(requests, 3);
   const size_t counts = ((size_t)requests * 4 + 255) & ~(size_t)255;
   p.stats = counts;
   p.best = p.stats + (size_t)rows * 2 * p.splits * 16;
