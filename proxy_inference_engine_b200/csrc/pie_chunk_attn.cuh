@@ -59,23 +59,25 @@ struct ChunkPiece {
 __device__ __forceinline__ const int4* chunk_words(const ChunkArgs& a, const int4* list, int begin, int at) {
   return at - begin < kChunkList ? list + 3 * (at - begin) : reinterpret_cast<const int4*>(a.pieces + at);
 }
+// false: an empty one
+__device__ __forceinline__ bool chunk_read(const ChunkArgs& a, const int4& x, const int4& y, const int4& z, ChunkPiece& p) {
+  p.row0 = x.x; p.pos0 = x.y; p.tokens = x.z; p.request = x.w;
+  p.head = y.x; p.k0 = y.y; p.n = y.z - y.y; p.first = y.w;
+  p.pieces = z.x;
+  p.kind = p.tokens > a.tile_tokens ? CHUNK_PAIR : p.tokens <= a.few_tokens ? CHUNK_FEW : CHUNK_ONE;
+  if (p.kind == CHUNK_PAIR) {
+    p.cnt0 = max(0, min(p.n, (p.pos0 + a.tile_tokens - 1) / kStepTile + 1 - p.k0));
+    p.cnt1 = p.n;
+  } else {
+    p.cnt0 = (p.n + 1) / 2;
+    p.cnt1 = p.n / 2;
+  }
+  return p.n > 0;
+}
 __device__ __forceinline__ bool chunk_piece(const ChunkArgs& a, const int4* list, int begin, int& at, int end, ChunkPiece& p) {
   while (at < end) {
     const int4* const e = chunk_words(a, list, begin, at++);
-    const int4 x = e[0], y = e[1], z = e[2];
-    p.row0 = x.x; p.pos0 = x.y; p.tokens = x.z; p.request = x.w;
-    p.head = y.x; p.k0 = y.y; p.n = y.z - y.y; p.first = y.w;
-    p.pieces = z.x;
-    if (p.n <= 0) continue;
-    p.kind = p.tokens > a.tile_tokens ? CHUNK_PAIR : p.tokens <= a.few_tokens ? CHUNK_FEW : CHUNK_ONE;
-    if (p.kind == CHUNK_PAIR) {
-      p.cnt0 = max(0, min(p.n, (p.pos0 + a.tile_tokens - 1) / kStepTile + 1 - p.k0));
-      p.cnt1 = p.n;
-    } else {
-      p.cnt0 = (p.n + 1) / 2;
-      p.cnt1 = p.n / 2;
-    }
-    return true;
+    if (chunk_read(a, e[0], e[1], e[2], p)) return true;
   }
   p.n = p.cnt0 = p.cnt1 = 0;
   return false;
@@ -120,6 +122,83 @@ struct ChunkFew {
   float2 share[kChunkFew];        // factors of the two groups' results
   int row[kChunkFew];             // a row's place among the step's rows x heads
 };
+
+// Adds up the pieces of a cut item: by the eight softmax warps of the CTA that came last.
+template <int D>
+__device__ __forceinline__ void chunk_merge(uint16_t* out, const float* part, int first, int pieces, int tokens, int row0, int head, int Hq, int G, bool few) {
+  const int tid = threadIdx.x;
+            // the item's pieces: the one that opens it, and the ones of the CTAs behind, in order
+            const float* const rec0 = part + (size_t)(2 * first + 1) * kChunkRecord<D>;
+            auto piece = [&](int i) { return rec0 + (i == 0 ? 0 : i * 2 * (ptrdiff_t)kChunkRecord<D> - kChunkRecord<D>); };
+            const int rows = tokens * G;
+            // What this costs is trips to L2 (and instructions that are run once), so all loads of a step are under way together.
+            auto store = [&](int q, int c4, const float4& o) {
+              const int t = q / G;
+              *reinterpret_cast<uint2*>(out + ((size_t)(row0 + t) * Hq + head * G + q - t * G) * D + 4 * c4) =
+                  make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+            };
+            // two parts of a row, (m, l, o) <- with (m2, l2, o2); a part without a key (m2 = -inf) may have left no results
+            auto join = [](float& m, float& l, float4& o, const float2& ml2, const float4& o2) {
+              if (ml2.x == -INFINITY && m != -INFINITY) return;
+              const float to = fmaxf(m, ml2.x), f = m == -INFINITY ? 0.f : exp2f(m - to), f2 = exp2f(ml2.x - to);
+              l = l * f + ml2.y * f2;
+              o.x = o.x * f + o2.x * f2; o.y = o.y * f + o2.y * f2; o.z = o.z * f + o2.z * f2; o.w = o.w * f + o2.w * f2;
+              m = to;
+            };
+            if (!few) {   // a row a thread, eight times four of its features at a time
+              if (tid < rows) {
+                const int from = 256 * D + 2 * tid;
+  #pragma unroll 1
+                for (int c0 = 0; c0 < D / 4; c0 += 8) {
+                  float4 o[8];
+                  float m = -INFINITY, l = 0.f;
+  #pragma unroll
+                  for (int k = 0; k < 8; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  #pragma unroll 1
+                  for (int i = 0; i < pieces; ++i) {
+                    float4 v[8];
+                    const float2 mi = __ldcg(reinterpret_cast<const float2*>(piece(i) + from));
+  #pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = __ldcg(reinterpret_cast<const float4*>(piece(i) + ((size_t)(c0 + k) * 256 + tid) * 4));
+                    float to = m, sum = l;
+  #pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                      to = m; sum = l;
+                      join(to, sum, o[k], mi, v[k]);
+                    }
+                    m = to; l = sum;
+                  }
+                  const float inv = 1.f / l;
+  #pragma unroll
+                  for (int k = 0; k < 8; ++k) store(tid, c0 + k, make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv));
+                }
+              }
+            } else {                     // four features of a row a lane, eight pieces at a time
+              constexpr int LANES = D / 4, STEP = 256 / LANES;
+  #pragma unroll 1
+              for (int q = tid / LANES; q < rows; q += STEP) {
+                const int c4 = tid % LANES;
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                float m = -INFINITY, l = 0.f;
+  #pragma unroll 1
+                for (int i0 = 0; i0 < pieces; i0 += 8) {
+                  float4 v[8];
+                  float2 mi[8];
+  #pragma unroll
+                  for (int k = 0; k < 8; ++k) {
+                    const float* const at_piece = piece(min(i0 + k, pieces - 1));
+                    mi[k] = __ldcg(reinterpret_cast<const float2*>(at_piece + 256 * D + 2 * q));
+                    v[k] = __ldcg(reinterpret_cast<const float4*>(at_piece + q * D + 4 * c4));
+                  }
+  #pragma unroll
+                  for (int k = 0; k < 8; ++k)
+                    if (i0 + k < pieces) join(m, l, o, mi[k], v[k]);
+                }
+                const float inv = 1.f / l;
+                store(q, c4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+              }
+            }
+}
 
 template <int D>
 __global__ void __launch_bounds__(ChunkTile<D>::THREADS, 1)
@@ -169,8 +248,13 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   pdl_launch_dependents();
   pdl_wait();   // (the set-up above ran under the end of the launch before this one)
   const int begin = __ldg(a.ranges + 2 * blockIdx.x), end = __ldg(a.ranges + 2 * blockIdx.x + 1);
-  for (int i = tid; i < 3 * min(end - begin, kChunkList); i += T::THREADS) list[i] = __ldg(reinterpret_cast<const int4*>(a.pieces + begin) + i);
-  __syncthreads();
+  // The CTA's pieces.  (The TMA warp reads the first one where it is and asks for its keys meanwhile.)
+  if (warp != 8) {
+    for (int i = warp < 8 ? tid : tid - 32; i < 3 * min(end - begin, kChunkList); i += T::THREADS - 32)
+      list[i] = __ldg(reinterpret_cast<const int4*>(a.pieces + begin) + i);
+    asm volatile("bar.sync 4, 352;" ::: "memory");
+    if (end - begin > 1) asm volatile("bar.arrive 5, 384;" ::: "memory");
+  }
 
   // All barriers are counted over the CTA's pieces: a role keeps the number of key tiles (of its group, of K and V) before its piece.
   // Registers: 384 threads x 168 at launch = 64512; 8 warps of 216 and 4 of 64 are 63488.
@@ -220,38 +304,49 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             chunk_ld16(tS + 32 * half, s);
             if (32 * half + 16 < rows) chunk_ld16(tS + 32 * half + 16, s + 16);
             tmem_ld_wait();
-            const int cut = step >= edge_step ? cut0 + step * 128 * a.G : 0;
-            if (step >= edge_step || 32 * half + 32 > rows)
+            if (step >= edge_step) {
+              const int cut = cut0 + step * 128 * a.G - 32 * half;
 #pragma unroll
               for (int n = 0; n < 32; ++n)
-                if (32 * half + n < cut || 32 * half + n >= rows) s[n] = -INFINITY;
+                if (n < cut) s[n] = -INFINITY;
+            }
+            if (rows & 3)   // (four rows are worked on at a time; what P has for the rows behind those does not matter)
+#pragma unroll
+              for (int n = 0; n < 32; ++n)
+                if (32 * half + n >= rows) s[n] = -INFINITY;
+          };
+          // the weights in the scores' place, and the largest
+          auto weigh = [&](int half) {
+            float mx = 0.f;
+#pragma unroll
+            for (int n = 0; n < 32; n += 4) {
+              if (32 * half + n >= rows) break;
+              const float4 less = *reinterpret_cast<const float4*>(&few.less[g][32 * half + n]);
+              s[n] = fap_exp2(fmaf(s[n], a.scale_log2e, less.x));
+              s[n + 1] = fap_exp2(fmaf(s[n + 1], a.scale_log2e, less.y));
+              s[n + 2] = fap_exp2(fmaf(s[n + 2], a.scale_log2e, less.z));
+              s[n + 3] = fap_exp2(fmaf(s[n + 3], a.scale_log2e, less.w));
+              mx = fmaxf(fmaxf(mx, fmaxf(s[n], s[n + 1])), fmaxf(s[n + 2], s[n + 3]));
+            }
+            return mx;
           };
           bool over = i == 0;
-#pragma unroll
-          for (int half = 1; half >= 0; --half)   // (the first 32 rows stay where they are)
-            if (32 * half < rows) {
-              load(half);
-              float mx = -INFINITY;
-              if (i > 0)
-#pragma unroll
-                for (int n = 0; n < 32; n += 4)
-                  if (n < 16 || 32 * half + 16 < rows) {
-                    const float4 less = *reinterpret_cast<const float4*>(&few.less[g][32 * half + n]);
-                    mx = fmaxf(fmaxf(mx, fmaxf(fmaf(s[n], a.scale_log2e, less.x), fmaf(s[n + 1], a.scale_log2e, less.y))),
-                               fmaxf(fmaf(s[n + 2], a.scale_log2e, less.z), fmaf(s[n + 3], a.scale_log2e, less.w)));
-                  }
-              over = over || mx > 8.f;
-            }
-          // the reference of a row moves where a score exceeds it by 8 (log2 units): same sums, and mostly the lanes need not know of one another
+          if (i > 0 && rows > 32) {
+            load(1);
+            over = weigh(1) > 256.f;
+          }
+          load(0);
+          if (i > 0) over = weigh(0) > 256.f || over;
+          // the reference of a row moves where a score exceeds it by 8 (log2 units: a weight of 256): same sums, and mostly the lanes need not know of one another
           if (chunk_group_any(g, over)) {
 #pragma unroll
             for (int half = 0; half < 2; ++half)
               if (32 * half < rows) {
-                if (half) load(half);
+                if (half || i > 0) load(half);
                 int mine = 0;
 #pragma unroll
-                for (int n = 0; n < 32; ++n)
-                  if (n < 16 || 32 * half + 16 < rows) {
+                for (int n = 0; n < 32; ++n) {
+                    if (32 * half + n >= rows) break;
                     const int v = __reduce_max_sync(0xffffffffu, chunk_order(s[n]));
                     if (lane == n) mine = v;
                   }
@@ -290,20 +385,21 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               tmem_st_wait();
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
-            if (rows > 32) load(0);
+            if (rows > 32 || i > 0) load(0);
+            weigh(0);
           }
 #pragma unroll
           for (int half = 0; half < 2; ++half)
             if (32 * half < rows) {
-              if (half) load(half);
+              if (half) {
+                load(1);
+                weigh(1);
+              }
 #pragma unroll
-              for (int n = 0; n < 32; n += 4)
-                if (n < 16 || 32 * half + 16 < rows) {
-                  const float4 less = *reinterpret_cast<const float4*>(&few.less[g][32 * half + n]);
-                  const float e0 = fap_exp2(fmaf(s[n], a.scale_log2e, less.x)), e1 = fap_exp2(fmaf(s[n + 1], a.scale_log2e, less.y));
-                  const float e2 = fap_exp2(fmaf(s[n + 2], a.scale_log2e, less.z)), e3 = fap_exp2(fmaf(s[n + 3], a.scale_log2e, less.w));
-                  l[32 * half + n] += e0; l[32 * half + n + 1] += e1; l[32 * half + n + 2] += e2; l[32 * half + n + 3] += e3;
-                  const uint32_t w[2] = {pack_bf16(e0, e1), pack_bf16(e2, e3)};
+              for (int n = 0; n < 32; n += 4) {
+                if (32 * half + n >= rows) break;
+                l[32 * half + n] += s[n]; l[32 * half + n + 1] += s[n + 1]; l[32 * half + n + 2] += s[n + 2]; l[32 * half + n + 3] += s[n + 3];
+                const uint32_t w[2] = {pack_bf16(s[n], s[n + 1]), pack_bf16(s[n + 2], s[n + 3])};
 #pragma unroll
                   for (int k = 0; k < 4; ++k)   // row n + k of the swizzled tile: 128 bytes, its 16-byte chunks in another order
                     asm volatile("st.shared.u16 [%0], %1;" ::"r"(sp + (32 * half + n + k) * 128 + ((chunk16 ^ ((n + k) & 7)) << 4)),
@@ -528,94 +624,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (last_flag) a.count[p.first] = 0;   // for the next launch: nobody else comes
         }
         chunk_sync();
-        if (last_flag) {
-          // the item's pieces: the one that opens it, and the ones of the CTAs behind, in order
-          const float* const rec0 = a.part + (size_t)(2 * p.first + 1) * kChunkRecord<D>;
-          auto piece = [&](int i) { return rec0 + (i == 0 ? 0 : i * 2 * (ptrdiff_t)kChunkRecord<D> - kChunkRecord<D>); };
-          const int rows = p.tokens * a.G, tile_rows = a.tile_tokens * a.G;
-          auto place = [&](int q) { return q < tile_rows ? q : q - tile_rows + 128; };   // of the item's row q in a record
-          // What this costs is trips to L2 (and instructions that are run once), so all loads of a step are under way together.
-          // Maximum and sum of a row: 1 to 32 lanes beside one another take every so manieth piece.
-          const int log = rows > 128 ? 0 : rows > 64 ? 1 : rows > 32 ? 2 : rows > 16 ? 3 : rows > 8 ? 4 : 5, row = min(tid >> log, rows - 1);
-          float mx = -INFINITY, ls = 0.f;
-          const int from = 256 * D + 2 * place(row);
-#pragma unroll 1
-          for (int i0 = tid & ((1 << log) - 1); i0 < p.pieces; i0 += 4 << log) {
-            float2 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = i0 + (k << log) < p.pieces ? __ldcg(reinterpret_cast<const float2*>(piece(i0 + (k << log)) + from)) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float to = fmaxf(mx, v[k].x);
-              ls = (ls == 0.f ? 0.f : ls * exp2f(mx - to)) + (v[k].y == 0.f ? 0.f : v[k].y * exp2f(v[k].x - to));
-              mx = to;
-            }
-          }
-#pragma unroll 1
-          for (int o = 1; o < 1 << log; o <<= 1) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, mx, o), l2 = __shfl_xor_sync(0xffffffffu, ls, o), to = fmaxf(mx, m2);
-            ls = (ls == 0.f ? 0.f : ls * exp2f(mx - to)) + (l2 == 0.f ? 0.f : l2 * exp2f(m2 - to));
-            mx = to;
-          }
-          (&ml[0][0])[row] = make_float2(mx, 1.f / ls);
-          chunk_sync();
-          auto add = [](float4& o, const float4& v, float mi, const float2& s) {   // (a piece without a key for this row may not have written results)
-            if (mi == -INFINITY && s.x != -INFINITY) return;
-            const float f = exp2f(mi - s.x) * s.y;
-            o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
-          };
-          auto store = [&](int q, int c4, const float4& o) {
-            const int t = q / a.G;
-            *reinterpret_cast<uint2*>(a.out + ((size_t)(p.row0 + t) * a.Hq + p.head * a.G + q - t * a.G) * D + 4 * c4) =
-                make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
-          };
-          if (p.kind != CHUNK_FEW) {   // a row a thread, eight times four of its features at a time
-            if (tid < rows) {
-              const float2 s = (&ml[0][0])[tid];
-#pragma unroll 1
-              for (int c0 = 0; c0 < D / 4; c0 += 8) {
-                float4 o[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-                for (int i = 0; i < p.pieces; ++i) {
-                  float4 v[8];
-                  const float mi = __ldcg(piece(i) + from);
-#pragma unroll
-                  for (int k = 0; k < 8; ++k) v[k] = __ldcg(reinterpret_cast<const float4*>(piece(i) + ((size_t)(c0 + k) * 256 + place(tid)) * 4));
-#pragma unroll
-                  for (int k = 0; k < 8; ++k) add(o[k], v[k], mi, s);
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) store(tid, c0 + k, o[k]);
-              }
-            }
-          } else {                     // four features of a row a lane, eight pieces at a time
-            constexpr int LANES = D / 4, STEP = 256 / LANES;
-#pragma unroll 1
-            for (int q = tid / LANES; q < rows; q += STEP) {
-              const float2 s = (&ml[0][0])[q];
-              const int c4 = tid % LANES;
-              float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-              for (int i0 = 0; i0 < p.pieces; i0 += 8) {
-                float4 v[8];
-                float mi[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  const float* const at_piece = piece(min(i0 + k, p.pieces - 1));
-                  mi[k] = __ldcg(at_piece + 256 * D + 2 * q);
-                  v[k] = __ldcg(reinterpret_cast<const float4*>(at_piece + q * D + 4 * c4));
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                  if (i0 + k < p.pieces) add(o, v[k], mi[k], s);
-              }
-              store(q, c4, o);
-            }
-          }
-          chunk_sync();   // (the sums are read before they are written again)
-        }
+        if (last_flag) chunk_merge<D>(a.out, a.part, p.first, p.pieces, p.tokens, p.row0, p.head, a.Hq, a.G, p.kind == CHUNK_FEW);
       } else if (p.kind != CHUNK_PAIR) {
         chunk_sync();     // both groups have read both accumulators
       }
@@ -627,9 +636,13 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       bool alive = true;
       int cq[2] = {0, 0}, ck = 0;   // pieces with a query tile g, key tiles, before this piece
       int turned = -RING - 1;       // the last key tile of the last piece of the turned kind
-      int at = begin;
-      ChunkPiece p;
-      while (alive && chunk_piece(a, list, begin, at, end, p)) {
+      for (int at = begin; alive && at < end; ++at) {
+        if (at == begin + 1) asm volatile("bar.sync 5, 384;" ::: "memory");   // (the list is there)
+        const int4* const e = at == begin ? reinterpret_cast<const int4*>(a.pieces + at) : chunk_words(a, list, begin, at);
+        const int4 z = e[2];
+        const int lead0 = z.y, lead1 = z.z;   // the pages of its first key tile
+        ChunkPiece p;
+        if (!chunk_read(a, e[0], e[1], z, p)) continue;
         const int32_t* const pages = a.table + (size_t)p.request * a.blocks;
         const int last_page = (p.pos0 + p.tokens - 1) / kStepPage;
         int first = 2 * p.k0, ids = __ldg(pages + min(first + lane, last_page));   // 32 pages from `first` on, a lane each; behind the last key: the last one
@@ -662,7 +675,8 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             first += 32;
             ids = __ldg(pages + min(first + lane, last_page));
           }
-          const int page0 = __shfl_sync(0xffffffffu, ids, 2 * (p.k0 + j) - first), page1 = __shfl_sync(0xffffffffu, ids, 2 * (p.k0 + j) + 1 - first);
+          const int page0 = j == 0 ? lead0 : __shfl_sync(0xffffffffu, ids, 2 * (p.k0 + j) - first);
+          const int page1 = j == 0 ? lead1 : __shfl_sync(0xffffffffu, ids, 2 * (p.k0 + j) + 1 - first);
           if (!(alive = gemm_wait_warp(smem_u32(&k_empty[i]), ph ^ 1, abortp))) break;
           fetch(&map_k, smK + i * T::TILE, &k_full[i], page0, page1);
           if (j == 0 && !(alive = fetch_q(1))) break;
@@ -676,34 +690,39 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (warp == 9) {
       // the whole warp walks the loop, one elected lane issues (as in the prompt's kernel)
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint64_t dq0 = umma_desc_sw128(smQ), dq1 = umma_desc_sw128(smQ1), dk0 = umma_desc_sw128(smK), dv0 = fap_desc_mn(smV);
+      // descriptors: their upper words are all the same
+      constexpr uint64_t UPPER = ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+      const uint32_t dq0 = (uint32_t)umma_desc_sw128(smQ), dq1 = (uint32_t)umma_desc_sw128(smQ1), dk0 = (uint32_t)umma_desc_sw128(smK), dv0 = (uint32_t)fap_desc_mn(smV);
       bool alive = true;   // a lane's own: once a wait expires it only keeps the lane from issuing
       int c[2] = {0, 0}, cq[2] = {0, 0}, ck = 0;   // tiles of group g, pieces with a query tile g, tiles of K and V, before this piece
       // scores of group g by query tile `tile`: S_g = Q K^T, or of the turned kind, whose rows' word of the instruction is `wide`, K Q^T
       auto qk = [&](int g, int tile, int t, uint32_t wide) {
-        const uint64_t dq = tile ? dq1 : dq0, dk = dk0 + (uint64_t)((t % RING) * (T::TILE >> 4));
+        uint32_t dq = tile ? dq1 : dq0, dk = dk0 + (t % RING) * (T::TILE >> 4);
+        asm volatile("" : "+r"(dq), "+r"(dk));   // (what is made of them is made here, and not kept in registers that the warp does not have)
         if (wide) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tm + COL_S + g * 128, dk + (k >> 2) * 1024 + 2 * (k & 3), dq + (k >> 2) * 1024 + 2 * (k & 3), ID_FEW | wide, k > 0 ? 1u : 0u);
+            umma_bf16(tm + COL_S + g * 128, UPPER | (dk + (k >> 2) * 1024 + 2 * (k & 3)), UPPER | (dq + (k >> 2) * 1024 + 2 * (k & 3)), ID_FEW | wide, k > 0 ? 1u : 0u);
         } else {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tm + COL_S + g * 128, dq + (k >> 2) * 1024 + 2 * (k & 3), dk + (k >> 2) * 1024 + 2 * (k & 3), ID_S, k > 0 ? 1u : 0u);
+            umma_bf16(tm + COL_S + g * 128, UPPER | (dq + (k >> 2) * 1024 + 2 * (k & 3)), UPPER | (dk + (k >> 2) * 1024 + 2 * (k & 3)), ID_S, k > 0 ? 1u : 0u);
         }
         fap_commit(&s_full[g]);
       };
       auto pv = [&](int g, int t, bool first, uint32_t wide) {
-        const uint64_t dv = dv0 + (uint64_t)((t % RING) * (T::TILE >> 4));
+        uint32_t dv = dv0 + (t % RING) * (T::TILE >> 4);
+        asm volatile("" : "+r"(dv));
         if (wide) {   // O^T += V^T P^T: V with its rows for K, P from shared memory
-          const uint64_t dp = dq1 + (uint64_t)(g * (T::P >> 4));
+          uint32_t dp = dq1 + g * (T::P >> 4);
+          asm volatile("" : "+r"(dp));
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_bf16(tm + COL_O + g * D, dv + k * (2048 >> 4), dp + (k >> 2) * (8192 >> 4) + 2 * (k & 3), ID_FEW | (1u << 15) | wide, (!first || k > 0) ? 1u : 0u);
+            umma_bf16(tm + COL_O + g * D, UPPER | (dv + k * (2048 >> 4)), UPPER | (dp + (k >> 2) * (8192 >> 4) + 2 * (k & 3)), ID_FEW | (1u << 15) | wide, (!first || k > 0) ? 1u : 0u);
         } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k)   // 16 keys: 8 columns of P, two 8-key atoms of V
-            umma_f16_ts(tm + COL_O + g * D, tm + COL_S + g * 128 + 8 * k, dv + k * (2048 >> 4), ID_O, (!first || k > 0) ? 1u : 0u);
+            umma_f16_ts(tm + COL_O + g * D, tm + COL_S + g * 128 + 8 * k, UPPER | (dv + k * (2048 >> 4)), ID_O, (!first || k > 0) ? 1u : 0u);
         }
         fap_commit(&o_full[g]);
       };
@@ -750,8 +769,9 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           ahead[g] = false;
         }
         // the next piece's scores, while this one's last tiles and its O are worked on
+        // (The second key tile's scores come behind the first's: the last ones give Q's place up.)
         auto go_on = [&](int g) {
-          if (more && next.cnt(g) > 0) {
+          if (more && next.cnt(g) > 0 && (next.kind == CHUNK_PAIR || g == 0 || ahead[0])) {
             open(next, g, tn, nq0, nq1);
             ahead[g] = true;
           }

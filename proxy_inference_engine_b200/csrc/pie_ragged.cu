@@ -33,8 +33,8 @@ struct PlanArgs {
 };
 constexpr int kPlanThreads = 512;
 constexpr int kCostPair = 2, kCostTile = 1;   // a key of an item with rows in both query tiles, in one
-constexpr int kCostItem = 256;                // queries in, results out
-constexpr long long kCostShare = 512;         // least share worth a CTA
+constexpr int kCostItem = 384;                // queries in, results out
+constexpr long long kCostShare = 512;         // least share worth a CTA; without pairs of query tiles, whose keys are sooner read than added up in pieces, twice that
 constexpr int kCutPair = 4, kCutTile = 2;     // least key tiles of a piece: what it costs to leave a piece's results and to add them up
 
 __device__ __forceinline__ long long warp_scan(long long v, int lane) {
@@ -211,7 +211,14 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
   // ---- attention's schedule
   const int Q = item[S];
   const long long W1 = cost[S], W = W1 * a.d.Hkv;
-  const long long want = max(1LL, min((long long)a.ctas, W / kCostShare)), share = (W + want - 1) / want;
+  bool pairs = false, large = false;   // requests with pairs, items of more than the least share: where there are none, a CTA an item
+  for (int s = s0; s < s1; ++s) {
+    const int n = row[s + 1] - row[s];
+    pairs = pairs || n > a.l.tile_tokens;
+    large = large || (n > 0 && ctx[s] + n + kCostItem > 2 * kCostShare);
+  }
+  const long long least = __syncthreads_or(pairs) || !__syncthreads_or(large) ? kCostShare : 2 * kCostShare;
+  const long long want = max(1LL, min((long long)a.ctas, W / least)), share = (W + want - 1) / want;
   int32_t* const ranges = w + a.l.ranges;
   if (blockIdx.x == 0)
     for (int c = tid; c < kStepMaxCtas; c += kPlanThreads)
@@ -222,13 +229,13 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     const int n = row[s + 1] - row[s], tokens = min(span, n - q * span), keys = ctx[s] + q * span + tokens;
     const int weight = tokens > a.l.tile_tokens ? kCostPair : kCostTile, tiles = (keys + kStepTile - 1) / kStepTile;
     const long long x = head * W1 + cost[s] + cost_before(q, ctx[s], span), end = x + (long long)weight * keys + kCostItem;
-    const int least = weight == kCostPair ? kCutPair : kCutTile;
+    const int cut = weight == kCostPair ? kCutPair : kCutTile;
     auto tile = [&](int c) {   // first key tile of CTA c's share.  A cut that would leave little on one side of it is not made.
       const long long past = c * share - x;
       if (past <= 0) return 0;
       const long long per = (long long)weight * kStepTile, k = (past + per - 1) / per;
-      if (k < least) return 2 * k <= tiles || tiles >= 2 * least ? 0 : tiles;
-      return tiles - k < least ? tiles : (int)k;
+      if (k < cut) return 2 * k <= tiles || tiles >= 2 * cut ? 0 : tiles;
+      return tiles - k < cut ? tiles : (int)k;
     };
     const int c0 = (int)(x / share), c1 = (int)((end - 1) / share);
     int mine = 0, opens = c0;
@@ -243,7 +250,9 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
       p.request = s; p.kv_head = head;
       p.k0 = tile(c); p.k1 = tile(c + 1);
       p.first_cta = opens; p.pieces = mine;
-      p.pad[0] = p.pad[1] = p.pad[2] = 0;
+      const int last_page = (keys - 1) / kStepPage;   // (behind the last key: its page again)
+      for (int i = 0; i < 2; ++i) p.pages[i] = p.k0 < p.k1 ? max(page_id(s, min(2 * p.k0 + i, last_page)), 0) : 0;
+      p.pad = 0;
       const int4* const from = reinterpret_cast<const int4*>(&p);
       int4* const to = reinterpret_cast<int4*>(pieces + i + c);   // the CTAs' lists lie one behind the other, with holes where an item ends with a share
       to[0] = from[0]; to[1] = from[1]; to[2] = from[2];

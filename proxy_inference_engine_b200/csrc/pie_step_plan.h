@@ -18,7 +18,8 @@ struct StepPiece {
   int request, kv_head;
   int k0, k1;               // key tiles [k0, k1); none: nothing to do
   int first_cta, pieces;    // the CTA of the item's first piece, and how many CTAs share it
-  int pad[3];
+  int pages[2];             // of key tile k0
+  int pad;
 };
 static_assert(sizeof(StepPiece) == 4 * kStepPieceWords, "read as three 16-byte words");
 

@@ -123,10 +123,11 @@ def test_chunk_attention(new, cached, Hq, Hkv, D):
 @pytest.mark.parametrize("Hq,Hkv,D", [(1, 1, 64), (3, 1, 128), (24, 8, 64), (64, 8, 128), (7, 1, 64), (40, 1, 128), (128, 1, 64), (16, 16, 128)])
 def test_chunk_attention_of_other_heads(Hq, Hkv, D):
     from proxy_inference_engine_b200 import ops
-    new, cached = [1, 45, 9, 4], [900, 30, 250, 2000]
-    plan, q, k, v, tables = attention_case(new, cached, Hq, Hkv, D, seed=Hq)
-    attention_holds(ops.chunk_attention(q, k, v, plan, D ** -0.5), q, k, v, new, cached, tables, D ** -0.5)
-    ops.check_pipeline()
+    # (long ones of two, three and more query tiles: items that are cut between key tiles)
+    for new, cached in (([1, 45, 9, 4], [900, 30, 250, 2000]), ([3, 7, 40, 140 * Hkv // Hq + 1], [5000, 6001, 4000, 9000])):
+        plan, q, k, v, tables = attention_case(new, cached, Hq, Hkv, D, seed=Hq)
+        attention_holds(ops.chunk_attention(q, k, v, plan, D ** -0.5), q, k, v, new, cached, tables, D ** -0.5)
+        ops.check_pipeline()
 
 
 @pytest.mark.parametrize("std", [0.0, 30.0])

@@ -47,16 +47,18 @@ def schedule_is_whole(plan):
     ranges, base = words[at:at + 384], at + 384
     G = d.Hq // d.Hkv
     tile, starts, ctx = 128 // G, plan.row_starts.tolist(), plan.contexts.tolist()
-    seen, opens, shares = {}, set(), []
+    seen, opens, shares, plan_table = {}, set(), [], plan.block_table.tolist()
     for c in range(192):
         lo, hi = ranges[2 * c], ranges[2 * c + 1]
         assert 0 <= lo <= hi and (base + 12 * hi <= len(words) or lo == hi)
         cost = 0
         for i in range(lo, hi):
-            row0, pos0, tokens, s, h, k0, k1, first, pieces = words[base + 12 * i:base + 12 * i + 9]
+            row0, pos0, tokens, s, h, k0, k1, first, pieces, page0, page1 = words[base + 12 * i:base + 12 * i + 11]
             assert 0 <= k0 <= k1
             if k0 == k1:
                 continue
+            mine = plan_table[s][:(pos0 + tokens + 63) // 64]
+            assert [page0, page1] == [mine[min(j, len(mine) - 1)] for j in (2 * k0, 2 * k0 + 1)]
             item = seen.setdefault((h, s, row0), [])
             item.append((k0, k1, c, first, pieces))
             cost += (k1 - k0) * (2 if tokens > tile else 1)
