@@ -9,7 +9,7 @@ int step_dims_status(const pie_step_dims* d) {
   if (!d) return PIE_ENULL;
   if (d->requests < 1 || d->requests > kStepMaxRequests || d->rows < 1 || d->logit_rows < 1 || d->blocks < 1 || d->pages < 1 || d->Hq < 1 || d->Hkv < 1 ||
       d->Hq % d->Hkv || d->Hq / d->Hkv > kStepTile || (long long)d->requests * d->blocks > 0x7fffffff || (long long)d->pages * kStepPage > 0x7fffffff ||
-      (long long)d->blocks * kStepPage > 0x7fffffff || step_layout(*d).items > 0x3fffffff)
+      (long long)d->blocks * kStepPage > 0x7fffffff || (long long)d->rows * d->Hq > 0x7fffffff || step_layout(*d).items > 0x3fffffff)
     return PIE_EINVAL_SHAPE;
   return PIE_OK;
 }
@@ -17,7 +17,8 @@ int step_dims_status(const pie_step_dims* d) {
 // ---------------------------------------------------------------------------------------------------- the plan
 // Every array of the plan is a function of four sums over the requests before one (rows, pages, logit rows, cost of attention).  One launch: each CTA takes the sums of
 // all requests itself, in shared memory (at most 4096 of them), and fills its part of every array, finding a row's request by bisection.  Kilobytes: what counts is one
-// launch and the length of the chain load, scan, bisection, page id, store.
+// launch and the length of the chain load, scan, bisection, page id, store.  8 requests 5.8 us, 212 requests of 11700 rows 7.3, in a row of such launches; a call costs its
+// host 8.
 //
 // Attention's work is dealt out to the SMs in equal shares: items (key / value head, request, pair of query tiles) lie on a line, as long as they have keys to multiply
 // (twice that where both query tiles have rows) and a constant for what an item costs besides; CTA c has [c share, (c + 1) share) of the line.  An item that lies in
@@ -33,7 +34,7 @@ struct PlanArgs {
 };
 constexpr int kPlanThreads = 512;
 constexpr int kCostPair = 2, kCostTile = 1;   // a key of an item with rows in both query tiles, in one
-constexpr int kCostItem = 384;                // queries in, results out
+constexpr int kCostItem = 576;                // queries in, results out (256: a step of three prompts and 29 answers 85 us, 81 with this)
 constexpr long long kCostShare = 512;         // least share worth a CTA; without pairs of query tiles, whose keys are sooner read than added up in pieces, twice that
 constexpr int kCutPair = 4, kCutTile = 2;     // least key tiles of a piece: what it costs to leave a piece's results and to add them up
 
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
       p.k0 = tile(c); p.k1 = tile(c + 1);
       p.first_cta = opens; p.pieces = mine;
       const int last_page = (keys - 1) / kStepPage;   // (behind the last key: its page again)
-      for (int i = 0; i < 2; ++i) p.pages[i] = p.k0 < p.k1 ? max(page_id(s, min(2 * p.k0 + i, last_page)), 0) : 0;
+      for (int h = 0; h < 2; ++h) p.pages[h] = p.k0 < p.k1 ? max(page_id(s, min(2 * p.k0 + h, last_page)), 0) : 0;
       p.pad = 0;
       const int4* const from = reinterpret_cast<const int4*>(&p);
       int4* const to = reinterpret_cast<int4*>(pieces + i + c);   // the CTAs' lists lie one behind the other, with holes where an item ends with a share
@@ -273,7 +274,8 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
 
 // ---------------------------------------------------------------------------------------------------- rotation and cache write
 // rope_kv_heads_kernel's way (pie_rope_kv.cu) over rows that each have a position and a slot of their own: a thread takes 8 pairs of features of one row for every HL-th
-// head, 16 bytes an access, so a sine serves H / HL heads.  HBM-bound where there are many rows, latency-bound where there are few.
+// head, 16 bytes an access, so a sine serves H / HL heads.  HBM-bound where there are many rows (8191 of 32 + 16 heads of 128 34.8 us, 5.8 TB/s), latency-bound where there
+// are few (32 rows 3 us).
 __global__ void __launch_bounds__(128) rope_kv_slots_kernel(uint16_t* q_out, uint16_t* kp, uint16_t* vp, long long tok_stride, long long head_stride, const RopeRows r,
                                                             const int32_t* positions, const int32_t* slots, const float* freqs, int rows, int n_slots, int Hq,
                                                             int Hkv, int D, int rest, int HL) {

@@ -2,8 +2,10 @@
 // token a step (PIE/engine/inference_engine.py:259-297); the log-probabilities are its own, f32(logits) - logsumexp (:268-269), at the temperature of the draw.
 //
 // Two launches.  verify_stats_kernel reads every row of logits once: maximum and sum of exponentials (greedy: and the first largest) of slices, in 32 bits.
-// verify_emit_kernel: each CTA of a request joins its rows' slices, finds how many drafted tokens are accepted, and takes a slice of the vocabulary of the one row behind
-// them; the last CTA to finish joins the slices' best.  All of it is bound by HBM: a row of 128256 logits is 257 KB.
+// verify_emit_kernel: each CTA of a request joins its rows' slices, finds how many drafted tokens are accepted, and takes slices of the one row behind them through the race for
+// its token; the last CTA to finish joins the slices' best.  (The joining by the last CTA of the first launch, once for a request, cost more in its tail than it saved: 39 -> 46 us.)
+// A row of 128256 logits is 257 KB: HBM at the least, but at seven instructions an exponential, all told, the issue slots are half taken, and a CTA's start and end are as long as its
+// slice.  Device time, in a row of such calls: 5 rows greedy 5.3 us, 16 x 8 12.7, 32 x 6 looked-up drafts 21.7, 64 x 6 rows against a drafter's 39.4 (3.2 TB/s).
 #include <algorithm>
 
 #include "pie_internal.h"

@@ -255,8 +255,8 @@ def _planned_step(model, plan: StepPlan, pools, all_logits: bool) -> torch.Tenso
 
 def speculative_step(model, plan: StepPlan, pools, *, max_draft: int, temp: float = 0.0, uniforms=None, noise=None, draft_logits=None):
     """One step of drafting decode: ragged_step over a plan whose requests bring their last token and some drafted ones (draft_lengths), then verify_draft.
-    Returns its (tokens, counts, logprobs).  A request then has context + new - drafted + counts - 1 tokens in the cache -- what lies behind them there is
-    written over -- and its last token, tokens[s, counts[s] - 1], is the next step's first."""
+    Returns its (tokens, counts, logprobs).  A request that took part then has context + new - drafted + counts - 1 tokens in the cache -- what lies behind them
+    there is written over -- and its last token, tokens[s, counts[s] - 1], is the next step's first; of one that sat the step out (counts 0) nothing changed."""
     logits = ragged_step(model, plan, pools)
     return ops.verify_draft(logits, plan.draft_tokens, plan.logit_starts, max_draft=max_draft, temp=temp, uniforms=uniforms, noise=noise, draft_logits=draft_logits)
 

@@ -130,6 +130,22 @@ def test_chunk_attention_of_other_heads(Hq, Hkv, D):
         ops.check_pipeline()
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_steps_of_all_kinds_of_requests(seed):
+    """Single tokens, drafts, portions of every size and requests that sit the step out, in any order: a CTA turns from one kind of item to another."""
+    from proxy_inference_engine_b200 import ops
+    rng = random.Random(seed)
+    D, Hkv, G = rng.choice([64, 128]), rng.choice([1, 2, 4]), rng.choice([1, 2, 3, 4, 8, 16])
+    kinds = [lambda: 1, lambda: rng.randint(1, 8), lambda: rng.randint(9, 70), lambda: rng.randint(60, 300), lambda: 0]
+    new = [rng.choice(kinds)() for _ in range(rng.randint(2, 14))] + [1]
+    cached = [rng.choice([0, rng.randint(0, 200), rng.randint(0, 2500)]) for _ in new]
+    plan, q, k, v, tables = attention_case(new, cached, Hkv * G, Hkv, D, seed=seed, pad=seed % 3, std=rng.choice([0.5, 2.0, 3.0]))
+    got = ops.chunk_attention(q, k, v, plan, D ** -0.5)
+    attention_holds(got, q, k, v, new, cached, tables, D ** -0.5)
+    assert torch.equal(got, ops.chunk_attention(q, k, v, plan, D ** -0.5)) and not got[sum(new):].any()
+    ops.check_pipeline()
+
+
 @pytest.mark.parametrize("std", [0.0, 30.0])
 def test_chunk_attention_of_flat_and_of_steep_scores(std):
     """All keys alike, and one key that takes all: the running maximum moves by hundreds."""
@@ -191,6 +207,72 @@ def test_attention_on_two_streams_at_once():
     torch.cuda.synchronize()
     for mine, w in zip(got, want):
         assert all(torch.equal(x, w) for x in mine)
+
+
+def test_what_other_requests_and_later_keys_hold_does_not_matter():
+    """NaN and infinities in one request's keys and values stay its own, and in the keys of later new tokens they are masked."""
+    from proxy_inference_engine_b200 import ops
+    for new, cached in (([3, 40, 1], [200, 100, 300]), ([200, 300, 5], [0, 70, 10])):
+        plan, q, k, v, tables = attention_case(new, cached, 8, 2, 128, seed=13)
+        want = ops.chunk_attention(q, k, v, plan, 0.1)
+        k2, v2 = k.clone(), v.clone()
+        k2[tables[1]], v2[tables[1]] = torch.inf, torch.nan
+        got = ops.chunk_attention(q, k2, v2, plan, 0.1)
+        rest = list(range(new[0])) + list(range(new[0] + new[1], sum(new)))
+        assert torch.equal(got[rest], want[rest]) and bool(torch.isnan(got[new[0]:new[0] + new[1]]).all())
+        k2, last = k.clone(), cached[1] + new[1] - 1
+        k2[tables[1][last // 64], last % 64] = torch.nan
+        got = ops.chunk_attention(q, k2, v, plan, 0.1)
+        but = [t for t in range(sum(new)) if t != new[0] + new[1] - 1]
+        assert torch.equal(got[but], want[but]) and bool(torch.isnan(got[new[0] + new[1] - 1]).all())
+
+
+def test_pages_behind_the_32_bit_offsets():
+    """Pools of 2.6e9 elements: pages at either end."""
+    from proxy_inference_engine_b200 import ops
+    from proxy_inference_engine_b200.ragged import StepPlan
+    g, n_pages, Hq, Hkv, D = gen(21), 40000, 32, 8, 128
+    k_pool, v_pool = (torch.empty((n_pages, 64, Hkv, D), dtype=BF, device="cuda") for _ in range(2))
+    tables, new, cached = [[39999, 3, 39990], [35000, 39998]], [5, 70], [130, 20]
+    for t in tables:
+        k_pool[t], v_pool[t] = randn(g, len(t), 64, Hkv, D), randn(g, len(t), 64, Hkv, D)
+    plan = StepPlan.build(ints([0] * 75), ints(new), ints(cached), ints(sum(tables, [])), num_pages=n_pages, max_blocks=3, num_heads=Hq, num_kv_heads=Hkv)
+    plan.check()
+    q, k, v = randn(g, 75, Hq, D, std=2.0), randn(g, 75, Hkv, D), randn(g, 75, Hkv, D)
+    turned = ops.rope_kv_slots(q, k, v, FREQS(D), plan.positions, plan.slots, k_pool, v_pool)
+    at = plan.slots.long()
+    assert torch.equal(v_pool.view(-1, Hkv, D)[at], v) and int(at.max()) * Hkv * D > 2 ** 31
+    some = sorted(set(sum(tables, [])))
+    small = [[some.index(p) for p in t] for t in tables]
+    attention_holds(ops.chunk_attention(turned, k_pool, v_pool, plan, 0.1), turned, k_pool[some], v_pool[some], new, cached, small, 0.1)
+
+
+def test_two_captured_graphs_at_once():
+    """... of calls whose items are cut: neither counts in the other's workspace, nor in an eager call's."""
+    from proxy_inference_engine_b200 import ops
+    cases = [attention_case([4, 1], [6000, 3000], 8, 2, 128, seed=s) for s in (3, 4)]
+    drafts = [verify_case([3, 4], 5000, 0.7, True, seed=s)[0] for s in (5, 6)]
+
+    def run(i):
+        plan, q, k, v, _ = cases[i]
+        kw = dict(drafts[i])
+        return (ops.chunk_attention(q, k, v, plan, 0.1), *ops.verify_draft(kw.pop("logits"), kw.pop("draft_tokens"), kw.pop("logit_starts"), max_draft=4, **kw))
+    want = [run(0), run(1)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run(i))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        eager = run(0)
+    torch.cuda.synchronize()
+    for got, w in ((outs[0], want[0]), (outs[1], want[1]), (eager, want[0])):
+        assert all(torch.equal(a, b) for a, b in zip(got, w))
 
 
 # ---------------------------------------------------------------------------------------------------- verification
