@@ -33,9 +33,10 @@ struct PlanArgs {
   int ctas;
 };
 constexpr int kPlanThreads = 512;
-constexpr int kCostPair = 2, kCostTile = 1;   // a key of an item with rows in both query tiles, in one
+constexpr int kCostPair = 2, kCostTile = 1;   // a key of an item with rows in both query tiles, in one (powers of two)
 constexpr int kCostItem = 576;                // queries in, results out (256: a step of three prompts and 29 answers 85 us, 81 with this)
 constexpr long long kCostShare = 512;         // least share worth a CTA; without pairs of query tiles, whose keys are sooner read than added up in pieces, twice that
+static_assert(kCostTile * kStepTile == 1 << 7 && kCostPair * kStepTile == 1 << 8, "key tiles are counted by shifts");
 constexpr int kCutPair = 4, kCutTile = 2;     // least key tiles of a piece: what it costs to leave a piece's results and to add them up
 
 __device__ __forceinline__ long long warp_scan(long long v, int lane) {
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
   extern __shared__ __align__(16) uint8_t plan_smem[];
   __shared__ long long scan_sm[3 * (kPlanThreads / 32)];
   __shared__ long long page_total;
-  __shared__ int bad;
+  __shared__ int bad, kinds;
   const int S = a.d.requests, T = a.d.rows, tid = threadIdx.x, span = 2 * a.l.tile_tokens;
   long long* const cost = reinterpret_cast<long long*>(plan_smem);   // [S + 1] each
   int* const row = reinterpret_cast<int*>(cost + S + 1);
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
   int* const ctx = item + S + 1;
   pdl_launch_dependents();
   pdl_wait();
-  if (tid == 0) bad = 0;
+  if (tid == 0) bad = kinds = 0;
   __syncthreads();
   int fault = 0;
 
@@ -148,13 +149,17 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     };
     for (int s = s0; s < s1; ++s) add(s, v);
     block_scan(v, scan_sm);
+    int kind = 0;   // 1: a pair of query tiles, 2: an item of more than the larger least share (where there is none, a CTA an item)
     for (int s = s0; s < s1; ++s) {
+      const int n = row[s + 1] - row[s];
+      kind |= (n > a.l.tile_tokens ? 1 : 0) | (n > 0 && ctx[s] + n + kCostItem > 2 * kCostShare ? 2 : 0);
       logit[s] = (int)min(v[0], (long long)a.d.logit_rows);
       item[s] = (int)v[1];
       cost[s] = v[2];
       add(s, v);
       if (v[0] > a.d.logit_rows) fault |= PIE_STEP_LOGITS;
     }
+    if (kind) atomicOr(&kinds, kind);
     if (s0 < S && s1 == S) { logit[S] = (int)min(v[0], (long long)a.d.logit_rows); item[S] = (int)v[1]; cost[S] = v[2]; }
   }
   __syncthreads();
@@ -181,7 +186,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     w[a.l.logit_starts + s] = logit[s];
     if (s < S) w[a.l.contexts + s] = ctx[s];
   }
-  for (int t = first; t < T; t += step) {
+  auto do_row = [&](int t) {
     int s = -1, p = 0, slot = -1;
     if (t < row[S]) {
       s = last_at_or_below(row, S, t);
@@ -192,13 +197,13 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     w[a.l.sequences + t] = s;
     w[a.l.positions + t] = p;
     w[a.l.slots + t] = slot;
-  }
+  };
   const unsigned cells = (unsigned)S * (unsigned)a.d.blocks;
-  for (unsigned e = first; e < cells; e += step) {
+  auto do_cell = [&](unsigned e) {
     const int s = e / (unsigned)a.d.blocks, j = e % (unsigned)a.d.blocks;
     w[a.l.block_table + e] = j < page[s + 1] - page[s] ? max(page_id(s, j), 0) : 0;
-  }
-  for (int r = first; r < a.d.logit_rows; r += step) {
+  };
+  auto do_logit = [&](int r) {
     int of = 0, token = -1;
     if (r < logit[S]) {
       const int s = last_at_or_below(logit, S, r), left = logit[s + 1] - 1 - r;
@@ -207,25 +212,20 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     }
     w[a.l.logit_rows + r] = of;
     w[a.l.draft_tokens + r] = token;
-  }
+  };
 
   // ---- attention's schedule
   const int Q = item[S];
   const long long W1 = cost[S], W = W1 * a.d.Hkv;
-  bool pairs = false, large = false;   // requests with pairs, items of more than the least share: where there are none, a CTA an item
-  for (int s = s0; s < s1; ++s) {
-    const int n = row[s + 1] - row[s];
-    pairs = pairs || n > a.l.tile_tokens;
-    large = large || (n > 0 && ctx[s] + n + kCostItem > 2 * kCostShare);
-  }
-  const long long least = __syncthreads_or(pairs) || !__syncthreads_or(large) ? kCostShare : 2 * kCostShare;
+  const long long least = kinds == 2 ? 2 * kCostShare : kCostShare;
   const long long want = max(1LL, min((long long)a.ctas, W / least)), share = (W + want - 1) / want;
   int32_t* const ranges = w + a.l.ranges;
   if (blockIdx.x == 0)
     for (int c = tid; c < kStepMaxCtas; c += kPlanThreads)
       if (c * share >= W) ranges[2 * c] = ranges[2 * c + 1] = 0;   // (the shares before it are written below)
   StepPiece* const pieces = reinterpret_cast<StepPiece*>(w + a.l.pieces);
-  for (int i = first; i < Q * a.d.Hkv; i += step) {
+  auto share_of = [&](long long at) { return W <= 0xffffffffLL ? (int)((uint32_t)at / (uint32_t)share) : (int)(at / share); };
+  auto do_item = [&](int i) {
     const int head = i / Q, at = i - head * Q, s = last_at_or_below(item, S, at), q = at - item[s];
     const int n = row[s + 1] - row[s], tokens = min(span, n - q * span), keys = ctx[s] + q * span + tokens;
     const int weight = tokens > a.l.tile_tokens ? kCostPair : kCostTile, tiles = (keys + kStepTile - 1) / kStepTile;
@@ -234,11 +234,12 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     auto tile = [&](int c) {   // first key tile of CTA c's share.  A cut that would leave little on one side of it is not made.
       const long long past = c * share - x;
       if (past <= 0) return 0;
-      const long long per = (long long)weight * kStepTile, k = (past + per - 1) / per;
+      const int log = weight == kCostPair ? 8 : 7;   // of the cost of a key tile
+      const long long k = (past + (1 << log) - 1) >> log;
       if (k < cut) return 2 * k <= tiles || tiles >= 2 * cut ? 0 : tiles;
       return tiles - k < cut ? tiles : (int)k;
     };
-    const int c0 = (int)(x / share), c1 = (int)((end - 1) / share);
+    const int c0 = share_of(x), c1 = share_of(end - 1);
     int mine = 0, opens = c0;
     for (int c = c0; c <= c1; ++c)
       if (tile(c) < tile(c + 1)) {
@@ -263,6 +264,15 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
       }
     }
     if (i == Q * a.d.Hkv - 1) ranges[2 * c1 + 1] = i + c1 + 1;
+  };
+
+  // ---- one entry a thread: the arrays lie behind one another here, so that no thread waits for memory once for each
+  const long long e0 = (long long)Q * a.d.Hkv, e1 = e0 + cells, e2 = e1 + T, e3 = e2 + a.d.logit_rows;
+  for (long long e = first; e < e3; e += step) {
+    if (e < e0) do_item((int)e);
+    else if (e < e1) do_cell((unsigned)(e - e0));
+    else if (e < e2) do_row((int)(e - e1));
+    else do_logit((int)(e - e2));
   }
 
   if (fault) atomicOr(&bad, fault);
