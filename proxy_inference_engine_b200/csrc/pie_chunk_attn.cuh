@@ -9,7 +9,7 @@
 //   * one tile of more than 64 rows: the groups take every other key tile of it, each with its own maximum, sum and accumulator, which meet at the end through tensor
 //     memory (the groups' warps read the same lanes).
 //   * few, up to 64 rows (an answer's token, drafted ones): every other key tile as well, but turned around.  S^T = K Q^T has a key a lane and the rows, padded to 16,
-//     for its columns; P goes to shared memory as the B operand of O^T = V^T P^T.  The softmax of 4 rows is then 16 exponentials of each of the 128 threads instead of 128 of four of
+//     for its columns; P goes to shared memory as the B operand of O^T = V^T P^T.  The softmax of 4 rows is then 4 exponentials of each of the 128 threads instead of 128 of four of
 //     them, and the MMAs are as narrow as the rows: bound by the stream of keys and values.  (A row a lane: one warp a group does all the work, and both of them on the same
 //     quarter of the SM; head size 64 40 x 12000 keys 259 us, 59 % of the stream's rate.)  A column's maximum is taken over all lanes only where some score exceeds the reference by
 //     2^8, which the group finds by a vote; the sums over the lanes wait for the end.
@@ -17,6 +17,10 @@
 // workspace, and the last CTA of the item to arrive adds all pieces up in their order: the same bits whichever that is.
 // Keys that a row must not see get weight 0; values behind the item's last key are cleared in shared memory, since 0 * NaN is not 0.
 // Every wait is bounded (pie_gemm.cuh); a warp whose wait ran out does nothing more, but walks on through the barriers of the softmax warps.
+// Device time in a row of such calls, inputs not in L2, 32 query / 8 kv heads: D 128, 2048 tokens behind 15000 460 us (1170 TFLOP/s, of cuBLAS's 1638 in a burst; the tensor pipe is
+// busy for 54 % of it, as in the prompt's kernel one tile's softmax is covered by the other's products in part); 16 answers with up to five drafted tokens over 4000 keys 50.8 (4.5 TB/s),
+// 40 over 12000 319 (6.2 TB/s), one with four over 9000 25.7; D 64, three portions of 700 tokens beside 29 answers over 1500 keys 80.6, 40 answers over 12000 192 (4.9 TB/s).  Short
+// steps pay 4 us from the launch to the first scores, some 3 at each turn from one piece to the next and 5 at the end: results, one counter, the last CTA's sums.
 #include "pie_step_plan.h"
 
 namespace pie {
@@ -127,77 +131,77 @@ struct ChunkFew {
 template <int D>
 __device__ __forceinline__ void chunk_merge(uint16_t* out, const float* part, int first, int pieces, int tokens, int row0, int head, int Hq, int G, bool few) {
   const int tid = threadIdx.x;
-            // the item's pieces: the one that opens it, and the ones of the CTAs behind, in order
-            const float* const rec0 = part + (size_t)(2 * first + 1) * kChunkRecord<D>;
-            auto piece = [&](int i) { return rec0 + (i == 0 ? 0 : i * 2 * (ptrdiff_t)kChunkRecord<D> - kChunkRecord<D>); };
-            const int rows = tokens * G;
-            // What this costs is trips to L2 (and instructions that are run once), so all loads of a step are under way together.
-            auto store = [&](int q, int c4, const float4& o) {
-              const int t = q / G;
-              *reinterpret_cast<uint2*>(out + ((size_t)(row0 + t) * Hq + head * G + q - t * G) * D + 4 * c4) =
-                  make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
-            };
-            // two parts of a row, (m, l, o) <- with (m2, l2, o2); a part without a key (m2 = -inf) may have left no results
-            auto join = [](float& m, float& l, float4& o, const float2& ml2, const float4& o2) {
-              if (ml2.x == -INFINITY && m != -INFINITY) return;
-              const float to = fmaxf(m, ml2.x), f = m == -INFINITY ? 0.f : exp2f(m - to), f2 = exp2f(ml2.x - to);
-              l = l * f + ml2.y * f2;
-              o.x = o.x * f + o2.x * f2; o.y = o.y * f + o2.y * f2; o.z = o.z * f + o2.z * f2; o.w = o.w * f + o2.w * f2;
-              m = to;
-            };
-            if (!few) {   // a row a thread, eight times four of its features at a time
-              if (tid < rows) {
-                const int from = 256 * D + 2 * tid;
-  #pragma unroll 1
-                for (int c0 = 0; c0 < D / 4; c0 += 8) {
-                  float4 o[8];
-                  float m = -INFINITY, l = 0.f;
-  #pragma unroll
-                  for (int k = 0; k < 8; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  #pragma unroll 1
-                  for (int i = 0; i < pieces; ++i) {
-                    float4 v[8];
-                    const float2 mi = __ldcg(reinterpret_cast<const float2*>(piece(i) + from));
-  #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = __ldcg(reinterpret_cast<const float4*>(piece(i) + ((size_t)(c0 + k) * 256 + tid) * 4));
-                    float to = m, sum = l;
-  #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                      to = m; sum = l;
-                      join(to, sum, o[k], mi, v[k]);
-                    }
-                    m = to; l = sum;
-                  }
-                  const float inv = 1.f / l;
-  #pragma unroll
-                  for (int k = 0; k < 8; ++k) store(tid, c0 + k, make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv));
-                }
-              }
-            } else {                     // four features of a row a lane, eight pieces at a time
-              constexpr int LANES = D / 4, STEP = 256 / LANES;
-  #pragma unroll 1
-              for (int q = tid / LANES; q < rows; q += STEP) {
-                const int c4 = tid % LANES;
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                float m = -INFINITY, l = 0.f;
-  #pragma unroll 1
-                for (int i0 = 0; i0 < pieces; i0 += 8) {
-                  float4 v[8];
-                  float2 mi[8];
-  #pragma unroll
-                  for (int k = 0; k < 8; ++k) {
-                    const float* const at_piece = piece(min(i0 + k, pieces - 1));
-                    mi[k] = __ldcg(reinterpret_cast<const float2*>(at_piece + 256 * D + 2 * q));
-                    v[k] = __ldcg(reinterpret_cast<const float4*>(at_piece + q * D + 4 * c4));
-                  }
-  #pragma unroll
-                  for (int k = 0; k < 8; ++k)
-                    if (i0 + k < pieces) join(m, l, o, mi[k], v[k]);
-                }
-                const float inv = 1.f / l;
-                store(q, c4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-              }
-            }
+  // the item's pieces: the one that opens it, and the ones of the CTAs behind, in order
+  const float* const rec0 = part + (size_t)(2 * first + 1) * kChunkRecord<D>;
+  auto piece = [&](int i) { return rec0 + (i == 0 ? 0 : i * 2 * (ptrdiff_t)kChunkRecord<D> - kChunkRecord<D>); };
+  const int rows = tokens * G;
+  // What this costs is trips to L2 (and instructions that are run once), so all loads of a step are under way together.
+  auto store = [&](int q, int c4, const float4& o) {
+    const int t = q / G;
+    *reinterpret_cast<uint2*>(out + ((size_t)(row0 + t) * Hq + head * G + q - t * G) * D + 4 * c4) =
+        make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+  };
+  // two parts of a row, (m, l, o) <- with (m2, l2, o2); a part without a key (m2 = -inf) may have left no results
+  auto join = [](float& m, float& l, float4& o, const float2& ml2, const float4& o2) {
+    if (ml2.x == -INFINITY && m != -INFINITY) return;
+    const float to = fmaxf(m, ml2.x), f = m == -INFINITY ? 0.f : exp2f(m - to), f2 = exp2f(ml2.x - to);
+    l = l * f + ml2.y * f2;
+    o.x = o.x * f + o2.x * f2; o.y = o.y * f + o2.y * f2; o.z = o.z * f + o2.z * f2; o.w = o.w * f + o2.w * f2;
+    m = to;
+  };
+  if (!few) {   // a row a thread, eight times four of its features at a time
+    if (tid < rows) {
+      const int from = 256 * D + 2 * tid;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D / 4; c0 += 8) {
+        float4 o[8];
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int i = 0; i < pieces; ++i) {
+          float4 v[8];
+          const float2 mi = __ldcg(reinterpret_cast<const float2*>(piece(i) + from));
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = __ldcg(reinterpret_cast<const float4*>(piece(i) + ((size_t)(c0 + k) * 256 + tid) * 4));
+          float to = m, sum = l;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            to = m; sum = l;
+            join(to, sum, o[k], mi, v[k]);
+          }
+          m = to; l = sum;
+        }
+        const float inv = 1.f / l;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) store(tid, c0 + k, make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv));
+      }
+    }
+  } else {                     // four features of a row a lane, eight pieces at a time
+    constexpr int LANES = D / 4, STEP = 256 / LANES;
+#pragma unroll 1
+    for (int q = tid / LANES; q < rows; q += STEP) {
+      const int c4 = tid % LANES;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+      for (int i0 = 0; i0 < pieces; i0 += 8) {
+        float4 v[8];
+        float2 mi[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float* const at_piece = piece(min(i0 + k, pieces - 1));
+          mi[k] = __ldcg(reinterpret_cast<const float2*>(at_piece + 256 * D + 2 * q));
+          v[k] = __ldcg(reinterpret_cast<const float4*>(at_piece + q * D + 4 * c4));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i0 + k < pieces) join(m, l, o, mi[k], v[k]);
+      }
+      const float inv = 1.f / l;
+      store(q, c4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    }
+  }
 }
 
 template <int D>
@@ -346,10 +350,10 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 int mine = 0;
 #pragma unroll
                 for (int n = 0; n < 32; ++n) {
-                    if (32 * half + n >= rows) break;
-                    const int v = __reduce_max_sync(0xffffffffu, chunk_order(s[n]));
-                    if (lane == n) mine = v;
-                  }
+                  if (32 * half + n >= rows) break;
+                  const int v = __reduce_max_sync(0xffffffffu, chunk_order(s[n]));
+                  if (lane == n) mine = v;
+                }
                 few.best[g][quad][32 * half + lane] = mine;
               }
             chunk_group_sync(g);
@@ -401,10 +405,10 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 l[32 * half + n] += s[n]; l[32 * half + n + 1] += s[n + 1]; l[32 * half + n + 2] += s[n + 2]; l[32 * half + n + 3] += s[n + 3];
                 const uint32_t w[2] = {pack_bf16(s[n], s[n + 1]), pack_bf16(s[n + 2], s[n + 3])};
 #pragma unroll
-                  for (int k = 0; k < 4; ++k)   // row n + k of the swizzled tile: 128 bytes, its 16-byte chunks in another order
-                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(sp + (32 * half + n + k) * 128 + ((chunk16 ^ ((n + k) & 7)) << 4)),
-                                 "h"((uint16_t)(k & 1 ? w[k >> 1] >> 16 : w[k >> 1])) : "memory");
-                }
+                for (int k = 0; k < 4; ++k)   // row n + k of the swizzled tile: 128 bytes, its 16-byte chunks in another order
+                  asm volatile("st.shared.u16 [%0], %1;" ::"r"(sp + (32 * half + n + k) * 128 + ((chunk16 ^ ((n + k) & 7)) << 4)),
+                               "h"((uint16_t)(k & 1 ? w[k >> 1] >> 16 : w[k >> 1])) : "memory");
+              }
             }
           if (step == tail_step) clear_tail(step, tail);
           fence_proxy_async();

@@ -17,7 +17,7 @@ int step_dims_status(const pie_step_dims* d) {
 // ---------------------------------------------------------------------------------------------------- the plan
 // Every array of the plan is a function of four sums over the requests before one (rows, pages, logit rows, cost of attention).  One launch: each CTA takes the sums of
 // all requests itself, in shared memory (at most 4096 of them), and fills its part of every array, finding a row's request by bisection.  Kilobytes: what counts is one
-// launch and the length of the chain load, scan, bisection, page id, store.  8 requests 5.8 us, 212 requests of 11700 rows 7.3, in a row of such launches; a call costs its
+// launch and the length of the chain load, scan, bisection, page id, store.  8 requests 6.0 us, 212 requests of 11700 rows 7.0, in a row of such launches; a call costs its
 // host 8.
 //
 // Attention's work is dealt out to the SMs in equal shares: items (key / value head, request, pair of query tiles) lie on a line, as long as they have keys to multiply
