@@ -5,7 +5,7 @@
 // verify_emit_kernel: each CTA of a request joins its rows' slices, finds how many drafted tokens are accepted, and takes slices of the one row behind them through the race for
 // its token; the last CTA to finish joins the slices' best.  (The joining by the last CTA of the first launch, once for a request, cost more in its tail than it saved: 39 -> 46 us.)
 // A row of 128256 logits is 257 KB: HBM at the least, but at seven instructions an exponential, all told, the issue slots are half taken, and a CTA's start and end are as long as its
-// slice.  Device time, in a row of such calls: 5 rows greedy 5.3 us, 16 x 8 12.7, 32 x 6 looked-up drafts 21.7, 64 x 6 rows against a drafter's 39.4 (3.2 TB/s).
+// slice.  Device time, in a row of such calls: 5 rows greedy 5.4 us, 16 x 8 12.8, 32 x 6 looked-up drafts 21.9, 64 x 6 rows against a drafter's 40.1 (3.1 TB/s).
 #include <algorithm>
 
 #include "pie_internal.h"
@@ -23,7 +23,7 @@ struct VerArgs {
   long long ld;
   const int32_t *draft, *starts;
   int requests, rows, vocab, most;
-  float itemp;                      // 1 / temp; greedy: 1
+  float itemp;                      // 1 / temp, at most 2^125 (times log2(e) it is finite); greedy: 1
   int greedy;
   const float *uniforms, *noise;
   int splits, emit_splits;          // slices of a row in either launch
@@ -92,14 +92,20 @@ __device__ __forceinline__ float ver_warp_max(float x) {   // of numbers, by int
   return __int_as_float(v ^ ((v >> 31) & 0x7fffffff));
 }
 // A thread's part of a row: maximum x and sum of exp2(c x + off), off = -c maximum rounded -- one fused multiply-add an exponential, and what the rounding does to all
-// of them alike (2^-24 of c x, more than a sum may be off by) is taken back at the end.  32 logits a turn; their maximum is taken in pairs of bf16, and moves the sum
-// once a turn.  Greedy: where it moves is where the first largest lies so far.
+// of them alike (2^-24 of c x, more than a sum may be off by) is taken back at the end.  Where it would do too much (steep: a maximum of thousands at an ordinary
+// temperature, a slice of nothing but the type's lowest value, a temperature near 0) the sum is of exp2(c (x - maximum)), an operation more.  32 logits a turn; their
+// maximum is taken in pairs of bf16, and moves the sum once a turn.  Greedy: where it moves is where the first largest lies so far.
 struct VerSum {
   float m = -INFINITY, off = 0.f, s = 0.f;
   int index = -1;
+  __device__ __forceinline__ bool steep() const { return fabsf(off) > 16384.f; }   // (at the border the factor is 2^(2^-11))
+  __device__ __forceinline__ float term(float x, float c) const { return x == -INFINITY ? 0.f : ver_exp2(steep() ? (x - m) * c : fmaf(x, c, off)); }
   __device__ __forceinline__ void move(float mx, float c) {
     const float to = -mx * c;
-    s = m == -INFINITY ? s : s * ver_exp2(to - off);        // (a NaN in s stays one)
+    if (m != -INFINITY) {                                    // (a NaN in s stays one)
+      if (fmaxf(fabsf(to), fabsf(off)) <= 16384.f) s *= ver_exp2(to - off);
+      else s = sum(c) * ver_exp2((m - mx) * c) * (fabsf(to) > 16384.f ? 1.f : ver_exp2(fmaf(mx, c, to)));
+    }
     m = mx;
     off = to;
   }
@@ -107,9 +113,9 @@ struct VerSum {
     x += 0.f;                                                // (-0 is 0)
     if (x > m) { move(x, c); index = i; }
     if (index < 0 && x == x) index = i;
-    s += x == -INFINITY ? 0.f : ver_exp2(fmaf(x, c, off));
+    s += term(x, c);
   }
-  __device__ __forceinline__ float sum(float c) const { return m == -INFINITY ? s : s * ver_exp2(-fmaf(m, c, off)); }   // of exp2(c (x - m))
+  __device__ __forceinline__ float sum(float c) const { return m == -INFINITY || steep() ? s : s * ver_exp2(-fmaf(m, c, off)); }   // of exp2(c (x - m))
 };
 
 // two fp32 operations an instruction
@@ -177,6 +183,16 @@ __global__ void __launch_bounds__(kVerThreads) verify_stats_kernel(const __grid_
             if (sum.index < 0 && f == sum.m && v0 + t * kVerThreads < hi) sum.index = row.head + 8 * (v0 + t * kVerThreads) + e;
           }
       }
+    }
+    if (sum.steep()) {
+#pragma unroll 1
+      for (int t = 0; t < kVerTurn; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t pair = t == 0 ? w[0][e] : t == 1 ? w[1][e] : t == 2 ? w[2][e] : w[3][e];
+          sum.s += sum.term(bf16lo(pair), c) + sum.term(bf16hi(pair), c);
+        }
+      continue;
     }
     const f32x2 c2 = v2_pack(c, c), off2 = v2_pack(sum.off, sum.off);
     f32x2 s01 = v2_pack(0.f, 0.f), s23 = s01;
@@ -284,9 +300,9 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
     const uint16_t* const g = refused && a.guess ? a.guess + (size_t)r * a.ld : nullptr;
     const int out = refused && !a.guess ? __ldg(a.draft + r) : -1;   // the token that was refused
     const float* const u = a.noise + (size_t)s * a.vocab;
-    // p = kp exp2(c x + op), as in the first launch
+    // p = exp2(c (x - maximum)) / sum
     const float2 dp = dist[0][k], dq = dist[1][k];
-    const float op = -dp.x * c, oq = -dq.x * c, kp = exp2f(-fmaf(dp.x, c, op)) / dp.y, kq = exp2f(-fmaf(dq.x, c, oq)) / dq.y;
+    const float kp = 1.f / dp.y, kq = 1.f / dq.y;
     const VerRow row = ver_row(x, a.vocab);
     const bool flat = !(reinterpret_cast<uintptr_t>(u + row.head) & 15);   // the draws can be read 16 bytes at a time as well
     // The race: of weights w and draws u, the largest w / E, E = -log(u), over turns i, i + n, ... of the row; whole: of the target's own weights.
@@ -298,8 +314,8 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
       const int not_this = whole ? -1 : out;
       unsigned long long key = 0;
       auto weight = [&](float xi, float qi) {
-        float w = __fmul_rn(ver_exp2(fmaf(xi, c, op)), kp);
-        if (q) w = __fsub_rn(w, __fmul_rn(ver_exp2(fmaf(qi, c, oq)), kq));   // (no fused form: p = q leaves nothing)
+        float w = __fmul_rn(ver_exp2((xi - dp.x) * c), kp);
+        if (q) w = __fsub_rn(w, __fmul_rn(ver_exp2((qi - dq.x) * c), kq));   // (no fused form: p = q leaves nothing)
         return w;
       };
       auto run = [&](int at) {   // exactly
@@ -395,10 +411,11 @@ static VerPlan ver_plan(int requests, int rows, int vocab) {
   VerPlan p;
   // as many slices of a row as give every SM some CTAs, all of the same power of two of turns but the last
   auto pick = [&](int units, int want) {
-    const int turns = (vocab / 8 + kVerTurn * kVerThreads - 1) / (kVerTurn * kVerThreads), most = std::max(1, turns * units / (want * 148));
-    int per = 1;
+    const int turns = (vocab / 8 + kVerTurn * kVerThreads - 1) / (kVerTurn * kVerThreads);
+    const long long most = std::max(1LL, (long long)turns * units / (want * 148));
+    long long per = 1;
     while (2 * per <= most || (turns + per - 1) / per > kVerMaxSplits) per *= 2;
-    return std::max(1, (turns + per - 1) / per);
+    return (int)std::max(1LL, (turns + per - 1) / per);
   };
   p.splits = pick(rows, 4);
   p.emit_splits = pick(requests, 3);
@@ -435,7 +452,7 @@ int pie_verify_draft(int32_t* tokens, int32_t* counts, float* logprobs, const vo
   a.logits = (const uint16_t*)logits; a.guess = (const uint16_t*)draft_logits; a.ld = ld;
   a.draft = draft_tokens; a.starts = logit_starts;
   a.requests = requests; a.rows = rows; a.vocab = vocab; a.most = max_draft;
-  a.greedy = temp == 0.f; a.itemp = a.greedy ? 1.f : 1.f / temp;
+  a.greedy = temp == 0.f; a.itemp = a.greedy ? 1.f : std::min(1.f / temp, 4.25352959e37f);
   a.uniforms = uniforms; a.noise = noise;
   a.splits = p.splits; a.emit_splits = a.greedy ? 1 : p.emit_splits;
   uint8_t* const ws = (uint8_t*)workspace;

@@ -640,7 +640,8 @@ def _head_rows(x) -> tuple:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-    return x, HeadRows(x.data_ptr(), 0, x.stride(1), x.stride(0))
+    T, H, D = x.shape   # (of one row or head the stride may be anything)
+    return x, HeadRows(x.data_ptr(), 0, x.stride(1) if H > 1 else D, x.stride(0) if T > 1 else H * D)
 
 
 def _slot_pools(what: str, k_pool, v_pool) -> KvLayout:
@@ -732,9 +733,10 @@ def chunk_attention(q, k_pool, v_pool, plan, scale: float, out=None):
         raise ValueError(f"[{what}] scale must be positive, but is {scale}")
     _check_out(what, out, (T, Hq * D))
     with _one_device(what, q, k_pool, v_pool, plan.words, *(() if out is None else (out,))):
+        L = _lib.load()
+        _step_ints(what, "plan.words", plan.words, (L.pie_step_plan_words(C.byref(d)),))
         out, rest = _fresh(out, (T, Hq * D), q.device)
         held, rows = _head_rows(q)
-        L = _lib.load()
         ws = workspaces.get("chunk", L.pie_chunk_attn_workspace_bytes(C.byref(d), D), q.device)
         _lib.check(L.pie_chunk_attn(_p(out), C.byref(rows), _p(k_pool), _p(v_pool), C.byref(lay), _p(plan.words), C.byref(d), D, float(scale), rest, _p(ws),
                                     ws.numel(), _stream()), what)
@@ -748,7 +750,8 @@ def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: fl
     p = softmax(logits / temp); q = softmax(draft_logits / temp) (bf16 [R, vocab]), or all of it on the drafted token where the drafter has no probabilities
     (draft_logits None).  In order, token x is accepted while uniforms[r] * q(x) < p(x) (f32 [R], in [0, 1)).  Behind the accepted ones comes one more, drawn by
     noise[s] (f32 [requests, vocab], in (0, 1)): the v of largest w_v / -log(noise[s, v]), w = max(p - q, 0) at a refusal, p with all accepted -- so that the
-    tokens are distributed as the target's own.  temp 0: greedy; a token is accepted if it is the first largest logit.  Filters (top-p, ...) are logits of -inf.
+    tokens are distributed as the target's own.  temp 0: greedy; a token is accepted if it is the first largest logit.  Filters (top-p, ...) are logits of -inf,
+    or of the type's lowest value.
 
     Returns (tokens int32 [requests, max_draft + 1], padded by -1; counts int32 [requests], 1 + accepted (0: a request without rows); log-probabilities f32
     [requests, max_draft + 1] of the tokens under p, padded by 0).  max_draft: at most 127; further drafts of a request are not looked at."""
@@ -786,6 +789,7 @@ def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: fl
             logits = aligned(logits)
         if draft_logits is not None and (draft_logits.stride() != logits.stride() or draft_logits.data_ptr() % 16):
             logits, draft_logits = aligned(logits), aligned(draft_logits)
+        ld = logits.stride(0) if R > 1 else vocab
         dev = logits.device
         tokens = torch.empty((S, max_draft + 1), dtype=torch.int32, device=dev)
         counts = torch.empty((S,), dtype=torch.int32, device=dev)
@@ -793,7 +797,7 @@ def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: fl
         L = _lib.load()
         # (keyed by the size of the counters' region, which has to be zero at a launch)
         ws = workspaces.get(("verify", (S * 4 + 255) // 256), L.pie_verify_workspace_bytes(S, R, vocab), dev)
-        _lib.check(L.pie_verify_draft(_p(tokens), _p(counts), _p(logprobs), _p(logits), _p(draft_logits), logits.stride(0), _p(draft_tokens), _p(logit_starts), S, R,
+        _lib.check(L.pie_verify_draft(_p(tokens), _p(counts), _p(logprobs), _p(logits), _p(draft_logits), ld, _p(draft_tokens), _p(logit_starts), S, R,
                                       vocab, max_draft, float(temp), _p(uniforms), _p(noise), _p(ws), ws.numel(), _stream()), what)
     return tokens, counts, logprobs
 

@@ -186,6 +186,8 @@ class StepPlan:
         draft_lengths int32 [S]: how many of a request's new tokens are drafted ones (fewer than its new ones).  num_logits: logit rows to make room for (default: S, none drafted).
         Lengths that do not fit one another cannot be seen from here: check() tells, and until then nothing is read or written out of bounds."""
         S = input_lengths.numel()
+        if max(S, token_ids.numel(), max_blocks, num_pages, num_heads, num_kv_heads, num_logits or 0) > 0x7fffffff:
+            raise ValueError("[StepPlan] not built here: a dimension of more than 31 bits")
         dims = _lib.StepDims(S, token_ids.numel(), S if num_logits is None else int(num_logits), int(max_blocks), int(num_pages), int(num_heads), int(num_kv_heads))
         got = ops.native_host().step_plan(token_ids, input_lengths, context_lengths, pages, draft_lengths, dims)
         if got is not None:

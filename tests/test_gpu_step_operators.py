@@ -1,5 +1,6 @@
 """The operators of a ragged step beside its plan: rotation and cache write through the slot map, attention of every request's new tokens over its pages, drafted tokens
 against the target's probabilities -- each against 64 bits, and all of them together."""
+import math
 import random
 
 import pytest
@@ -381,6 +382,50 @@ def test_filters_and_rows_without_a_distribution():
     assert ops.verify_draft(greedy, ints([7, 0]), ints([0, 2]), max_draft=1)[0].tolist() == [[7, 0]]
 
 
+@pytest.mark.parametrize("model", [False, True])
+def test_filters_of_the_lowest_value(model):
+    """A filter that writes the type's lowest value leaves what one that writes -inf does, bit for bit; a row of nothing else is flat."""
+    from proxy_inference_engine_b200 import ops
+    V, low = 40000, torch.finfo(BF).min
+    kw, starts = verify_case([3] * 8, V, 0.8, model, seed=21)
+    keep = torch.rand(V, generator=gen(6), device="cuda") < 0.001
+    keep[:100], keep[39000:] = False, False
+    results = []
+    for masked in (-torch.inf, low):
+        given = {n: torch.where(keep, kw[n], torch.tensor(masked, dtype=BF, device="cuda")) for n in ("logits", "draft_logits") if kw[n] is not None}
+        results.append(ops.verify_draft(max_draft=3, **{**kw, **given}))
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and not bool(torch.isnan(a).any())
+    assert bool(keep[results[0][0][results[0][0] >= 0].long()].all())
+    kw["logits"].fill_(low)
+    kw["uniforms"].fill_(1.0 - 2.0 ** -24)
+    tokens, counts, logprobs = ops.verify_draft(max_draft=3, **kw)
+    assert bool(((logprobs[:, 0] + math.log(V)).abs() <= 4e-6).all())
+    if not model:   # every other token is as likely, so that the largest draw has it
+        noise = kw["noise"].clone().scatter_(1, kw["draft_tokens"].view(8, 4)[:, :1].long(), 0.0)
+        assert counts.tolist() == [1] * 8 and tokens[:, 0].tolist() == noise.argmax(1).tolist()
+
+
+@pytest.mark.parametrize("temp,factor", [(1e-3, 1.0), (1e-8, 1.0), (1e-30, 1.0), (1e-42, 1.0), (1.0, 1e4), (1.0, 1e30), (0.7, 1e37)])
+@pytest.mark.parametrize("model", [False, True])
+def test_temperatures_near_0_and_logits_of_any_size_are_greedy(temp, factor, model):
+    """One logit of each row is larger than the others by 2^-3 of itself at least: p is 1 there."""
+    from proxy_inference_engine_b200 import ops
+    kw, starts = verify_case([5] * 8, 9001, 1.0, model, seed=31)
+    R = kw["logits"].shape[0]
+    best = torch.randint(0, 9001, (R,), generator=gen(32), device="cuda")
+    x = kw["logits"].float().clamp(-8, 8).scatter(1, best[:, None], 10.0)
+    kw["logits"] = (x * factor).to(BF)
+    kw["draft_tokens"] = torch.where(torch.rand(R, generator=gen(33), device="cuda") < 0.6, best, (best + 1) % 9001).to(torch.int32)
+    if model:
+        kw["draft_logits"] = (x.scatter(1, kw["draft_tokens"][:, None].long(), 13.0) * factor).to(BF)
+    kw["temp"] = temp
+    got = ops.verify_draft(max_draft=5, **kw)
+    want = ops.verify_draft(kw["logits"], kw["draft_tokens"], kw["logit_starts"], max_draft=5)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert 0 < int((want[1] > 1).sum()) and bool((got[2] == 0).all())
+
+
 def test_tokens_outside_the_vocabulary_and_starts_outside_the_rows():
     from proxy_inference_engine_b200 import ops
     kw, starts = verify_case([2, 2, 2], 900, 0.8, False, seed=2)
@@ -568,6 +613,30 @@ def test_the_native_host_form_is_the_python_one(monkeypatch):
     assert len(native) == len(python)
     for i, (a, b) in enumerate(zip(native, python)):
         assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride() and torch.equal(a.view(torch.int16) if a.dtype == BF else a, b.view(torch.int16) if b.dtype == BF else b), i
+
+
+@pytest.mark.parametrize("stride", [0, 1, 24])
+def test_one_row_of_any_stride(stride):
+    """The stride of a dimension of one is anything at all."""
+    import dataclasses
+    from proxy_inference_engine_b200 import ops
+    from proxy_inference_engine_b200.ragged import StepPlan
+    Hq, Hkv, D, V = 4, 2, 64, 4001
+    pools = [torch.randn((4, 64, Hkv, D), generator=gen(1), device="cuda").to(BF) for _ in range(2)]
+    q, k, v = (torch.randn((1, H, D), generator=gen(2), device="cuda").to(BF) for H in (Hq, Hkv, Hkv))
+    freqs = torch.linspace(1.0, 9.0, D // 2, device="cuda")
+    plan = StepPlan.build(ints([1]), ints([1]), ints([70]), ints([2, 1]), num_pages=4, max_blocks=2, num_heads=Hq, num_kv_heads=Hkv)
+    odd = lambda x: x.as_strided(x.shape, (stride, *x.stride()[1:]))
+    other = [p.clone() for p in pools]
+    got = ops.rope_kv_slots(odd(q), odd(k), odd(v), freqs, plan.positions, plan.slots, *pools)
+    want = ops.rope_kv_slots(q, k, v, freqs, plan.positions, plan.slots, *other)
+    assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(pools, other))
+    assert torch.equal(ops.chunk_attention(odd(q), *pools, plan, 0.125), ops.chunk_attention(q, *pools, plan, 0.125))
+    x = torch.randn((1, V), generator=gen(3), device="cuda").to(BF)
+    for a, b in zip(*(ops.verify_draft(t, ints([-1]), ints([0, 1]), max_draft=0) for t in (odd(x), x))):
+        assert torch.equal(a, b)
+    with pytest.raises(ValueError, match="plan.words"):
+        ops.chunk_attention(q, *pools, dataclasses.replace(plan, words=plan.words[:-4].clone()), 0.125)
 
 
 def test_a_planned_step_refuses():
