@@ -315,7 +315,7 @@ int pie_rope_kv_slots(void* q_out, void* kpool, void* vpool, const pie_kv_layout
                       const int32_t* positions, const int32_t* slots, const float* freqs, int rows, int pages, int Hq, int Hkv, int D, int rest, void* stream);
 
 /* Causal attention of every request's new tokens over its pages, which hold them already: row t of out [rows, Hq * D] is
- * softmax(scale q_t . K[0 .. position t]) V of its request.  scale > 0.  q as above.  rest: rows behind the last request's are set to zero (1) or left as they are (0).
+ * softmax(scale q_t . K[0 .. position t]) V of its request.  scale > 0; scores (scale q . K) up to 2^30.  q as above.  rest: rows behind the last request's are set to zero (1) or left as they are (0).
  * Workspace: pie_chunk_attn_workspace_bytes() bytes, ZEROED ONCE at allocation (counters are left at zero), for launches that come one after the other. */
 size_t pie_chunk_attn_workspace_bytes(const pie_step_dims* dims, int D);
 int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const void* vpool, const pie_kv_layout* kv_host, const int32_t* plan,
@@ -328,7 +328,7 @@ int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const v
  * is accepted if it is the first largest logit, which is what comes behind; p = softmax(logits) is for the log-probabilities alone, and uniforms and noise are not read.
  * tokens int32 [requests, max_draft + 1]: accepted ones, that one, -1; counts int32 [requests]: how many; logprobs f32 [requests, max_draft + 1]: log p of
  * each, 0 behind them.  A request without rows gets none; of one with more than max_draft + 1 the first max_draft + 1 count (max_draft <= 127).  A drafted token
- * outside the vocabulary is refused.  -inf logits are tokens that cannot be; a row with a NaN, +inf or nothing else has no distribution: it refuses its
+ * outside the vocabulary is refused.  -inf logits are tokens that cannot be (a draw in noise of 0 counts as the smallest number, a temp below 2^-125 as that); a row with a NaN, +inf or nothing else has no distribution: it refuses its
  * token, and what comes behind is token 0 (temp 0: NaN is passed over).  Workspace: as pie_chunk_attn's. */
 size_t pie_verify_workspace_bytes(int requests, int rows, int vocab);
 int pie_verify_draft(int32_t* tokens, int32_t* counts, float* logprobs, const void* logits, const void* draft_logits, long long ld, const int32_t* draft_tokens,

@@ -292,7 +292,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (p.kind == CHUNK_FEW) {
         // ---------------------------------------------------------------------------------- a key a lane, a row a column
         const int rows = p.tokens * a.G;
-        const int cut0 = (p.k0 * 128 + r - p.pos0) * a.G, edge_step = (p.pos0 + 1) / 128 - p.k0;   // the first key tile with a key that some row must not see
+        const int beyond = p.k0 * 128 + r - p.pos0, edge_step = (p.pos0 + 1) / 128 - p.k0;   // the first key tile with a key that some row must not see
         const uint32_t sp = smQ1 + g * T::P + (r >> 6) * 8192 + (r & 7) * 2;
         const int chunk16 = (r & 63) >> 3;
         float l[kChunkFew];
@@ -309,7 +309,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             if (32 * half + 16 < rows) chunk_ld16(tS + 32 * half + 16, s + 16);
             tmem_ld_wait();
             if (step >= edge_step) {
-              const int cut = cut0 + step * 128 * a.G - 32 * half;
+              const int cut = (beyond + step * 128) * a.G - 32 * half;   // (a key that far beyond the first row's own: the place in the cache times G may not fit)
 #pragma unroll
               for (int n = 0; n < 32; ++n)
                 if (n < cut) s[n] = -INFINITY;
