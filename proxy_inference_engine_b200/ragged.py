@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from dataclasses import dataclass, field
 
 import torch
@@ -148,6 +149,9 @@ class BatchDetails:
         return self.consolidated_block_table[seq_of_token].contiguous()
 
 
+_DIMS = struct.Struct("7i").pack   # pie_step_dims
+
+
 @dataclass
 class StepPlan:
     """A ragged step described on the device: BatchDetails for callers whose requests' lengths live there -- after drafted tokens were verified, or in a captured
@@ -186,9 +190,10 @@ class StepPlan:
         draft_lengths int32 [S]: how many of a request's new tokens are drafted ones (fewer than its new ones).  num_logits: logit rows to make room for (default: S, none drafted).
         Lengths that do not fit one another cannot be seen from here: check() tells, and until then nothing is read or written out of bounds."""
         S = input_lengths.numel()
-        if max(S, token_ids.numel(), max_blocks, num_pages, num_heads, num_kv_heads, num_logits or 0) > 0x7fffffff:
-            raise ValueError("[StepPlan] not built here: a dimension of more than 31 bits")
-        dims = _lib.StepDims(S, token_ids.numel(), S if num_logits is None else int(num_logits), int(max_blocks), int(num_pages), int(num_heads), int(num_kv_heads))
+        try:   # (packed, since a ctypes field takes what does not fit it modulo 2^32)
+            dims = _lib.StepDims.from_buffer_copy(_DIMS(S, token_ids.numel(), S if num_logits is None else num_logits, max_blocks, num_pages, num_heads, num_kv_heads))
+        except struct.error as e:
+            raise ValueError(f"[StepPlan] not built here: numbers of anything have to be integers of 31 bits ({e})") from None
         got = ops.native_host().step_plan(token_ids, input_lengths, context_lengths, pages, draft_lengths, dims)
         if got is not None:
             return cls(token_ids, got[0], dims, *got[1:])

@@ -69,7 +69,7 @@ def _plan(**kw):
 @pytest.mark.parametrize("kw", [
     dict(), dict(token_ids=torch.tensor([1, 2, 3])), dict(token_ids=ints()), dict(token_ids=ints(1, 2).view(1, 2)), dict(input_lengths=ints(1)), dict(context_lengths=ints(1)),
     dict(pages=torch.tensor([1, 2])), dict(pages=ints(1, 2, 3).view(3, 1)), dict(draft_lengths=ints(0)), dict(num_heads=3), dict(max_blocks=0), dict(num_pages=0), dict(num_logits=0),
-    dict(num_pages=(1 << 32) + 4), dict(max_blocks=(1 << 32) + 2), dict(num_logits=(1 << 32) + 2), dict(input_lengths=torch.tensor([[1, 2], [3, 4]], dtype=torch.int32).t()[0])])
+    dict(num_pages=(1 << 32) + 4), dict(max_blocks=(1 << 32) + 2), dict(num_logits=(1 << 32) + 2), dict(num_heads=4.0), dict(input_lengths=torch.tensor([[1, 2], [3, 4]], dtype=torch.int32).t()[0])])
 def test_plan_refuses(kw):
     refuses(_plan, kw)
 
