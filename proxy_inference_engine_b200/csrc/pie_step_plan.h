@@ -1,4 +1,4 @@
-// A ragged step's plan: one buffer of 32-bit words on the device, laid out by what its dimensions are (pie_ragged.cu writes it, pie_chunk_attn.cu and
+// A ragged step's plan: one buffer of 32-bit words on the device, laid out by what its dimensions are (pie_ragged.cu writes it, pie_chunk_attn.cuh and
 // the callers read it).  Nothing here is part of the public ABI but the words' order, which pie_step_plan_offsets tells.
 #pragma once
 #include "pie_internal.h"
