@@ -329,7 +329,8 @@ int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const v
  * tokens int32 [requests, max_draft + 1]: accepted ones, that one, -1; counts int32 [requests]: how many; logprobs f32 [requests, max_draft + 1]: log p of
  * each, 0 behind them.  A request without rows gets none; of one with more than max_draft + 1 the first max_draft + 1 count (max_draft <= 127).  A drafted token
  * outside the vocabulary is refused.  -inf logits are tokens that cannot be (a draw in noise of 0 counts as the smallest number, a temp below 2^-125 as that); a row with a NaN, +inf or nothing else has no distribution: it refuses its
- * token, and what comes behind is token 0 (temp 0: NaN is passed over).  Workspace: as pie_chunk_attn's. */
+ * token, and what comes behind is token 0 (temp 0: NaN is passed over).  Workspace: pie_verify_workspace_bytes() bytes, 16-byte aligned, for launches that come one after the
+ * other; what it holds does not matter. */
 size_t pie_verify_workspace_bytes(int requests, int rows, int vocab);
 int pie_verify_draft(int32_t* tokens, int32_t* counts, float* logprobs, const void* logits, const void* draft_logits, long long ld, const int32_t* draft_tokens,
                      const int32_t* logit_starts, int requests, int rows, int vocab, int max_draft, float temp, const float* uniforms, const float* noise,

@@ -517,7 +517,7 @@ PyObject* verify_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!dev) return nullptr;
   at::Tensor ws;
   const size_t need = lib.pie_verify_workspace_bytes((int)S, (int)R, (int)V);
-  if (const Answer a = buffer(Py_BuildValue("((sn)nO)", "verify", (Py_ssize_t)((S * 4 + 255) / 256), (Py_ssize_t)need, dev.get()), args[8], ws)) {
+  if (const Answer a = buffer(Py_BuildValue("(snO)", "verify", (Py_ssize_t)need, dev.get()), args[8], ws)) {
     if (a == FAILED) return nullptr;
     Py_RETURN_NONE;
   }

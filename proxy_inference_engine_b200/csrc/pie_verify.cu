@@ -29,7 +29,7 @@ struct VerArgs {
   int splits, emit_splits;          // slices of a row in either launch
   float* stats;                     // [rows][2][splits][4]: maximum, sum of exp, index of the maximum (greedy)
   unsigned long long* best;         // [requests][emit_splits]
-  unsigned int* count;              // [requests], zero between launches
+  unsigned int* count;              // [requests], set to zero by the first launch for the second
 };
 
 // larger keys are larger scores, of equal scores the lower index; 0: none
@@ -143,6 +143,9 @@ __global__ void __launch_bounds__(kVerThreads) verify_stats_kernel(const __grid_
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
+  // (Here, and not by the last CTA to count: where the counters lie depends on the call, and a call of another shape may have left numbers there.)
+  if (blockIdx.x == 0 && r == 0 && !which)
+    for (int i = tid; i < a.requests; i += kVerThreads) a.count[i] = 0;
   if (which) {   // a request's last row judges no token: its draft's logits are not read
     bool last = false;
     for (int i = tid; i < a.requests; i += kVerThreads) last = last || __ldg(a.starts + i + 1) == r + 1;
@@ -382,7 +385,6 @@ __global__ void __launch_bounds__(kVerThreads) verify_emit_kernel(const __grid_c
         unsigned int before;
         asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.count + s) : "memory");
         s_last = before == (unsigned)a.emit_splits - 1;
-        if (s_last) a.count[s] = 0;
       }
       __syncthreads();
       if (!s_last) return;

@@ -796,8 +796,7 @@ def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: fl
         counts = torch.empty((S,), dtype=torch.int32, device=dev)
         logprobs = torch.empty((S, max_draft + 1), dtype=torch.float32, device=dev)
         L = _lib.load()
-        # (keyed by the size of the counters' region, which has to be zero at a launch)
-        ws = workspaces.get(("verify", (S * 4 + 255) // 256), L.pie_verify_workspace_bytes(S, R, vocab), dev)
+        ws = workspaces.get("verify", L.pie_verify_workspace_bytes(S, R, vocab), dev)
         _lib.check(L.pie_verify_draft(_p(tokens), _p(counts), _p(logprobs), _p(logits), _p(draft_logits), ld, _p(draft_tokens), _p(logit_starts), S, R,
                                       vocab, max_draft, float(temp), _p(uniforms), _p(noise), _p(ws), ws.numel(), _stream()), what)
     return tokens, counts, logprobs

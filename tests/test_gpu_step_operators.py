@@ -437,6 +437,26 @@ def test_tokens_outside_the_vocabulary_and_starts_outside_the_rows():
         assert all(0 <= c <= 3 for c in counts.tolist())
 
 
+def test_one_workspace_for_calls_of_all_shapes():
+    """What a call leaves in it does not reach the next one, whose counters lie where others' sums did; nor does what was there before the first."""
+    from proxy_inference_engine_b200 import _lib, ops
+    L, V = _lib.load(), 50000
+    ptr = lambda t: None if t is None else t.data_ptr()
+
+    def call(kw, S, R, ws):
+        out = torch.full((S, 2), -7, dtype=torch.int32, device="cuda"), torch.full((S,), -7, dtype=torch.int32, device="cuda"), torch.full((S, 2), 9.0, device="cuda")
+        _lib.check(L.pie_verify_draft(*map(ptr, out), ptr(kw["logits"]), ptr(kw["draft_logits"]), V, ptr(kw["draft_tokens"]), ptr(kw["logit_starts"]), S, R, V, 1, kw["temp"],
+                                      ptr(kw["uniforms"]), ptr(kw["noise"]), ptr(ws), ws.numel(), ops._stream()), "verify_draft")
+        return out
+    most = L.pie_verify_workspace_bytes(300, 600, V)
+    shared = torch.full((most,), 0x5A, dtype=torch.uint8, device="cuda")
+    for S in (64, 65, 300, 1, 65):
+        kw, _ = verify_case([1] * S, V, 0.8, True, seed=S)
+        got, want = call(kw, S, 2 * S, shared), call(kw, S, 2 * S, torch.zeros_like(shared))
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and bool((got[1] > 0).all())
+        assert all(torch.equal(a, b) for a, b in zip(got, ops.verify_draft(max_draft=1, **kw)))
+
+
 def test_draws_follow_the_target():
     """Drafts from q, verified against p: the first token behind them is distributed as p.  4000 draws of 6 tokens: five standard deviations."""
     from proxy_inference_engine_b200 import ops
