@@ -327,7 +327,8 @@ int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const v
  * w_v / -log(noise[s, v]), w = max(p - q, 0) (p where that is nowhere positive), and with all accepted of w = p; the lowest index where two are largest.  temp 0: greedy, a token
  * is accepted if it is the first largest logit, which is what comes behind; p = softmax(logits) is for the log-probabilities alone, and uniforms and noise are not read.
  * tokens int32 [requests, max_draft + 1]: accepted ones, that one, -1; counts int32 [requests]: how many; logprobs f32 [requests, max_draft + 1]: log p of
- * each, 0 behind them.  A request without rows gets none; of one with more than max_draft + 1 the first max_draft + 1 count (max_draft <= 127).  A drafted token
+ * each, 0 behind them.  A request without rows gets none (starts have to rise; the answers of those
+ * that do not mean nothing, and are made of the inputs alone); of one with more than max_draft + 1 the first max_draft + 1 count (max_draft <= 127).  A drafted token
  * outside the vocabulary is refused.  -inf logits are tokens that cannot be (a draw in noise of 0 counts as the smallest number, a temp below 2^-125 as that); a row with a NaN, +inf or nothing else has no distribution: it refuses its
  * token, and what comes behind is token 0 (temp 0: NaN is passed over).  Workspace: pie_verify_workspace_bytes() bytes, 16-byte aligned, for launches that come one after the
  * other; what it holds does not matter. */

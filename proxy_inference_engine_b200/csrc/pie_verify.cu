@@ -149,7 +149,11 @@ __global__ void __launch_bounds__(kVerThreads) verify_stats_kernel(const __grid_
   if (which) {   // a request's last row judges no token: its draft's logits are not read
     bool last = false;
     for (int i = tid; i < a.requests; i += kVerThreads) last = last || __ldg(a.starts + i + 1) == r + 1;
-    if (__syncthreads_or(last)) return;
+    if (__syncthreads_or(last)) {   // (where starts do not rise, another request may judge its token all the same: without a distribution, as it finds here, it refuses it)
+      if (tid == 0)
+        *reinterpret_cast<float4*>(a.stats + (((size_t)r * 2 + 1) * a.splits + blockIdx.x) * 4) = make_float4(-INFINITY, __int_as_float(0x7fffffff), 0.f, 0.f);
+      return;
+    }
   }
   const VerRow row = ver_row((which ? a.guess : a.logits) + (size_t)r * a.ld, a.vocab);
   const float c = a.itemp * 1.4426950408889634f;

@@ -457,6 +457,23 @@ def test_one_workspace_for_calls_of_all_shapes():
         assert all(torch.equal(a, b) for a, b in zip(got, ops.verify_draft(max_draft=1, **kw)))
 
 
+def test_starts_that_do_not_rise_meet_no_other_calls_sums():
+    """A row that is one request's last and lies within another: what a call before this one left of its draft's logits does not matter."""
+    from proxy_inference_engine_b200 import ops
+    kw, _ = verify_case([5], 9000, 0.8, True, seed=1)
+    kw["logit_starts"], kw["noise"], kw["uniforms"] = ints([0, 3, 2, 6]), torch.rand((3, 9000), generator=gen(2), device="cuda"), torch.full((6,), 0.5, device="cuda")
+    results = []
+    for level in (0.0, 40.0):
+        other, _ = verify_case([5], 9000, 0.8, True, seed=2)
+        other["logit_starts"], other["noise"] = ints([0, 1, 2, 6]), torch.rand((3, 9000), generator=gen(3), device="cuda")
+        other["draft_logits"].fill_(level)
+        ops.verify_draft(max_draft=5, **other)
+        results.append(ops.verify_draft(max_draft=5, **kw))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert results[0][1].tolist()[1:] == [0, 1]      # (and refuses its token)
+
+
 def test_draws_follow_the_target():
     """Drafts from q, verified against p: the first token behind them is distributed as p.  4000 draws of 6 tokens: five standard deviations."""
     from proxy_inference_engine_b200 import ops
