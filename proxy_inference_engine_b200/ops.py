@@ -756,7 +756,10 @@ def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: fl
 
     Returns (tokens int32 [requests, max_draft + 1], padded by -1; counts int32 [requests], 1 + accepted (0: a request without rows); log-probabilities f32
     [requests, max_draft + 1] of the tokens under p, padded by 0).  max_draft: at most 127; further drafts of a request are not looked at."""
-    got = native_host().verify_draft(logits, draft_tokens, logit_starts, max_draft, float(temp), uniforms, noise, draft_logits, workspaces.get)
+    temp = float(temp)
+    if 0 < temp < 1e-38:   # (as a 32-bit number it might be 0, which is another thing)
+        temp = 1e-38
+    got = native_host().verify_draft(logits, draft_tokens, logit_starts, max_draft, temp, uniforms, noise, draft_logits, workspaces.get)
     if got is not None:
         return got
     what = "verify_draft"
@@ -798,7 +801,7 @@ def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: fl
         L = _lib.load()
         ws = workspaces.get("verify", L.pie_verify_workspace_bytes(S, R, vocab), dev)
         _lib.check(L.pie_verify_draft(_p(tokens), _p(counts), _p(logprobs), _p(logits), _p(draft_logits), ld, _p(draft_tokens), _p(logit_starts), S, R,
-                                      vocab, max_draft, float(temp), _p(uniforms), _p(noise), _p(ws), ws.numel(), _stream()), what)
+                                      vocab, max_draft, temp, _p(uniforms), _p(noise), _p(ws), ws.numel(), _stream()), what)
     return tokens, counts, logprobs
 
 

@@ -426,6 +426,19 @@ def test_temperatures_near_0_and_logits_of_any_size_are_greedy(temp, factor, mod
     assert 0 < int((want[1] > 1).sum()) and bool((got[2] == 0).all())
 
 
+@pytest.mark.parametrize("model", [False, True])
+@pytest.mark.parametrize("native", [True, False])
+def test_a_temperature_that_32_bits_do_not_hold_is_none_of_0(model, native, monkeypatch):
+    """It is a draw at the lowest temperature there is, log-probabilities included, and not a greedy answer, whose log-probabilities are the model's own."""
+    from proxy_inference_engine_b200 import ops
+    if not native:
+        monkeypatch.setattr(ops, "native_host", lambda: ops._NoHost)
+    kw, _ = verify_case([5] * 4, 9001, 1.0, model, seed=41)
+    want = ops.verify_draft(max_draft=5, **{**kw, "temp": 1e-42})
+    for temp in (1e-50, 5e-324):
+        assert all(torch.equal(a, b) for a, b in zip(ops.verify_draft(max_draft=5, **{**kw, "temp": temp}), want))
+
+
 def test_tokens_outside_the_vocabulary_and_starts_outside_the_rows():
     from proxy_inference_engine_b200 import ops
     kw, starts = verify_case([2, 2, 2], 900, 0.8, False, seed=2)
