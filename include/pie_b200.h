@@ -284,7 +284,7 @@ int pie_sample(int32_t* tokens, const void* logits, int rows, int vocab, int ld,
  * The reference declares the descriptor of such a step (BatchDetails, CORE/include/engine/batch_details.hpp:10-90) and no kernel that
  * reads it.  Lengths, page ids and plan are DEVICE memory, so that a captured step runs again on other lengths; the host knows the
  * dimensions below, which are upper bounds: rows behind the last request's belong to nobody.
- *   requests <= 4096, rows >= 1, logit_rows >= 1 (rows whose logits are wanted), blocks (of a row of the block table), pages (of the pools, 64 tokens each),
+ *   requests <= 4096, rows >= 1, logit_rows >= 1 (rows whose logits are wanted), blocks (of a row of the block table, 64 tokens each: below 2^31 - 1024 in all), pages (of the pools, 64 tokens each),
  *   Hq / Hkv <= 128.
  * pie_step_plan_build fills a plan of pie_step_plan_words() 32-bit words, 16-byte aligned, whose parts begin at the words that pie_step_plan_offsets gives:
  *   0 row_starts [requests + 1]   first row of each request          1 contexts [requests]          tokens it has in the cache

@@ -9,7 +9,7 @@ int step_dims_status(const pie_step_dims* d) {
   if (!d) return PIE_ENULL;
   if (d->requests < 1 || d->requests > kStepMaxRequests || d->rows < 1 || d->logit_rows < 1 || d->blocks < 1 || d->pages < 1 || d->Hq < 1 || d->Hkv < 1 ||
       d->Hq % d->Hkv || d->Hq / d->Hkv > kStepTile || (long long)d->requests * d->blocks > 0x7fffffff || (long long)d->pages * kStepPage > 0x7fffffff ||
-      (long long)d->blocks * kStepPage > 0x7fffffff || (long long)d->rows * d->Hq > 0x7fffffff || step_layout(*d).items > 0x3fffffff)
+      (long long)d->blocks * kStepPage > 0x7fffffff - kStepRoom || (long long)d->rows * d->Hq > 0x7fffffff || step_layout(*d).items > 0x3fffffff)
     return PIE_EINVAL_SHAPE;
   return PIE_OK;
 }
@@ -35,6 +35,7 @@ struct PlanArgs {
 constexpr int kPlanThreads = 512;
 constexpr int kCostPair = 2, kCostTile = 1;   // a key of an item with rows in both query tiles, in one (powers of two)
 constexpr int kCostItem = 576;                // queries in, results out (256: a step of three prompts and 29 answers 85 us, 81 with this)
+static_assert(kCostItem < kStepRoom && kStepTile < kStepRoom, "added to keys in 32 bits");
 constexpr long long kCostShare = 512;         // least share worth a CTA; without pairs of query tiles, whose keys are sooner read than added up in pieces, twice that
 static_assert(kCostTile * kStepTile == 1 << 7 && kCostPair * kStepTile == 1 << 8, "key tiles are counted by shifts");
 constexpr int kCutPair = 4, kCutTile = 2;     // least key tiles of a piece: what it costs to leave a piece's results and to add them up

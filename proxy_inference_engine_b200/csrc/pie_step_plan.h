@@ -10,6 +10,7 @@ constexpr int kStepMaxRequests = 4096; // the scans of a step's lengths are held
 constexpr int kStepMaxCtas = 192;      // CTAs that the attention's work is dealt out to, at most
 constexpr int kStepTile = 128;         // rows of a query tile, keys of a key tile
 constexpr int kStepPieceWords = 12;
+constexpr int kStepRoom = 1024;        // what is added to a number of keys in 32 bits (a tile, an item's cost) is less
 
 // One CTA's share of an item of attention: some of the key tiles of up to two query tiles of one key / value head of one request.  A query tile's rows are
 // its tokens' query heads of that key / value head, token by token.

@@ -34,6 +34,13 @@ def test_dimensions(kw):
     assert L.pie_step_plan_offsets(C.byref(d), (C.c_longlong * 10)()) == 1
 
 
+@pytest.mark.parametrize("blocks,fits", [((2 ** 31 - 1) // 64, False), ((2 ** 31 - 1025) // 64 + 1, False), ((2 ** 31 - 1025) // 64, True)])
+def test_positions_leave_room_for_a_tile_behind_them(blocks, fits):
+    """A request of as many keys as its row of the table holds: what is added to them -- a tile, an item's cost -- has to fit 32 bits."""
+    assert (_lib.load().pie_step_plan_words(C.byref(_dims(blocks=blocks))) > 0) == fits
+    assert not fits or blocks * 64 + 1024 <= 2 ** 31 - 1
+
+
 def test_offsets_are_apart_and_aligned():
     L, d, at = _lib.load(), _dims(requests=3, rows=11, logit_rows=5), (C.c_longlong * 10)()
     assert L.pie_step_plan_offsets(C.byref(d), at) == 0
