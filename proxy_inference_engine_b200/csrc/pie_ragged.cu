@@ -154,14 +154,14 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     for (int s = s0; s < s1; ++s) {
       const int n = row[s + 1] - row[s];
       kind |= (n > a.l.tile_tokens ? 1 : 0) | (n > 0 && ctx[s] + n + kCostItem > 2 * kCostShare ? 2 : 0);
-      logit[s] = (int)min(v[0], (long long)a.d.logit_rows);
+      logit[s] = (int)v[0];   // (at most T; what lies behind the last logit row is cut off below)
       item[s] = (int)v[1];
       cost[s] = v[2];
       add(s, v);
       if (v[0] > a.d.logit_rows) fault |= PIE_STEP_LOGITS;
     }
     if (kind) atomicOr(&kinds, kind);
-    if (s0 < S && s1 == S) { logit[S] = (int)min(v[0], (long long)a.d.logit_rows); item[S] = (int)v[1]; cost[S] = v[2]; }
+    if (s0 < S && s1 == S) { logit[S] = (int)v[0]; item[S] = (int)v[1]; cost[S] = v[2]; }
   }
   __syncthreads();
 
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
   };
   for (int s = first; s <= S; s += step) {
     w[a.l.row_starts + s] = row[s];
-    w[a.l.logit_starts + s] = logit[s];
+    w[a.l.logit_starts + s] = min(logit[s], a.d.logit_rows);
     if (s < S) w[a.l.contexts + s] = ctx[s];
   }
   auto do_row = [&](int t) {
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     if (r < logit[S]) {
       const int s = last_at_or_below(logit, S, r), left = logit[s + 1] - 1 - r;
       of = row[s + 1] - 1 - left;
-      if (left > 0) token = __ldg(a.ids + of + 1);
+      if (left > 0 && r + 1 < a.d.logit_rows) token = __ldg(a.ids + of + 1);   // (a row that is the last one because of the cut judges none)
     }
     w[a.l.logit_rows + r] = of;
     w[a.l.draft_tokens + r] = token;

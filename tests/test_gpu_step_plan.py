@@ -153,6 +153,21 @@ def test_what_does_not_fit_is_told_and_stays_in_bounds(text, kw):
     schedule_is_whole(plan)
 
 
+@pytest.mark.parametrize("rows", range(1, 9))
+def test_logit_rows_that_do_not_fit_are_cut_off_at_the_end(rows):
+    """What is left is what it would have been: a request's first drafts, judged in order, and none behind an unjudged one."""
+    plan = _build([9, 3], [0, 0], [1, 2], drafted=[4, 2], num_logits=rows)
+    assert plan.logit_rows.tolist() == [4, 5, 6, 7, 8, 9, 10, 11][:rows] and plan.logit_starts.tolist() == [0, min(rows, 5), rows if rows > 5 else min(rows, 5)]
+    want = [5, 6, 7, 8, -1, 10, 11, -1][:rows]
+    want[-1] = -1
+    assert plan.draft_tokens.tolist() == want
+    if rows < 8:
+        with pytest.raises(ValueError, match="more logit rows"):
+            plan.check()
+    else:
+        plan.check()
+
+
 def test_a_table_that_is_too_narrow():
     plan = _build([9, 3], [60, 0], ints([[1], [2]]))
     with pytest.raises(ValueError, match="more pages than"):
