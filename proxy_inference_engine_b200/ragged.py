@@ -243,10 +243,16 @@ def _planned_step(model, plan: StepPlan, pools, all_logits: bool) -> torch.Tenso
         raise ValueError("[ragged_step] a StepPlan is for one GPU's whole model with rotation by halves")
     if len(pools) != len(model.layers):
         raise ValueError(f"[ragged_step] {len(pools)} pools for {len(model.layers)} layers")
-    h = model.model.embed_tokens(plan.token_ids[None])
-    for ly, (kp, vp) in zip(model.layers, pools):
+    d = plan.dims   # (all of it before the first layer writes to its pools: slots of another plan's pools are other requests' places)
+    for kp, vp in pools:
         if isinstance(kp, (tuple, list)):
             raise ValueError("[ragged_step] a StepPlan's attention reads bfloat16 pools; 8-bit pools are for BatchDetails")
+        ops._slot_pools("ragged_step", kp, vp)
+        if (d.Hq, d.Hkv, d.pages) != (Hq, Hkv, kp.shape[0]) or kp.shape[2:] != (Hkv, D):
+            raise ValueError(f"[ragged_step] the plan is for {d.Hq} heads over {d.pages} pages of {d.Hkv} heads, but the model has {Hq} over {Hkv} of {D} features and a pool is "
+                             f"{tuple(kp.shape)}")
+    h = model.model.embed_tokens(plan.token_ids[None])
+    for ly, (kp, vp) in zip(model.layers, pools):
         at = ly.self_attn
         x = ly.input_layernorm(h)
         q = ops.rope_kv_slots(at.q_proj(x).view(T, Hq, D), at.k_proj(x).view(T, Hkv, D), at.v_proj(x).view(T, Hkv, D), at.rope._freqs, plan.positions, plan.slots, kp, vp)

@@ -689,6 +689,24 @@ def test_one_row_of_any_stride(stride):
         ops.chunk_attention(q, *pools, dataclasses.replace(plan, words=plan.words[:-4].clone()), 0.125)
 
 
+def test_a_planned_step_that_is_refused_writes_nothing():
+    """A plan of other heads or pools, and pools of which the last layer's do not fit: the first layer's are left as they were."""
+    from proxy_inference_engine_b200.ragged import StepPlan, ragged_step
+    args, w, model, mk = _model(64)
+    Hq, Hkv = args.num_attention_heads, args.num_key_value_heads
+    plan_of = lambda pages, hq, hkv: StepPlan.build(ints([1]), ints([1]), ints([0]), ints([0]), num_pages=pages, max_blocks=1, num_heads=hq, num_kv_heads=hkv)
+    pools = [tuple(torch.zeros_like(t) for t in pair) for pair in mk()]
+    short, eights = [(k[:39], v[:39]) for k, v in pools], [((k,), (v,)) for k, v in pools]
+    for plan, given, match in ((plan_of(39, Hq, Hkv), pools, "the plan is for"), (plan_of(40, 2 * Hq, Hkv), pools, "the plan is for"), (plan_of(40, Hq, Hq), pools, "the plan is for"),
+                               (plan_of(40, Hq, Hkv), pools[:-1] + short[-1:], "the plan is for"), (plan_of(40, Hq, Hkv), pools[:-1] + eights[-1:], "8-bit"),
+                               (plan_of(40, Hq, Hkv), pools[:-1] + [(pools[-1][0], pools[-1][1].float())], "bfloat16")):
+        with pytest.raises(ValueError, match=match):
+            ragged_step(model, plan, given)
+    assert not any(bool(t.any()) for pair in pools for t in pair)
+    ragged_step(model, plan_of(40, Hq, Hkv), pools)
+    assert all(bool(t[0, 0].any()) for pair in pools for t in pair)
+
+
 def test_a_planned_step_refuses():
     from proxy_inference_engine_b200.ragged import StepPlan, ragged_step
     args, w, model, mk = _model(64)
