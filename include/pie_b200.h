@@ -315,7 +315,8 @@ int pie_rope_kv_slots(void* q_out, void* kpool, void* vpool, const pie_kv_layout
                       const int32_t* positions, const int32_t* slots, const float* freqs, int rows, int pages, int Hq, int Hkv, int D, int rest, void* stream);
 
 /* Causal attention of every request's new tokens over its pages, which hold them already: row t of out [rows, Hq * D] is
- * softmax(scale q_t . K[0 .. position t]) V of its request.  scale > 0; scores (scale q . K) up to 2^30.  q as above.  rest: rows behind the last request's are set to zero (1) or left as they are (0).
+ * softmax(scale q_t . K[0 .. position t]) V of its request.  scale > 0; scores (scale q . K) up to 2^30.  Weights are rounded to 16 bits for their
+ * product with V where a request's rows x Hq / Hkv are at most 64 (48 at D 128), to bf16 otherwise.  q as above.  rest: rows behind the last request's are set to zero (1) or left as they are (0).
  * Workspace: pie_chunk_attn_workspace_bytes() bytes, ZEROED ONCE at allocation (counters are left at zero), for launches that come one after the other. */
 size_t pie_chunk_attn_workspace_bytes(const pie_step_dims* dims, int D);
 int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const void* vpool, const pie_kv_layout* kv_host, const int32_t* plan,

@@ -6,20 +6,25 @@
 // The rows of a query tile are the query heads of one key / value head, token by token (32 tokens of 4 heads): keys and values are read once for all of them, and a tile
 // of few tokens crosses the diagonal in few key tiles.  An item (pie_step_plan.h) is of one of three kinds:
 //   * pair: rows in both query tiles.  They walk the same key tiles, one tile's softmax under the other's MMAs, as in the prompt's kernel -- bound by softmax and tensor pipe.
-//   * one tile of more than 64 rows: the groups take every other key tile of it, each with its own maximum, sum and accumulator, which meet at the end through tensor
+//   * one tile of more rows than that has: the groups take every other key tile of it, each with its own maximum, sum and accumulator, which meet at the end through tensor
 //     memory (the groups' warps read the same lanes).
-//   * few, up to 64 rows (an answer's token, drafted ones): every other key tile as well, but turned around.  S^T = K Q^T has a key a lane and the rows, padded to 16,
+//   * few, up to 64 rows, 48 at head size 128 (an answer's token, drafted ones): every other key tile as well, but turned around.  S^T = K Q^T has a key a lane and the rows, padded to 16,
 //     for its columns; P goes to shared memory as the B operand of O^T = V^T P^T.  The softmax of 4 rows is then 4 exponentials of each of the 128 threads instead of 128 of four of
 //     them, and the MMAs are as narrow as the rows: bound by the stream of keys and values.  (A row a lane: one warp a group does all the work, and both of them on the same
 //     quarter of the SM; head size 64 40 x 12000 keys 259 us, 59 % of the stream's rate.)  A column's maximum is taken over all lanes only where some score exceeds the reference by
 //     2^8, which the group finds by a vote; the sums over the lanes wait for the end.
+// Weights are multiplied with V as bf16, and so rounded, in the two kinds of more rows as in the prompt's kernel (2^-8 of a weight; pairs would take the tensor pipe,
+// which bounds there, half as long again).  The few rows' are pairs of bf16, first and second 8 bits, as in the decode kernels: an answer must not depend on which of them it is given.  A row's
+// second halves are eight rows of P behind its first ones -- so both lie at offsets known beforehand -- and the same MMA, twice as wide, gives them columns of their own, added up with the results.
+// (Two MMAs into the same columns: head size 64, 40 answers with up to five drafts over 12000 keys 236 us, 220 so; rounded once: 191.  Head size 128: 309 and 305.  Shared memory has room
+// for 48 rows' pairs at head size 128; 64 / 8 heads, 16 answers with up to seven drafts over 4000 keys, the longest as one tile 79.7 us, all turned around with weights rounded once 75.9.)
 // A CTA per SM walks the pieces that the plan dealt out to it.  A piece of a cut item leaves its maxima, sums and unnormalised results (fp32) in its CTA's place of the
 // workspace, and the last CTA of the item to arrive adds all pieces up in their order: the same bits whichever that is.
 // Keys that a row must not see get weight 0; values behind the item's last key are cleared in shared memory, since 0 * NaN is not 0.
 // Every wait is bounded (pie_gemm.cuh); a warp whose wait ran out does nothing more, but walks on through the barriers of the softmax warps.
 // Device time in a row of such calls, inputs not in L2, 32 query / 8 kv heads: D 128, 2048 tokens behind 15000 460 us (1170 TFLOP/s, of cuBLAS's 1638 in a burst; the tensor pipe is
-// busy for 54 % of it, as in the prompt's kernel one tile's softmax is covered by the other's products in part); 16 answers with up to five drafted tokens over 4000 keys 50.8 (4.5 TB/s),
-// 40 over 12000 319 (6.2 TB/s), one with four over 9000 25.7; D 64, three portions of 700 tokens beside 29 answers over 1500 keys 80.6, 40 answers over 12000 192 (4.9 TB/s).  Short
+// busy for 54 % of it, as in the prompt's kernel one tile's softmax is covered by the other's products in part); 16 answers with up to five drafted tokens over 4000 keys 51.6 (4.4 TB/s),
+// 40 over 12000 309 (6.4 TB/s), one with four over 9000 26.3; D 64, three portions of 700 tokens beside 29 answers over 1500 keys 83.9, 40 answers over 12000 220 (4.5 TB/s).  Short
 // steps pay 4 us from the launch to the first scores, some 3 at each turn from one piece to the next and 5 at the end: results, one counter, the last CTA's sums.
 #include "pie_step_plan.h"
 
@@ -40,14 +45,16 @@ struct ChunkArgs {
 };
 template <int D>
 constexpr int kChunkRecord = 256 * D + 512;   // floats: results, [64 rows][D] of the turned kind, [D / 4][256 rows][4] of the others; [256] maxima and sums
-constexpr int kChunkFew = 64;                 // rows of an item of the turned kind, at most
+constexpr int kChunkFew = 64;                 // rows of an item of the turned kind, at most (ChunkTile::FEW)
 constexpr int kChunkList = 32;                // pieces held in shared memory; a CTA that has more reads them where they are
 
 template <int D>
 struct ChunkTile {
   static constexpr int CH = D / 64, TILE = 128 * D * 2;          // 64-feature chunks of a row, bytes of 128 rows
   static constexpr int RING = D == 64 ? 4 : 2;                   // tiles of K, and of V: 64 KB of each
-  static constexpr int P = 128 * 64 * 2;                         // bytes of a group's P of the turned kind: 2 x 64 rows x 64 keys
+  static constexpr int FEW = D == 64 ? 64 : 48;                  // rows of an item of the turned kind, at most: as shared memory has room for their weights
+  static constexpr int PCHUNK = 2 * FEW * 128;                   // bytes of 64 keys of a group's P of the turned kind: eight rows' first halves, their second halves, ...
+  static constexpr int P = 2 * PCHUNK;
   static constexpr int Q1 = TILE > 2 * P ? TILE : 2 * P;         // the second query tile; the turned kind's P
   static constexpr int SMEM = 1024 + TILE + Q1 + 2 * RING * TILE;
   static constexpr int THREADS = 384;
@@ -106,11 +113,6 @@ __device__ __forceinline__ void chunk_st16(uint32_t taddr, const float* v) {
       "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void chunk_ld16(uint32_t taddr, float* v) { tmem_ld16(taddr, *reinterpret_cast<uint32_t(*)[16]>(v)); }   // not waited for
-__device__ __forceinline__ void chunk_ld8(uint32_t taddr, float* v) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(v);
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "r"(taddr) : "memory");
-}
 __device__ __forceinline__ int chunk_order(float x) {   // integers in the order of the numbers
   const int i = __float_as_int(x);
   return i ^ ((i >> 31) & 0x7fffffff);
@@ -213,7 +215,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   constexpr uint32_t ID_S = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
   constexpr uint32_t ID_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
   constexpr uint32_t ID_FEW = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);   // | N
-  constexpr int COL_S = 0, COL_O = 256;   // + g * 128, + g * D
+  constexpr int COL_S = 0, COL_O = 256, OST = 128;   // + g * 128, + g * OST
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[RING], k_empty[RING], v_full[RING], v_empty[RING], s_full[2], p_full[2], o_full[2];
   __shared__ __align__(16) int4 list[3 * kChunkList];
@@ -293,7 +295,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         // ---------------------------------------------------------------------------------- a key a lane, a row a column
         const int rows = p.tokens * a.G;
         const int beyond = p.k0 * 128 + r - p.pos0, edge_step = (p.pos0 + 1) / 128 - p.k0;   // the first key tile with a key that some row must not see
-        const uint32_t sp = smQ1 + g * T::P + (r >> 6) * 8192 + (r & 7) * 2;
+        const uint32_t sp = smQ1 + g * T::P + (r >> 6) * T::PCHUNK + (r & 7) * 2;
         const int chunk16 = (r & 63) >> 3;
         float l[kChunkFew];
 #pragma unroll
@@ -334,6 +336,14 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             }
             return mx;
           };
+          // four rows' weights into the swizzled tile: 128 bytes a row, its 16-byte chunks in another order
+          auto put = [&](int row, uint32_t w01, uint32_t w23) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t w = k < 2 ? w01 : w23;
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(sp + (row + k) * 128 + ((chunk16 ^ ((row + k) & 7)) << 4)), "h"((uint16_t)(k & 1 ? w >> 16 : w)) : "memory");
+            }
+          };
           bool over = i == 0;
           if (i > 0 && rows > 32) {
             load(1);
@@ -373,18 +383,19 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               alive = alive && gemm_wait_warp(smem_u32(&o_full[g]), (c[g] + i - 1) & 1, abortp);
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-              for (int b = 0; b < 4; ++b)
-                if (16 * b < rows) {
+              for (int b = 0; b < T::FEW / 8; ++b)
+                if (8 * b < rows) {
                   float o[16];
-                  chunk_ld16(tO + g * D + 16 * b, o);
+                  chunk_ld16(tO + g * OST + 16 * b, o);
                   tmem_ld_wait();
 #pragma unroll
-                  for (int n = 0; n < 16; ++n) {
-                    const float f = few.factor[g][16 * b + n];
-                    l[16 * b + n] *= f;
+                  for (int n = 0; n < 8; ++n) {
+                    const float f = few.factor[g][8 * b + n];
+                    l[8 * b + n] *= f;
                     o[n] *= f;
+                    o[8 + n] *= f;
                   }
-                  chunk_st16(tO + g * D + 16 * b, o);
+                  chunk_st16(tO + g * OST + 16 * b, o);
                 }
               tmem_st_wait();
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -401,13 +412,12 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               }
 #pragma unroll
               for (int n = 0; n < 32; n += 4) {
-                if (32 * half + n >= rows) break;
+                if (32 * half + n >= T::FEW || 32 * half + n >= rows) break;
                 l[32 * half + n] += s[n]; l[32 * half + n + 1] += s[n + 1]; l[32 * half + n + 2] += s[n + 2]; l[32 * half + n + 3] += s[n + 3];
-                const uint32_t w[2] = {pack_bf16(s[n], s[n + 1]), pack_bf16(s[n + 2], s[n + 3])};
-#pragma unroll
-                for (int k = 0; k < 4; ++k)   // row n + k of the swizzled tile: 128 bytes, its 16-byte chunks in another order
-                  asm volatile("st.shared.u16 [%0], %1;" ::"r"(sp + (32 * half + n + k) * 128 + ((chunk16 ^ ((n + k) & 7)) << 4)),
-                               "h"((uint16_t)(k & 1 ? w[k >> 1] >> 16 : w[k >> 1])) : "memory");
+                const uint32_t w01 = pack_bf16(s[n], s[n + 1]), w23 = pack_bf16(s[n + 2], s[n + 3]);
+                const int row = 2 * (32 * half + n) - n % 8;
+                put(row, w01, w23);
+                put(row + 8, pack_bf16(s[n] - bf16lo(w01), s[n + 1] - bf16hi(w01)), pack_bf16(s[n + 2] - bf16lo(w23), s[n + 3] - bf16hi(w23)));
               }
             }
           if (step == tail_step) clear_tail(step, tail);
@@ -458,17 +468,25 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll 1
           for (int b = 0; 16 * b < rows; ++b) {
             const int n0 = 16 * b + 8 * g;
-            float o[8], u[8];
-            chunk_ld8(tO + n0, o);
-            if (p.cnt1 > 0) chunk_ld8(tO + D + n0, u);
-            tmem_ld_wait();
+            float v[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) v[n] = 0.f;
+#pragma unroll 1
+            for (int h = 0; h < (p.cnt1 > 0 ? 2 : 1); ++h) {   // the groups' results: by the first halves of the weights, by the second
+              float o[16];
+              chunk_ld16(tO + h * OST + 2 * n0, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int n = 0; n < 8; ++n) {
+                const float2 f = few.share[n0 + n];
+                v[n] += (o[n] + o[8 + n]) * (h ? f.y : f.x);
+              }
+            }
 #pragma unroll
             for (int n = 0; n < 8; ++n)
               if (n0 + n < rows) {
-                const float2 f = few.share[n0 + n];
-                const float v = o[n] * f.x + (p.cnt1 > 0 ? u[n] * f.y : 0.f);
-                if (whole) a.out[(size_t)few.row[n0 + n] * D + r] = f2bf(v);
-                else __stcg(rec + (n0 + n) * D + r, v);
+                if (whole) a.out[(size_t)few.row[n0 + n] * D + r] = f2bf(v[n]);
+                else __stcg(rec + (n0 + n) * D + r, v[n]);
               }
           }
         }
@@ -516,11 +534,11 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll 1
               for (int c0 = 0; c0 < D; c0 += 32) {
                 float o[32];
-                fap_tmem_ld(tO + g * D + c0, o);
+                fap_tmem_ld(tO + g * OST + c0, o);
                 tmem_ld_wait();
 #pragma unroll
                 for (int k = 0; k < 32; ++k) o[k] *= f;
-                tmem_st32(tO + g * D + c0, reinterpret_cast<uint32_t*>(o));
+                tmem_st32(tO + g * OST + c0, reinterpret_cast<uint32_t*>(o));
               }
               tmem_st_wait();
             }
@@ -583,7 +601,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         // columns of this group: its own accumulator, or half of both of one tile's
         const int col0 = pair ? 0 : g * (D / 2), col1 = pair ? D : col0 + D / 2, rr = t0 * a.G + r;   // row of the item
-        const uint32_t from = pair ? tO + g * D : tO;
+        const uint32_t from = pair ? tO + g * OST : tO;
         const bool two = !pair && p.cnt1 > 0;
         if (alive && busy && (cnt > 0 || !pair)) {
           const float inv = whole ? 1.f / l : 1.f;
@@ -595,7 +613,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             tmem_ld_wait();
             if (two) {
               float u[32];
-              fap_tmem_ld(from + D + c0, u);
+              fap_tmem_ld(from + OST + c0, u);
               tmem_ld_wait();
 #pragma unroll
               for (int k = 0; k < 32; ++k) o[k] = o[k] * f0 + u[k] * f1;
@@ -722,11 +740,12 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           asm volatile("" : "+r"(dp));
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_bf16(tm + COL_O + g * D, UPPER | (dv + k * (2048 >> 4)), UPPER | (dp + (k >> 2) * (8192 >> 4) + 2 * (k & 3)), ID_FEW | (1u << 15) | wide, (!first || k > 0) ? 1u : 0u);
+            umma_bf16(tm + COL_O + g * OST, UPPER | (dv + k * (2048 >> 4)), UPPER | (dp + (k >> 2) * (T::PCHUNK >> 4) + 2 * (k & 3)), ID_FEW | (1u << 15) | wide,
+                      (!first || k > 0) ? 1u : 0u);
         } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k)   // 16 keys: 8 columns of P, two 8-key atoms of V
-            umma_f16_ts(tm + COL_O + g * D, tm + COL_S + g * 128 + 8 * k, UPPER | (dv + k * (2048 >> 4)), ID_O, (!first || k > 0) ? 1u : 0u);
+            umma_f16_ts(tm + COL_O + g * OST, tm + COL_S + g * 128 + 8 * k, UPPER | (dv + k * (2048 >> 4)), ID_O, (!first || k > 0) ? 1u : 0u);
         }
         fap_commit(&o_full[g]);
       };
@@ -816,7 +835,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             alive &= gemm_wait(smem_u32(&p_full[g]), (c[g] + (j >> 1)) & 1, abortp);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (elect_one() && alive) {
-              pv(g, t, j < 2, wide);
+              pv(g, t, j < 2, 2 * wide);   // (P with the second halves of its weights)
               fap_commit(&v_empty[t % RING]);
             }
             if (j + 2 < p.n) {
@@ -902,7 +921,7 @@ int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const v
   CUtensorMap maps[4];
   const cuuint32_t one[4] = {1, 1, 1, 1};
   // a query tile, and one of the turned kind: 64 features of G heads of their tokens
-  a.few_tokens = kChunkFew / a.G;
+  a.few_tokens = (D == 128 ? ChunkTile<128>::FEW : ChunkTile<64>::FEW) / a.G;
   for (int i = 0; i < 2; ++i) {
     const long long head = (d->Hq > 1 ? q->stride_h : D) * 2, row = (d->rows > 1 ? q->stride_l : (long long)d->Hq * D) * 2;
     const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)d->Hq, (cuuint64_t)d->rows}, strides[2] = {(cuuint64_t)head, (cuuint64_t)row};
