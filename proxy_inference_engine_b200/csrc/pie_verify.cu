@@ -418,7 +418,7 @@ static VerPlan ver_plan(int requests, int rows, int vocab) {
   // as many slices of a row as give every SM some CTAs, all of the same power of two of turns but the last
   auto pick = [&](int units, int want) {
     const int turns = (vocab / 8 + kVerTurn * kVerThreads - 1) / (kVerTurn * kVerThreads);
-    const long long most = std::max(1LL, (long long)turns * units / (want * 148));
+    const long long most = std::max(1LL, (long long)turns * units / (want * num_sms()));
     long long per = 1;
     while (2 * per <= most || (turns + per - 1) / per > kVerMaxSplits) per *= 2;
     return (int)std::max(1LL, (turns + per - 1) / per);
