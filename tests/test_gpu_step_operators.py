@@ -209,6 +209,44 @@ def test_pools_inside_larger_ones():
     assert torch.equal(ops.chunk_attention(q, both[:, :, 0:2], both[:, :, 2:4], plan, 0.1), ops.chunk_attention(q, k, v, plan, 0.1))
 
 
+def test_rows_and_heads_that_lie_anywhere():
+    """Queries, keys and values with heads outside rows, pools with heads outside pages."""
+    from proxy_inference_engine_b200 import ops
+    for D in (64, 128):
+        new, cached, Hq, Hkv = [3, 90, 17], [300, 40, 0], 8, 2
+        plan, q, k, v, tables = attention_case(new, cached, Hq, Hkv, D, seed=D)
+        outside = lambda x, *order: x.permute(*order).contiguous().permute(*[order.index(i) for i in range(x.dim())])
+        oq, ok, ov = outside(q, 1, 0, 2), outside(k, 2, 0, 1, 3), outside(v, 2, 0, 1, 3)
+        assert oq.stride(1) > oq.stride(0) and ok.stride(2) > ok.stride(0)
+        want = ops.chunk_attention(q, k, v, plan, D ** -0.5)
+        attention_holds(want, q, k, v, new, cached, tables, D ** -0.5)
+        assert torch.equal(ops.chunk_attention(oq, ok, ov, plan, D ** -0.5), want)
+        g = gen(D)
+        nk, nv = randn(g, 110, Hkv, D), randn(g, 110, Hkv, D)
+        turned = ops.rope_kv_slots(q, nk, nv, FREQS(D), plan.positions, plan.slots, k, v)
+        assert torch.equal(ops.rope_kv_slots(oq, outside(nk, 1, 0, 2), outside(nv, 1, 0, 2), FREQS(D), plan.positions, plan.slots, ok, ov), turned)
+        assert torch.equal(ok.view(torch.int16), k.view(torch.int16)) and torch.equal(ov.view(torch.int16), v.view(torch.int16))
+        ops.check_pipeline()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_pieces_than_a_cta_holds_at_once(D):
+    """Seven hundred requests, a portion of a prompt among every few: some CTAs have more than 32 pieces, of all kinds."""
+    from proxy_inference_engine_b200 import ops
+    rng, Hkv = random.Random(D), 8
+    new = [rng.choice([1, 1, 1, 1, 1, 1, 1, 2, 5, 70, 130, 300]) if s % 5 == 0 else 1 for s in range(700)]
+    cached = [rng.choice([0, 1, 63, 64, 100, 127, 128]) for _ in new]
+    plan, q, k, v, tables = attention_case(new, cached, Hkv, Hkv, D, seed=D)
+    plan.check()
+    at = plan.status.storage_offset() + 192
+    ranges = plan.words[at:at + 384].view(192, 2)
+    assert int((ranges[:, 1] - ranges[:, 0]).max()) > 34
+    got = ops.chunk_attention(q, k, v, plan, D ** -0.5)
+    attention_holds(got, q, k, v, new, cached, tables, D ** -0.5)
+    assert torch.equal(got, ops.chunk_attention(q, k, v, plan, D ** -0.5))
+    ops.check_pipeline()
+
+
 def test_attention_on_two_streams_at_once():
     from proxy_inference_engine_b200 import ops
     cases = [attention_case([4, 1], [6000, 3000], 8, 2, 128, seed=s) for s in (1, 2)]
@@ -361,6 +399,36 @@ def test_the_same_draft_is_always_accepted():
     counts = ops.verify_draft(kw["logits"], kw["draft_tokens"], kw["logit_starts"], max_draft=5, temp=1.0, uniforms=kw["uniforms"], noise=kw["noise"],
                               draft_logits=kw["draft_logits"])[1]
     assert counts.tolist() == [6] * 8
+
+
+@pytest.mark.parametrize("temp,model", [(0.0, False), (0.8, False), (1.0, True)])
+def test_rows_behind_the_last_request_judge_nothing(temp, model):
+    """A captured step's room for logit rows is an upper bound: what the rows have that belong to nobody does not matter, NaN included, nor what lies there at a replay."""
+    from proxy_inference_engine_b200 import ops
+    drafted, V, room = [4, 0, 7, -1, 2], 128256, 68
+    kw, starts = verify_case(drafted, V, temp, model, seed=51)
+    live = starts[-1]
+    kw["draft_tokens"][live - 1] = -1
+    want = ops.verify_draft(max_draft=7, **kw)
+    wide = dict(kw)
+    for name in ("logits", "draft_logits", "uniforms"):
+        if kw[name] is not None:
+            wide[name] = torch.full((room, *kw[name].shape[1:]), torch.nan, dtype=kw[name].dtype, device="cuda")
+            wide[name][:live] = kw[name]
+    wide["draft_tokens"] = torch.full((room,), -1, dtype=torch.int32, device="cuda")
+    wide["draft_tokens"][:live] = kw["draft_tokens"]
+    bits = lambda got: [t.view(torch.int32) for t in got]
+    assert all(torch.equal(a, b) for a, b in zip(bits(ops.verify_draft(max_draft=7, **wide)), bits(want)))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.verify_draft(max_draft=7, **wide)
+    for fill, token in ((torch.nan, -1), (torch.inf, V - 1), (0.0, 1 << 30)):
+        wide["logits"][live:], wide["draft_tokens"][live:] = fill, token
+        for t in got:
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(bits(got), bits(want)))
 
 
 def test_ties_go_to_the_first():
