@@ -144,16 +144,16 @@ __global__ void __launch_bounds__(kVerThreads) verify_stats_kernel(const __grid_
   pdl_wait();
   const int r = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
   // (Here, and not by the last CTA to count: where the counters lie depends on the call, and a call of another shape may have left numbers there.)
-  if (blockIdx.x == 0 && r == 0 && !which)
+  if (a.emit_splits > 1 && blockIdx.x == 0 && r == 0 && !which)
     for (int i = tid; i < a.requests; i += kVerThreads) a.count[i] = 0;
-  int vocab = a.vocab;
   if (which) {   // a request's last row judges no token: its draft's logits are not read
+    // (Where starts do not rise, another request may judge its token all the same: by a sum of 0 it refuses it.  Said ahead of the look at them, which costs the others no registers.)
+    if (tid == 0) *reinterpret_cast<float2*>(a.stats + (((size_t)r * 2 + 1) * a.splits + blockIdx.x) * 4) = make_float2(-INFINITY, 0.f);
     bool last = false;
     for (int i = tid; i < a.requests; i += kVerThreads) last = last || __ldg(a.starts + i + 1) == r + 1;
-    // (Where starts do not rise, another request may judge its token all the same: by a row of nothing, whose sum is 0, it refuses it.)
-    if (__syncthreads_or(last)) vocab = 0;
+    if (__syncthreads_or(last)) return;
   }
-  const VerRow row = ver_row((which ? a.guess : a.logits) + (size_t)r * a.ld, vocab);
+  const VerRow row = ver_row((which ? a.guess : a.logits) + (size_t)r * a.ld, a.vocab);
   const float c = a.itemp * 1.4426950408889634f;
   VerSum sum;
   if (blockIdx.x == 0 && tid < row.head) sum.one(bf16lo((uint32_t)__ldg(row.x + tid)), tid, c);
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_stats_kernel(const __grid_
     v2_unpack(v2_add(s01, s23), s0, s1);
     sum.s += s0 + s1;
   }
-  if ((int)blockIdx.x == a.splits - 1 && tid < vocab - row.tail) sum.one(bf16lo((uint32_t)__ldg(row.x + row.tail + tid)), row.tail + tid, c);
+  if ((int)blockIdx.x == a.splits - 1 && tid < a.vocab - row.tail) sum.one(bf16lo((uint32_t)__ldg(row.x + row.tail + tid)), row.tail + tid, c);
   const unsigned long long mine = a.greedy && sum.index >= 0 ? ver_key(sum.m, sum.index) : 0;
   const float m = ver_warp_max(sum.m), part = sum.sum(c);
   float s = part == 0.f ? 0.f : part * exp2f((sum.m - m) * c);
