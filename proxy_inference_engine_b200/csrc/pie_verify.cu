@@ -4,8 +4,9 @@
 // Two launches.  verify_stats_kernel reads every row of logits once: maximum and sum of exponentials (greedy: and the first largest) of slices, in 32 bits.
 // verify_emit_kernel: each CTA of a request joins its rows' slices, finds how many drafted tokens are accepted, and takes slices of the one row behind them through the race for
 // its token; the last CTA to finish joins the slices' best.  (The joining by the last CTA of the first launch, once for a request, cost more in its tail than it saved: 39 -> 46 us.)
-// A row of 128256 logits is 257 KB: HBM at the least, but at seven instructions an exponential, all told, the issue slots are half taken, and a CTA's start and end are as long as its
-// slice.  Device time, in a row of such calls: 5 rows greedy 5.4 us, 16 x 8 12.8, 32 x 6 looked-up drafts 21.9, 64 x 6 rows against a drafter's 40.1 (3.1 TB/s).
+// A row of 128256 logits is 257 KB: HBM at the least, but it gives 1.3 to 3.8 TB/s, and the issue slots are 27 to 42 % active: what bounds is latency.  A CTA's start and end are as long as its
+// slice, and a turn of the race uses its loads at once, between barriers.  Device time in a captured row of such calls, inputs not in L2: 5 rows greedy 5.5 us, 16 x 8 13.0, 32 x 6 looked-up
+// drafts 22.0, 64 x 6 rows against a drafter's 40.4 (3.1 TB/s).
 #include <algorithm>
 
 #include "pie_internal.h"
