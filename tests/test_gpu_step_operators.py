@@ -93,13 +93,13 @@ def attention_case(new, cached, Hq, Hkv, D, seed=0, pad=0, std=2.0, strided=Fals
     return plan, q, k, v, tables
 
 
-def attention_holds(got, q, k, v, new, cached, tables, scale, weights=2.0 ** -8):
+def attention_holds(got, q, k, v, new, cached, tables, scale):
     """A weight in [0, 1] is rounded to bf16 at most once (2^-8 of it), the result once; scores are sums of D products in fp32 (2^-24 D of the sum of
     |q k| scale, up to 2^-13 here, and so for the weights and for their sum), exponentials are off by a few 2^-22."""
     want, weight = O.attention(q, k, v, new, cached, tables, scale)
     T = sum(new)
     got = got.view(got.shape[0], *q.shape[1:]).cpu().double()
-    off = (got[:T] - want[:T]).abs() - (2.0 ** -8 * want[:T].abs() + (weights + 2.0 ** -12) * weight[:T])
+    off = (got[:T] - want[:T]).abs() - (2.0 ** -8 * want[:T].abs() + (2.0 ** -8 + 2.0 ** -12) * weight[:T])
     assert bool((off <= 0).all()), float(off.max())     # (a NaN is not below)
 
 
@@ -158,7 +158,9 @@ def test_an_answers_weights_hold_16_bits(Hq, Hkv, D, long):
     for cached in ([(9000, 4000, 63, 700)[i] if long else (0, 9, 64, 200)[i] for i in range(len(new))], [3000 if long else 30] * len(new)):
         plan, q, k, v, tables = attention_case(new, cached, Hq, Hkv, D, seed=Hq + D, std=0.7)
         got = ops.chunk_attention(q, k, v, plan, D ** -0.5)
-        attention_holds(got, q, k, v, new, cached, tables, D ** -0.5, weights=2.0 ** -16)
+        want, weight = O.attention(q, k, v, new, cached, tables, D ** -0.5)
+        off = (got.view(want.shape).cpu().double() - want).abs() - (2.0 ** -8 * want.abs() + (2.0 ** -16 + 2.0 ** -12) * weight)      # (attention_holds', with 2^-16 for the weights)
+        assert bool((off <= 0).all()), float(off.max())
         ops.check_pipeline()
 
 
