@@ -89,7 +89,7 @@ __device__ __forceinline__ long long cost_before(long long q, int context, int s
 __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_constant__ PlanArgs a) {
   extern __shared__ __align__(16) uint8_t plan_smem[];
   __shared__ long long scan_sm[3 * (kPlanThreads / 32)];
-  __shared__ long long page_total;
+  __shared__ long long page_total, row_total;
   __shared__ int bad, kinds;
   const int S = a.d.requests, T = a.d.rows, tid = threadIdx.x, span = 2 * a.l.tile_tokens;
   long long* const cost = reinterpret_cast<long long*>(plan_smem);   // [S + 1] each
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
       v[1] += (n + c + kStepPage - 1) / kStepPage;
       if (v[0] > T) fault |= PIE_STEP_ROWS;
     }
-    if (s0 < S && s1 == S) { row[S] = (int)min(v[0], (long long)T); page[S] = (int)min(v[1], 0x7fffffffLL); page_total = v[1]; }
+    if (s0 < S && s1 == S) { row[S] = (int)min(v[0], (long long)T); page[S] = (int)min(v[1], 0x7fffffffLL); row_total = v[0]; page_total = v[1]; }
   }
   __syncthreads();
   if (!a.page_stride && page_total > a.n_page_ids) fault |= PIE_STEP_PAGES;
@@ -144,7 +144,13 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
       const int n = row[s + 1] - row[s];
       if (n == 0) return;
       int dr = a.draft ? __ldg(a.draft + s) : 0;
-      if (dr < 0 || dr >= n) { fault |= PIE_STEP_DRAFT; dr = 0; }
+      int all = n;
+      if (row_total > T) {   // rows that are cut off take their drafts with them
+        int c;
+        lengths(s, all, c);
+      }
+      if (dr < 0 || dr >= all) { fault |= PIE_STEP_DRAFT; dr = 0; }
+      dr = max(0, dr - (all - n));
       const int full = (n - 1) / span, rest = n - full * span;
       v[0] += dr + 1;
       v[1] += full + 1;

@@ -168,6 +168,20 @@ def test_logit_rows_that_do_not_fit_are_cut_off_at_the_end(rows):
         plan.check()
 
 
+@pytest.mark.parametrize("new,drafted,rows,starts,tokens", [
+    ([9, 4], [0, 2], [8, 10, 11], [0, 1, 3], [-1, 11, -1]),          # of 10, 11, 12: the last draft has no row
+    ([9, 5], [0, 1], [8, 11], [0, 1, 2], [-1, -1]),                  # none of its drafts has
+    ([9, 6], [3, 5], [5, 6, 7, 8, 9, 10, 11], [0, 4, 7], [6, 7, 8, -1, 10, 11, -1]),
+])
+def test_rows_that_do_not_fit_take_their_drafts_with_them(new, drafted, rows, starts, tokens):
+    """What is left of a request judges the drafts that it would have, and no token that was not drafted."""
+    plan = _build(new, [0, 0], [1, 2], drafted=drafted, num_logits=10)
+    assert plan.logit_rows.tolist() == rows + [0] * (10 - len(rows)) and plan.logit_starts.tolist() == starts
+    assert plan.draft_tokens.tolist() == tokens + [-1] * (10 - len(tokens)) and plan.row_starts.tolist() == [0, 9, 12]
+    with pytest.raises(ValueError, match="more tokens than token_ids$"):
+        plan.check()
+
+
 def test_a_table_that_is_too_narrow():
     plan = _build([9, 3], [60, 0], ints([[1], [2]]))
     with pytest.raises(ValueError, match="more pages than"):
