@@ -34,7 +34,7 @@ struct PlanArgs {
 };
 constexpr int kPlanThreads = 512;
 constexpr int kCostPair = 2, kCostTile = 1;   // a key of an item with rows in both query tiles, in one (powers of two)
-// Queries in, results out.  Over 27 steps of both head sizes, 1 to 212 requests, answers, drafts and portions, a flat choice: 256 and 960 stay within 4 % of it either way but for one answer of
+// Queries in, results out.  Over 27 steps of both head sizes, 1 to 212 requests, answers, drafts and portions, a flat choice: 256 and 960 stay within 5 % of it either way but for one answer of
 // 9000 keys (256: 28.6 us, this 26.2), a prompt of 8192 (528, 500), 4 answers with drafts over 1000 (21.0, 19.6; 960: 17.9) and 16 with up to 14 drafts over 4000 (960: 84.8, 79.0).
 constexpr int kCostItem = 576;
 static_assert(kCostItem < kStepRoom && kStepTile < kStepRoom, "added to keys in 32 bits");

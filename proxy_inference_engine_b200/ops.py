@@ -714,7 +714,8 @@ def chunk_attention(q, k_pool, v_pool, plan, scale: float, out=None):
     """Causal attention of a ragged step: row t of q [T, Hq, D] (rows may lie anywhere) attends to the keys 0 .. position of its own request, which the pools
     [pages, 64, Hkv, D] hold already (rope_kv_slots).  plan: the step's ragged.StepPlan, built for these numbers of heads and pages.  Returns [T, Hq * D].
     Rows that belong to nobody are zero, or with ``out`` given what that held.  What lies in the pages behind a request's last token does not matter, nor what other
-    requests hold; a NaN or an infinity among the values of a request's own new tokens may reach all of its new tokens (0 * NaN), as it does in the other prompt kernels.  Softmax weights are
+    requests hold; a NaN or an infinity among the values of a request's own new tokens may reach all of its new tokens (0 * NaN), as it does in the other prompt kernels, and where a
+    row sees an infinite value it may have NaN.  Softmax weights are
     rounded for their product with the values: to 16 bits (two bfloat16) where a request's rows, its new tokens x Hq / Hkv, are few -- 64, 48 at head size 128 -- as in a decode
     step's attention, and to bfloat16 otherwise, as in a prompt's.  Scores are scaled in 32 bits: scale q . k of more than 2^30 has no result."""
     got = native_host().chunk_attention(q, k_pool, v_pool, plan.words, plan.dims, float(scale), out, workspaces.get)
