@@ -108,6 +108,9 @@ SIGNATURES = {
     "pie_qmm_swiglu": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "pie_qmm_rows": (_i, [_vp, _i, _vp, C.POINTER(QmvSeg), _i, _vp, _i, _i, _i, _i, _vp]),
     "pie_qmm": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "pie_int8_rows": (_i, [_vp, _vp, _vp, _ll, _i, _i, _vp, _f, _vp]),
+    "pie_int8_workspace_bytes": (_sz, [_i, _i]),
+    "pie_int8_matmul": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _sz, _vp]),
     "pie_rms_norm": (_i, [_vp, _vp, _vp, _ll, _i, _f, _vp]),
     "pie_rope": (_i, [_vp, _vp, _ll, _i, _i, _i, _i, _f, _f, _i, _vp, _vp]),
     "pie_rope_kv_append": (_i, [_vp, _vp, _vp, _vp, C.POINTER(KvLayout), _vp, _vp, _i, _i, _i, _i, _vp]),

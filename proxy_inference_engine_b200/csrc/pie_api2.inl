@@ -230,6 +230,26 @@ int pie_pipeline_words(unsigned int* words, void* stream) {
   return cuda_status(fa_prefill_pipeline_post(words + 1, (cudaStream_t)stream));
 }
 
+int pie_int8_rows(int8_t* codes, float* scales, const void* x, long long x_ld, int rows, int K, const void* norm_weight, float eps, void* stream) {
+  if (rows == 0) return PIE_OK;
+  if (!codes || !scales || !x) return PIE_ENULL;
+  if (rows < 0 || K <= 0 || K % 16 || x_ld % 8 || x_ld < 0) return PIE_EINVAL_SHAPE;
+  if (!aligned16(codes) || !aligned16(x) || !aligned16(norm_weight)) return PIE_EALIGN;
+  return cuda_status(launch_int8_rows(codes, scales, (const uint16_t*)x, x_ld, rows, K, (const uint16_t*)norm_weight, eps, (cudaStream_t)stream));
+}
+size_t pie_int8_workspace_bytes(int M, int N) { return M <= 0 || N <= 0 ? 0 : int8_workspace_bytes(M, N); }
+int pie_int8_matmul(void* y, const int8_t* codes, const float* scales, const int8_t* w, const float* w_scales, const void* residual, int M, int N, int K,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  if (M == 0) return PIE_OK;
+  if (!y || !codes || !scales || !w || !w_scales) return PIE_ENULL;
+  // (products of two -128 are 2^14: below 2^17 of them fit 32 bits)
+  if (M < 0 || N <= 0 || K <= 0 || K % 16 || K >= 131072 || ((M + 127LL) / 128) * ((N + 127LL) / 128) > (1 << 30)) return PIE_EINVAL_SHAPE;
+  if (!aligned16(y) || !aligned16(codes) || !aligned16(scales) || !aligned16(w) || !aligned16(w_scales) || !aligned16(residual) || !aligned16(workspace)) return PIE_EALIGN;
+  const size_t need = int8_workspace_bytes(M, N);
+  if (need && (!workspace || workspace_bytes < need)) return PIE_EWORKSPACE;
+  return cuda_status(launch_int8_matmul((uint16_t*)y, codes, scales, w, w_scales, (const uint16_t*)residual, M, N, K, workspace, (cudaStream_t)stream));
+}
+
 int pie_silu_mul(void* out, const void* gate, const void* up, long long n, void* stream) {
   if (n == 0) return PIE_OK;
   if (!out || !gate || !up) return PIE_ENULL;

@@ -122,9 +122,19 @@ __device__ __forceinline__ void gemm_tma_3d(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void gemm_prefetch_3d(const CUtensorMap* map, int c0, int c1, int c2) {
   asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
-template <int CG>
+template <int CG, bool I8 = false>
 __device__ __forceinline__ void gemm_mma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accum) {
-  if (CG == 2)
+  if (I8 && CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accum)
+        : "memory");
+  else if (I8)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accum)
+        : "memory");
+  else if (CG == 2)
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accum)
@@ -217,6 +227,13 @@ template <class E> struct gemm_paired<E, decltype((void)E::PAIRED)> { static con
 template <class E, class = void> struct gemm_segments { static constexpr bool value = false; };
 template <class E> struct gemm_segments<E, decltype((void)E::SEGMENTS)> { static constexpr bool value = true; };
 
+// An epilogue with a member INTEGER has operands of signed 8-bit integers and is given 32-bit integers: sums of integers are exact in any order, and nothing else
+// changes, since two of them lie where one bf16 does.  K, and with it the maps, counts such pairs: a step is 128 bytes of a row either way.
+template <class E, class = void> struct gemm_integer { static constexpr bool value = false; };
+template <class E> struct gemm_integer<E, decltype((void)E::INTEGER)> { static constexpr bool value = true; };
+// signed 8-bit A and B, 32-bit integers out, both K-major (cute::UMMA::InstrDescriptor)
+template <int M, int N> constexpr uint32_t umma_idesc_i8 = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+
 // Epi: void operator()(int z, int row0, int col0, const uint32_t (&v)[32], uint32_t buf, int lane), called by whole warps: 32 columns
 // of rows row0 .. row0 + 31, lane l holding row l's; any row and column, the callee checks the bounds.  buf: 4 KB of shared memory
 // of the warp's own, to turn the tile so that rows are written in whole runs.
@@ -230,7 +247,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
   static_assert(!SEGMENTS || (QB && !PAIRED), "matrices side by side are dequantised ones");
   constexpr int COLS = PAIRED ? T::NB : BN;   // columns of y in a tile
   constexpr int S = T::S, RING = T::RING > 0 ? T::RING : 1, KPC = QB == 4 ? 4 : 2;   // K steps per packed chunk
-  constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(T::BM >> 4) << 24);
+  constexpr bool I8 = gemm_integer<Epi>::value;
+  static_assert(!I8 || !QB, "integers are multiplied as they are");
+  constexpr uint32_t IDESC = I8 ? umma_idesc_i8<T::BM, BN> : (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(T::BM >> 4) << 24);
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], tfull_bar[2], tempty_bar[2], pfull_bar[RING], pempty_bar[RING];
   __shared__ uint32_t tmem_slot;
@@ -381,7 +400,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
           if (elect_one() && alive) {
 #pragma unroll
             for (int k4 = 0; k4 < 4; ++k4)   // 16 elements of K: 32 bytes inside the swizzle atom
-              gemm_mma<CG>(acc + b * T::ACC, da + 2 * k4, db + 2 * k4, IDESC, (kb > k_lo || k4 > 0) ? 1u : 0u);
+              gemm_mma<CG, I8>(acc + b * T::ACC, da + 2 * k4, db + 2 * k4, IDESC, (kb > k_lo || k4 > 0) ? 1u : 0u);
             gemm_commit<CG>(smem_u32(&empty_bar[s]));
             if (kb == k_hi - 1) gemm_commit<CG>(smem_u32(&tfull_bar[b]));
           }
@@ -540,12 +559,19 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const uint4 u = lds128(p + q * 128 * 16);
-            acc[4 * q] += __uint_as_float(u.x); acc[4 * q + 1] += __uint_as_float(u.y);
-            acc[4 * q + 2] += __uint_as_float(u.z); acc[4 * q + 3] += __uint_as_float(u.w);
+            if constexpr (I8) {   // (bits of integers, which nothing but these sums touches)
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[4 * q + e] = src ? v[4 * q + e] + w[e] : w[e];
+            } else {
+              acc[4 * q] += __uint_as_float(u.x); acc[4 * q + 1] += __uint_as_float(u.y);
+              acc[4 * q + 2] += __uint_as_float(u.z); acc[4 * q + 3] += __uint_as_float(u.w);
+            }
           }
         }
+        if constexpr (!I8)
 #pragma unroll
-        for (int q = 0; q < 32; ++q) v[q] = __float_as_uint(acc[q]);
+          for (int q = 0; q < 32; ++q) v[q] = __float_as_uint(acc[q]);
         if constexpr (SEGMENTS) {
           const int g = epi.segment(at.n);
           epi(g, at.m * T::BM + (warp & 3) * 32, (at.n - epi.tile0[g]) * BN + (gi * (int)ranks + (int)rank) * 32, v,

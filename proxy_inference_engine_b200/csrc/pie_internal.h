@@ -135,6 +135,11 @@ bool qmt_shape_ok(int M, int K, int group_size, int bits);
 size_t qmt_ws_bytes(int M, long long ntiles, int K, int bits);
 cudaError_t launch_qmt(void* out, int out_ld, const void* x, int x_ld, int M, int K, const pie_qmv_seg* segs, int nseg, int bits,
                        const void* norm_w, float eps, int epi, const void* residual, void* ws, cudaStream_t st);
+// products in 8-bit integers (pie_int8.cuh, compiled with pie_qmm.cu as well)
+size_t int8_workspace_bytes(int M, int N);
+cudaError_t launch_int8_rows(int8_t* codes, float* scales, const uint16_t* x, long long x_ld, int rows, int K, const uint16_t* norm, float eps, cudaStream_t st);
+cudaError_t launch_int8_matmul(uint16_t* y, const int8_t* codes, const float* sx, const int8_t* w, const float* sw, const uint16_t* residual, int M, int N, int K, void* ws,
+                               cudaStream_t st);
 unsigned int qmm_pipeline_error();
 cudaError_t qmm_pipeline_post(unsigned int* host, cudaStream_t st);
 cudaError_t qmm_pipeline_clear();

@@ -216,3 +216,5 @@ cudaError_t qmm_pipeline_post(unsigned int* host, cudaStream_t st) { return gemm
 cudaError_t qmm_pipeline_clear() { return gemm_error_clear(); }
 
 }  // namespace pie
+
+#include "pie_int8.cuh"

@@ -807,6 +807,99 @@ def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: fl
     return tokens, counts, logprobs
 
 
+def _rows_of(x, K: int):
+    """x [..., K] as rows that a kernel can read 16 bytes at a time: (tensor to be held until the launch is queued, elements between rows)."""
+    if x.dim() != 2:
+        x = x.reshape(-1, K)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < 0)) or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x, x.stride(0) if x.shape[0] > 1 else K
+
+
+def _int8_features(what: str, x, norm_weight) -> int:
+    """What int8_rows and int8_linear take: bfloat16 rows of a multiple of 16 features, and a norm's weight for them."""
+    if x.dim() < 1 or x.dtype != _BF16:
+        raise ValueError(f"[{what}] x must be bfloat16 [..., K], but is {x.dtype} {tuple(x.shape)}")
+    K = x.shape[-1]
+    if K == 0 or K % 16:
+        raise ValueError(f"[{what}] rows of {K} features are not built here (a multiple of 16)")
+    if norm_weight is not None and (norm_weight.dtype != _BF16 or tuple(norm_weight.shape) != (K,)):
+        raise ValueError(f"[{what}] norm_weight must be bfloat16 [{K}], but is {norm_weight.dtype} {list(norm_weight.shape)}")
+    return K
+
+
+def int8_rows(x, *, norm_weight=None, eps: float = 1e-5):
+    """Rows of 8-bit integers with a scale each: of x bfloat16 [..., K] (K a multiple of 16) the codes int8 [..., K] and scales f32 [...], with s = max |x| / 127 and codes
+    x / s rounded to the nearest, of two the even one, so that x is about codes * s.  With norm_weight (bfloat16 [K]) of rms_norm(x, norm_weight, eps).  A row of zeros has scale
+    0; a row with an infinity or a NaN has scale NaN, so that its products are NaN.  A weight [N, K] becomes integers with a scale for each output channel the same way."""
+    what = "int8_rows"
+    K = _int8_features(what, x, norm_weight)
+    with _one_device(what, x, *(() if norm_weight is None else (norm_weight,))):
+        rows, ld = _rows_of(x, K)
+        norm = None if norm_weight is None else _rows_of(norm_weight.view(1, K), K)[0]
+        codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        _lib.check(_lib.load().pie_int8_rows(_p(codes), _p(scales), _p(rows), ld, rows.shape[0], K, _p(norm), float(eps), _stream()), what)
+    return codes, scales
+
+
+def _int8_weight(what: str, weight, weight_scales, K: int) -> int:
+    if weight.dtype != torch.int8 or weight.dim() != 2 or weight.shape[1] != K or not weight.is_contiguous() or weight.data_ptr() % 16:
+        raise ValueError(f"[{what}] weight must be contiguous int8 [N, {K}], but is {weight.dtype} {tuple(weight.shape)}")
+    N = weight.shape[0]
+    if weight_scales.dtype != torch.float32 or tuple(weight_scales.shape) != (N,) or not weight_scales.is_contiguous() or weight_scales.data_ptr() % 16:
+        raise ValueError(f"[{what}] weight_scales must be contiguous float32 [{N}], but is {weight_scales.dtype} {list(weight_scales.shape)}")
+    if K >= 131072:
+        raise ValueError(f"[{what}] sums of {K} products are not built here (below 131072)")
+    return N
+
+
+def int8_matmul(codes, scales, weight, weight_scales, *, residual=None):
+    """Product of 8-bit integers with a scale for each token and each channel: y[..., n] = bf16((sum_k codes[..., k] weight[n, k]) scales[...] weight_scales[n]), and
+    bf16(residual + y) with a residual (bfloat16 [..., N]).  codes int8 [..., K] and scales f32 [...] as int8_rows gives them, weight int8 [N, K] and weight_scales f32 [N] (int8_rows
+    of a weight).  K: a multiple of 16 below 131072.  The sum is exact, and a row's result does not depend on the rows beside it."""
+    what = "int8_matmul"
+    if codes.dim() < 1 or codes.dtype != torch.int8 or codes.shape[-1] == 0 or codes.shape[-1] % 16:
+        raise ValueError(f"[{what}] codes must be int8 [..., K] with K a multiple of 16, but are {codes.dtype} {tuple(codes.shape)}")
+    K = codes.shape[-1]
+    if scales.dtype != torch.float32 or scales.shape != codes.shape[:-1]:
+        raise ValueError(f"[{what}] scales must be float32 {list(codes.shape[:-1])}, but are {scales.dtype} {list(scales.shape)}")
+    N = _int8_weight(what, weight, weight_scales, K)
+    shape = codes.shape[:-1] + (N,)
+    if residual is not None and (residual.dtype != _BF16 or residual.shape != shape):
+        raise ValueError(f"[{what}] residual must be bfloat16 {list(shape)}, but is {residual.dtype} {list(residual.shape)}")
+
+    def aligned(t):
+        t = t.contiguous()
+        return t if t.data_ptr() % 16 == 0 else t.clone()
+    with _one_device(what, codes, scales, weight, weight_scales, *(() if residual is None else (residual,))):
+        codes, scales, residual = aligned(codes), aligned(scales), None if residual is None else aligned(residual)
+        y = torch.empty(shape, dtype=_BF16, device=codes.device)
+        M = scales.numel()
+        L = _lib.load()
+        need = L.pie_int8_workspace_bytes(M, N)
+        ws = workspaces.get("int8", need, codes.device) if need else None
+        _lib.check(L.pie_int8_matmul(_p(y), _p(codes), _p(scales), _p(weight), _p(weight_scales), _p(residual), M, N, K, _p(ws), 0 if ws is None else ws.numel(),
+                                     _stream()), what)
+    return y
+
+
+def int8_linear(x, weight, weight_scales, *, norm_weight=None, eps: float = 1e-5, residual=None):
+    """A linear layer of 8-bit integers: int8_rows of x (bfloat16 [..., K], through the layer's norm with norm_weight), int8_matmul of those with weight int8 [N, K] and
+    weight_scales f32 [N], and the residual added.  Returns bfloat16 [..., N]."""
+    what = "int8_linear"
+    K = _int8_features(what, x, norm_weight)
+    N = _int8_weight(what, weight, weight_scales, K)
+    shape = x.shape[:-1] + (N,)
+    if residual is not None and (residual.dtype != _BF16 or residual.shape != shape):
+        raise ValueError(f"[{what}] residual must be bfloat16 {list(shape)}, but is {residual.dtype} {list(residual.shape)}")
+    _one_device(what, x, weight, weight_scales, *(t for t in (norm_weight, residual) if t is not None))
+    codes, scales = int8_rows(x, norm_weight=norm_weight, eps=eps)
+    return int8_matmul(codes, scales, weight, weight_scales, residual=residual)
+
+
 _VOID = ("a bounded wait inside a tensor-core pipeline expired: results since the last check that passed are void "
          "(and every check fails until {}_pipeline_error_clear())")
 
