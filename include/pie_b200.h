@@ -335,6 +335,18 @@ size_t pie_chunk_attn_workspace_bytes(const pie_step_dims* dims, int D);
 int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const void* vpool, const pie_kv_layout* kv_host, const int32_t* plan,
                    const pie_step_dims* dims, int D, float scale, int rest, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The same step over a cache of 8 bits: pools of e4m3 codes [pages, Hkv, 64, D], a page of a head in one piece, and scales f32 [pages, Hkv]; a feature is its code times its page's and
+ * head's scale, which is the lowest power of two, 2^-60 at least, with which all that was written since the page's first token is 448 or less.
+ * pie_rope_kv_fp8 is pie_rope_kv_slots into such pools (keys are not rounded between rotation and code).  A row at a page's first place begins the page anew; where a row needs a
+ * larger scale than the page has, what the page holds in front of it is brought to that.  Rows of one request go to a page together: no two requests of a plan may write to the same page.
+ * A block with an infinity or a NaN has scale NaN, and stays so until it begins anew.
+ * pie_chunk_attn_fp8 is pie_chunk_attn over such pools (scales > 0; codes are taken as finite).  Up to 32 rows of a request (its rows x Hq / Hkv) have the weights of 16 bits; weights are
+ * rounded after they are multiplied with the values' scale.  The same workspace. */
+int pie_rope_kv_fp8(void* q_out, uint8_t* kpool, float* k_scales, uint8_t* vpool, float* v_scales, const pie_head_rows* q, const pie_head_rows* k, const pie_head_rows* v,
+                    const int32_t* plan, const pie_step_dims* dims, const float* freqs, int D, int rest, void* stream);
+int pie_chunk_attn_fp8(void* out, const pie_head_rows* q, const uint8_t* kpool, const float* k_scales, const uint8_t* vpool, const float* v_scales, const int32_t* plan,
+                       const pie_step_dims* dims, int D, float scale, int rest, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Drafted tokens against the target's probabilities.  Request s has the rows logit_starts[s] .. logit_starts[s + 1] - 1 of logits (bf16 [rows, ld >= vocab]); row r
  * judges draft_tokens[r], the last one none.  p = softmax(logits / temp); q = softmax(draft_logits / temp) (laid out as logits), or with draft_logits NULL all of it on
  * the drafted token.  In order, a token x is accepted while uniforms[r] q(x) < p(x).  Behind the accepted ones comes one more: at the first refusal the one of largest

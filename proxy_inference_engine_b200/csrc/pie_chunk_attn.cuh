@@ -42,23 +42,35 @@ struct ChunkArgs {
   float* part;                 // [2 CTAs] records
   int rest;
   int few_tokens;              // tokens of an item of the turned kind, at most
+  // 8-bit pages: codes [pages, Hkv, 64, D], scales [pages, Hkv]
+  const uint8_t *k8, *v8;
+  const float *k_scales, *v_scales;
+  int Hkv;
 };
 template <int D>
 constexpr int kChunkRecord = 256 * D + 512;   // floats: results, [64 rows][D] of the turned kind, [D / 4][256 rows][4] of the others; [256] maxima and sums
 constexpr int kChunkFew = 64;                 // rows of an item of the turned kind, at most (ChunkTile::FEW)
 constexpr int kChunkList = 32;                // pieces held in shared memory; a CTA that has more reads them where they are
 
-template <int D>
+template <int D, bool F8 = false>
 struct ChunkTile {
   static constexpr int CH = D / 64, TILE = 128 * D * 2;          // 64-feature chunks of a row, bytes of 128 rows
-  static constexpr int RING = D == 64 ? 4 : 2;                   // tiles of K, and of V: 64 KB of each
-  static constexpr int FEW = D == 64 ? 64 : 48;                  // rows of an item of the turned kind, at most: as shared memory has room for their weights
+  static constexpr int RK = F8 ? (D == 64 ? 2 : 1) : D == 64 ? 4 : 2;   // tiles of K
+  static constexpr int RV = F8 ? 2 : RK;                         // tiles of V
+  static constexpr int FEW = F8 ? 32 : D == 64 ? 64 : 48;        // rows of an item of the turned kind, at most: as shared memory has room for their weights
+  static constexpr int HALVES = (FEW + 31) / 32;                 // of 32 rows
   static constexpr int PCHUNK = 2 * FEW * 128;                   // bytes of 64 keys of a group's P of the turned kind: eight rows' first halves, their second halves, ...
   static constexpr int P = 2 * PCHUNK;
   static constexpr int Q1 = TILE > 2 * P ? TILE : 2 * P;         // the second query tile; the turned kind's P
-  static constexpr int SMEM = 1024 + TILE + Q1 + 2 * RING * TILE;
-  static constexpr int THREADS = 384;
+  static constexpr int PAGE = 64 * D, PAGES = F8 ? (D == 64 ? 16 : 6) : 1;   // bytes of a page of one head in 8 bits, and how many of them wait to be converted
+  static constexpr int SMEM = 1024 + TILE + Q1 + (RK + RV) * TILE + (F8 ? PAGES * PAGE : 0);
+  static constexpr int THREADS = F8 ? 512 : 384;
+  // warps 0-7 softmax, 8 TMA, 9 MMAs, 10 scales (8-bit pages), W_REST rows of nobody, 12-15 conversion (8-bit pages)
+  static constexpr int W_REST = F8 ? 11 : 10;
+  // Registers, which must not exceed what the block is launched with: 384 x 168 = 64512, 256 x 216 and 128 x 64 are 63488; 512 x 128 = 65536 = 256 x 208 and 256 x 48
+  static constexpr int REGS_SOFTMAX = F8 ? 208 : 216, REGS_REST = F8 ? 48 : 64;
 };
+constexpr int kChunkScales = 4;               // 8-bit pages: key tiles of a group whose scales are held
 
 enum ChunkKind { CHUNK_PAIR, CHUNK_ONE, CHUNK_FEW };
 // a piece as the roles walk it
@@ -206,18 +218,32 @@ __device__ __forceinline__ void chunk_merge(uint16_t* out, const float* part, in
   }
 }
 
-template <int D>
-__global__ void __launch_bounds__(ChunkTile<D>::THREADS, 1)
+// 16 codes of 8 bits as bf16, exactly: the code's bits in the places of a bf16's are a number 2^120 times smaller (and e4m3's subnormals bf16's)
+__device__ __forceinline__ uint32_t chunk_widen(uint32_t w, uint32_t sel) {
+  const uint32_t x = __byte_perm(w, 0, sel), y = ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u);
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(y), "r"(0x7b807b80u));
+  return d;
+}
+__device__ __forceinline__ void chunk_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+template <int D, bool F8>
+__global__ void __launch_bounds__(ChunkTile<D, F8>::THREADS, 1)
 chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_few, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ChunkArgs a) {
-  using T = ChunkTile<D>;
-  constexpr int RING = T::RING;
+  using T = ChunkTile<D, F8>;
+  constexpr int RK = T::RK, RV = T::RV;
   constexpr uint32_t ID_S = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
   constexpr uint32_t ID_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
   constexpr uint32_t ID_FEW = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);   // | N
   constexpr int COL_S = 0, COL_O = 256, OST = 128;   // + g * 128, + g * OST
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[RING], k_empty[RING], v_full[RING], v_empty[RING], s_full[2], p_full[2], o_full[2];
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[RK], k_empty[RK], v_full[RV], v_empty[RV], s_full[2], p_full[2], o_full[2];
+  // 8-bit pages: pages as they lie, scales of a group's key tiles, products behind which the turned kind's P is free (pieces of that kind in turn)
+  __shared__ __align__(8) uint64_t c_full[T::PAGES], c_empty[T::PAGES], sc_full[2][F8 ? kChunkScales : 1], sc_empty[2][F8 ? kChunkScales : 1], turn_free[2];
+  __shared__ __align__(16) float sc[2][F8 ? kChunkScales : 1][8];   // of the two pages: scores to log2 units, log2 of the values' scale, its reciprocal, itself
   __shared__ __align__(16) int4 list[3 * kChunkList];
   __shared__ __align__(16) ChunkFew few;
   __shared__ float2 ml[2][128];           // a row's maximum and sum: of the two groups of a tile, of the rows of a cut item
@@ -227,16 +253,19 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   // (The turned kind's P lies where Q1 does.  Its V^T has 128 rows whatever the head size: at 64 the upper ones are what lies 16 KB behind, so V does not lie last.)
-  const uint32_t smV = base, smK = smV + RING * T::TILE, smQ = smK + RING * T::TILE, smQ1 = smQ + T::TILE;
+  const uint32_t smV = base, smK = smV + RV * T::TILE, smQ = smK + RK * T::TILE, smQ1 = smQ + T::TILE, smC = smQ1 + T::Q1;
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1);
     }
-    for (int i = 0; i < RING; ++i) {
-      mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
+    for (int i = 0; i < RK; ++i) { mbar_init(&k_full[i], F8 ? 4 : 1); mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < RV; ++i) { mbar_init(&v_full[i], F8 ? 4 : 1); mbar_init(&v_empty[i], 1); }
+    if (F8) {
+      for (int i = 0; i < T::PAGES; ++i) { mbar_init(&c_full[i], 1); mbar_init(&c_empty[i], 4); }
+      for (int i = 0; i < 2 * kChunkScales; ++i) { mbar_init(&sc_full[0][0] + i, 1); mbar_init(&sc_empty[0][0] + i, 4); }
+      for (int i = 0; i < 2; ++i) mbar_init(&turn_free[i], 1);
     }
     abort_flag = 0;
     fence_mbar_init();
@@ -245,7 +274,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (warp == 8 && lane < 4) tma_prefetch_desc(lane == 0 ? &map_q : lane == 1 ? &map_few : lane == 2 ? &map_k : &map_v);
+  if (warp == 8 && lane < (F8 ? 2 : 4)) tma_prefetch_desc(lane == 0 ? &map_q : lane == 1 ? &map_few : lane == 2 ? &map_k : &map_v);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -258,14 +287,13 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (warp != 8) {
     for (int i = warp < 8 ? tid : tid - 32; i < 3 * min(end - begin, kChunkList); i += T::THREADS - 32)
       list[i] = __ldg(reinterpret_cast<const int4*>(a.pieces + begin) + i);
-    asm volatile("bar.sync 4, 352;" ::: "memory");
-    if (end - begin > 1) asm volatile("bar.arrive 5, 384;" ::: "memory");
+    asm volatile("bar.sync 4, %0;" ::"n"(T::THREADS - 32) : "memory");
+    if (end - begin > 1) asm volatile("bar.arrive 5, %0;" ::"n"(T::THREADS) : "memory");
   }
 
   // All barriers are counted over the CTA's pieces: a role keeps the number of key tiles (of its group, of K and V) before its piece.
-  // Registers: 384 threads x 168 at launch = 64512; 8 warps of 216 and 4 of 64 are 63488.
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::REGS_SOFTMAX));
     // ------------------------------------------------------------------------------------------------ softmax of group g
     const int g = warp >> 2, quad = warp & 3, r = quad * 32 + lane, tok = r / a.G;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
@@ -277,12 +305,21 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // values behind the item's last key may be anything: this thread's row of the key tile they lie in
     auto clear_tail = [&](int step, int tail) {
       const int v = cv + step;
-      alive = alive && gemm_wait_warp(smem_u32(&v_full[v % RING]), (v / RING) & 1, abortp);
+      alive = alive && gemm_wait_warp(smem_u32(&v_full[v % RV]), (v / RV) & 1, abortp);
       if (alive && r >= tail)
 #pragma unroll
         for (int q = 0; q < 8 * T::CH; ++q)
-          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(smV + (v % RING) * T::TILE + (q >> 3) * 16384 + r * 128 + (q & 7) * 16), "r"(0) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(smV + (v % RV) * T::TILE + (q >> 3) * 16384 + r * 128 + (q & 7) * 16), "r"(0) : "memory");
       fence_proxy_async();
+    };
+    // 8-bit pages: the scales of this group's key tile n, before its scores are there (both pages'; (c, log2 v, 1 / v, v) of page h at h, 2 + h, ...)
+    auto take_scales = [&](int n, float (&to)[8]) {
+      const int i = n % kChunkScales;
+      alive = alive && gemm_wait_warp(smem_u32(&sc_full[g][i]), (n / kChunkScales) & 1, abortp);
+      *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(sc[g][i]);
+      *reinterpret_cast<float4*>(to + 4) = *reinterpret_cast<const float4*>(sc[g][i] + 4);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc_empty[g][i]);
     };
     // Registers are short where a thread holds a row of scores: the loops keep a few numbers, and the piece is read again behind them.
     auto read_again = [&]() {
@@ -297,11 +334,18 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const int beyond = p.k0 * 128 + r - p.pos0, edge_step = (p.pos0 + 1) / 128 - p.k0;   // the first key tile with a key that some row must not see
         const uint32_t sp = smQ1 + g * T::P + (r >> 6) * T::PCHUNK + (r & 7) * 2;
         const int chunk16 = (r & 63) >> 3;
-        float l[kChunkFew];
+        float l[32 * T::HALVES];
 #pragma unroll
-        for (int n = 0; n < kChunkFew; ++n) l[n] = 0.f;
+        for (int n = 0; n < 32 * T::HALVES; ++n) l[n] = 0.f;
         for (int i = 0; i < cnt; ++i) {
           const int step = 2 * i + g;
+          float to_log2 = a.scale_log2e, value = 1.f;   // of this lane's key: of its page
+          if constexpr (F8) {
+            float of[8];
+            take_scales(c[g] + i, of);
+            to_log2 = quad < 2 ? of[0] : of[1];
+            value = quad < 2 ? of[6] : of[7];
+          }
           alive = alive && gemm_wait_warp(smem_u32(&s_full[g]), (c[g] + i) & 1, abortp);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           float s[32];
@@ -328,10 +372,10 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             for (int n = 0; n < 32; n += 4) {
               if (32 * half + n >= rows) break;
               const float4 less = *reinterpret_cast<const float4*>(&few.less[g][32 * half + n]);
-              s[n] = fap_exp2(fmaf(s[n], a.scale_log2e, less.x));
-              s[n + 1] = fap_exp2(fmaf(s[n + 1], a.scale_log2e, less.y));
-              s[n + 2] = fap_exp2(fmaf(s[n + 2], a.scale_log2e, less.z));
-              s[n + 3] = fap_exp2(fmaf(s[n + 3], a.scale_log2e, less.w));
+              s[n] = fap_exp2(fmaf(s[n], to_log2, less.x));
+              s[n + 1] = fap_exp2(fmaf(s[n + 1], to_log2, less.y));
+              s[n + 2] = fap_exp2(fmaf(s[n + 2], to_log2, less.z));
+              s[n + 3] = fap_exp2(fmaf(s[n + 3], to_log2, less.w));
               mx = fmaxf(fmaxf(mx, fmaxf(s[n], s[n + 1])), fmaxf(s[n + 2], s[n + 3]));
             }
             return mx;
@@ -345,7 +389,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             }
           };
           bool over = i == 0;
-          if (i > 0 && rows > 32) {
+          if (T::HALVES > 1 && i > 0 && rows > 32) {
             load(1);
             over = weigh(1) > 256.f;
           }
@@ -354,14 +398,14 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           // the reference of a row moves where a score exceeds it by 8 (log2 units: a weight of 256): same sums, and mostly the lanes need not know of one another
           if (chunk_group_any(g, over)) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int half = 0; half < T::HALVES; ++half)
               if (32 * half < rows) {
                 if (half || i > 0) load(half);
                 int mine = 0;
 #pragma unroll
                 for (int n = 0; n < 32; ++n) {
                   if (32 * half + n >= rows) break;
-                  const int v = __reduce_max_sync(0xffffffffu, chunk_order(s[n]));
+                  const int v = __reduce_max_sync(0xffffffffu, chunk_order(F8 ? s[n] * to_log2 : s[n]));
                   if (lane == n) mine = v;
                 }
                 few.best[g][quad][32 * half + lane] = mine;
@@ -370,7 +414,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             if (quad == 0)
               for (int n = lane; n < rows; n += 32) {
                 const float was = i == 0 ? -INFINITY : few.m[g][n];
-                const float now = chunk_unorder(max(max(few.best[g][0][n], few.best[g][1][n]), max(few.best[g][2][n], few.best[g][3][n]))) * a.scale_log2e;
+                const float now = chunk_unorder(max(max(few.best[g][0][n], few.best[g][1][n]), max(few.best[g][2][n], few.best[g][3][n]))) * (F8 ? 1.f : a.scale_log2e);
                 const bool move = i == 0 || now > was + 8.f;
                 const float m = move ? now : was;
                 few.factor[g][n] = !move ? 1.f : was == -INFINITY ? 0.f : fap_exp2(was - m);
@@ -400,11 +444,11 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               tmem_st_wait();
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
-            if (rows > 32 || i > 0) load(0);
+            if ((T::HALVES > 1 && rows > 32) || i > 0) load(0);
             weigh(0);
           }
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
+          for (int half = 0; half < T::HALVES; ++half)
             if (32 * half < rows) {
               if (half) {
                 load(1);
@@ -414,13 +458,14 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               for (int n = 0; n < 32; n += 4) {
                 if (32 * half + n >= T::FEW || 32 * half + n >= rows) break;
                 l[32 * half + n] += s[n]; l[32 * half + n + 1] += s[n + 1]; l[32 * half + n + 2] += s[n + 2]; l[32 * half + n + 3] += s[n + 3];
+                if constexpr (F8) { s[n] *= value; s[n + 1] *= value; s[n + 2] *= value; s[n + 3] *= value; }
                 const uint32_t w01 = pack_bf16(s[n], s[n + 1]), w23 = pack_bf16(s[n + 2], s[n + 3]);
                 const int row = 2 * (32 * half + n) - n % 8;
                 put(row, w01, w23);
                 put(row + 8, pack_bf16(s[n] - bf16lo(w01), s[n + 1] - bf16hi(w01)), pack_bf16(s[n + 2] - bf16lo(w23), s[n + 3] - bf16hi(w23)));
               }
             }
-          if (step == tail_step) clear_tail(step, tail);
+          if (!F8 && step == tail_step) clear_tail(step, tail);   // (8-bit codes are finite as they are converted)
           fence_proxy_async();
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
@@ -428,7 +473,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         // a row's sum over the warp's lanes: half of the columns a step, until a lane has one
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int half = 0; half < T::HALVES; ++half)
           if (32 * half < rows) {
             float* const v = l + 32 * half;
 #pragma unroll
@@ -500,6 +545,8 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         float m = -INFINITY, l = 0.f;
         for (int i = 0; i < cnt; ++i) {
           const int step = pair ? i : 2 * i + g;
+          float of[F8 ? 8 : 1];
+          if constexpr (F8) take_scales(c[g] + i, of);
           alive = alive && gemm_wait_warp(smem_u32(&s_full[g]), (c[g] + i) & 1, abortp);
           if (!alive) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -514,12 +561,25 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               for (int k = 0; k < 128; ++k)
                 if (k > last) s[k] = -INFINITY;
             }
-            float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
+            float mx;
+            if constexpr (F8) {   // a page's half of the row at a time
+              float x[4];
 #pragma unroll
-            for (int k = 4; k < 128; k += 4) {
-              x0 = fmaxf(x0, s[k]); x1 = fmaxf(x1, s[k + 1]); x2 = fmaxf(x2, s[k + 2]); x3 = fmaxf(x3, s[k + 3]);
+              for (int q = 0; q < 4; ++q) {
+                const int k0 = 64 * (q >> 1) + 32 * (q & 1);
+                x[q] = s[k0];
+#pragma unroll
+                for (int k = 1; k < 32; ++k) x[q] = fmaxf(x[q], s[k0 + k]);
+              }
+              mx = fmaxf(fmaxf(x[0], x[1]) * of[0], fmaxf(x[2], x[3]) * of[1]);
+            } else {
+              float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
+#pragma unroll
+              for (int k = 4; k < 128; k += 4) {
+                x0 = fmaxf(x0, s[k]); x1 = fmaxf(x1, s[k + 1]); x2 = fmaxf(x2, s[k + 2]); x3 = fmaxf(x3, s[k + 3]);
+              }
+              mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale_log2e;   // (the scale is positive)
             }
-            const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale_log2e;   // (the scale is positive)
             const bool move = mx > m + 8.f;
             if (i == 0) {
               m = mx;
@@ -543,10 +603,17 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               tmem_st_wait();
             }
             const float ms = m == -INFINITY ? 0.f : m;
-            const f32x2 sc2 = f2_pack(a.scale_log2e, a.scale_log2e), ms2 = f2_pack(-ms, -ms);
+            f32x2 sc2 = f2_pack(a.scale_log2e, a.scale_log2e), ms2 = f2_pack(-ms, -ms);
             f32x2 l01 = f2_pack(0.f, 0.f), l23 = l01;
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
+              // (8-bit pages: weights times the values' scale, which the row's sum is rid of again)
+              if constexpr (F8) {
+                sc2 = f2_pack(of[hf], of[hf]);
+                ms2 = f2_pack(of[2 + hf] - ms, of[2 + hf] - ms);
+                l01 = f2_pack(0.f, 0.f);
+                l23 = l01;
+              }
               uint32_t w[32];
 #pragma unroll
               for (int k = 0; k < 32; ++k) {
@@ -565,13 +632,20 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 else l01 = f2_add(l01, f2_pack(e0, e1));
               }
               tmem_st32(tS + 32 * hf, w);
+              if constexpr (F8) {
+                float l0, l1;
+                f2_unpack(f2_add(l01, l23), l0, l1);
+                l += (l0 + l1) * of[4 + hf];
+              }
             }
-            float l0, l1;
-            f2_unpack(f2_add(l01, l23), l0, l1);
-            l += l0 + l1;
+            if constexpr (!F8) {
+              float l0, l1;
+              f2_unpack(f2_add(l01, l23), l0, l1);
+              l += l0 + l1;
+            }
             tmem_st_wait();
           }
-          if (step == tail_step) clear_tail(step, tail);
+          if (!F8 && step == tail_step) clear_tail(step, tail);
           if (!alive) break;
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
@@ -652,14 +726,16 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::REGS_REST));
     // ------------------------------------------------------------------------------------------------ TMA
     if (warp == 8) {
       bool alive = true;
       int cq[2] = {0, 0}, ck = 0;   // pieces with a query tile g, key tiles, before this piece
-      int turned = -RING - 1;       // the last key tile of the last piece of the turned kind
+      int turned = -RV - 1;         // the last key tile of the last piece of the turned kind
+      int cp = 0, few_pieces = 0;   // 8-bit pages: pages of K and V, pieces of the turned kind, before this piece
+      bool was_few = false;         // the piece before this one was of that kind
       for (int at = begin; alive && at < end; ++at) {
-        if (at == begin + 1) asm volatile("bar.sync 5, 384;" ::: "memory");   // (the list is there)
+        if (at == begin + 1) asm volatile("bar.sync 5, %0;" ::"n"(T::THREADS) : "memory");   // (the list is there)
         const int4* const e = at == begin ? reinterpret_cast<const int4*>(a.pieces + at) : chunk_words(a, list, begin, at);
         const int4 z = e[2];
         const int lead0 = z.y, lead1 = z.z;   // the pages of its first key tile
@@ -673,7 +749,12 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (!gemm_wait_warp(smem_u32(&q_empty[g]), (cq[g] & 1) ^ 1, abortp)) return false;
           ++cq[g];
           // Q1 lies where P of the turned kind did: behind its last product, which frees the last tile of V (where that place was used since, it has)
-          if (g && ck - turned <= RING && !gemm_wait_warp(smem_u32(&v_empty[turned % RING]), (turned / RING) & 1, abortp)) return false;
+          if constexpr (F8) {
+            // (of pieces before the one before this, the last products are done: their successor's queries have been asked for)
+            if (g && was_few && !gemm_wait_warp(smem_u32(&turn_free[(few_pieces - 1) & 1]), ((few_pieces - 1) >> 1) & 1, abortp)) return false;
+          } else {
+            if (g && ck - turned <= RV && !gemm_wait_warp(smem_u32(&v_empty[turned % RV]), (turned / RV) & 1, abortp)) return false;
+          }
           if (lane == 0) {
             const bool few = p.kind == CHUNK_FEW;
             mbar_arrive_expect_tx(&q_full[g], T::CH * a.G * (few ? a.few_tokens : a.tile_tokens) * 128);
@@ -691,21 +772,41 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         // In the order in which the MMAs ask for them.
         if (!(alive = fetch_q(0))) break;
         const int t0 = ck;
+        // two pages as they lie, one behind the other in memory each
+        auto fetch_codes = [&](const uint8_t* pool, int page0, int page1) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r, ++cp) {
+            const int i = cp % T::PAGES;
+            if (!gemm_wait_warp(smem_u32(&c_empty[i]), ((cp / T::PAGES) & 1) ^ 1, abortp)) return false;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&c_full[i], T::PAGE);
+              chunk_bulk(smC + i * T::PAGE, pool + ((size_t)(r ? page1 : page0) * a.Hkv + p.head) * T::PAGE, T::PAGE, smem_u32(&c_full[i]));
+            }
+          }
+          return true;
+        };
         for (int j = 0; j < p.n; ++j, ++ck) {
-          const int i = ck % RING, ph = (ck / RING) & 1;
           if (2 * (p.k0 + j) >= first + 32) {
             first += 32;
             ids = __ldg(pages + min(first + lane, last_page));
           }
           const int page0 = j == 0 ? lead0 : __shfl_sync(0xffffffffu, ids, 2 * (p.k0 + j) - first);
           const int page1 = j == 0 ? lead1 : __shfl_sync(0xffffffffu, ids, 2 * (p.k0 + j) + 1 - first);
-          if (!(alive = gemm_wait_warp(smem_u32(&k_empty[i]), ph ^ 1, abortp))) break;
-          fetch(&map_k, smK + i * T::TILE, &k_full[i], page0, page1);
-          if (j == 0 && !(alive = fetch_q(1))) break;
-          if (!(alive = gemm_wait_warp(smem_u32(&v_empty[i]), ph ^ 1, abortp))) break;
-          fetch(&map_v, smV + i * T::TILE, &v_full[i], page0, page1);
+          if constexpr (F8) {
+            if (!(alive = fetch_codes(a.k8, page0, page1))) break;
+            if (j == 0 && !(alive = fetch_q(1))) break;
+            if (!(alive = fetch_codes(a.v8, page0, page1))) break;
+          } else {
+            const int i = ck % RK, iv = ck % RV;
+            if (!(alive = gemm_wait_warp(smem_u32(&k_empty[i]), ((ck / RK) & 1) ^ 1, abortp))) break;
+            fetch(&map_k, smK + i * T::TILE, &k_full[i], page0, page1);
+            if (j == 0 && !(alive = fetch_q(1))) break;
+            if (!(alive = gemm_wait_warp(smem_u32(&v_empty[iv]), ((ck / RV) & 1) ^ 1, abortp))) break;
+            fetch(&map_v, smV + iv * T::TILE, &v_full[iv], page0, page1);
+          }
         }
-        if (p.kind == CHUNK_FEW) turned = t0 + p.n - 1;
+        if (p.kind == CHUNK_FEW) { turned = t0 + p.n - 1; ++few_pieces; }
+        was_few = p.kind == CHUNK_FEW;
       }
     }
     // ------------------------------------------------------------------------------------------------ MMAs
@@ -717,9 +818,10 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const uint32_t dq0 = (uint32_t)umma_desc_sw128(smQ), dq1 = (uint32_t)umma_desc_sw128(smQ1), dk0 = (uint32_t)umma_desc_sw128(smK), dv0 = (uint32_t)fap_desc_mn(smV);
       bool alive = true;   // a lane's own: once a wait expires it only keeps the lane from issuing
       int c[2] = {0, 0}, cq[2] = {0, 0}, ck = 0;   // tiles of group g, pieces with a query tile g, tiles of K and V, before this piece
+      int few_pieces = 0;                          // 8-bit pages: pieces of the turned kind before this one
       // scores of group g by query tile `tile`: S_g = Q K^T, or of the turned kind, whose rows' word of the instruction is `wide`, K Q^T
       auto qk = [&](int g, int tile, int t, uint32_t wide) {
-        uint32_t dq = tile ? dq1 : dq0, dk = dk0 + (t % RING) * (T::TILE >> 4);
+        uint32_t dq = tile ? dq1 : dq0, dk = dk0 + (t % RK) * (T::TILE >> 4);
         asm volatile("" : "+r"(dq), "+r"(dk));   // (what is made of them is made here, and not kept in registers that the warp does not have)
         if (wide) {
 #pragma unroll
@@ -733,7 +835,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         fap_commit(&s_full[g]);
       };
       auto pv = [&](int g, int t, bool first, uint32_t wide) {
-        uint32_t dv = dv0 + (t % RING) * (T::TILE >> 4);
+        uint32_t dv = dv0 + (t % RV) * (T::TILE >> 4);
         asm volatile("" : "+r"(dv));
         if (wide) {   // O^T += V^T P^T: V with its rows for K, P from shared memory
           uint32_t dp = dq1 + g * (T::P >> 4);
@@ -761,8 +863,8 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         p.cnt1 = __shfl_sync(0xffffffffu, p.cnt1, 0);
         return __shfl_sync(0xffffffffu, (int)more, 0) != 0;
       };
-      auto wait_k = [&](int t) { alive &= gemm_wait(smem_u32(&k_full[t % RING]), (t / RING) & 1, abortp); };
-      auto wait_v = [&](int t) { alive &= gemm_wait(smem_u32(&v_full[t % RING]), (t / RING) & 1, abortp); };
+      auto wait_k = [&](int t) { alive &= gemm_wait(smem_u32(&k_full[t % RK]), (t / RK) & 1, abortp); };
+      auto wait_v = [&](int t) { alive &= gemm_wait(smem_u32(&v_full[t % RV]), (t / RV) & 1, abortp); };
       // the first scores of group g of piece p, whose key tiles begin at tile t and whose query tiles are number q0, q1
       auto open = [&](const ChunkPiece& p, int g, int t, int q0, int q1) {
         const bool pair = p.kind == CHUNK_PAIR;
@@ -772,7 +874,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (elect_one() && alive) {
           qk(g, tile, t + step, wide_of(p));
-          if (!pair) fap_commit(&k_empty[(t + step) % RING]);                    // (of a pair, both tiles read the same keys)
+          if (!pair) fap_commit(&k_empty[(t + step) % RK]);                    // (of a pair, both tiles read the same keys)
           if (pair ? p.cnt(g) == 1 : step == p.n - 1) fap_commit(&q_empty[tile]);   // behind the last scores Q's place is free
         }
       };
@@ -800,31 +902,42 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           }
         };
         if (pair) {
-          if (elect_one() && alive) fap_commit(&k_empty[ck % RING]);
+          if (elect_one() && alive) fap_commit(&k_empty[ck % RK]);
           for (int j = 0; j < p.n; ++j) {
             const int t = ck + j;
             wait_v(t);
-            if (j + 1 < p.n) wait_k(t + 1);
+            if (!F8 && j + 1 < p.n) wait_k(t + 1);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               const int ng = p.cnt(g);
               if (j < ng) {
                 alive &= gemm_wait(smem_u32(&p_full[g]), (c[g] + j) & 1, abortp);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (elect_one() && alive) {
+                if constexpr (F8) {   // (the next keys are being converted: the product does not wait for them)
+                  if (elect_one() && alive) pv(g, t, j == 0, 0);
+                  if (j + 1 < ng) {
+                    wait_k(t + 1);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_one() && alive) {
+                      qk(g, g, t + 1, 0);
+                      if (j + 2 == ng) fap_commit(&q_empty[g]);
+                    }
+                  }
+                } else if (elect_one() && alive) {
                   pv(g, t, j == 0, 0);
                   if (j + 1 < ng) {
                     qk(g, g, t + 1, 0);
                     if (j + 2 == ng) fap_commit(&q_empty[g]);
                   }
                 }
-                // (the turned kind's P goes where Q1 is: not before this piece's last scores of tile 1 are on their way)
-                if (j + 1 == ng && (next.kind != CHUNK_FEW || g || j + 1 == p.n)) go_on(g);
+                // (the turned kind's P goes where Q1 is: not before this piece's last scores of tile 1 are on their way.  Where K has one place, the next piece's
+                // first keys come behind this one's last.)
+                if (j + 1 == ng && (!F8 || j + 1 == p.n) && (next.kind != CHUNK_FEW || g || j + 1 == p.n)) go_on(g);
               }
             }
             if (elect_one() && alive) {
-              fap_commit(&v_empty[t % RING]);
-              if (j + 1 < p.n) fap_commit(&k_empty[(t + 1) % RING]);
+              fap_commit(&v_empty[t % RV]);
+              if (j + 1 < p.n) fap_commit(&k_empty[(t + 1) % RK]);
             }
           }
         } else {
@@ -836,14 +949,15 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (elect_one() && alive) {
               pv(g, t, j < 2, 2 * wide);   // (P with the second halves of its weights)
-              fap_commit(&v_empty[t % RING]);
+              fap_commit(&v_empty[t % RV]);
+              if (F8 && wide && j + 1 == p.n) fap_commit(&turn_free[few_pieces & 1]);
             }
             if (j + 2 < p.n) {
               wait_k(t + 2);
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
               if (elect_one() && alive) {
                 qk(g, 0, t + 2, wide);
-                fap_commit(&k_empty[(t + 2) % RING]);
+                fap_commit(&k_empty[(t + 2) % RK]);
                 if (j + 3 == p.n) fap_commit(&q_empty[0]);
               }
             } else if (!(wide && next.kind == CHUNK_PAIR && g && j + 1 < p.n)) {   // (Q1 of a pair comes behind the last product that reads P)
@@ -853,10 +967,100 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         c[0] += p.cnt0; c[1] += p.cnt1; ck = tn;
         cq[0] = nq0; cq[1] = nq1;
+        few_pieces += p.kind == CHUNK_FEW;
+      }
+    }
+    // ------------------------------------------------------------------------------------------------ scales of 8-bit pages
+    if (F8 && warp == 10) {
+      bool alive = true;
+      int c[2] = {0, 0};
+      int at = begin;
+      ChunkPiece p;
+      while (alive && chunk_piece(a, list, begin, at, end, p)) {
+        const int32_t* const pages = a.table + (size_t)p.request * a.blocks;
+        const int last_page = (p.pos0 + p.tokens - 1) / kStepPage;
+        int first = 2 * p.k0;
+        float to_log2, value;   // of 32 pages from `first` on, a lane each
+        auto read = [&]() {
+          const size_t e = (size_t)__ldg(pages + min(first + lane, last_page)) * a.Hkv + p.head;
+          to_log2 = __ldg(a.k_scales + e) * a.scale_log2e;
+          value = __ldg(a.v_scales + e);
+        };
+        read();
+        for (int j = 0; alive && j < p.n; ++j) {
+          if (2 * (p.k0 + j) >= first + 32) {
+            first += 32;
+            read();
+          }
+          const int h = lane - (2 * (p.k0 + j) - first);   // 0, 1: the tile's pages
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (p.kind == CHUNK_PAIR ? j >= p.cnt(g) : (j & 1) != g) continue;
+            const int n = c[g]++, i = n % kChunkScales;
+            if (!(alive = gemm_wait_warp(smem_u32(&sc_empty[g][i]), ((n / kChunkScales) & 1) ^ 1, abortp))) break;
+            if (h == 0 || h == 1) {
+              float* const to = sc[g][i] + h;
+              to[0] = to_log2;
+              to[2] = log2f(value);
+              to[4] = 1.f / value;
+              to[6] = value;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sc_full[g][i]);
+          }
+        }
+      }
+    }
+    // ------------------------------------------------------------------------------------------------ 8-bit pages to bf16 tiles
+    // 16 codes of a row a thread at a time: 16 bytes read, two pieces of 16 bytes written, whose places in the swizzled tile are other banks for each of eight lanes
+    // (at head size 128 a row's second 64 features lie 16 KB behind: half of the lanes write their second piece first).
+    if (F8 && warp >= 12) {
+      const int ct = tid - 384;
+      constexpr int ROW = D / 16, PIECES = 64 * ROW / 128;   // 16-byte pieces of a row; of a page, a thread
+      const int c16 = ct % ROW, row0 = ct / ROW;
+      const int f0 = 2 * c16 + (D == 128 && c16 >= 4 ? 1 : 0);
+      bool alive = true;
+      int ck = 0, cp = 0;
+      int at = begin;
+      ChunkPiece p;
+      while (alive && chunk_piece(a, list, begin, at, end, p)) {
+        for (int j = 0; alive && j < p.n; ++j, ++ck) {
+#pragma unroll 1
+          for (int kv = 0; alive && kv < 2; ++kv) {
+            const int i = kv ? ck % RV : ck % RK, ph = kv ? (ck / RV) & 1 : (ck / RK) & 1;
+            uint64_t* const full = kv ? &v_full[i] : &k_full[i];
+            const uint32_t tile = kv ? smV + i * T::TILE : smK + i * T::TILE;
+#pragma unroll 1
+            for (int r = 0; r < 2; ++r, ++cp) {
+              const int q = cp % T::PAGES;
+              if (!(alive = gemm_wait_warp(smem_u32(&c_full[q]), (cp / T::PAGES) & 1, abortp))) break;
+              uint4 w[PIECES];
+#pragma unroll
+              for (int e = 0; e < PIECES; ++e) w[e] = lds128(smC + q * T::PAGE + (e * 128 + ct) * 16);
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&c_empty[q]);
+              if (r == 0 && !(alive = gemm_wait_warp(kv ? smem_u32(&v_empty[i]) : smem_u32(&k_empty[i]), ph ^ 1, abortp))) break;
+#pragma unroll
+              for (int e = 0; e < PIECES; ++e) {
+                const int row = r * 64 + row0 + e * (128 / ROW);
+                uint4 lo = make_uint4(chunk_widen(w[e].x, 0x1404), chunk_widen(w[e].x, 0x3424), chunk_widen(w[e].y, 0x1404), chunk_widen(w[e].y, 0x3424));
+                uint4 hi = make_uint4(chunk_widen(w[e].z, 0x1404), chunk_widen(w[e].z, 0x3424), chunk_widen(w[e].w, 0x1404), chunk_widen(w[e].w, 0x3424));
+                if (f0 & 1) { const uint4 t = lo; lo = hi; hi = t; }
+                const uint32_t dst = tile + (f0 >> 3) * 16384 + row * 128;
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (((f0 & 7) ^ (row & 7)) << 4)), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + ((((f0 ^ 1) & 7) ^ (row & 7)) << 4)), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+              }
+            }
+            if (!alive) break;
+            fence_proxy_async();   // generic-proxy stores -> the tensor core's async proxy
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full);
+          }
+        }
       }
     }
     // ------------------------------------------------------------------------------------------------ rows behind the last request's
-    if (warp == 10 && a.rest) {
+    if (warp == T::W_REST && a.rest) {
       const int row_words = a.Hq * D / 8;   // of 16 bytes
       for (long long e = ((long long)__ldg(a.row_starts + a.requests) + blockIdx.x) * row_words; e < (long long)a.rows * row_words; e += (long long)gridDim.x * row_words)
         for (int i = lane; i < row_words; i += 32) reinterpret_cast<uint4*>(a.out)[e + i] = make_uint4(0, 0, 0, 0);
@@ -869,21 +1073,57 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
 }
 
-template <int D>
+template <int D, bool F8 = false>
 static cudaError_t launch_chunk(const CUtensorMap (&m)[4], const ChunkArgs& a, cudaStream_t st) {
-  using T = ChunkTile<D>;
+  using T = ChunkTile<D, F8>;
   static std::atomic<unsigned long long> served{0};
   const cudaError_t set = once_per_device(served, [] {
     cudaFuncAttributes at;
-    const cudaError_t e = cudaFuncGetAttributes(&at, chunk_attn_kernel<D>);
+    const cudaError_t e = cudaFuncGetAttributes(&at, chunk_attn_kernel<D, F8>);
     if (e != cudaSuccess) return e;
     // the warps' register shares must fit what the block is launched with, or they would wait for registers for good
-    if (at.numRegs * T::THREADS < 8 * 32 * 216 + 4 * 32 * 64) return cudaErrorInvalidConfiguration;
-    return cudaFuncSetAttribute(chunk_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+    if (at.numRegs * T::THREADS < 8 * 32 * T::REGS_SOFTMAX + (T::THREADS - 256) * T::REGS_REST) return cudaErrorInvalidConfiguration;
+    return cudaFuncSetAttribute(chunk_attn_kernel<D, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
   });
   if (set != cudaSuccess) return set;
   count_launch();
-  return launch_pdl(chunk_attn_kernel<D>, dim3((unsigned)(num_sms() < kStepMaxCtas ? num_sms() : kStepMaxCtas)), dim3(T::THREADS), T::SMEM, st, m[0], m[1], m[2], m[3], a);
+  return launch_pdl(chunk_attn_kernel<D, F8>, dim3((unsigned)(num_sms() < kStepMaxCtas ? num_sms() : kStepMaxCtas)), dim3(T::THREADS), T::SMEM, st, m[0], m[1], m[2], m[3], a);
+}
+
+static size_t chunk_workspace_bytes(int D) { return kStepMaxCtas * 4 + (size_t)2 * kStepMaxCtas * (D == 128 ? kChunkRecord<128> : kChunkRecord<64>) * 4; }
+// the common part: q's maps, the plan's arrays
+template <bool F8>
+static int chunk_common(ChunkArgs& a, CUtensorMap* maps, void* out, const pie_head_rows* q, const int32_t* plan, const pie_step_dims* d, int D, float scale, int rest,
+                        void* workspace, size_t workspace_bytes) {
+  if ((D != 64 && D != 128) || !(scale > 0.f) || scale > 3.4028234e38f / 1.5f || q->stride_h % 8 || q->stride_l % 8 || (d->rows > 1 && q->stride_l <= 0) ||
+      (d->Hq > 1 && q->stride_h <= 0))
+    return PIE_EINVAL_SHAPE;
+  for (const void* p : {(const void*)out, q->p, (const void*)plan, (const void*)workspace})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return PIE_EALIGN;
+  if (!workspace || workspace_bytes < chunk_workspace_bytes(D)) return PIE_EWORKSPACE;
+  const StepLayout l = step_layout(*d);
+  a = {};
+  a.out = (uint16_t*)out; a.Hq = d->Hq; a.Hkv = d->Hkv; a.G = d->Hq / d->Hkv; a.tile_tokens = l.tile_tokens; a.rows = d->rows; a.requests = d->requests;
+  a.scale_log2e = scale * 1.4426950408889634f;
+  a.ranges = plan + l.ranges; a.table = plan + l.block_table; a.row_starts = plan + l.row_starts;
+  a.pieces = reinterpret_cast<const StepPiece*>(plan + l.pieces);
+  a.blocks = d->blocks; a.rest = rest;
+  a.count = (unsigned int*)workspace;
+  a.part = (float*)((uint8_t*)workspace + kStepMaxCtas * 4);
+  const GemmEncodeFn fn = gemm_encode_fn();
+  if (!fn) return PIE_ECUDA;
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  // a query tile, and one of the turned kind: 64 features of G heads of their tokens
+  a.few_tokens = (D == 128 ? ChunkTile<128, F8>::FEW : ChunkTile<64, F8>::FEW) / a.G;
+  for (int i = 0; i < 2; ++i) {
+    const long long head = (d->Hq > 1 ? q->stride_h : D) * 2, row = (d->rows > 1 ? q->stride_l : (long long)d->Hq * D) * 2;
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)d->Hq, (cuuint64_t)d->rows}, strides[2] = {(cuuint64_t)head, (cuuint64_t)row};
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)(i && a.few_tokens ? a.few_tokens : a.tile_tokens)};
+    if (fn(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q->p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return PIE_EUNSUPPORTED;
+  }
+  return PIE_OK;
 }
 
 }  // namespace pie
@@ -894,42 +1134,21 @@ using namespace pie;
 
 size_t pie_chunk_attn_workspace_bytes(const pie_step_dims* d, int D) {
   if (step_dims_status(d) || (D != 64 && D != 128)) return 0;
-  return kStepMaxCtas * 4 + (size_t)2 * kStepMaxCtas * (D == 128 ? kChunkRecord<128> : kChunkRecord<64>) * 4;
+  return chunk_workspace_bytes(D);
 }
 
 int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const void* vpool, const pie_kv_layout* kv, const int32_t* plan, const pie_step_dims* d, int D,
                    float scale, int rest, void* workspace, size_t workspace_bytes, void* stream) {
   if (int s = step_dims_status(d)) return s;
   if (!out || !q || !q->p || !kpool || !vpool || !kv || !plan) return PIE_ENULL;
-  if ((D != 64 && D != 128) || !(scale > 0.f) || scale > 3.4028234e38f / 1.5f || kv->tok_stride <= 0 || kv->tok_stride % 8 || kv->head_stride % 8 || q->stride_h % 8 ||
-      q->stride_l % 8 || (d->rows > 1 && q->stride_l <= 0) || (d->Hq > 1 && q->stride_h <= 0) || (d->Hkv > 1 && kv->head_stride <= 0))
-    return PIE_EINVAL_SHAPE;
-  for (const void* p : {(const void*)out, q->p, kpool, vpool, (const void*)plan, (const void*)workspace})
-    if (reinterpret_cast<uintptr_t>(p) & 15) return PIE_EALIGN;
-  if (!workspace || workspace_bytes < pie_chunk_attn_workspace_bytes(d, D)) return PIE_EWORKSPACE;
-  const StepLayout l = step_layout(*d);
+  if (kv->tok_stride <= 0 || kv->tok_stride % 8 || kv->head_stride % 8 || (d->Hkv > 1 && kv->head_stride <= 0)) return PIE_EINVAL_SHAPE;
   ChunkArgs a;
-  a.out = (uint16_t*)out; a.Hq = d->Hq; a.G = d->Hq / d->Hkv; a.tile_tokens = l.tile_tokens; a.rows = d->rows; a.requests = d->requests;
-  a.scale_log2e = scale * 1.4426950408889634f;
-  a.ranges = plan + l.ranges; a.table = plan + l.block_table; a.row_starts = plan + l.row_starts;
-  a.pieces = reinterpret_cast<const StepPiece*>(plan + l.pieces);
-  a.blocks = d->blocks; a.rest = rest;
-  a.count = (unsigned int*)workspace;
-  a.part = (float*)((uint8_t*)workspace + kStepMaxCtas * 4);
-  const GemmEncodeFn fn = gemm_encode_fn();
-  if (!fn) return PIE_ECUDA;
   CUtensorMap maps[4];
+  if (int s = chunk_common<false>(a, maps, out, q, plan, d, D, scale, rest, workspace, workspace_bytes)) return s;
+  for (const void* p : {kpool, vpool})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return PIE_EALIGN;
+  const GemmEncodeFn fn = gemm_encode_fn();
   const cuuint32_t one[4] = {1, 1, 1, 1};
-  // a query tile, and one of the turned kind: 64 features of G heads of their tokens
-  a.few_tokens = (D == 128 ? ChunkTile<128>::FEW : ChunkTile<64>::FEW) / a.G;
-  for (int i = 0; i < 2; ++i) {
-    const long long head = (d->Hq > 1 ? q->stride_h : D) * 2, row = (d->rows > 1 ? q->stride_l : (long long)d->Hq * D) * 2;
-    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)d->Hq, (cuuint64_t)d->rows}, strides[2] = {(cuuint64_t)head, (cuuint64_t)row};
-    const cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)(i && a.few_tokens ? a.few_tokens : a.tile_tokens)};
-    if (fn(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q->p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return PIE_EUNSUPPORTED;
-  }
   for (int i = 0; i < 2; ++i) {   // a page of one head: 64 features of its 64 slots
     const long long tok = kv->tok_stride * 2, head = d->Hkv > 1 ? kv->head_stride * 2 : tok;
     const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)kStepPage, (cuuint64_t)d->Hkv, (cuuint64_t)d->pages};
@@ -941,6 +1160,20 @@ int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const v
       return PIE_EUNSUPPORTED;
   }
   return status_of(D == 128 ? launch_chunk<128>(maps, a, (cudaStream_t)stream) : launch_chunk<64>(maps, a, (cudaStream_t)stream));
+}
+
+int pie_chunk_attn_fp8(void* out, const pie_head_rows* q, const uint8_t* kpool, const float* k_scales, const uint8_t* vpool, const float* v_scales, const int32_t* plan,
+                       const pie_step_dims* d, int D, float scale, int rest, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int s = step_dims_status(d)) return s;
+  if (!out || !q || !q->p || !kpool || !k_scales || !vpool || !v_scales || !plan) return PIE_ENULL;
+  ChunkArgs a;
+  CUtensorMap maps[4];
+  if (int s = chunk_common<true>(a, maps, out, q, plan, d, D, scale, rest, workspace, workspace_bytes)) return s;
+  for (const void* p : {(const void*)kpool, (const void*)vpool})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return PIE_EALIGN;
+  maps[2] = maps[3] = maps[0];   // (its keys and values come by address)
+  a.k8 = kpool; a.v8 = vpool; a.k_scales = k_scales; a.v_scales = v_scales;
+  return status_of(D == 128 ? launch_chunk<128, true>(maps, a, (cudaStream_t)stream) : launch_chunk<64, true>(maps, a, (cudaStream_t)stream));
 }
 
 }  // extern "C"

@@ -746,6 +746,81 @@ def chunk_attention(q, k_pool, v_pool, plan, scale: float, out=None):
     return out
 
 
+_F8 = torch.float8_e4m3fn
+
+
+def _fp8_pools(what: str, k_pool, k_scales, v_pool, v_scales, d: StepDims, D: int):
+    for pool, scales in ((k_pool, k_scales), (v_pool, v_scales)):
+        if pool.dtype != _F8 or tuple(pool.shape) != (d.pages, d.Hkv, 64, D) or not pool.is_contiguous() or pool.data_ptr() % 16:
+            raise ValueError(f"[{what}] the plan is for {d.pages} pages of {d.Hkv} heads: pools must be contiguous float8_e4m3fn {[d.pages, d.Hkv, 64, D]}, but one is {pool.dtype} "
+                             f"{list(pool.shape)}")
+        if scales.dtype != torch.float32 or tuple(scales.shape) != (d.pages, d.Hkv) or not scales.is_contiguous():
+            raise ValueError(f"[{what}] scales must be contiguous float32 {[d.pages, d.Hkv]}, but are {scales.dtype} {list(scales.shape)}")
+
+
+def _fp8_plan(what: str, plan, T: int, Hq: int, D: int):
+    if D not in (64, 128):
+        raise ValueError(f"[{what}] head size {D} is not built here (64 or 128)")
+    if (T, Hq) != (plan.dims.rows, plan.dims.Hq):
+        raise ValueError(f"[{what}] the plan is for {plan.dims.rows} rows of {plan.dims.Hq} heads, but queries are {[T, Hq, D]}")
+    _step_ints(what, "plan.words", plan.words, (_lib.load().pie_step_plan_words(C.byref(plan.dims)),))
+
+
+def rope_kv_fp8(queries, keys, values, freqs, plan, k_pool, k_scales, v_pool, v_scales, out=None):
+    """rope_kv_slots into a cache of 8 bits: queries [T, Hq, D] and keys [T, Hkv, D] rotated at each row's own position, keys and values [T, Hkv, D] written to the pages of their
+    requests (plan: the step's ragged.StepPlan) as float8_e4m3fn pools [pages, Hkv, 64, D] with scales f32 [pages, Hkv]: a feature is its code times its page's and head's scale.  The
+    scale is the lowest power of two, 2^-60 at least, with which all features that were written since the page's first token are 448 or less; a row at a page's first place begins the
+    page anew, and a row that needs a larger scale has what the page holds in front of it brought to that, by a power of two and so without another rounding, but below e4m3's lowest.  A
+    page and head that an infinity or a NaN was written to has scale NaN.  No two requests of a plan may write to the same page.  Returns the rotated queries, [T, Hq, D]; rows that
+    belong to nobody as rope_kv_slots has them."""
+    what = "rope_kv_fp8"
+    if queries.dim() != 3 or keys.dim() != 3 or values.shape != keys.shape or keys.shape[0] != queries.shape[0] or keys.shape[2] != queries.shape[2]:
+        raise ValueError(f"[{what}] queries [T, Hq, D], keys and values [T, Hkv, D] expected, but they are {tuple(queries.shape)}, {tuple(keys.shape)} and "
+                         f"{tuple(values.shape)}")
+    T, Hq, D = queries.shape
+    if any(t.dtype != _BF16 for t in (queries, keys, values)):
+        raise ValueError(f"[{what}] only bfloat16 is built here")
+    if freqs.dtype != torch.float32 or tuple(freqs.shape) != (D // 2,) or not freqs.is_contiguous():
+        raise ValueError(f"[{what}] freqs must be contiguous float32 [{D // 2}], but is {freqs.dtype} {list(freqs.shape)}")
+    _fp8_plan(what, plan, T, Hq, D)
+    d = plan.dims
+    if keys.shape[1] != d.Hkv:
+        raise ValueError(f"[{what}] the plan is for {d.Hkv} heads of keys, but they are {tuple(keys.shape)}")
+    _fp8_pools(what, k_pool, k_scales, v_pool, v_scales, d, D)
+    _check_out(what, out, (T, Hq, D))
+    with _one_device(what, queries, keys, values, freqs, plan.words, k_pool, k_scales, v_pool, v_scales, *(() if out is None else (out,))):
+        out, rest = _fresh(out, (T, Hq, D), queries.device)
+        held = [_head_rows(t) for t in (queries, keys, values)]
+        _lib.check(_lib.load().pie_rope_kv_fp8(_p(out), _p(k_pool), _p(k_scales), _p(v_pool), _p(v_scales), *(C.byref(r) for _, r in held), _p(plan.words), C.byref(d),
+                                               _p(freqs), D, rest, _stream()), what)
+    return out
+
+
+def chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan, scale: float, out=None):
+    """chunk_attention over a cache of 8 bits (rope_kv_fp8): row t of q [T, Hq, D] attends to the keys 0 .. position of its own request, a key and a value being their codes times their
+    pages' scales.  Returns [T, Hq * D].  Softmax weights are multiplied with the values' scales and then rounded for their product with the codes: to 16 bits (two bfloat16) where a
+    request's rows, its new tokens x Hq / Hkv, are at most 32, and to bfloat16 otherwise.  A page of scale NaN may make all of its request's new tokens NaN; a code of NaN counts as 480.
+    Rows that belong to nobody are zero, or with ``out`` given what that held."""
+    what = "chunk_attention_fp8"
+    if q.dim() != 3 or q.dtype != _BF16:
+        raise ValueError(f"[{what}] queries must be bfloat16 [T, Hq, D], but are {q.dtype} {tuple(q.shape)}")
+    T, Hq, D = q.shape
+    _fp8_plan(what, plan, T, Hq, D)
+    d = plan.dims
+    _fp8_pools(what, k_pool, k_scales, v_pool, v_scales, d, D)
+    if not scale > 0:
+        raise ValueError(f"[{what}] scale must be positive, but is {scale}")
+    _check_out(what, out, (T, Hq * D))
+    with _one_device(what, q, k_pool, k_scales, v_pool, v_scales, plan.words, *(() if out is None else (out,))):
+        L = _lib.load()
+        out, rest = _fresh(out, (T, Hq * D), q.device)
+        held, rows = _head_rows(q)
+        ws = workspaces.get("chunk", L.pie_chunk_attn_workspace_bytes(C.byref(d), D), q.device)
+        _lib.check(L.pie_chunk_attn_fp8(_p(out), C.byref(rows), _p(k_pool), _p(k_scales), _p(v_pool), _p(v_scales), _p(plan.words), C.byref(d), D, float(scale), rest, _p(ws),
+                                        ws.numel(), _stream()), what)
+    return out
+
+
 def verify_draft(logits, draft_tokens, logit_starts, *, max_draft: int, temp: float = 0.0, uniforms=None, noise=None, draft_logits=None):
     """Drafted tokens against the target's probabilities, and the token behind the accepted ones.  Request s has rows logit_starts[s] .. logit_starts[s + 1] - 1
     of logits (bf16 [R, vocab]): row r judges draft_tokens[r] (int32 [R]), a request's last row none (StepPlan has both arrays).
