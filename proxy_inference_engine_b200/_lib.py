@@ -168,6 +168,7 @@ SIGNATURES = {
     "pie_chunk_attn_workspace_bytes": (_sz, [C.POINTER(StepDims), _i]),
     "pie_chunk_attn": (_i, [_vp, C.POINTER(HeadRows), _vp, _vp, C.POINTER(KvLayout), _vp, C.POINTER(StepDims), _i, _f, _i, _vp, _sz, _vp]),
     "pie_rope_kv_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, C.POINTER(HeadRows), C.POINTER(HeadRows), C.POINTER(HeadRows), _vp, C.POINTER(StepDims), _vp, _i, _i, _vp]),
+    "pie_chunk_attn_fp8_workspace_bytes": (_sz, [C.POINTER(StepDims), _i]),
     "pie_chunk_attn_fp8": (_i, [_vp, C.POINTER(HeadRows), _vp, _vp, _vp, _vp, _vp, C.POINTER(StepDims), _i, _f, _i, _vp, _sz, _vp]),
     "pie_verify_workspace_bytes": (_sz, [_i, _i, _i]),
     "pie_verify_draft": (_i, [_vp, _vp, _vp, _vp, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp, _vp, _sz, _vp]),

@@ -26,6 +26,8 @@
 // busy for 54 % of it, as in the prompt's kernel one tile's softmax is covered by the other's products in part); 16 answers with up to five drafted tokens over 4000 keys 51.6 (4.4 TB/s),
 // 40 over 12000 309 (6.4 TB/s), one with four over 9000 26.3; D 64, three portions of 700 tokens beside 29 answers over 1500 keys 83.9, 40 answers over 12000 220 (4.5 TB/s).  Short
 // steps pay 4 us from the launch to the first scores, some 3 at each turn from one piece to the next and 5 at the end: results, one counter, the last CTA's sums.
+#include <type_traits>
+
 #include "pie_step_plan.h"
 
 namespace pie {
@@ -42,10 +44,12 @@ struct ChunkArgs {
   float* part;                 // [2 CTAs] records
   int rest;
   int few_tokens;              // tokens of an item of the turned kind, at most
-  // 8-bit pages: codes [pages, Hkv, 64, D], scales [pages, Hkv]
-  const uint8_t *k8, *v8;
+  // 8-bit pages: their scales [pages, Hkv], and queries as they lie (elements between rows, between heads)
   const float *k_scales, *v_scales;
+  const int32_t* contexts;
   int Hkv;
+  const uint16_t* q;
+  long long q_row, q_head;
 };
 template <int D>
 constexpr int kChunkRecord = 256 * D + 512;   // floats: results, [64 rows][D] of the turned kind, [D / 4][256 rows][4] of the others; [256] maxima and sums
@@ -55,22 +59,16 @@ constexpr int kChunkList = 32;                // pieces held in shared memory; a
 template <int D, bool F8 = false>
 struct ChunkTile {
   static constexpr int CH = D / 64, TILE = 128 * D * 2;          // 64-feature chunks of a row, bytes of 128 rows
-  static constexpr int RK = F8 ? (D == 64 ? 2 : 1) : D == 64 ? 4 : 2;   // tiles of K
-  static constexpr int RV = F8 ? 2 : RK;                         // tiles of V
-  static constexpr int FEW = F8 ? 32 : D == 64 ? 64 : 48;        // rows of an item of the turned kind, at most: as shared memory has room for their weights
-  static constexpr int HALVES = (FEW + 31) / 32;                 // of 32 rows
+  static constexpr int RING = D == 64 ? 4 : 2;                   // tiles of K, and of V: 64 KB of each
+  static constexpr int FEW = F8 || D == 64 ? 64 : 48;            // rows of an item of the turned kind, at most: as shared memory has room for their weights
   static constexpr int PCHUNK = 2 * FEW * 128;                   // bytes of 64 keys of a group's P of the turned kind: eight rows' first halves, their second halves, ...
   static constexpr int P = 2 * PCHUNK;
-  static constexpr int Q1 = TILE > 2 * P ? TILE : 2 * P;         // the second query tile; the turned kind's P
-  static constexpr int PAGE = 64 * D, PAGES = F8 ? (D == 64 ? 16 : 6) : 1;   // bytes of a page of one head in 8 bits, and how many of them wait to be converted
-  static constexpr int SMEM = 1024 + TILE + Q1 + (RK + RV) * TILE + (F8 ? PAGES * PAGE : 0);
-  static constexpr int THREADS = F8 ? 512 : 384;
-  // warps 0-7 softmax, 8 TMA, 9 MMAs, 10 scales (8-bit pages), W_REST rows of nobody, 12-15 conversion (8-bit pages)
-  static constexpr int W_REST = F8 ? 11 : 10;
-  // Registers, which must not exceed what the block is launched with: 384 x 168 = 64512, 256 x 216 and 128 x 64 are 63488; 512 x 128 = 65536 = 256 x 208 and 256 x 48
-  static constexpr int REGS_SOFTMAX = F8 ? 208 : 216, REGS_REST = F8 ? 48 : 64;
+  static constexpr int Q1 = F8 || TILE > 2 * P ? TILE : 2 * P;   // the second query tile; the turned kind's P (8-bit pages: its warps' results)
+  static constexpr int PLACES = 2 * RING;                        // 8-bit pages, turned kind: a key tile's codes of K and of V take one tile's place
+  static constexpr int SMEM = 1024 + TILE + Q1 + 2 * RING * TILE;
+  static constexpr int THREADS = 384;
 };
-constexpr int kChunkScales = 4;               // 8-bit pages: key tiles of a group whose scales are held
+constexpr int kChunkScales = 8;               // 8-bit pages: key tiles whose scales are held
 
 enum ChunkKind { CHUNK_PAIR, CHUNK_ONE, CHUNK_FEW };
 // a piece as the roles walk it
@@ -218,34 +216,351 @@ __device__ __forceinline__ void chunk_merge(uint16_t* out, const float* part, in
   }
 }
 
-// 16 codes of 8 bits as bf16, exactly: the code's bits in the places of a bf16's are a number 2^120 times smaller (and e4m3's subnormals bf16's)
-__device__ __forceinline__ uint32_t chunk_widen(uint32_t w, uint32_t sel) {
-  const uint32_t x = __byte_perm(w, 0, sel), y = ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u);
+struct ChunkMaps8 { CUtensorMap k, v; };   // of the codes, a page of a head
+struct ChunkNone {};
+// what the turned kind over 8-bit pages keeps of its rows: a warp's maxima and sums
+struct ChunkFew8 { float2 ml[8][16]; };
+struct ChunkFew8Bars { uint64_t *f_full, *f_empty, *sc_full, *sc_empty; const float4* sc; };
+// two codes as fp16, exactly; numbers to codes
+__device__ __forceinline__ uint32_t chunk_f16(uint32_t two) {
   uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(y), "r"(0x7b807b80u));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"((uint16_t)two));
   return d;
 }
-__device__ __forceinline__ void chunk_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+__device__ __forceinline__ void chunk_f32(uint32_t f16x2, float& lo, float& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(lo), "=f"(hi) : "r"(f16x2));
+}
+__device__ __forceinline__ uint32_t chunk_codes4(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return lo | ((uint32_t)hi << 16);
+}
+__device__ __forceinline__ void chunk_mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void chunk_mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t chunk_pack_f16(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ uint32_t chunk_turn8x8(uint32_t x) {   // an 8 x 8 matrix of 16-bit numbers, two of a row a lane, turned around
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
+// where 16 bytes of a row of a page lie in its place in shared memory
+template <int D>
+__device__ __forceinline__ uint32_t chunk_code_at(int row, int c16) {
+  return D == 128 ? row * 128 + ((c16 ^ (row & 7)) << 4) : row * 64 + ((c16 ^ ((row >> 1) & 3)) << 4);
+}
+
+// A piece of few rows over 8-bit pages, by the eight softmax warps, whose A operand is made of the codes in registers: what bounds it is the stream of pages, and a detour of widened codes
+// through shared memory (store, fence, barrier, tcgen05) took 2.9 us a key tile where the stream takes 0.75.
+// S^T = K Q^T of 16 keys at a time: codes are an e4m3 MMA's operand as they lie.  A query, brought to 2^7 .. 2^8 by a power of two for each row, is the sum of two e4m3 numbers -- its first
+// four and its last four bits, nothing else is lost but what is 2^-17 of the row's largest -- and the products of both are added up.  (That MMA has four times fp16's rate: 1.1 cycles of an SM
+// for 16 x 8 x 32, fp16's 2.0 for 16 x 8 x 16.)  O^T = V^T P^T in fp16, the codes widened (exactly), weights rounded to 2^-12 of one; sums are fp32.
+// A lane (g, t = lane / 4, lane % 4) has rows g and g + 8 of A and the columns 2 t, 2 t + 1 of the results.  Which features make up a step and which rows are V's features is free, so that a
+// lane's codes are whole pieces: of K the features D / 4 t .. of its two keys; of V the features D / 8 g .. of its four keys, two to a tile, neighbouring keys' codes put together by a byte
+// permutation.  A page's scale of K is applied to the scores; that of V to the weights, relative to the largest so far, which the results are in units of, or where it is below
+// 2^-16 of that, whose weights fp16 might not hold, to the page's product.
+// 16 rows a warp: up to 16 of an item go to eight slices of 16 keys of a tile, 32 to two sets of four slices of 32, 64 to four of two.  Every warp has its own running maximum; the warps'
+// results meet at the end in shared memory, eight rows of each set at a time.
+template <int D, int NT>
+__device__ __forceinline__ bool chunk_few8(const ChunkArgs& a, const ChunkPiece& p, ChunkFew8& few, uint32_t smP, uint32_t smO, const ChunkFew8Bars& bars, volatile int* abortp, int cf,
+                                           bool alive, int rows, bool whole, float* rec) {
+  using T = ChunkTile<D, true>;
+  constexpr int KC = D / 64, VW = D / 32;          // 16-byte pieces of K of a key, 32-bit words of V of a key, a lane
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int sets_log = rows <= 16 ? 0 : rows <= 32 ? 1 : 2, slices = 8 >> sets_log, slice = warp & (slices - 1), set = warp >> (3 - sets_log), row_first = 16 * set;
+  const int keys = 16 << sets_log, key0 = slice * keys, page = key0 >> 6, in_page = key0 & 63;
+  // queries: the rows 8 n + g, as two codes a feature
+  uint32_t qh[NT][D / 16], ql[NT][D / 16];
+  float scale[NT][2];                               // of the columns' rows
+  int own[NT][2];                                   // and their tokens
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = row_first + 8 * n + g, tok = row / a.G;
+    uint4 x[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (row < rows)
+        x[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (p.row0 + tok) * a.q_row + (p.head * a.G + row - tok * a.G) * a.q_head + t * (D / 4)) + i);
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      constexpr uint32_t ABS = 0x7fff7fffu;
+      m = __vmaxu2(__vmaxu2(__vmaxu2(m, x[i].x & ABS), __vmaxu2(x[i].y & ABS, x[i].z & ABS)), x[i].w & ABS);
+    }
+    m = max(m & 0xffffu, m >> 16);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    // (rows of less than 2^-95, whose scores are 0, as they are; an infinity or a NaN makes the row's scores NaN)
+    const int e = m < 0x1000u ? 127 + 7 : min((int)(m >> 7), 254);
+    const float up = __uint_as_float((uint32_t)(127 + 7 + 127 - e) << 23), down = m >= 0x7f80u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(e - 7) << 23);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float v0 = bf16lo(w[2 * h]) * up, v1 = bf16hi(w[2 * h]) * up, v2 = bf16lo(w[2 * h + 1]) * up, v3 = bf16hi(w[2 * h + 1]) * up;
+        const uint32_t c = chunk_codes4(v0, v1, v2, v3);
+        float c0, c1, c2, c3;
+        chunk_f32(chunk_f16(c), c0, c1);
+        chunk_f32(chunk_f16(c >> 16), c2, c3);
+        qh[n][2 * i + h] = c;
+        ql[n][2 * i + h] = chunk_codes4(v0 - c0, v1 - c1, v2 - c2, v3 - c3);
+      }
+    }
+    scale[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+    scale[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+    own[n][0] = (row_first + 8 * n + 2 * t) / a.G;
+    own[n][1] = (row_first + 8 * n + 2 * t + 1) / a.G;
+  }
+  float o[NT][D / 16][4], m[NT][2], l[NT][2], unit = 0.f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.f;
+  }
+  for (int j = 0; j < p.n; ++j, ++cf) {
+    const int place = cf % T::PLACES, is = cf % kChunkScales;
+    alive = alive && gemm_wait_warp(smem_u32(&bars.sc_full[is]), (cf / kChunkScales) & 1, abortp);
+    const float4 of = bars.sc[is];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars.sc_empty[is]);
+    alive = alive && gemm_wait_warp(smem_u32(&bars.f_full[place]), (cf / T::PLACES) & 1, abortp);
+    if (!alive) break;   // (and on through the barriers)
+    const float to_log2 = page ? of.y : of.x, value = page ? of.w : of.z;
+    const uint32_t sk = smP + place * T::TILE + page * (64 * D), sv = sk + 2 * (64 * D);
+    const int beyond = (p.k0 + j) * 128 + 64 * page - p.pos0;   // the page's first key, from the first row's own on
+    if (value > unit) {
+      const float f = unit / value;
+      unit = value;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][i][e] *= f;
+    }
+    const float ratio = value / unit;
+    const bool near = ratio >= 0x1p-16f;
+    const float weight = near ? 16.f * ratio : 16.f;   // (results are 16 times what they are: the weights' lowest are 2^-29 of one)
+#pragma unroll 1
+    for (int kk = 0; kk < keys; kk += 16) {
+      const int k_row = in_page + kk;
+      float s[NT][4], s2[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.f;
+#pragma unroll
+      for (int h = 0; h < KC; ++h) {
+        const uint4 u = lds128(sk + chunk_code_at<D>(k_row + g, KC * t + h)), v = lds128(sk + chunk_code_at<D>(k_row + g + 8, KC * t + h));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          chunk_mma_e4m3(s[n], u.x, v.x, u.y, v.y, qh[n][4 * h], qh[n][4 * h + 1]);
+          chunk_mma_e4m3(s2[n], u.x, v.x, u.y, v.y, ql[n][4 * h], ql[n][4 * h + 1]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          chunk_mma_e4m3(s[n], u.z, v.z, u.w, v.w, qh[n][4 * h + 2], qh[n][4 * h + 3]);
+          chunk_mma_e4m3(s2[n], u.z, v.z, u.w, v.w, ql[n][4 * h + 2], ql[n][4 * h + 3]);
+        }
+      }
+      // values of the keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+      uint32_t w[4][VW];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = k_row + 2 * t + (i & 1) + 8 * (i >> 1);
+        if (D == 128) {
+          const uint4 u = lds128(sv + chunk_code_at<D>(r, g));
+          w[i][0] = u.x; w[i][1] = u.y; w[i][VW - 2] = u.z; w[i][VW - 1] = u.w;
+        } else {
+          const uint2 u = lds64(sv + chunk_code_at<D>(r, g >> 1) + 8 * (g & 1));
+          w[i][0] = u.x; w[i][1] = u.y;
+        }
+      }
+      // scores in log2 units; keys beyond a row's own
+      bool over = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + s2[n][e]) * (to_log2 * scale[n][e & 1]);
+      if (beyond + k_row + 15 > 0) {
+        const int key = beyond + k_row + g;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (key > own[n][e]) s[n][e] = -INFINITY;
+            if (key + 8 > own[n][e]) s[n][2 + e] = -INFINITY;
+          }
+        // behind the item's last key there may be anything: 0 * NaN is not 0
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (beyond + k_row + 2 * t + (i & 1) + 8 * (i >> 1) >= p.tokens)
+#pragma unroll
+            for (int h = 0; h < VW; ++h) w[i][h] = 0;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) over = over || fmaxf(s[n][e], s[n][2 + e]) > m[n][e] + 8.f;
+      // the reference of a row moves where a score exceeds it by 8
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(s[n][e], s[n][2 + e]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            if (x > m[n][e] + 8.f) {
+              const float f = m[n][e] == -INFINITY ? 0.f : fap_exp2(m[n][e] - x);
+              m[n][e] = x;
+              l[n][e] *= f;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) { o[n][i][e] *= f; o[n][i][2 + e] *= f; }
+            }
+          }
+      }
+      uint32_t b[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+        s[n][0] = fap_exp2(s[n][0] - m0); s[n][1] = fap_exp2(s[n][1] - m1);
+        s[n][2] = fap_exp2(s[n][2] - m0); s[n][3] = fap_exp2(s[n][3] - m1);
+        l[n][0] += s[n][0] + s[n][2];
+        l[n][1] += s[n][1] + s[n][3];
+        b[n][0] = chunk_turn8x8(chunk_pack_f16(s[n][0] * weight, s[n][1] * weight));
+        b[n][1] = chunk_turn8x8(chunk_pack_f16(s[n][2] * weight, s[n][3] * weight));
+      }
+      auto values = [&](int i, uint32_t (&v)[4]) {
+        const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
+        const uint32_t lo = __byte_perm(w[0][i >> 1], w[1][i >> 1], sel), hi = __byte_perm(w[2][i >> 1], w[3][i >> 1], sel);
+        v[0] = chunk_f16(lo); v[1] = chunk_f16(lo >> 16); v[2] = chunk_f16(hi); v[3] = chunk_f16(hi >> 16);
+      };
+      if (near) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t v[4];
+          values(i, v);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) chunk_mma_f16(o[n][i], v[0], v[1], v[2], v[3], b[n][0], b[n][1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t v[4];
+          values(i, v);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            chunk_mma_f16(d, v[0], v[1], v[2], v[3], b[n][0], b[n][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][i][e] = fmaf(d[e], ratio, o[n][i][e]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars.f_empty[place]);
+  }
+  // sums over the lanes of a column, then the slices' maxima and sums
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[n][e];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      if (g == 0) few.ml[warp][8 * n + 2 * t + e] = make_float2(m[n][e], x);
+    }
+  chunk_sync();
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int col = 8 * n + 2 * t + e, row = row_first + col;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+      for (int w = 0; w < slices; ++w) top = fmaxf(top, few.ml[set * slices + w][col].x);
+#pragma unroll 1
+      for (int w = 0; w < slices; ++w) {
+        const float2 x = few.ml[set * slices + w][col];
+        sum += x.x == -INFINITY ? 0.f : x.y * fap_exp2(x.x - top);
+      }
+      float f = m[n][e] == -INFINITY ? 0.f : fap_exp2(m[n][e] - top) * (unit * 0.0625f);
+      if (whole) f /= sum;
+      else if (slice == 0 && g == 0 && row < rows) __stcg(reinterpret_cast<float2*>(rec + 256 * D + 2 * row), make_float2(top, sum));
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) { o[n][i][e] *= f; o[n][i][2 + e] *= f; }
+    }
+  // eight rows of each set at a time: [warp][row][D] fp32, the 16-byte pieces of a row in another order for every other row
+  constexpr int LANES = D / 4;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (n > 0) chunk_sync();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t to = smO + (warp * 8 + 2 * t + e) * D * 4;
+#pragma unroll
+      for (int i = 0; i < D / 16; i += 2)   // features D / 8 g + 2 i ..
+        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((g * (D / 32) + (i >> 1)) ^ t) << 4)), "f"(o[n][i][e]), "f"(o[n][i][2 + e]), "f"(o[n][i + 1][e]),
+                     "f"(o[n][i + 1][2 + e]) : "memory");
+    }
+    chunk_sync();
+#pragma unroll 1
+    for (int x = tid; x < (8 << sets_log) * LANES; x += 256) {
+      const int c4 = x % LANES, r8 = x / LANES % 8, of_set = x / (8 * LANES), row = 16 * of_set + 8 * n + r8;
+      if (row >= rows) continue;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int w = 0; w < slices; ++w) {
+        const uint4 u = lds128(smO + ((of_set * slices + w) * 8 + r8) * D * 4 + ((c4 ^ (r8 >> 1)) << 4));
+        sum.x += __uint_as_float(u.x); sum.y += __uint_as_float(u.y); sum.z += __uint_as_float(u.z); sum.w += __uint_as_float(u.w);
+      }
+      const int tok = row / a.G;
+      if (whole)
+        *reinterpret_cast<uint2*>(a.out + ((size_t)(p.row0 + tok) * a.Hq + p.head * a.G + row - tok * a.G) * D + 4 * c4) = make_uint2(pack_bf16(sum.x, sum.y), pack_bf16(sum.z, sum.w));
+      else
+        __stcg(reinterpret_cast<float4*>(rec + row * D + 4 * c4), sum);
+    }
+  }
+  fence_proxy_async();   // (what lies there is read: a query tile may be copied there)
+  chunk_sync();
+  return alive;
 }
 
 template <int D, bool F8>
 __global__ void __launch_bounds__(ChunkTile<D, F8>::THREADS, 1)
 chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_few, const __grid_constant__ CUtensorMap map_k,
-                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ChunkArgs a) {
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ typename std::conditional<F8, ChunkMaps8, ChunkNone>::type codes8,
+                  const __grid_constant__ ChunkArgs a) {
   using T = ChunkTile<D, F8>;
-  constexpr int RK = T::RK, RV = T::RV;
+  constexpr int RING = T::RING;
   constexpr uint32_t ID_S = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
   constexpr uint32_t ID_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
   constexpr uint32_t ID_FEW = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);   // | N
   constexpr int COL_S = 0, COL_O = 256, OST = 128;   // + g * 128, + g * OST
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[RK], k_empty[RK], v_full[RV], v_empty[RV], s_full[2], p_full[2], o_full[2];
-  // 8-bit pages: pages as they lie, scales of a group's key tiles, products behind which the turned kind's P is free (pieces of that kind in turn)
-  __shared__ __align__(8) uint64_t c_full[T::PAGES], c_empty[T::PAGES], sc_full[2][F8 ? kChunkScales : 1], sc_empty[2][F8 ? kChunkScales : 1], turn_free[2];
-  __shared__ __align__(16) float sc[2][F8 ? kChunkScales : 1][8];   // of the two pages: scores to log2 units, log2 of the values' scale, its reciprocal, itself
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[RING], k_empty[RING], v_full[RING], v_empty[RING], s_full[2], p_full[2], o_full[2];
   __shared__ __align__(16) int4 list[3 * kChunkList];
-  __shared__ __align__(16) ChunkFew few;
+  // 8-bit pages: places of the turned kind's tiles, scales of its tiles, and whether a piece's results have left the place of the second query tile (in turn)
+  __shared__ __align__(8) uint64_t f_full[F8 ? T::PLACES : 1], f_empty[F8 ? T::PLACES : 1], sc_full[F8 ? kChunkScales : 1], sc_empty[F8 ? kChunkScales : 1], turn_free[2];
+  __shared__ __align__(16) float4 sc[F8 ? kChunkScales : 1];   // of the two pages: scores to log2 units, the values' scale
+  __shared__ __align__(16) typename std::conditional<F8, ChunkFew8, ChunkFew>::type few;
   __shared__ float2 ml[2][128];           // a row's maximum and sum: of the two groups of a tile, of the rows of a cut item
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag, last_flag;
@@ -253,18 +568,20 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   // (The turned kind's P lies where Q1 does.  Its V^T has 128 rows whatever the head size: at 64 the upper ones are what lies 16 KB behind, so V does not lie last.)
-  const uint32_t smV = base, smK = smV + RV * T::TILE, smQ = smK + RK * T::TILE, smQ1 = smQ + T::TILE, smC = smQ1 + T::Q1;
+  const uint32_t smV = base, smK = smV + RING * T::TILE, smQ = smK + RING * T::TILE, smQ1 = smQ + T::TILE;
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1);
     }
-    for (int i = 0; i < RK; ++i) { mbar_init(&k_full[i], F8 ? 4 : 1); mbar_init(&k_empty[i], 1); }
-    for (int i = 0; i < RV; ++i) { mbar_init(&v_full[i], F8 ? 4 : 1); mbar_init(&v_empty[i], 1); }
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
+    }
     if (F8) {
-      for (int i = 0; i < T::PAGES; ++i) { mbar_init(&c_full[i], 1); mbar_init(&c_empty[i], 4); }
-      for (int i = 0; i < 2 * kChunkScales; ++i) { mbar_init(&sc_full[0][0] + i, 1); mbar_init(&sc_empty[0][0] + i, 4); }
+      for (int i = 0; i < T::PLACES; ++i) { mbar_init(&f_full[i], 1); mbar_init(&f_empty[i], 8); }
+      for (int i = 0; i < kChunkScales; ++i) { mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 8); }
       for (int i = 0; i < 2; ++i) mbar_init(&turn_free[i], 1);
     }
     abort_flag = 0;
@@ -274,7 +591,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (warp == 8 && lane < (F8 ? 2 : 4)) tma_prefetch_desc(lane == 0 ? &map_q : lane == 1 ? &map_few : lane == 2 ? &map_k : &map_v);
+  if (warp == 8 && lane < 4) tma_prefetch_desc(lane == 0 ? &map_q : lane == 1 ? &map_few : lane == 2 ? &map_k : &map_v);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -287,39 +604,32 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (warp != 8) {
     for (int i = warp < 8 ? tid : tid - 32; i < 3 * min(end - begin, kChunkList); i += T::THREADS - 32)
       list[i] = __ldg(reinterpret_cast<const int4*>(a.pieces + begin) + i);
-    asm volatile("bar.sync 4, %0;" ::"n"(T::THREADS - 32) : "memory");
-    if (end - begin > 1) asm volatile("bar.arrive 5, %0;" ::"n"(T::THREADS) : "memory");
+    asm volatile("bar.sync 4, 352;" ::: "memory");
+    if (end - begin > 1) asm volatile("bar.arrive 5, 384;" ::: "memory");
   }
 
   // All barriers are counted over the CTA's pieces: a role keeps the number of key tiles (of its group, of K and V) before its piece.
+  // Registers: 384 threads x 168 at launch = 64512; 8 warps of 216 and 4 of 64 are 63488.
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::REGS_SOFTMAX));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ------------------------------------------------------------------------------------------------ softmax of group g
     const int g = warp >> 2, quad = warp & 3, r = quad * 32 + lane, tok = r / a.G;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t tS = tmem + COL_S + g * 128 + lanes, tO = tmem + COL_O + lanes;
     int c[2] = {0, 0}, cv = 0;     // key tiles of either group, tiles of V, before this piece
+    int cf = 0, few_pieces = 0;    // 8-bit pages: key tiles and pieces of the turned kind before this one, which the other counts leave out
     bool alive = true;
     int at = begin;
     ChunkPiece p;
     // values behind the item's last key may be anything: this thread's row of the key tile they lie in
     auto clear_tail = [&](int step, int tail) {
       const int v = cv + step;
-      alive = alive && gemm_wait_warp(smem_u32(&v_full[v % RV]), (v / RV) & 1, abortp);
+      alive = alive && gemm_wait_warp(smem_u32(&v_full[v % RING]), (v / RING) & 1, abortp);
       if (alive && r >= tail)
 #pragma unroll
         for (int q = 0; q < 8 * T::CH; ++q)
-          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(smV + (v % RV) * T::TILE + (q >> 3) * 16384 + r * 128 + (q & 7) * 16), "r"(0) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(smV + (v % RING) * T::TILE + (q >> 3) * 16384 + r * 128 + (q & 7) * 16), "r"(0) : "memory");
       fence_proxy_async();
-    };
-    // 8-bit pages: the scales of this group's key tile n, before its scores are there (both pages'; (c, log2 v, 1 / v, v) of page h at h, 2 + h, ...)
-    auto take_scales = [&](int n, float (&to)[8]) {
-      const int i = n % kChunkScales;
-      alive = alive && gemm_wait_warp(smem_u32(&sc_full[g][i]), (n / kChunkScales) & 1, abortp);
-      *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(sc[g][i]);
-      *reinterpret_cast<float4*>(to + 4) = *reinterpret_cast<const float4*>(sc[g][i] + 4);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sc_empty[g][i]);
     };
     // Registers are short where a thread holds a row of scores: the loops keep a few numbers, and the piece is read again behind them.
     auto read_again = [&]() {
@@ -328,24 +638,32 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     };
     while (chunk_piece(a, list, begin, at, end, p)) {
       const int keys = p.pos0 + p.tokens, tail = keys & 127, tail_step = tail ? (keys - 1) / 128 - p.k0 : -1, cnt = p.cnt(g);
-      if (p.kind == CHUNK_FEW) {
+      if (F8 && p.kind == CHUNK_FEW) {
+        // ---------------------------------------------------------------------------------- 8-bit pages, few rows: every warp its keys
+        if constexpr (F8) {
+          const int rows = p.tokens * a.G;
+          const bool whole = p.pieces == 1;
+          float* const rec = a.part + (size_t)(2 * blockIdx.x + ((int)blockIdx.x == p.first)) * kChunkRecord<D>;
+          const ChunkFew8Bars bars = {f_full, f_empty, sc_full, sc_empty, sc};
+          if (rows > 8) alive = chunk_few8<D, 2>(a, p, few, smV, smQ1, bars, abortp, cf, alive, rows, whole, rec);
+          else alive = chunk_few8<D, 1>(a, p, few, smV, smQ1, bars, abortp, cf, alive, rows, whole, rec);
+          cf += p.n;
+          read_again();
+          if (tid == 0) mbar_arrive(&turn_free[few_pieces & 1]);   // (behind a barrier of the eight warps)
+          ++few_pieces;
+        }
+      } else if (!F8 && p.kind == CHUNK_FEW) {
+        if constexpr (!F8) {
         // ---------------------------------------------------------------------------------- a key a lane, a row a column
         const int rows = p.tokens * a.G;
         const int beyond = p.k0 * 128 + r - p.pos0, edge_step = (p.pos0 + 1) / 128 - p.k0;   // the first key tile with a key that some row must not see
         const uint32_t sp = smQ1 + g * T::P + (r >> 6) * T::PCHUNK + (r & 7) * 2;
         const int chunk16 = (r & 63) >> 3;
-        float l[32 * T::HALVES];
+        float l[kChunkFew];
 #pragma unroll
-        for (int n = 0; n < 32 * T::HALVES; ++n) l[n] = 0.f;
+        for (int n = 0; n < kChunkFew; ++n) l[n] = 0.f;
         for (int i = 0; i < cnt; ++i) {
           const int step = 2 * i + g;
-          float to_log2 = a.scale_log2e, value = 1.f;   // of this lane's key: of its page
-          if constexpr (F8) {
-            float of[8];
-            take_scales(c[g] + i, of);
-            to_log2 = quad < 2 ? of[0] : of[1];
-            value = quad < 2 ? of[6] : of[7];
-          }
           alive = alive && gemm_wait_warp(smem_u32(&s_full[g]), (c[g] + i) & 1, abortp);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           float s[32];
@@ -372,10 +690,10 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             for (int n = 0; n < 32; n += 4) {
               if (32 * half + n >= rows) break;
               const float4 less = *reinterpret_cast<const float4*>(&few.less[g][32 * half + n]);
-              s[n] = fap_exp2(fmaf(s[n], to_log2, less.x));
-              s[n + 1] = fap_exp2(fmaf(s[n + 1], to_log2, less.y));
-              s[n + 2] = fap_exp2(fmaf(s[n + 2], to_log2, less.z));
-              s[n + 3] = fap_exp2(fmaf(s[n + 3], to_log2, less.w));
+              s[n] = fap_exp2(fmaf(s[n], a.scale_log2e, less.x));
+              s[n + 1] = fap_exp2(fmaf(s[n + 1], a.scale_log2e, less.y));
+              s[n + 2] = fap_exp2(fmaf(s[n + 2], a.scale_log2e, less.z));
+              s[n + 3] = fap_exp2(fmaf(s[n + 3], a.scale_log2e, less.w));
               mx = fmaxf(fmaxf(mx, fmaxf(s[n], s[n + 1])), fmaxf(s[n + 2], s[n + 3]));
             }
             return mx;
@@ -389,7 +707,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             }
           };
           bool over = i == 0;
-          if (T::HALVES > 1 && i > 0 && rows > 32) {
+          if (i > 0 && rows > 32) {
             load(1);
             over = weigh(1) > 256.f;
           }
@@ -398,14 +716,14 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           // the reference of a row moves where a score exceeds it by 8 (log2 units: a weight of 256): same sums, and mostly the lanes need not know of one another
           if (chunk_group_any(g, over)) {
 #pragma unroll
-            for (int half = 0; half < T::HALVES; ++half)
+            for (int half = 0; half < 2; ++half)
               if (32 * half < rows) {
                 if (half || i > 0) load(half);
                 int mine = 0;
 #pragma unroll
                 for (int n = 0; n < 32; ++n) {
                   if (32 * half + n >= rows) break;
-                  const int v = __reduce_max_sync(0xffffffffu, chunk_order(F8 ? s[n] * to_log2 : s[n]));
+                  const int v = __reduce_max_sync(0xffffffffu, chunk_order(s[n]));
                   if (lane == n) mine = v;
                 }
                 few.best[g][quad][32 * half + lane] = mine;
@@ -414,7 +732,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             if (quad == 0)
               for (int n = lane; n < rows; n += 32) {
                 const float was = i == 0 ? -INFINITY : few.m[g][n];
-                const float now = chunk_unorder(max(max(few.best[g][0][n], few.best[g][1][n]), max(few.best[g][2][n], few.best[g][3][n]))) * (F8 ? 1.f : a.scale_log2e);
+                const float now = chunk_unorder(max(max(few.best[g][0][n], few.best[g][1][n]), max(few.best[g][2][n], few.best[g][3][n]))) * a.scale_log2e;
                 const bool move = i == 0 || now > was + 8.f;
                 const float m = move ? now : was;
                 few.factor[g][n] = !move ? 1.f : was == -INFINITY ? 0.f : fap_exp2(was - m);
@@ -444,11 +762,11 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               tmem_st_wait();
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
-            if ((T::HALVES > 1 && rows > 32) || i > 0) load(0);
+            if (rows > 32 || i > 0) load(0);
             weigh(0);
           }
 #pragma unroll
-          for (int half = 0; half < T::HALVES; ++half)
+          for (int half = 0; half < 2; ++half)
             if (32 * half < rows) {
               if (half) {
                 load(1);
@@ -458,14 +776,13 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               for (int n = 0; n < 32; n += 4) {
                 if (32 * half + n >= T::FEW || 32 * half + n >= rows) break;
                 l[32 * half + n] += s[n]; l[32 * half + n + 1] += s[n + 1]; l[32 * half + n + 2] += s[n + 2]; l[32 * half + n + 3] += s[n + 3];
-                if constexpr (F8) { s[n] *= value; s[n + 1] *= value; s[n + 2] *= value; s[n + 3] *= value; }
                 const uint32_t w01 = pack_bf16(s[n], s[n + 1]), w23 = pack_bf16(s[n + 2], s[n + 3]);
                 const int row = 2 * (32 * half + n) - n % 8;
                 put(row, w01, w23);
                 put(row + 8, pack_bf16(s[n] - bf16lo(w01), s[n + 1] - bf16hi(w01)), pack_bf16(s[n + 2] - bf16lo(w23), s[n + 3] - bf16hi(w23)));
               }
             }
-          if (!F8 && step == tail_step) clear_tail(step, tail);   // (8-bit codes are finite as they are converted)
+          if (step == tail_step) clear_tail(step, tail);
           fence_proxy_async();
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
@@ -473,7 +790,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         // a row's sum over the warp's lanes: half of the columns a step, until a lane has one
 #pragma unroll
-        for (int half = 0; half < T::HALVES; ++half)
+        for (int half = 0; half < 2; ++half)
           if (32 * half < rows) {
             float* const v = l + 32 * half;
 #pragma unroll
@@ -535,6 +852,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               }
           }
         }
+        }
       } else {
         // ---------------------------------------------------------------------------------- a row a lane
         const bool pair = p.kind == CHUNK_PAIR;
@@ -545,8 +863,6 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         float m = -INFINITY, l = 0.f;
         for (int i = 0; i < cnt; ++i) {
           const int step = pair ? i : 2 * i + g;
-          float of[F8 ? 8 : 1];
-          if constexpr (F8) take_scales(c[g] + i, of);
           alive = alive && gemm_wait_warp(smem_u32(&s_full[g]), (c[g] + i) & 1, abortp);
           if (!alive) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -561,25 +877,12 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               for (int k = 0; k < 128; ++k)
                 if (k > last) s[k] = -INFINITY;
             }
-            float mx;
-            if constexpr (F8) {   // a page's half of the row at a time
-              float x[4];
+            float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const int k0 = 64 * (q >> 1) + 32 * (q & 1);
-                x[q] = s[k0];
-#pragma unroll
-                for (int k = 1; k < 32; ++k) x[q] = fmaxf(x[q], s[k0 + k]);
-              }
-              mx = fmaxf(fmaxf(x[0], x[1]) * of[0], fmaxf(x[2], x[3]) * of[1]);
-            } else {
-              float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
-#pragma unroll
-              for (int k = 4; k < 128; k += 4) {
-                x0 = fmaxf(x0, s[k]); x1 = fmaxf(x1, s[k + 1]); x2 = fmaxf(x2, s[k + 2]); x3 = fmaxf(x3, s[k + 3]);
-              }
-              mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale_log2e;   // (the scale is positive)
+            for (int k = 4; k < 128; k += 4) {
+              x0 = fmaxf(x0, s[k]); x1 = fmaxf(x1, s[k + 1]); x2 = fmaxf(x2, s[k + 2]); x3 = fmaxf(x3, s[k + 3]);
             }
+            const float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale_log2e;   // (the scale is positive)
             const bool move = mx > m + 8.f;
             if (i == 0) {
               m = mx;
@@ -603,17 +906,10 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               tmem_st_wait();
             }
             const float ms = m == -INFINITY ? 0.f : m;
-            f32x2 sc2 = f2_pack(a.scale_log2e, a.scale_log2e), ms2 = f2_pack(-ms, -ms);
+            const f32x2 sc2 = f2_pack(a.scale_log2e, a.scale_log2e), ms2 = f2_pack(-ms, -ms);
             f32x2 l01 = f2_pack(0.f, 0.f), l23 = l01;
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-              // (8-bit pages: weights times the values' scale, which the row's sum is rid of again)
-              if constexpr (F8) {
-                sc2 = f2_pack(of[hf], of[hf]);
-                ms2 = f2_pack(of[2 + hf] - ms, of[2 + hf] - ms);
-                l01 = f2_pack(0.f, 0.f);
-                l23 = l01;
-              }
               uint32_t w[32];
 #pragma unroll
               for (int k = 0; k < 32; ++k) {
@@ -632,20 +928,13 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 else l01 = f2_add(l01, f2_pack(e0, e1));
               }
               tmem_st32(tS + 32 * hf, w);
-              if constexpr (F8) {
-                float l0, l1;
-                f2_unpack(f2_add(l01, l23), l0, l1);
-                l += (l0 + l1) * of[4 + hf];
-              }
             }
-            if constexpr (!F8) {
-              float l0, l1;
-              f2_unpack(f2_add(l01, l23), l0, l1);
-              l += l0 + l1;
-            }
+            float l0, l1;
+            f2_unpack(f2_add(l01, l23), l0, l1);
+            l += l0 + l1;
             tmem_st_wait();
           }
-          if (!F8 && step == tail_step) clear_tail(step, tail);
+          if (step == tail_step) clear_tail(step, tail);
           if (!alive) break;
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
@@ -721,39 +1010,55 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         chunk_sync();
         if (last_flag) chunk_merge<D>(a.out, a.part, p.first, p.pieces, p.tokens, p.row0, p.head, a.Hq, a.G, p.kind == CHUNK_FEW);
-      } else if (p.kind != CHUNK_PAIR) {
+      } else if (p.kind != CHUNK_PAIR && !(F8 && p.kind == CHUNK_FEW)) {
         chunk_sync();     // both groups have read both accumulators
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::REGS_REST));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // ------------------------------------------------------------------------------------------------ TMA
     if (warp == 8) {
       bool alive = true;
       int cq[2] = {0, 0}, ck = 0;   // pieces with a query tile g, key tiles, before this piece
-      int turned = -RV - 1;         // the last key tile of the last piece of the turned kind
-      int cp = 0, few_pieces = 0;   // 8-bit pages: pages of K and V, pieces of the turned kind, before this piece
-      bool was_few = false;         // the piece before this one was of that kind
+      int turned = -RING - 1;       // the last key tile of the last piece of the turned kind
+      // 8-bit pages: key tiles and pieces of the turned kind so far; of each place (those of V, then those of K) whether a tile of that kind, or another, was put there since it was last
+      // waited for, and the parity of the wait.  (Each round of each barrier is waited for once, so that its parity tells it.)
+      int cf = 0, few_pieces = 0;
+      uint32_t few_in = 0, dense_in = 0, few_round = 0, dense_round = 0;
+      auto acquire = [&](int place) {
+        const uint32_t bit = 1u << place;
+        if (few_in & bit) {
+          if (!gemm_wait_warp(smem_u32(&f_empty[place]), (few_round >> place) & 1, abortp)) return false;
+          few_in &= ~bit;
+          few_round ^= bit;
+        } else if (dense_in & bit) {
+          if (!gemm_wait_warp(place < RING ? smem_u32(&v_empty[place]) : smem_u32(&k_empty[place - RING]), (dense_round >> place) & 1, abortp)) return false;
+          dense_in &= ~bit;
+          dense_round ^= bit;
+        }
+        return true;
+      };
       for (int at = begin; alive && at < end; ++at) {
-        if (at == begin + 1) asm volatile("bar.sync 5, %0;" ::"n"(T::THREADS) : "memory");   // (the list is there)
+        if (at == begin + 1) asm volatile("bar.sync 5, 384;" ::: "memory");   // (the list is there)
         const int4* const e = at == begin ? reinterpret_cast<const int4*>(a.pieces + at) : chunk_words(a, list, begin, at);
         const int4 z = e[2];
         const int lead0 = z.y, lead1 = z.z;   // the pages of its first key tile
         ChunkPiece p;
         if (!chunk_read(a, e[0], e[1], z, p)) continue;
+        // 8-bit pages: pieces of the turned kind leave their results where Q1 is.  Those before the last two are known here to be done, so that the two barriers tell them apart.
+        if (F8 && p.kind == CHUNK_FEW && few_pieces > 1 && !(alive = gemm_wait_warp(smem_u32(&turn_free[few_pieces & 1]), ((few_pieces >> 1) - 1) & 1, abortp))) break;
         const int32_t* const pages = a.table + (size_t)p.request * a.blocks;
         const int last_page = (p.pos0 + p.tokens - 1) / kStepPage;
         int first = 2 * p.k0, ids = __ldg(pages + min(first + lane, last_page));   // 32 pages from `first` on, a lane each; behind the last key: the last one
         auto fetch_q = [&](int g) {
-          if ((p.kind == CHUNK_PAIR ? p.cnt(g) : 1 - g) == 0) return true;
+          if ((p.kind == CHUNK_PAIR ? p.cnt(g) : F8 && p.kind == CHUNK_FEW ? 0 : 1 - g) == 0) return true;
           if (!gemm_wait_warp(smem_u32(&q_empty[g]), (cq[g] & 1) ^ 1, abortp)) return false;
           ++cq[g];
           // Q1 lies where P of the turned kind did: behind its last product, which frees the last tile of V (where that place was used since, it has)
           if constexpr (F8) {
-            // (of pieces before the one before this, the last products are done: their successor's queries have been asked for)
-            if (g && was_few && !gemm_wait_warp(smem_u32(&turn_free[(few_pieces - 1) & 1]), ((few_pieces - 1) >> 1) & 1, abortp)) return false;
+            if (g && few_pieces > 0 && !gemm_wait_warp(smem_u32(&turn_free[(few_pieces - 1) & 1]), ((few_pieces - 1) >> 1) & 1, abortp)) return false;
           } else {
-            if (g && ck - turned <= RV && !gemm_wait_warp(smem_u32(&v_empty[turned % RV]), (turned / RV) & 1, abortp)) return false;
+            if (g && ck - turned <= RING && !gemm_wait_warp(smem_u32(&v_empty[turned % RING]), (turned / RING) & 1, abortp)) return false;
           }
           if (lane == 0) {
             const bool few = p.kind == CHUNK_FEW;
@@ -772,20 +1077,9 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         // In the order in which the MMAs ask for them.
         if (!(alive = fetch_q(0))) break;
         const int t0 = ck;
-        // two pages as they lie, one behind the other in memory each
-        auto fetch_codes = [&](const uint8_t* pool, int page0, int page1) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r, ++cp) {
-            const int i = cp % T::PAGES;
-            if (!gemm_wait_warp(smem_u32(&c_empty[i]), ((cp / T::PAGES) & 1) ^ 1, abortp)) return false;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&c_full[i], T::PAGE);
-              chunk_bulk(smC + i * T::PAGE, pool + ((size_t)(r ? page1 : page0) * a.Hkv + p.head) * T::PAGE, T::PAGE, smem_u32(&c_full[i]));
-            }
-          }
-          return true;
-        };
-        for (int j = 0; j < p.n; ++j, ++ck) {
+        const bool codes = F8 && p.kind == CHUNK_FEW;
+        for (int j = 0; j < p.n; ++j, codes ? ++cf : ++ck) {
+          const int i = ck % RING, ph = (ck / RING) & 1;
           if (2 * (p.k0 + j) >= first + 32) {
             first += 32;
             ids = __ldg(pages + min(first + lane, last_page));
@@ -793,20 +1087,30 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           const int page0 = j == 0 ? lead0 : __shfl_sync(0xffffffffu, ids, 2 * (p.k0 + j) - first);
           const int page1 = j == 0 ? lead1 : __shfl_sync(0xffffffffu, ids, 2 * (p.k0 + j) + 1 - first);
           if constexpr (F8) {
-            if (!(alive = fetch_codes(a.k8, page0, page1))) break;
-            if (j == 0 && !(alive = fetch_q(1))) break;
-            if (!(alive = fetch_codes(a.v8, page0, page1))) break;
-          } else {
-            const int i = ck % RK, iv = ck % RV;
-            if (!(alive = gemm_wait_warp(smem_u32(&k_empty[i]), ((ck / RK) & 1) ^ 1, abortp))) break;
-            fetch(&map_k, smK + i * T::TILE, &k_full[i], page0, page1);
-            if (j == 0 && !(alive = fetch_q(1))) break;
-            if (!(alive = gemm_wait_warp(smem_u32(&v_empty[iv]), ((ck / RV) & 1) ^ 1, abortp))) break;
-            fetch(&map_v, smV + iv * T::TILE, &v_full[iv], page0, page1);
-          }
+            if (codes) {   // both pages of K, both of V, rows of D bytes in the swizzle of their length
+              const int place = cf % T::PLACES;
+              if (!(alive = acquire(place))) break;
+              few_in |= 1u << place;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&f_full[place], T::TILE);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  fap_tma_4d(smV + place * T::TILE + r * (64 * D), r < 2 ? &codes8.k : &codes8.v, smem_u32(&f_full[place]), 0, 0, p.head, r & 1 ? page1 : page0);
+              }
+              continue;
+            }
+            if (!(alive = acquire(RING + i))) break;
+            dense_in |= 1u << (RING + i);
+          } else if (!(alive = gemm_wait_warp(smem_u32(&k_empty[i]), ph ^ 1, abortp))) break;
+          fetch(&map_k, smK + i * T::TILE, &k_full[i], page0, page1);
+          if (j == 0 && !(alive = fetch_q(1))) break;
+          if constexpr (F8) {
+            if (!(alive = acquire(i))) break;
+            dense_in |= 1u << i;
+          } else if (!(alive = gemm_wait_warp(smem_u32(&v_empty[i]), ph ^ 1, abortp))) break;
+          fetch(&map_v, smV + i * T::TILE, &v_full[i], page0, page1);
         }
         if (p.kind == CHUNK_FEW) { turned = t0 + p.n - 1; ++few_pieces; }
-        was_few = p.kind == CHUNK_FEW;
       }
     }
     // ------------------------------------------------------------------------------------------------ MMAs
@@ -818,10 +1122,9 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const uint32_t dq0 = (uint32_t)umma_desc_sw128(smQ), dq1 = (uint32_t)umma_desc_sw128(smQ1), dk0 = (uint32_t)umma_desc_sw128(smK), dv0 = (uint32_t)fap_desc_mn(smV);
       bool alive = true;   // a lane's own: once a wait expires it only keeps the lane from issuing
       int c[2] = {0, 0}, cq[2] = {0, 0}, ck = 0;   // tiles of group g, pieces with a query tile g, tiles of K and V, before this piece
-      int few_pieces = 0;                          // 8-bit pages: pieces of the turned kind before this one
       // scores of group g by query tile `tile`: S_g = Q K^T, or of the turned kind, whose rows' word of the instruction is `wide`, K Q^T
       auto qk = [&](int g, int tile, int t, uint32_t wide) {
-        uint32_t dq = tile ? dq1 : dq0, dk = dk0 + (t % RK) * (T::TILE >> 4);
+        uint32_t dq = tile ? dq1 : dq0, dk = dk0 + (t % RING) * (T::TILE >> 4);
         asm volatile("" : "+r"(dq), "+r"(dk));   // (what is made of them is made here, and not kept in registers that the warp does not have)
         if (wide) {
 #pragma unroll
@@ -835,7 +1138,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         fap_commit(&s_full[g]);
       };
       auto pv = [&](int g, int t, bool first, uint32_t wide) {
-        uint32_t dv = dv0 + (t % RV) * (T::TILE >> 4);
+        uint32_t dv = dv0 + (t % RING) * (T::TILE >> 4);
         asm volatile("" : "+r"(dv));
         if (wide) {   // O^T += V^T P^T: V with its rows for K, P from shared memory
           uint32_t dp = dq1 + g * (T::P >> 4);
@@ -852,9 +1155,17 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         fap_commit(&o_full[g]);
       };
       auto wide_of = [&](const ChunkPiece& p) { return p.kind == CHUNK_FEW ? (uint32_t)((p.tokens * a.G + 15) / 16 * 2) << 17 : 0u; };
+      bool apart = false;                          // 8-bit pages: pieces of few rows lie in front of the next one
       // the next piece; warp-uniform, and known to be
       auto fetch = [&](int& at, ChunkPiece& p) {
-        const bool more = chunk_piece(a, list, begin, at, end, p);
+        bool more = chunk_piece(a, list, begin, at, end, p);
+        if constexpr (F8) {   // (those are the softmax warps' own, and what comes behind one is not begun before it: its operands wait for it)
+          apart = false;
+          while (more && p.kind == CHUNK_FEW) {
+            apart = true;
+            more = chunk_piece(a, list, begin, at, end, p);
+          }
+        }
         at = __shfl_sync(0xffffffffu, at, 0);
         p.n = __shfl_sync(0xffffffffu, p.n, 0);
         p.kind = __shfl_sync(0xffffffffu, p.kind, 0);
@@ -863,8 +1174,8 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         p.cnt1 = __shfl_sync(0xffffffffu, p.cnt1, 0);
         return __shfl_sync(0xffffffffu, (int)more, 0) != 0;
       };
-      auto wait_k = [&](int t) { alive &= gemm_wait(smem_u32(&k_full[t % RK]), (t / RK) & 1, abortp); };
-      auto wait_v = [&](int t) { alive &= gemm_wait(smem_u32(&v_full[t % RV]), (t / RV) & 1, abortp); };
+      auto wait_k = [&](int t) { alive &= gemm_wait(smem_u32(&k_full[t % RING]), (t / RING) & 1, abortp); };
+      auto wait_v = [&](int t) { alive &= gemm_wait(smem_u32(&v_full[t % RING]), (t / RING) & 1, abortp); };
       // the first scores of group g of piece p, whose key tiles begin at tile t and whose query tiles are number q0, q1
       auto open = [&](const ChunkPiece& p, int g, int t, int q0, int q1) {
         const bool pair = p.kind == CHUNK_PAIR;
@@ -874,7 +1185,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (elect_one() && alive) {
           qk(g, tile, t + step, wide_of(p));
-          if (!pair) fap_commit(&k_empty[(t + step) % RK]);                    // (of a pair, both tiles read the same keys)
+          if (!pair) fap_commit(&k_empty[(t + step) % RING]);                    // (of a pair, both tiles read the same keys)
           if (pair ? p.cnt(g) == 1 : step == p.n - 1) fap_commit(&q_empty[tile]);   // behind the last scores Q's place is free
         }
       };
@@ -896,48 +1207,37 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         // the next piece's scores, while this one's last tiles and its O are worked on
         // (The second key tile's scores come behind the first's: the last ones give Q's place up.)
         auto go_on = [&](int g) {
-          if (more && next.cnt(g) > 0 && (next.kind == CHUNK_PAIR || g == 0 || ahead[0])) {
+          if (more && !apart && next.cnt(g) > 0 && (next.kind == CHUNK_PAIR || g == 0 || ahead[0])) {
             open(next, g, tn, nq0, nq1);
             ahead[g] = true;
           }
         };
         if (pair) {
-          if (elect_one() && alive) fap_commit(&k_empty[ck % RK]);
+          if (elect_one() && alive) fap_commit(&k_empty[ck % RING]);
           for (int j = 0; j < p.n; ++j) {
             const int t = ck + j;
             wait_v(t);
-            if (!F8 && j + 1 < p.n) wait_k(t + 1);
+            if (j + 1 < p.n) wait_k(t + 1);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               const int ng = p.cnt(g);
               if (j < ng) {
                 alive &= gemm_wait(smem_u32(&p_full[g]), (c[g] + j) & 1, abortp);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if constexpr (F8) {   // (the next keys are being converted: the product does not wait for them)
-                  if (elect_one() && alive) pv(g, t, j == 0, 0);
-                  if (j + 1 < ng) {
-                    wait_k(t + 1);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (elect_one() && alive) {
-                      qk(g, g, t + 1, 0);
-                      if (j + 2 == ng) fap_commit(&q_empty[g]);
-                    }
-                  }
-                } else if (elect_one() && alive) {
+                if (elect_one() && alive) {
                   pv(g, t, j == 0, 0);
                   if (j + 1 < ng) {
                     qk(g, g, t + 1, 0);
                     if (j + 2 == ng) fap_commit(&q_empty[g]);
                   }
                 }
-                // (the turned kind's P goes where Q1 is: not before this piece's last scores of tile 1 are on their way.  Where K has one place, the next piece's
-                // first keys come behind this one's last.)
-                if (j + 1 == ng && (!F8 || j + 1 == p.n) && (next.kind != CHUNK_FEW || g || j + 1 == p.n)) go_on(g);
+                // (the turned kind's P goes where Q1 is: not before this piece's last scores of tile 1 are on their way)
+                if (j + 1 == ng && (next.kind != CHUNK_FEW || g || j + 1 == p.n)) go_on(g);
               }
             }
             if (elect_one() && alive) {
-              fap_commit(&v_empty[t % RV]);
-              if (j + 1 < p.n) fap_commit(&k_empty[(t + 1) % RK]);
+              fap_commit(&v_empty[t % RING]);
+              if (j + 1 < p.n) fap_commit(&k_empty[(t + 1) % RING]);
             }
           }
         } else {
@@ -949,15 +1249,14 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (elect_one() && alive) {
               pv(g, t, j < 2, 2 * wide);   // (P with the second halves of its weights)
-              fap_commit(&v_empty[t % RV]);
-              if (F8 && wide && j + 1 == p.n) fap_commit(&turn_free[few_pieces & 1]);
+              fap_commit(&v_empty[t % RING]);
             }
             if (j + 2 < p.n) {
               wait_k(t + 2);
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
               if (elect_one() && alive) {
                 qk(g, 0, t + 2, wide);
-                fap_commit(&k_empty[(t + 2) % RK]);
+                fap_commit(&k_empty[(t + 2) % RING]);
                 if (j + 3 == p.n) fap_commit(&q_empty[0]);
               }
             } else if (!(wide && next.kind == CHUNK_PAIR && g && j + 1 < p.n)) {   // (Q1 of a pair comes behind the last product that reads P)
@@ -967,16 +1266,16 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         c[0] += p.cnt0; c[1] += p.cnt1; ck = tn;
         cq[0] = nq0; cq[1] = nq1;
-        few_pieces += p.kind == CHUNK_FEW;
       }
     }
     // ------------------------------------------------------------------------------------------------ scales of 8-bit pages
     if (F8 && warp == 10) {
       bool alive = true;
-      int c[2] = {0, 0};
+      int cf = 0;
       int at = begin;
       ChunkPiece p;
       while (alive && chunk_piece(a, list, begin, at, end, p)) {
+        if (p.kind != CHUNK_FEW) continue;
         const int32_t* const pages = a.table + (size_t)p.request * a.blocks;
         const int last_page = (p.pos0 + p.tokens - 1) / kStepPage;
         int first = 2 * p.k0;
@@ -987,80 +1286,24 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           value = __ldg(a.v_scales + e);
         };
         read();
-        for (int j = 0; alive && j < p.n; ++j) {
+        for (int j = 0; j < p.n; ++j, ++cf) {
           if (2 * (p.k0 + j) >= first + 32) {
             first += 32;
             read();
           }
-          const int h = lane - (2 * (p.k0 + j) - first);   // 0, 1: the tile's pages
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            if (p.kind == CHUNK_PAIR ? j >= p.cnt(g) : (j & 1) != g) continue;
-            const int n = c[g]++, i = n % kChunkScales;
-            if (!(alive = gemm_wait_warp(smem_u32(&sc_empty[g][i]), ((n / kChunkScales) & 1) ^ 1, abortp))) break;
-            if (h == 0 || h == 1) {
-              float* const to = sc[g][i] + h;
-              to[0] = to_log2;
-              to[2] = log2f(value);
-              to[4] = 1.f / value;
-              to[6] = value;
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sc_full[g][i]);
-          }
-        }
-      }
-    }
-    // ------------------------------------------------------------------------------------------------ 8-bit pages to bf16 tiles
-    // 16 codes of a row a thread at a time: 16 bytes read, two pieces of 16 bytes written, whose places in the swizzled tile are other banks for each of eight lanes
-    // (at head size 128 a row's second 64 features lie 16 KB behind: half of the lanes write their second piece first).
-    if (F8 && warp >= 12) {
-      const int ct = tid - 384;
-      constexpr int ROW = D / 16, PIECES = 64 * ROW / 128;   // 16-byte pieces of a row; of a page, a thread
-      const int c16 = ct % ROW, row0 = ct / ROW;
-      const int f0 = 2 * c16 + (D == 128 && c16 >= 4 ? 1 : 0);
-      bool alive = true;
-      int ck = 0, cp = 0;
-      int at = begin;
-      ChunkPiece p;
-      while (alive && chunk_piece(a, list, begin, at, end, p)) {
-        for (int j = 0; alive && j < p.n; ++j, ++ck) {
-#pragma unroll 1
-          for (int kv = 0; alive && kv < 2; ++kv) {
-            const int i = kv ? ck % RV : ck % RK, ph = kv ? (ck / RV) & 1 : (ck / RK) & 1;
-            uint64_t* const full = kv ? &v_full[i] : &k_full[i];
-            const uint32_t tile = kv ? smV + i * T::TILE : smK + i * T::TILE;
-#pragma unroll 1
-            for (int r = 0; r < 2; ++r, ++cp) {
-              const int q = cp % T::PAGES;
-              if (!(alive = gemm_wait_warp(smem_u32(&c_full[q]), (cp / T::PAGES) & 1, abortp))) break;
-              uint4 w[PIECES];
-#pragma unroll
-              for (int e = 0; e < PIECES; ++e) w[e] = lds128(smC + q * T::PAGE + (e * 128 + ct) * 16);
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&c_empty[q]);
-              if (r == 0 && !(alive = gemm_wait_warp(kv ? smem_u32(&v_empty[i]) : smem_u32(&k_empty[i]), ph ^ 1, abortp))) break;
-#pragma unroll
-              for (int e = 0; e < PIECES; ++e) {
-                const int row = r * 64 + row0 + e * (128 / ROW);
-                uint4 lo = make_uint4(chunk_widen(w[e].x, 0x1404), chunk_widen(w[e].x, 0x3424), chunk_widen(w[e].y, 0x1404), chunk_widen(w[e].y, 0x3424));
-                uint4 hi = make_uint4(chunk_widen(w[e].z, 0x1404), chunk_widen(w[e].z, 0x3424), chunk_widen(w[e].w, 0x1404), chunk_widen(w[e].w, 0x3424));
-                if (f0 & 1) { const uint4 t = lo; lo = hi; hi = t; }
-                const uint32_t dst = tile + (f0 >> 3) * 16384 + row * 128;
-                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (((f0 & 7) ^ (row & 7)) << 4)), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
-                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + ((((f0 ^ 1) & 7) ^ (row & 7)) << 4)), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
-              }
-            }
-            if (!alive) break;
-            fence_proxy_async();   // generic-proxy stores -> the tensor core's async proxy
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full);
+          const int i = cf % kChunkScales, at0 = 2 * (p.k0 + j) - first;
+          if (!(alive = gemm_wait_warp(smem_u32(&sc_empty[i]), ((cf / kChunkScales) & 1) ^ 1, abortp))) break;
+          const float4 of = make_float4(__shfl_sync(0xffffffffu, to_log2, at0), __shfl_sync(0xffffffffu, to_log2, at0 + 1), __shfl_sync(0xffffffffu, value, at0),
+                                        __shfl_sync(0xffffffffu, value, at0 + 1));
+          if (lane == 0) {
+            sc[i] = of;
+            mbar_arrive(&sc_full[i]);
           }
         }
       }
     }
     // ------------------------------------------------------------------------------------------------ rows behind the last request's
-    if (warp == T::W_REST && a.rest) {
+    if (warp == (F8 ? 11 : 10) && a.rest) {
       const int row_words = a.Hq * D / 8;   // of 16 bytes
       for (long long e = ((long long)__ldg(a.row_starts + a.requests) + blockIdx.x) * row_words; e < (long long)a.rows * row_words; e += (long long)gridDim.x * row_words)
         for (int i = lane; i < row_words; i += 32) reinterpret_cast<uint4*>(a.out)[e + i] = make_uint4(0, 0, 0, 0);
@@ -1073,8 +1316,8 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
 }
 
-template <int D, bool F8 = false>
-static cudaError_t launch_chunk(const CUtensorMap (&m)[4], const ChunkArgs& a, cudaStream_t st) {
+template <int D, bool F8, class Codes>
+static cudaError_t launch_chunk(const CUtensorMap (&m)[4], const Codes& codes, const ChunkArgs& a, cudaStream_t st) {
   using T = ChunkTile<D, F8>;
   static std::atomic<unsigned long long> served{0};
   const cudaError_t set = once_per_device(served, [] {
@@ -1082,14 +1325,74 @@ static cudaError_t launch_chunk(const CUtensorMap (&m)[4], const ChunkArgs& a, c
     const cudaError_t e = cudaFuncGetAttributes(&at, chunk_attn_kernel<D, F8>);
     if (e != cudaSuccess) return e;
     // the warps' register shares must fit what the block is launched with, or they would wait for registers for good
-    if (at.numRegs * T::THREADS < 8 * 32 * T::REGS_SOFTMAX + (T::THREADS - 256) * T::REGS_REST) return cudaErrorInvalidConfiguration;
+    if (at.numRegs * T::THREADS < 8 * 32 * 216 + 4 * 32 * 64) return cudaErrorInvalidConfiguration;
     return cudaFuncSetAttribute(chunk_attn_kernel<D, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
   });
   if (set != cudaSuccess) return set;
   count_launch();
-  return launch_pdl(chunk_attn_kernel<D, F8>, dim3((unsigned)(num_sms() < kStepMaxCtas ? num_sms() : kStepMaxCtas)), dim3(T::THREADS), T::SMEM, st, m[0], m[1], m[2], m[3], a);
+  return launch_pdl(chunk_attn_kernel<D, F8>, dim3((unsigned)(num_sms() < kStepMaxCtas ? num_sms() : kStepMaxCtas)), dim3(T::THREADS), T::SMEM, st, m[0], m[1], m[2], m[3], codes, a);
 }
 
+// 8-bit pages of the requests that have more rows than the turned kind takes, as bf16 where they will be read as those are: the tensor cores' operands of that kind come from shared memory
+// alone, and every query tile would turn the same codes around again.  (Done so, by four warps beside the softmax's: 2048 tokens behind 15000 1024 us, with products of the operands as they
+// lay 970.)  A block (page, head) a CTA at a time.
+__global__ void __launch_bounds__(256) chunk_widen_kernel(const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs, uint16_t* k16, uint16_t* v16, const int32_t* row_starts,
+                                                          const int32_t* contexts, const int32_t* table, int requests, int blocks, int Hkv, int D, int few_tokens) {
+  __shared__ int list[256];   // requests of this round that have so many
+  __shared__ int of_warp[8];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, pieces = 64 * D / 16;   // of 16 codes, of a block of K or of V
+  int done = 0;                                        // blocks before this request's, so that the CTAs have equal shares of all
+  for (int s0 = 0; s0 < requests; s0 += 256) {
+    const int s = s0 + tid;
+    const bool many = s < requests && __ldg(row_starts + s + 1) - __ldg(row_starts + s) > few_tokens;
+    const unsigned who = __ballot_sync(0xffffffffu, many);
+    if ((tid & 31) == 0) of_warp[tid >> 5] = __popc(who);
+    __syncthreads();
+    int n = 0, before = __popc(who & ((1u << (tid & 31)) - 1));
+    for (int w = 0; w < 8; ++w) {
+      if (w == tid >> 5) before += n;
+      n += of_warp[w];
+    }
+    if (many) list[before] = s;
+    __syncthreads();
+    for (int i = 0; i < n; ++i) {
+      const int r = list[i], keys = __ldg(contexts + r) + __ldg(row_starts + r + 1) - __ldg(row_starts + r), units = (keys + kStepPage - 1) / kStepPage * Hkv;
+      for (int u = ((int)blockIdx.x + (int)gridDim.x - done % (int)gridDim.x) % (int)gridDim.x; u < units; u += gridDim.x) {
+        const size_t block = (size_t)__ldg(table + (size_t)r * blocks + u / Hkv) * Hkv + u % Hkv;
+        const float fk = __ldg(ks + block), fv = __ldg(vs + block);
+        for (int e = tid; e < 2 * pieces; e += 256) {
+          const bool v = e >= pieces;
+          const size_t at = block * pieces + (v ? e - pieces : e);
+          const uint4 w = __ldg(reinterpret_cast<const uint4*>(v ? v8 : k8) + at);
+          const float f = v ? fv : fk;
+          const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+          uint32_t out[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const uint32_t two = chunk_f16(in[q >> 1] >> (16 * (q & 1)));
+            float lo, hi;
+            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(lo), "=f"(hi) : "r"(two));
+            out[q] = pack_bf16(lo * f, hi * f);   // (exact: the scale is a power of two)
+          }
+          uint4* const to = reinterpret_cast<uint4*>(v ? v16 : k16) + 2 * at;
+          to[0] = make_uint4(out[0], out[1], out[2], out[3]);
+          to[1] = make_uint4(out[4], out[5], out[6], out[7]);
+        }
+      }
+      done += units % (int)gridDim.x;
+    }
+    __syncthreads();
+  }
+}
+// whether some request may have more rows than the turned kind takes
+static bool chunk_wide8(const pie_step_dims& d) { return d.rows > ChunkTile<128, true>::FEW / (d.Hq / d.Hkv); }
+static cudaError_t launch_chunk_widen(const ChunkArgs& a, const pie_step_dims& d, int D, const uint8_t* k8, const uint8_t* v8, uint16_t* k16, uint16_t* v16, cudaStream_t st) {
+  count_launch();
+  return launch_pdl(chunk_widen_kernel, dim3((unsigned)(num_sms() * 4)), dim3(256), 0, st, k8, v8, a.k_scales, a.v_scales, k16, v16, a.row_starts, a.contexts, a.table, d.requests, d.blocks,
+                    d.Hkv, D, a.few_tokens);
+}
 static size_t chunk_workspace_bytes(int D) { return kStepMaxCtas * 4 + (size_t)2 * kStepMaxCtas * (D == 128 ? kChunkRecord<128> : kChunkRecord<64>) * 4; }
 // the common part: q's maps, the plan's arrays
 template <bool F8>
@@ -1105,7 +1408,7 @@ static int chunk_common(ChunkArgs& a, CUtensorMap* maps, void* out, const pie_he
   a = {};
   a.out = (uint16_t*)out; a.Hq = d->Hq; a.Hkv = d->Hkv; a.G = d->Hq / d->Hkv; a.tile_tokens = l.tile_tokens; a.rows = d->rows; a.requests = d->requests;
   a.scale_log2e = scale * 1.4426950408889634f;
-  a.ranges = plan + l.ranges; a.table = plan + l.block_table; a.row_starts = plan + l.row_starts;
+  a.ranges = plan + l.ranges; a.table = plan + l.block_table; a.row_starts = plan + l.row_starts; a.contexts = plan + l.contexts;
   a.pieces = reinterpret_cast<const StepPiece*>(plan + l.pieces);
   a.blocks = d->blocks; a.rest = rest;
   a.count = (unsigned int*)workspace;
@@ -1159,7 +1462,13 @@ int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const v
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)   // (256 bytes at head size 64 are two heads: half as much again was read from HBM)
       return PIE_EUNSUPPORTED;
   }
-  return status_of(D == 128 ? launch_chunk<128>(maps, a, (cudaStream_t)stream) : launch_chunk<64>(maps, a, (cudaStream_t)stream));
+  return status_of(D == 128 ? launch_chunk<128, false>(maps, ChunkNone{}, a, (cudaStream_t)stream) : launch_chunk<64, false>(maps, ChunkNone{}, a, (cudaStream_t)stream));
+}
+
+// the workspace: that of pie_chunk_attn, and room for a layer's pools in 16 bits where a request may have more rows than the turned kind takes
+size_t pie_chunk_attn_fp8_workspace_bytes(const pie_step_dims* d, int D) {
+  if (step_dims_status(d) || (D != 64 && D != 128)) return 0;
+  return chunk_workspace_bytes(D) + (chunk_wide8(*d) ? (size_t)d->pages * d->Hkv * kStepPage * D * 4 : 0);
 }
 
 int pie_chunk_attn_fp8(void* out, const pie_head_rows* q, const uint8_t* kpool, const float* k_scales, const uint8_t* vpool, const float* v_scales, const int32_t* plan,
@@ -1171,9 +1480,31 @@ int pie_chunk_attn_fp8(void* out, const pie_head_rows* q, const uint8_t* kpool, 
   if (int s = chunk_common<true>(a, maps, out, q, plan, d, D, scale, rest, workspace, workspace_bytes)) return s;
   for (const void* p : {(const void*)kpool, (const void*)vpool})
     if (reinterpret_cast<uintptr_t>(p) & 15) return PIE_EALIGN;
-  maps[2] = maps[3] = maps[0];   // (its keys and values come by address)
-  a.k8 = kpool; a.v8 = vpool; a.k_scales = k_scales; a.v_scales = v_scales;
-  return status_of(D == 128 ? launch_chunk<128, true>(maps, a, (cudaStream_t)stream) : launch_chunk<64, true>(maps, a, (cudaStream_t)stream));
+  if (workspace_bytes < pie_chunk_attn_fp8_workspace_bytes(d, D)) return PIE_EWORKSPACE;
+  a.k_scales = k_scales; a.v_scales = v_scales;
+  a.q = (const uint16_t*)q->p; a.q_row = d->rows > 1 ? q->stride_l : 0; a.q_head = d->Hq > 1 ? q->stride_h : 0;
+  const GemmEncodeFn fn = gemm_encode_fn();
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  const bool wide = chunk_wide8(*d);
+  const cuuint64_t block = (cuuint64_t)kStepPage * D, dims[4] = {(cuuint64_t)D, (cuuint64_t)kStepPage, (cuuint64_t)d->Hkv, (cuuint64_t)d->pages};
+  const size_t half = (size_t)d->pages * d->Hkv * kStepPage * D;
+  uint16_t* const k16 = (uint16_t*)((uint8_t*)workspace + chunk_workspace_bytes(D));
+  ChunkMaps8 codes;
+  for (int i = 0; i < 2; ++i) {   // a page of one head: 64 rows of D bytes; and in 16 bits, 64 features of them
+    const cuuint64_t strides[3] = {(cuuint64_t)D, block, block * d->Hkv}, strides16[3] = {2 * (cuuint64_t)D, 2 * block, 2 * block * d->Hkv};
+    const cuuint32_t box[4] = {(cuuint32_t)D, (cuuint32_t)kStepPage, 1, 1}, box16[4] = {64, 64, 1, 1};
+    if (fn(i ? &codes.v : &codes.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(i ? vpool : kpool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return PIE_EUNSUPPORTED;
+    maps[2 + i] = maps[0];        // (no piece asks for it)
+    if (wide && fn(&maps[2 + i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, i ? k16 + half : k16, dims, strides16, box16, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return PIE_EUNSUPPORTED;
+  }
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (wide)
+    if (const cudaError_t e = launch_chunk_widen(a, *d, D, kpool, vpool, k16, k16 + half, st); e != cudaSuccess) return status_of(e);
+  return status_of(D == 128 ? launch_chunk<128, true>(maps, codes, a, st) : launch_chunk<64, true>(maps, codes, a, st));
 }
 
 }  // extern "C"

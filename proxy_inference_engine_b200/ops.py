@@ -798,9 +798,9 @@ def rope_kv_fp8(queries, keys, values, freqs, plan, k_pool, k_scales, v_pool, v_
 
 def chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan, scale: float, out=None):
     """chunk_attention over a cache of 8 bits (rope_kv_fp8): row t of q [T, Hq, D] attends to the keys 0 .. position of its own request, a key and a value being their codes times their
-    pages' scales.  Returns [T, Hq * D].  Softmax weights are multiplied with the values' scales and then rounded for their product with the codes: to 16 bits (two bfloat16) where a
-    request's rows, its new tokens x Hq / Hkv, are at most 32, and to bfloat16 otherwise.  A page of scale NaN may make all of its request's new tokens NaN; a code of NaN counts as 480.
-    Rows that belong to nobody are zero, or with ``out`` given what that held."""
+    pages' scales.  Returns [T, Hq * D].  Softmax weights are rounded for their product with the values: to fp16, 2^-12 of one, where a request's rows, its new tokens x Hq / Hkv, are at
+    most 64 (and for the last ones of longer requests), otherwise to bfloat16; the pages of those are first brought to bfloat16 in a workspace of twice the pools' bytes, which all layers
+    share.  A page of scale NaN may make all of its request's new tokens NaN.  Rows that belong to nobody are zero, or with ``out`` given what that held."""
     what = "chunk_attention_fp8"
     if q.dim() != 3 or q.dtype != _BF16:
         raise ValueError(f"[{what}] queries must be bfloat16 [T, Hq, D], but are {q.dtype} {tuple(q.shape)}")
@@ -815,7 +815,7 @@ def chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan, scale: floa
         L = _lib.load()
         out, rest = _fresh(out, (T, Hq * D), q.device)
         held, rows = _head_rows(q)
-        ws = workspaces.get("chunk", L.pie_chunk_attn_workspace_bytes(C.byref(d), D), q.device)
+        ws = workspaces.get("chunk8", L.pie_chunk_attn_fp8_workspace_bytes(C.byref(d), D), q.device)
         _lib.check(L.pie_chunk_attn_fp8(_p(out), C.byref(rows), _p(k_pool), _p(k_scales), _p(v_pool), _p(v_scales), _p(plan.words), C.byref(d), D, float(scale), rest, _p(ws),
                                         ws.numel(), _stream()), what)
     return out
