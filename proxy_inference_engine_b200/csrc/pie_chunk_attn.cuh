@@ -269,20 +269,20 @@ __device__ __forceinline__ uint32_t chunk_code_at(int row, int c16) {
 // lane's codes are whole pieces: of K the features D / 4 t .. of its two keys; of V the features D / 8 g .. of its four keys, two to a tile, neighbouring keys' codes put together by a byte
 // permutation.  A page's scale of K is applied to the scores; that of V to the weights, relative to the largest so far, which the results are in units of, or where it is below
 // 2^-16 of that, whose weights fp16 might not hold, to the page's product.
-// 16 rows a warp: up to 16 of an item go to eight slices of 16 keys of a tile, 32 to two sets of four slices of 32, 64 to four of two.  Every warp has its own running maximum; the warps'
-// results meet at the end in shared memory, eight rows of each set at a time.
-template <int D, int NT>
+// A group of four warps takes every other tile, 16 rows a warp: up to 16 rows of an item are four slices of 32 keys, 32 two sets of two slices, 64 four sets of one.  U times 16 keys are
+// worked on side by side.  Every warp has its own running maximum; the warps' results meet at the end in shared memory, eight rows of each set at a time.
+template <int D, int NT, int U>
 __device__ __forceinline__ bool chunk_few8(const ChunkArgs& a, const ChunkPiece& p, ChunkFew8& few, uint32_t smP, uint32_t smO, const ChunkFew8Bars& bars, volatile int* abortp, int cf,
                                            bool alive, int rows, bool whole, float* rec) {
   using T = ChunkTile<D, true>;
   constexpr int KC = D / 64, VW = D / 32;          // 16-byte pieces of K of a key, 32-bit words of V of a key, a lane
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int sets_log = rows <= 16 ? 0 : rows <= 32 ? 1 : 2, slices = 8 >> sets_log, slice = warp & (slices - 1), set = warp >> (3 - sets_log), row_first = 16 * set;
-  const int keys = 16 << sets_log, key0 = slice * keys, page = key0 >> 6, in_page = key0 & 63;
+  const int group = warp >> 2, quad = warp & 3, sets_log = rows <= 16 ? 0 : rows <= 32 ? 1 : 2, slices = 4 >> sets_log, slice = quad & (slices - 1), set = quad >> (2 - sets_log);
+  const int row_first = 16 * set, keys = 32 << sets_log, key0 = slice * keys;
+  const int parts = 2 * slices, part = set * parts + group * slices + slice;   // a set's, of the groups and slices; this warp's among all
   // queries: the rows 8 n + g, as two codes a feature
   uint32_t qh[NT][D / 16], ql[NT][D / 16];
   float scale[NT][2];                               // of the columns' rows
-  int own[NT][2];                                   // and their tokens
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int row = row_first + 8 * n + g, tok = row / a.G;
@@ -321,8 +321,6 @@ __device__ __forceinline__ bool chunk_few8(const ChunkArgs& a, const ChunkPiece&
     }
     scale[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
     scale[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
-    own[n][0] = (row_first + 8 * n + 2 * t) / a.G;
-    own[n][1] = (row_first + 8 * n + 2 * t + 1) / a.G;
   }
   float o[NT][D / 16][4], m[NT][2], l[NT][2], unit = 0.f;
 #pragma unroll
@@ -332,96 +330,107 @@ __device__ __forceinline__ bool chunk_few8(const ChunkArgs& a, const ChunkPiece&
     m[n][0] = m[n][1] = -INFINITY;
     l[n][0] = l[n][1] = 0.f;
   }
-  for (int j = 0; j < p.n; ++j, ++cf) {
-    const int place = cf % T::PLACES, is = cf % kChunkScales;
-    alive = alive && gemm_wait_warp(smem_u32(&bars.sc_full[is]), (cf / kChunkScales) & 1, abortp);
+  // (by the tile's number among all, so that a place, and its rounds, are always the same group's)
+  for (int j = (group - cf) & 1; j < p.n; j += 2) {
+    const int tile = cf + j, place = tile % T::PLACES, is = tile % kChunkScales;
+    alive = alive && gemm_wait_warp(smem_u32(&bars.sc_full[is]), (tile / kChunkScales) & 1, abortp);
     const float4 of = bars.sc[is];
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars.sc_empty[is]);
-    alive = alive && gemm_wait_warp(smem_u32(&bars.f_full[place]), (cf / T::PLACES) & 1, abortp);
+    alive = alive && gemm_wait_warp(smem_u32(&bars.f_full[place]), (tile / T::PLACES) & 1, abortp);
     if (!alive) break;   // (and on through the barriers)
-    const float to_log2 = page ? of.y : of.x, value = page ? of.w : of.z;
-    const uint32_t sk = smP + place * T::TILE + page * (64 * D), sv = sk + 2 * (64 * D);
-    const int beyond = (p.k0 + j) * 128 + 64 * page - p.pos0;   // the page's first key, from the first row's own on
-    if (value > unit) {
-      const float f = unit / value;
-      unit = value;
+#pragma unroll 1
+    for (int key = key0; key < key0 + keys; key += 16 * U) {
+      const int page = key >> 6, k_row = key & 63;
+      const float to_log2 = page ? of.y : of.x, value = page ? of.w : of.z;
+      const uint32_t sk = smP + place * T::TILE + page * (64 * D), sv = sk + 2 * (64 * D);
+      const int beyond = (p.k0 + j) * 128 + key - p.pos0;   // the first key, from the first row's own on
+      float ratio = 1.f;
+      if (value != unit) {
+        if (value > unit) {
+          const float f = unit / value;
+          unit = value;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[n][i][e] *= f;
+        }
+        ratio = value / unit;
+      }
+      const bool near = ratio >= 0x1p-16f;
+      const float weight = near ? 16.f * ratio : 16.f;   // (results are 16 times what they are: the weights' lowest are 2^-29 of one)
+      float s[U][NT][4];
+      float s2[U][NT][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = s2[u][n][0] = s2[u][n][1] = s2[u][n][2] = s2[u][n][3] = 0.f;
+#pragma unroll
+      for (int h = 0; h < KC; ++h) {
+        uint4 x[U], y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          x[u] = lds128(sk + chunk_code_at<D>(k_row + 16 * u + g, KC * t + h));
+          y[u] = lds128(sk + chunk_code_at<D>(k_row + 16 * u + g + 8, KC * t + h));
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            chunk_mma_e4m3(s[u][n], x[u].x, y[u].x, x[u].y, y[u].y, qh[n][4 * h], qh[n][4 * h + 1]);
+            chunk_mma_e4m3(s2[u][n], x[u].x, y[u].x, x[u].y, y[u].y, ql[n][4 * h], ql[n][4 * h + 1]);
+          }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            chunk_mma_e4m3(s[u][n], x[u].z, y[u].z, x[u].w, y[u].w, qh[n][4 * h + 2], qh[n][4 * h + 3]);
+            chunk_mma_e4m3(s2[u][n], x[u].z, y[u].z, x[u].w, y[u].w, ql[n][4 * h + 2], ql[n][4 * h + 3]);
+          }
+      }
+      // scores in log2 units
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
+        for (int e = 0; e < 4; ++e) {
+          const float f = to_log2 * scale[n][e & 1];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][i][e] *= f;
-    }
-    const float ratio = value / unit;
-    const bool near = ratio >= 0x1p-16f;
-    const float weight = near ? 16.f * ratio : 16.f;   // (results are 16 times what they are: the weights' lowest are 2^-29 of one)
-#pragma unroll 1
-    for (int kk = 0; kk < keys; kk += 16) {
-      const int k_row = in_page + kk;
-      float s[NT][4], s2[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.f;
-#pragma unroll
-      for (int h = 0; h < KC; ++h) {
-        const uint4 u = lds128(sk + chunk_code_at<D>(k_row + g, KC * t + h)), v = lds128(sk + chunk_code_at<D>(k_row + g + 8, KC * t + h));
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          chunk_mma_e4m3(s[n], u.x, v.x, u.y, v.y, qh[n][4 * h], qh[n][4 * h + 1]);
-          chunk_mma_e4m3(s2[n], u.x, v.x, u.y, v.y, ql[n][4 * h], ql[n][4 * h + 1]);
+          for (int u = 0; u < U; ++u) s[u][n][e] = (s[u][n][e] + s2[u][n][e]) * f;
         }
+      if (beyond + 16 * U - 1 > 0) {   // keys beyond a row's own
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          chunk_mma_e4m3(s[n], u.z, v.z, u.w, v.w, qh[n][4 * h + 2], qh[n][4 * h + 3]);
-          chunk_mma_e4m3(s2[n], u.z, v.z, u.w, v.w, ql[n][4 * h + 2], ql[n][4 * h + 3]);
+        for (int u = 0; u < U; ++u) {
+          const int of_lane = beyond + 16 * u + g;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int own = (row_first + 8 * n + 2 * t + e) / a.G;
+              if (of_lane > own) s[u][n][e] = -INFINITY;
+              if (of_lane + 8 > own) s[u][n][2 + e] = -INFINITY;
+            }
         }
       }
-      // values of the keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-      uint32_t w[4][VW];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = k_row + 2 * t + (i & 1) + 8 * (i >> 1);
-        if (D == 128) {
-          const uint4 u = lds128(sv + chunk_code_at<D>(r, g));
-          w[i][0] = u.x; w[i][1] = u.y; w[i][VW - 2] = u.z; w[i][VW - 1] = u.w;
-        } else {
-          const uint2 u = lds64(sv + chunk_code_at<D>(r, g >> 1) + 8 * (g & 1));
-          w[i][0] = u.x; w[i][1] = u.y;
-        }
-      }
-      // scores in log2 units; keys beyond a row's own
+      float top[NT][2];
       bool over = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + s2[n][e]) * (to_log2 * scale[n][e & 1]);
-      if (beyond + k_row + 15 > 0) {
-        const int key = beyond + k_row + g;
+        for (int e = 0; e < 2; ++e) {
+          top[n][e] = fmaxf(s[0][n][e], s[0][n][2 + e]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if (key > own[n][e]) s[n][e] = -INFINITY;
-            if (key + 8 > own[n][e]) s[n][2 + e] = -INFINITY;
-          }
-        // behind the item's last key there may be anything: 0 * NaN is not 0
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (beyond + k_row + 2 * t + (i & 1) + 8 * (i >> 1) >= p.tokens)
-#pragma unroll
-            for (int h = 0; h < VW; ++h) w[i][h] = 0;
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) over = over || fmaxf(s[n][e], s[n][2 + e]) > m[n][e] + 8.f;
+          for (int u = 1; u < U; ++u) top[n][e] = fmaxf(top[n][e], fmaxf(s[u][n][e], s[u][n][2 + e]));
+          over = over || top[n][e] > m[n][e] + 8.f;
+        }
       // the reference of a row moves where a score exceeds it by 8
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(s[n][e], s[n][2 + e]);
+            float x = top[n][e];
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -434,43 +443,79 @@ __device__ __forceinline__ bool chunk_few8(const ChunkArgs& a, const ChunkPiece&
             }
           }
       }
-      uint32_t b[NT][2];
+      uint32_t b[U][NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-        s[n][0] = fap_exp2(s[n][0] - m0); s[n][1] = fap_exp2(s[n][1] - m1);
-        s[n][2] = fap_exp2(s[n][2] - m0); s[n][3] = fap_exp2(s[n][3] - m1);
-        l[n][0] += s[n][0] + s[n][2];
-        l[n][1] += s[n][1] + s[n][3];
-        b[n][0] = chunk_turn8x8(chunk_pack_f16(s[n][0] * weight, s[n][1] * weight));
-        b[n][1] = chunk_turn8x8(chunk_pack_f16(s[n][2] * weight, s[n][3] * weight));
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+          const float e0 = fap_exp2(s[u][n][0] - m0), e1 = fap_exp2(s[u][n][1] - m1), e2 = fap_exp2(s[u][n][2] - m0), e3 = fap_exp2(s[u][n][3] - m1);
+          l[n][0] += e0 + e2;
+          l[n][1] += e1 + e3;
+          b[u][n][0] = chunk_turn8x8(chunk_pack_f16(e0 * weight, e1 * weight));
+          b[u][n][1] = chunk_turn8x8(chunk_pack_f16(e2 * weight, e3 * weight));
+        }
+      uint32_t w[U][4][VW];   // values of the keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = k_row + 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
+          if (D == 128) {
+            const uint4 x = lds128(sv + chunk_code_at<D>(r, g));
+            w[u][i][0] = x.x; w[u][i][1] = x.y; w[u][i][VW - 2] = x.z; w[u][i][VW - 1] = x.w;
+          } else {
+            const uint2 x = lds64(sv + chunk_code_at<D>(r, g >> 1) + 8 * (g & 1));
+            w[u][i][0] = x.x; w[u][i][1] = x.y;
+          }
+        }
+      if (beyond + 16 * U > p.tokens) {   // behind the item's last key there may be anything: 0 * NaN is not 0
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (beyond + 16 * u + 2 * t + (i & 1) + 8 * (i >> 1) >= p.tokens)
+#pragma unroll
+              for (int h = 0; h < VW; ++h) w[u][i][h] = 0;
       }
-      auto values = [&](int i, uint32_t (&v)[4]) {
+      auto values = [&](int u, int i, uint32_t (&v)[4]) {
         const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
-        const uint32_t lo = __byte_perm(w[0][i >> 1], w[1][i >> 1], sel), hi = __byte_perm(w[2][i >> 1], w[3][i >> 1], sel);
+        const uint32_t lo = __byte_perm(w[u][0][i >> 1], w[u][1][i >> 1], sel), hi = __byte_perm(w[u][2][i >> 1], w[u][3][i >> 1], sel);
         v[0] = chunk_f16(lo); v[1] = chunk_f16(lo >> 16); v[2] = chunk_f16(hi); v[3] = chunk_f16(hi >> 16);
       };
       if (near) {
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t v[4];
-          values(i, v);
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) chunk_mma_f16(o[n][i], v[0], v[1], v[2], v[3], b[n][0], b[n][1]);
-        }
-      } else {
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t v[4];
+            values(u, i, v);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t v[4];
-          values(i, v);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            chunk_mma_f16(d, v[0], v[1], v[2], v[3], b[n][0], b[n][1]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][i][e] = fmaf(d[e], ratio, o[n][i][e]);
+            for (int n = 0; n < NT; ++n) chunk_mma_f16(o[n][i], v[0], v[1], v[2], v[3], b[u][n][0], b[u][n][1]);
           }
-        }
+      } else {
+#pragma unroll 1
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t v[4];
+            values(0, i, v);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              float d[4] = {0.f, 0.f, 0.f, 0.f};
+              chunk_mma_f16(d, v[0], v[1], v[2], v[3], b[0][n][0], b[0][n][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[n][i][e] = fmaf(d[e], ratio, o[n][i][e]);
+            }
+            if (i == D / 16 - 1 && U > 1) {   // (the other keys in the same registers)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int h = 0; h < VW; ++h) w[0][k][h] = w[U - 1][k][h];
+#pragma unroll
+              for (int n = 0; n < NT; ++n) { b[0][n][0] = b[U - 1][n][0]; b[0][n][1] = b[U - 1][n][1]; }
+            }
+          }
       }
     }
     __syncwarp();
@@ -485,7 +530,7 @@ __device__ __forceinline__ bool chunk_few8(const ChunkArgs& a, const ChunkPiece&
       x += __shfl_xor_sync(0xffffffffu, x, 4);
       x += __shfl_xor_sync(0xffffffffu, x, 8);
       x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (g == 0) few.ml[warp][8 * n + 2 * t + e] = make_float2(m[n][e], x);
+      if (g == 0) few.ml[part][8 * n + 2 * t + e] = make_float2(m[n][e], x);
     }
   chunk_sync();
 #pragma unroll
@@ -495,15 +540,15 @@ __device__ __forceinline__ bool chunk_few8(const ChunkArgs& a, const ChunkPiece&
       const int col = 8 * n + 2 * t + e, row = row_first + col;
       float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
-      for (int w = 0; w < slices; ++w) top = fmaxf(top, few.ml[set * slices + w][col].x);
+      for (int w = 0; w < parts; ++w) top = fmaxf(top, few.ml[set * parts + w][col].x);
 #pragma unroll 1
-      for (int w = 0; w < slices; ++w) {
-        const float2 x = few.ml[set * slices + w][col];
+      for (int w = 0; w < parts; ++w) {
+        const float2 x = few.ml[set * parts + w][col];
         sum += x.x == -INFINITY ? 0.f : x.y * fap_exp2(x.x - top);
       }
       float f = m[n][e] == -INFINITY ? 0.f : fap_exp2(m[n][e] - top) * (unit * 0.0625f);
       if (whole) f /= sum;
-      else if (slice == 0 && g == 0 && row < rows) __stcg(reinterpret_cast<float2*>(rec + 256 * D + 2 * row), make_float2(top, sum));
+      else if (part == set * parts && g == 0 && row < rows) __stcg(reinterpret_cast<float2*>(rec + 256 * D + 2 * row), make_float2(top, sum));
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) { o[n][i][e] *= f; o[n][i][2 + e] *= f; }
     }
@@ -514,7 +559,7 @@ __device__ __forceinline__ bool chunk_few8(const ChunkArgs& a, const ChunkPiece&
     if (n > 0) chunk_sync();
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const uint32_t to = smO + (warp * 8 + 2 * t + e) * D * 4;
+      const uint32_t to = smO + (part * 8 + 2 * t + e) * D * 4;
 #pragma unroll
       for (int i = 0; i < D / 16; i += 2)   // features D / 8 g + 2 i ..
         asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((g * (D / 32) + (i >> 1)) ^ t) << 4)), "f"(o[n][i][e]), "f"(o[n][i][2 + e]), "f"(o[n][i + 1][e]),
@@ -527,8 +572,8 @@ __device__ __forceinline__ bool chunk_few8(const ChunkArgs& a, const ChunkPiece&
       if (row >= rows) continue;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-      for (int w = 0; w < slices; ++w) {
-        const uint4 u = lds128(smO + ((of_set * slices + w) * 8 + r8) * D * 4 + ((c4 ^ (r8 >> 1)) << 4));
+      for (int w = 0; w < parts; ++w) {
+        const uint4 u = lds128(smO + ((of_set * parts + w) * 8 + r8) * D * 4 + ((c4 ^ (r8 >> 1)) << 4));
         sum.x += __uint_as_float(u.x); sum.y += __uint_as_float(u.y); sum.z += __uint_as_float(u.z); sum.w += __uint_as_float(u.w);
       }
       const int tok = row / a.G;
@@ -580,8 +625,8 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
     }
     if (F8) {
-      for (int i = 0; i < T::PLACES; ++i) { mbar_init(&f_full[i], 1); mbar_init(&f_empty[i], 8); }
-      for (int i = 0; i < kChunkScales; ++i) { mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 8); }
+      for (int i = 0; i < T::PLACES; ++i) { mbar_init(&f_full[i], 1); mbar_init(&f_empty[i], 4); }
+      for (int i = 0; i < kChunkScales; ++i) { mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 4); }
       for (int i = 0; i < 2; ++i) mbar_init(&turn_free[i], 1);
     }
     abort_flag = 0;
@@ -645,8 +690,8 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           const bool whole = p.pieces == 1;
           float* const rec = a.part + (size_t)(2 * blockIdx.x + ((int)blockIdx.x == p.first)) * kChunkRecord<D>;
           const ChunkFew8Bars bars = {f_full, f_empty, sc_full, sc_empty, sc};
-          if (rows > 8) alive = chunk_few8<D, 2>(a, p, few, smV, smQ1, bars, abortp, cf, alive, rows, whole, rec);
-          else alive = chunk_few8<D, 1>(a, p, few, smV, smQ1, bars, abortp, cf, alive, rows, whole, rec);
+          if (rows > 8) alive = chunk_few8<D, 2, 2>(a, p, few, smV, smQ1, bars, abortp, cf, alive, rows, whole, rec);
+          else alive = chunk_few8<D, 1, 2>(a, p, few, smV, smQ1, bars, abortp, cf, alive, rows, whole, rec);
           cf += p.n;
           read_again();
           if (tid == 0) mbar_arrive(&turn_free[few_pieces & 1]);   // (behind a barrier of the eight warps)

@@ -40,8 +40,8 @@ class Walk:
         self.q_full, self.q_empty = bars(2, 1), bars(2, 1)
         self.k_full, self.k_empty, self.v_full, self.v_empty = (bars(self.R, 1) for _ in range(4))
         self.s_full, self.p_full, self.o_full = bars(2, 1), bars(2, 4), bars(2, 1)
-        self.f_full, self.f_empty = bars(self.PLACES, 1), bars(self.PLACES, 8)
-        self.sc_full, self.sc_empty = bars(self.SC, 1), bars(self.SC, 8)
+        self.f_full, self.f_empty = bars(self.PLACES, 1), bars(self.PLACES, 4)
+        self.sc_full, self.sc_empty = bars(self.SC, 1), bars(self.SC, 4)
         self.turn_free = bars(2, 1)
         self.pipe, self.copies, self.at_sync = [], [], 0
         self.sync_round = 0
@@ -219,15 +219,18 @@ class Walk:
         for n, (kind, tiles, cnt, cut) in enumerate(self.pieces):
             if kind == FEW:
                 for j in range(tiles):
-                    place, i = cf % self.PLACES, cf % self.SC
-                    yield from self.wait(self.sc_full[i], cf // self.SC)
+                    if (cf + j) % 2 != g:   # (the other group's)
+                        continue
+                    tile = cf + j
+                    place, i = tile % self.PLACES, tile % self.SC
+                    yield from self.wait(self.sc_full[i], tile // self.SC)
                     self.sc_empty[i].arrive()
-                    yield from self.wait(self.f_full[place], cf // self.PLACES)
+                    yield from self.wait(self.f_full[place], tile // self.PLACES)
                     assert self.place_in[place] == (n, j), "another tile"
                     yield
                     assert self.place_in[place] == (n, j), "another tile"
                     self.f_empty[place].arrive()
-                    cf += 1
+                cf += tiles
                 yield from self.sync()
                 self.q_in[1] = ("results", n)
                 yield from self.sync()
