@@ -1,6 +1,6 @@
 // The host side of calls of few rows, natively: nn.fused_rows (a norm, matrices of one input, and what follows them), the two launches of a
-// feed-forward, a decode step's attention (rotation and cache write, attention), and the operators of a ragged step (its plan, rotation and cache write,
-// attention, verification of drafts).  Each looks the layers and the activations over and makes the
+// feed-forward, a decode step's attention (rotation and cache write, attention), the operators of a ragged step (its plan, rotation and cache write,
+// attention, verification of drafts; the middle ones over 8-bit pages too), and products in 8-bit integers.  Each looks the layers and the activations over and makes the
 // launches.  From Python a launch spends 13 of its 19 us on attributes, checks, argument tables and conversions, and a decode layer makes
 // eight.  Launches are programmatic dependents of whatever is before them on the stream and only ask L2 for weights ahead of their wait; the
 // second of a native call reads them ahead of it: the first does not write them, and starts its dependents behind its own wait for all before it.  One row of a 1B feed-forward, whose kernels take 9 us: 39 us
@@ -26,7 +26,8 @@ namespace {
   X(pie_qmv_fused) X(pie_qmv_workspace_bytes) X(pie_qmt) X(pie_qmt_scratch_bytes) X(pie_rope_kv_rows) X(pie_rope_kvq_rows)                \
   X(pie_decode_attn) X(pie_decode_attn_pick_splits_for) X(pie_decode_attn_q8) X(pie_decode_attn_q8_pick_splits) X(pie_decode_attn_workspace_bytes) \
   X(pie_step_plan_words) X(pie_step_plan_offsets) X(pie_step_plan_build) X(pie_rope_kv_slots) X(pie_chunk_attn) X(pie_chunk_attn_workspace_bytes)     \
-  X(pie_verify_draft) X(pie_verify_workspace_bytes)
+  X(pie_verify_draft) X(pie_verify_workspace_bytes) X(pie_rope_kv_fp8) X(pie_chunk_attn_fp8) X(pie_chunk_attn_fp8_workspace_bytes)                            \
+  X(pie_int8_rows) X(pie_int8_matmul) X(pie_int8_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
   PIE_FUNCTIONS(X)
@@ -486,6 +487,214 @@ PyObject* chunk_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// a plan's dims, as the Python side's structure has them
+bool dims_of(PyObject* v, pie_step_dims& d) {
+  Py_buffer view;
+  if (PyObject_GetBuffer(v, &view, PyBUF_SIMPLE) < 0) { PyErr_Clear(); return false; }
+  const bool whole = view.len == sizeof(d);
+  if (whole) memcpy(&d, view.buf, sizeof(d));
+  PyBuffer_Release(&view);
+  return whole;
+}
+// codes [pages, Hkv, 64, D] and scales [pages, Hkv]
+bool fp8_pool(const at::Tensor* pool, const at::Tensor* scales, int device, const pie_step_dims& d, int64_t D) {
+  return here(pool, device) && here(scales, device) && pool->scalar_type() == at::kFloat8_e4m3fn && scales->scalar_type() == at::kFloat && pool->dim() == 4 && scales->dim() == 2 &&
+         pool->size(0) == d.pages && pool->size(1) == d.Hkv && pool->size(2) == 64 && pool->size(3) == D && scales->size(0) == d.pages && scales->size(1) == d.Hkv &&
+         pool->is_contiguous() && scales->is_contiguous() && aligned(pool->const_data_ptr(), 16);
+}
+
+// rope_kv_fp8(queries, keys, values, freqs, plan's words, plan's dims, k_pool, k_scales, v_pool, v_scales, out or None) -> rotated queries, or None
+PyObject* rope_kv_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 11 || !bound || !on_gpu(args[0])) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const at::Tensor *t[3], *freqs = tensor_of(args[3]), *words = tensor_of(args[4]), *pool[4];
+  for (int i = 0; i < 3; ++i) t[i] = tensor_of(args[i]);
+  for (int i = 0; i < 4; ++i) pool[i] = tensor_of(args[6 + i]);
+  pie_head_rows rows[3];
+  pie_step_dims d;
+  for (int i = 0; i < 3; ++i)
+    if (!head_rows(t[i], device, rows[i])) Py_RETURN_NONE;
+  const int64_t T = t[0]->size(0), Hq = t[0]->size(1), D = t[0]->size(2);
+  if (!dims_of(args[5], d) || (D != 64 && D != 128) || T != d.rows || Hq != d.Hq || t[1]->size(0) != T || t[1]->size(1) != d.Hkv || t[1]->size(2) != D ||
+      t[1]->sizes() != t[2]->sizes() || !here(freqs, device) || freqs->scalar_type() != at::kFloat || freqs->dim() != 1 || freqs->size(0) != D / 2 || !freqs->is_contiguous() ||
+      !ints(words, device, -1) || (size_t)words->size(0) != lib.pie_step_plan_words(&d) || !fp8_pool(pool[0], pool[1], device, d, D) || !fp8_pool(pool[2], pool[3], device, d, D))
+    Py_RETURN_NONE;
+  at::Tensor out;
+  bool fresh;
+  if (!result(args[10], {T, Hq, D}, *t[0], device, out, fresh)) Py_RETURN_NONE;
+  void* const stream = c10::cuda::getCurrentCUDAStream().stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = lib.pie_rope_kv_fp8(out.data_ptr(), (uint8_t*)pool[0]->data_ptr(), (float*)pool[1]->data_ptr(), (uint8_t*)pool[2]->data_ptr(), (float*)pool[3]->data_ptr(), &rows[0],
+                               &rows[1], &rows[2], (const int32_t*)words->const_data_ptr(), &d, (const float*)freqs->const_data_ptr(), (int)D, fresh, stream);
+  Py_END_ALLOW_THREADS
+  if (status != PIE_OK) Py_RETURN_NONE;
+  if (!fresh) return Py_NewRef(args[10]);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan's words, plan's dims, scale, out or None, workspace) -> [T, Hq D], or None.  workspace(key, bytes, device)
+PyObject* chunk_attention_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10 || !bound || !on_gpu(args[0]) || !PyFloat_CheckExact(args[7])) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const at::Tensor *q = tensor_of(args[0]), *words = tensor_of(args[5]), *pool[4];
+  for (int i = 0; i < 4; ++i) pool[i] = tensor_of(args[1 + i]);
+  pie_head_rows rows;
+  pie_step_dims d;
+  if (!dims_of(args[6], d) || !head_rows(q, device, rows) || !ints(words, device, -1) || q->size(0) != d.rows || q->size(1) != d.Hq ||
+      !fp8_pool(pool[0], pool[1], device, d, q->size(2)) || !fp8_pool(pool[2], pool[3], device, d, q->size(2)) || (size_t)words->size(0) != lib.pie_step_plan_words(&d))
+    Py_RETURN_NONE;
+  const int64_t T = q->size(0), D = q->size(2);
+  const size_t need = lib.pie_chunk_attn_fp8_workspace_bytes(&d, (int)D);
+  if (!need) Py_RETURN_NONE;
+  THPObjectPtr dev(PyObject_GetAttr(args[0], s_device));
+  if (!dev) return nullptr;
+  at::Tensor ws, out;
+  if (const Answer a = buffer(Py_BuildValue("(snO)", "chunk8", (Py_ssize_t)need, dev.get()), args[9], ws)) {
+    if (a == FAILED) return nullptr;
+    Py_RETURN_NONE;
+  }
+  bool fresh;
+  if (!result(args[8], {T, (int64_t)d.Hq * D}, *q, device, out, fresh)) Py_RETURN_NONE;
+  const float scale = (float)PyFloat_AS_DOUBLE(args[7]);
+  void* const stream = c10::cuda::getCurrentCUDAStream().stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = lib.pie_chunk_attn_fp8(out.data_ptr(), &rows, (const uint8_t*)pool[0]->const_data_ptr(), (const float*)pool[1]->const_data_ptr(), (const uint8_t*)pool[2]->const_data_ptr(),
+                                  (const float*)pool[3]->const_data_ptr(), (const int32_t*)words->const_data_ptr(), &d, (int)D, scale, fresh, ws.data_ptr(), (size_t)ws.numel(), stream);
+  Py_END_ALLOW_THREADS
+  if (status != PIE_OK) Py_RETURN_NONE;
+  if (!fresh) return Py_NewRef(args[8]);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// what int8_rows reads: rows of x as a kernel reads them, 16 bytes at a time, and the norm's weight
+struct Int8In { const void *x, *norm; int64_t ld, rows, K; float eps; };
+bool int8_in(PyObject* x_obj, PyObject* norm_obj, PyObject* eps, int device, Int8In& in) {
+  const at::Tensor *x = tensor_of(x_obj), *norm = norm_obj == Py_None ? nullptr : tensor_of(norm_obj);
+  if (!here(x, device) || x->scalar_type() != at::kBFloat16 || x->dim() < 1 || !PyFloat_CheckExact(eps)) return false;
+  const int64_t K = x->size(-1);
+  if (K < 16 || K % 16 || K > INT32_MAX || x->numel() == 0 || x->numel() / K > INT32_MAX) return false;
+  in = {x->const_data_ptr(), nullptr, K, x->numel() / K, K, (float)PyFloat_AS_DOUBLE(eps)};
+  if (!x->is_contiguous()) {
+    if (x->dim() != 2 || x->stride(1) != 1 || x->stride(0) < 0 || x->stride(0) % 8) return false;
+    in.ld = x->stride(0);
+  }
+  if (norm_obj != Py_None) {
+    if (!here(norm, device) || norm->scalar_type() != at::kBFloat16 || norm->dim() != 1 || norm->size(0) != K || !norm->is_contiguous()) return false;
+    in.norm = norm->const_data_ptr();
+  }
+  return aligned(in.x, 16) && aligned(in.norm, 16);
+}
+bool int8_weight(const at::Tensor* w, const at::Tensor* s, int device, int64_t K) {
+  return here(w, device) && here(s, device) && w->scalar_type() == at::kChar && s->scalar_type() == at::kFloat && w->dim() == 2 && s->dim() == 1 && w->size(1) == K && w->size(0) >= 1 &&
+         w->size(0) <= INT32_MAX && s->size(0) == w->size(0) && w->is_contiguous() && s->is_contiguous() && aligned(w->const_data_ptr(), 16) && aligned(s->const_data_ptr(), 16);
+}
+// the product's result, and its workspace
+Answer int8_out(PyObject* device_of, const at::Tensor& like, PyObject* residual, int device, int64_t M, int64_t N, PyObject* workspace, at::Tensor& y, at::Tensor& ws, const void*& add) {
+  c10::SmallVector<int64_t, 6> shape(like.sizes().begin(), like.sizes().end());
+  shape.back() = N;
+  add = nullptr;
+  if (residual != Py_None) {
+    const at::Tensor* r = tensor_of(residual);
+    if (!here(r, device) || r->scalar_type() != at::kBFloat16 || r->sizes() != at::IntArrayRef(shape) || !r->is_contiguous() || !aligned(r->const_data_ptr(), 16)) return NOT_MINE;
+    add = r->const_data_ptr();
+  }
+  if (const size_t need = lib.pie_int8_workspace_bytes((int)M, (int)N)) {
+    THPObjectPtr dev(PyObject_GetAttr(device_of, s_device));
+    if (!dev) return FAILED;
+    if (const Answer a = buffer(Py_BuildValue("(snO)", "int8", (Py_ssize_t)need, dev.get()), workspace, ws)) return a;
+  }
+  y = at::empty(shape, like.options().dtype(at::kBFloat16));
+  return plain(y) ? DONE : NOT_MINE;
+}
+
+// int8_rows(x, norm_weight or None, eps) -> (codes, scales), or None
+PyObject* int8_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Int8In in;
+  if (n != 3 || !bound || !on_gpu(args[0])) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  if (!int8_in(args[0], args[1], args[2], device, in)) Py_RETURN_NONE;
+  const at::Tensor& x = *tensor_of(args[0]);
+  at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar)), scales = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  if (!plain(codes)) Py_RETURN_NONE;
+  void* const stream = c10::cuda::getCurrentCUDAStream().stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = lib.pie_int8_rows((int8_t*)codes.data_ptr(), (float*)scales.data_ptr(), in.x, in.ld, (int)in.rows, (int)in.K, in.norm, in.eps, stream);
+  Py_END_ALLOW_THREADS
+  if (status != PIE_OK) Py_RETURN_NONE;
+  THPObjectPtr a(THPVariable_Wrap(std::move(codes))), b(THPVariable_Wrap(std::move(scales)));
+  return a && b ? PyTuple_Pack(2, a.get(), b.get()) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_matmul(codes, scales, weight, weight_scales, residual or None, workspace) -> y, or None
+PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !bound || !on_gpu(args[0])) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const at::Tensor *c = tensor_of(args[0]), *s = tensor_of(args[1]), *w = tensor_of(args[2]), *ws_of = tensor_of(args[3]);
+  if (!here(c, device) || !here(s, device) || c->scalar_type() != at::kChar || s->scalar_type() != at::kFloat || c->dim() < 1 || s->dim() != c->dim() - 1 ||
+      s->sizes() != c->sizes().slice(0, c->dim() - 1) || !c->is_contiguous() || !s->is_contiguous() || c->numel() == 0 || !aligned(c->const_data_ptr(), 16) ||
+      !aligned(s->const_data_ptr(), 16) || !int8_weight(w, ws_of, device, c->size(-1)) || s->numel() > INT32_MAX || c->size(-1) > INT32_MAX)
+    Py_RETURN_NONE;
+  const int64_t M = s->numel(), N = w->size(0), K = c->size(-1);
+  at::Tensor y, ws;
+  const void* add;
+  if (const Answer a = int8_out(args[0], *c, args[4], device, M, N, args[5], y, ws, add)) {
+    if (a == FAILED) return nullptr;
+    Py_RETURN_NONE;
+  }
+  void* const stream = c10::cuda::getCurrentCUDAStream().stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = lib.pie_int8_matmul(y.data_ptr(), (const int8_t*)c->const_data_ptr(), (const float*)s->const_data_ptr(), (const int8_t*)w->const_data_ptr(),
+                               (const float*)ws_of->const_data_ptr(), add, (int)M, (int)N, (int)K, ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, stream);
+  Py_END_ALLOW_THREADS
+  if (status != PIE_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_linear(x, weight, weight_scales, norm_weight or None, eps, residual or None, workspace) -> y, or None
+PyObject* int8_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Int8In in;
+  if (n != 7 || !bound || !on_gpu(args[0])) Py_RETURN_NONE;
+  const int device = c10::cuda::current_device();
+  const at::Tensor *w = tensor_of(args[1]), *ws_of = tensor_of(args[2]);
+  if (!int8_in(args[0], args[3], args[4], device, in) || in.K >= 131072 || !int8_weight(w, ws_of, device, in.K)) Py_RETURN_NONE;
+  const at::Tensor& x = *tensor_of(args[0]);
+  const int64_t M = in.rows, N = w->size(0);
+  at::Tensor y, ws;
+  const void* add;
+  if (const Answer a = int8_out(args[0], x, args[5], device, M, N, args[6], y, ws, add)) {
+    if (a == FAILED) return nullptr;
+    Py_RETURN_NONE;
+  }
+  // codes, and behind them the scales (K is a multiple of 16)
+  at::Tensor rows = at::empty({M * (in.K + 4)}, x.options().dtype(at::kByte));
+  int8_t* const codes = (int8_t*)rows.data_ptr();
+  float* const scales = (float*)(codes + M * in.K);
+  void* const stream = c10::cuda::getCurrentCUDAStream().stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = lib.pie_int8_rows(codes, scales, in.x, in.ld, (int)M, (int)in.K, in.norm, in.eps, stream);
+  if (status == PIE_OK)
+    status = lib.pie_int8_matmul(y.data_ptr(), codes, scales, (const int8_t*)w->const_data_ptr(), (const float*)ws_of->const_data_ptr(), add, (int)M, (int)N, (int)in.K,
+                                 ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, stream);
+  Py_END_ALLOW_THREADS
+  if (status != PIE_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
 // verify_draft(logits, draft_tokens, logit_starts, max_draft, temp, uniforms, noise, draft_logits (or None each), workspace) -> (tokens, counts, logprobs), or None
 PyObject* verify_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -562,6 +771,11 @@ PyMethodDef methods[] = {{"fused_rows", (PyCFunction)(void (*)(void))fused_rows,
                          {"rope_kv_slots", (PyCFunction)(void (*)(void))rope_kv_slots, METH_FASTCALL, "ops.rope_kv_slots, or None"},
                          {"chunk_attention", (PyCFunction)(void (*)(void))chunk_attention, METH_FASTCALL, "ops.chunk_attention, or None"},
                          {"verify_draft", (PyCFunction)(void (*)(void))verify_draft, METH_FASTCALL, "ops.verify_draft, or None"},
+                         {"rope_kv_fp8", (PyCFunction)(void (*)(void))rope_kv_fp8, METH_FASTCALL, "ops.rope_kv_fp8, or None"},
+                         {"chunk_attention_fp8", (PyCFunction)(void (*)(void))chunk_attention_fp8, METH_FASTCALL, "ops.chunk_attention_fp8, or None"},
+                         {"int8_rows", (PyCFunction)(void (*)(void))int8_rows, METH_FASTCALL, "ops.int8_rows, or None"},
+                         {"int8_matmul", (PyCFunction)(void (*)(void))int8_matmul, METH_FASTCALL, "ops.int8_matmul, or None"},
+                         {"int8_linear", (PyCFunction)(void (*)(void))int8_linear, METH_FASTCALL, "ops.int8_linear, or None"},
                          {"bind", bind, METH_VARARGS, "addresses of the library's functions"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pie_host", nullptr, -1, methods};

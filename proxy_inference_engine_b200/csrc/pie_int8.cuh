@@ -1,7 +1,7 @@
 // Products in 8-bit integers with a scale for each token and each channel (include/pie_b200.h): y[m, n] = bf16(s_m t_n sum_k c[m, k] w[n, k]).  Compiled with pie_qmm.cu,
 // whose pipeline word it shares.
 //
-//   * int8_rows_kernel: a token's features as integers, c = x / s rounded to the nearest, s = max |x| / 127; the layer's norm in front of it.
+//   * int8_rows_kernel: a token's features as integers, c = x / s rounded to the nearest, s = max |x| / 127 (times the 32-bit 1 / 127); the layer's norm in front of it.
 //   * more than kInt8Few rows: the GEMM core of pie_gemm.cuh on the integer tensor pipe (tcgen05 kind::i8, twice the multiply-adds of bf16 in a byte of shared memory and of
 //     time), scales and residual in its epilogue.
 //   * up to that: int8_few_kernel, bound by the stream of weights.
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(int8_t* codes, float* sc
 #pragma unroll
   for (int w = 0; w < 8; ++w) m = max(m, most[w]);
   // an infinity or a NaN: nothing of the row has a value, and its products are NaN
-  const float amax = __uint_as_float(m << 16), s = m < 0x7f80u ? __fdiv_rn(amax, 127.f) : __uint_as_float(0x7fc00000u);
+  const float amax = __uint_as_float(m << 16), s = m < 0x7f80u ? amax * (1.f / 127.f) : __uint_as_float(0x7fc00000u);
   if (tid == 0) scales[blockIdx.x] = s;
   const bool some = s > 0.f;
   // (scales below 1e-30: every quotient is taken by division, since 1 / s may not be a number.  t = 0.5 takes it there.)

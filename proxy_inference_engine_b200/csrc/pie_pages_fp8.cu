@@ -19,6 +19,7 @@ struct Fp8Args {
   const float* freqs;
   int requests, rows, pages, Hq, Hkv, rest;
   int page_ctas, HL;       // CTAs of pages; threads that share a row's queries / 8 pairs
+  int heads;               // of a CTA of pages, one after the other
 };
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -52,6 +53,23 @@ __device__ __forceinline__ void angles8(float position, const float* freqs, floa
 #pragma unroll
   for (int e = 0; e < 8; ++e) rope_sincos(position * (1.0f / freqs[e]), &sn[e], &cs[e]);
 }
+// sin / cos of an angle of up to 2^17 to the last place or so (rope_sincos is off by 5e-7, which a rounding to bf16 hides and one to a code, next to a border, shows): the angle less the nearest
+// multiple k of pi / 2, taken off in three pieces -- k has 17 bits, so that the first difference is exact --, and Taylor's polynomials on what is left, at most pi / 4 (next terms 2e-9).
+__device__ __forceinline__ void sincos_of(float theta, float& sn, float& cs) {
+  const float k = rintf(theta * 0.636619772f);
+  float r = fmaf(-k, 1.57079637f, theta);
+  r = fmaf(-k, -4.37113883e-8f, r);
+  r = fmaf(-k, -1.71512451e-15f, r);
+  const float z = r * r;
+  float s = fmaf(z, fmaf(z, fmaf(z, 2.75573192e-6f, -1.98412698e-4f), 8.33333333e-3f), -0.166666667f);
+  s = fmaf(r * z, s, r);
+  float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, -2.75573192e-7f, 2.48015873e-5f), -1.38888889e-3f), 4.16666667e-2f), -0.5f);
+  c = fmaf(z, c, 1.f);
+  const int q = (int)k;
+  const float a = q & 1 ? c : s, b = q & 1 ? s : c;
+  sn = q & 2 ? -a : a;
+  cs = (q + 1) & 2 ? -b : b;
+}
 // the lowest power of two, 2^-60 at least, with which a magnitude is 448 or less; NaN for what is not finite
 __device__ __forceinline__ float e4m3_scale(uint32_t bits) {
   if (bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
@@ -63,7 +81,7 @@ template <int D>
 __global__ void __launch_bounds__(256) rope_kv_fp8_kernel(const __grid_constant__ Fp8Args a) {
   constexpr int half = D / 2, PB = half / 8, VC = D / 8;     // pieces of eight: pairs of a head, features of a head
   constexpr int KN = 64 * PB / 256, VN = 64 * VC / 256;      // of a page, a thread
-  __shared__ uint32_t most[2][8];
+  __shared__ uint32_t most[2][2][8];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -103,7 +121,7 @@ __global__ void __launch_bounds__(256) rope_kv_fp8_kernel(const __grid_constant_
     return;
   }
   // -------------------------------------------------------------------------------------------------- a page of a head
-  const int head = (int)blockIdx.x % a.Hkv, place = (int)blockIdx.x / a.Hkv;
+  const int sets = (a.Hkv + a.heads - 1) / a.heads, head0 = (int)blockIdx.x % sets * a.heads, place = (int)blockIdx.x / sets;
   // the last request whose places begin at or below this one: every so many-th of them, then those between
   int s = 0, n_rows = 0, row0 = 0;
   for (int stride = (a.requests + 255) / 256, span = a.requests;; span = stride, stride = 1) {
@@ -121,84 +139,91 @@ __global__ void __launch_bounds__(256) rope_kv_fp8_kernel(const __grid_constant_
   row0 += skipped;
   const int slot = __ldg(a.slots + row0);
   if (slot < 0 || slot >= a.pages * kStepPage) return;
-  const size_t block = (size_t)(slot / kStepPage) * a.Hkv + head;
-  uint8_t* const kp = a.kp + block * kStepPage * D;
-  uint8_t* const vp = a.vp + block * kStepPage * D;
-  const float had_k = lies ? a.ks[block] : 0.f, had_v = lies ? a.vs[block] : 0.f;
-
-  uint4 v[VN], k1[KN], k2[KN];
-#pragma unroll
-  for (int i = 0; i < KN; ++i) {
-    const int t = (tid + 256 * i) / PB, pb = tid % PB;
-    k1[i] = k2[i] = make_uint4(0, 0, 0, 0);
-    if (t < count) {
-      const uint16_t* const src = a.r.k + (row0 + t) * a.r.ks.sl + head * a.r.ks.sh + pb * 8;
-      k1[i] = *reinterpret_cast<const uint4*>(src);
-      k2[i] = *reinterpret_cast<const uint4*>(src + half);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < VN; ++i) {
-    const int t = (tid + 256 * i) / VC, c = tid % VC;
-    v[i] = make_uint4(0, 0, 0, 0);
-    if (t < count) v[i] = *reinterpret_cast<const uint4*>(a.r.v + (row0 + t) * a.r.vs.sl + head * a.r.vs.sh + c * 8);
-  }
-  float o1[KN][8], o2[KN][8];
-  uint32_t mk = 0, mv = 0;   // magnitudes in the order of their bits
+  float sn[KN][8], cs[KN][8];
 #pragma unroll
   for (int i = 0; i < KN; ++i) {
     const int t = (tid + 256 * i) / PB;
-    if (t < count) {
-      float sn[8], cs[8];
-      angles8((float)(page * kStepPage + lies + t), a.freqs + tid % PB * 8, cs, sn);
-      turn8(k1[i], k2[i], cs, sn, o1[i], o2[i]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) mk = max(mk, max(__float_as_uint(o1[i][e]) & 0x7fffffffu, __float_as_uint(o2[i][e]) & 0x7fffffffu));
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < VN; ++i) {
-    constexpr uint32_t ABS = 0x7fff7fffu;
-    const uint32_t m = __vmaxu2(__vmaxu2(v[i].x & ABS, v[i].y & ABS), __vmaxu2(v[i].z & ABS, v[i].w & ABS));
-    mv = max(mv, max(m << 16, m & 0xffff0000u));
-  }
-  mk = __reduce_max_sync(0xffffffffu, mk);
-  mv = __reduce_max_sync(0xffffffffu, mv);
-  if (lane == 0) { most[0][warp] = mk; most[1][warp] = mv; }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) { mk = max(mk, most[0][w]); mv = max(mv, most[1][w]); }
-  const float need_k = e4m3_scale(mk), need_v = e4m3_scale(mv);
-  const float sk = had_k >= need_k || had_k != had_k ? had_k : need_k, sv = had_v >= need_v || had_v != had_v ? had_v : need_v;
-  const float ik = 1.f / sk, iv = 1.f / sv;
-  if (tid == 0) { a.ks[block] = sk; a.vs[block] = sv; }
-#pragma unroll
-  for (int i = 0; i < KN; ++i) {
-    const int t = (tid + 256 * i) / PB, pb = tid % PB;
-    if (t < count) {
-      uint8_t* const to = kp + (lies + t) * D + pb * 8;
-      *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(o1[i][0] * ik, o1[i][1] * ik, o1[i][2] * ik, o1[i][3] * ik), e4m3x4(o1[i][4] * ik, o1[i][5] * ik, o1[i][6] * ik, o1[i][7] * ik));
-      *reinterpret_cast<uint2*>(to + half) = make_uint2(e4m3x4(o2[i][0] * ik, o2[i][1] * ik, o2[i][2] * ik, o2[i][3] * ik), e4m3x4(o2[i][4] * ik, o2[i][5] * ik, o2[i][6] * ik, o2[i][7] * ik));
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < VN; ++i) {
-    const int t = (tid + 256 * i) / VC, c = tid % VC;
     if (t < count)
-      *reinterpret_cast<uint2*>(vp + (lies + t) * D + c * 8) =
-          make_uint2(e4m3x4(bf16lo(v[i].x) * iv, bf16hi(v[i].x) * iv, bf16lo(v[i].y) * iv, bf16hi(v[i].y) * iv),
-                     e4m3x4(bf16lo(v[i].z) * iv, bf16hi(v[i].z) * iv, bf16lo(v[i].w) * iv, bf16hi(v[i].w) * iv));
-  }
-  // what the page held, where its scale has grown
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const float had = kv ? had_v : had_k, now = kv ? sv : sk;
-    if (!(now > had)) continue;
-    const float f = had / now;
-    uint4* const p = reinterpret_cast<uint4*>(kv ? vp : kp);
-    for (int i = tid; i < lies * (D / 16); i += 256) {
-      const uint4 w = p[i];
-      p[i] = make_uint4(e4m3x4_times(w.x, f), e4m3x4_times(w.y, f), e4m3x4_times(w.z, f), e4m3x4_times(w.w, f));
+      for (int e = 0; e < 8; ++e) sincos_of((float)(page * kStepPage + lies + t) * (1.0f / __ldg(a.freqs + tid % PB * 8 + e)), sn[i][e], cs[i][e]);
+  }
+#pragma unroll 1
+  for (int head = head0; head < min(head0 + a.heads, a.Hkv); ++head) {
+    const size_t block = (size_t)(slot / kStepPage) * a.Hkv + head;
+    uint8_t* const kp = a.kp + block * kStepPage * D;
+    uint8_t* const vp = a.vp + block * kStepPage * D;
+    const float had_k = lies ? a.ks[block] : 0.f, had_v = lies ? a.vs[block] : 0.f;
+
+    uint4 v[VN], k1[KN], k2[KN];
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const int t = (tid + 256 * i) / PB, pb = tid % PB;
+      k1[i] = k2[i] = make_uint4(0, 0, 0, 0);
+      if (t < count) {
+        const uint16_t* const src = a.r.k + (row0 + t) * a.r.ks.sl + head * a.r.ks.sh + pb * 8;
+        k1[i] = *reinterpret_cast<const uint4*>(src);
+        k2[i] = *reinterpret_cast<const uint4*>(src + half);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int t = (tid + 256 * i) / VC, c = tid % VC;
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (t < count) v[i] = *reinterpret_cast<const uint4*>(a.r.v + (row0 + t) * a.r.vs.sl + head * a.r.vs.sh + c * 8);
+    }
+    float o1[KN][8], o2[KN][8];
+    uint32_t mk = 0, mv = 0;   // magnitudes in the order of their bits
+#pragma unroll
+    for (int i = 0; i < KN; ++i)
+      if ((tid + 256 * i) / PB < count) {
+        turn8(k1[i], k2[i], cs[i], sn[i], o1[i], o2[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mk = max(mk, max(__float_as_uint(o1[i][e]) & 0x7fffffffu, __float_as_uint(o2[i][e]) & 0x7fffffffu));
+      }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      constexpr uint32_t ABS = 0x7fff7fffu;
+      const uint32_t m = __vmaxu2(__vmaxu2(v[i].x & ABS, v[i].y & ABS), __vmaxu2(v[i].z & ABS, v[i].w & ABS));
+      mv = max(mv, max(m << 16, m & 0xffff0000u));
+    }
+    mk = __reduce_max_sync(0xffffffffu, mk);
+    mv = __reduce_max_sync(0xffffffffu, mv);
+    if (lane == 0) { most[head & 1][0][warp] = mk; most[head & 1][1][warp] = mv; }   // (two of them: a warp may be at the next head)
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) { mk = max(mk, most[head & 1][0][w]); mv = max(mv, most[head & 1][1][w]); }
+    const float need_k = e4m3_scale(mk), need_v = e4m3_scale(mv);
+    const float sk = had_k >= need_k || had_k != had_k ? had_k : need_k, sv = had_v >= need_v || had_v != had_v ? had_v : need_v;
+    const float ik = 1.f / sk, iv = 1.f / sv;
+    if (tid == 0) { a.ks[block] = sk; a.vs[block] = sv; }   // (every thread's had_k, had_v lie behind the barrier's other side)
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const int t = (tid + 256 * i) / PB, pb = tid % PB;
+      if (t < count) {
+        uint8_t* const to = kp + (lies + t) * D + pb * 8;
+        *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(o1[i][0] * ik, o1[i][1] * ik, o1[i][2] * ik, o1[i][3] * ik), e4m3x4(o1[i][4] * ik, o1[i][5] * ik, o1[i][6] * ik, o1[i][7] * ik));
+        *reinterpret_cast<uint2*>(to + half) = make_uint2(e4m3x4(o2[i][0] * ik, o2[i][1] * ik, o2[i][2] * ik, o2[i][3] * ik), e4m3x4(o2[i][4] * ik, o2[i][5] * ik, o2[i][6] * ik, o2[i][7] * ik));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int t = (tid + 256 * i) / VC, c = tid % VC;
+      if (t < count)
+        *reinterpret_cast<uint2*>(vp + (lies + t) * D + c * 8) =
+            make_uint2(e4m3x4(bf16lo(v[i].x) * iv, bf16hi(v[i].x) * iv, bf16lo(v[i].y) * iv, bf16hi(v[i].y) * iv),
+                       e4m3x4(bf16lo(v[i].z) * iv, bf16hi(v[i].z) * iv, bf16lo(v[i].w) * iv, bf16hi(v[i].w) * iv));
+    }
+    // what the page held, where its scale has grown
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const float had = kv ? had_v : had_k, now = kv ? sv : sk;
+      if (!(now > had)) continue;
+      const float f = had / now;
+      uint4* const p = reinterpret_cast<uint4*>(kv ? vp : kp);
+      for (int i = tid; i < lies * (D / 16); i += 256) {
+        const uint4 w = p[i];
+        p[i] = make_uint4(e4m3x4_times(w.x, f), e4m3x4_times(w.y, f), e4m3x4_times(w.z, f), e4m3x4_times(w.w, f));
+      }
     }
   }
 }
@@ -231,7 +256,9 @@ extern "C" int pie_rope_kv_fp8(void* q_out, uint8_t* kpool, float* k_scales, uin
   const int lanes = 256 / (D / 16);
   a.HL = d->rows >= 1024 ? 4 : lanes;
   const int per = lanes / a.HL;
-  const long long pages = (2LL * d->requests + d->rows / kStepPage) * d->Hkv, grid = pages + (d->rows + per - 1) / per;
+  // Heads that share a row's angles: as many as leave each SM some CTAs of full pages (8191 rows of 8 heads: one a CTA 43 us, two 40, four 42).
+  a.heads = d->rows / kStepPage * (long long)d->Hkv >= 4LL * num_sms() ? 2 : 1;
+  const long long pages = (2LL * d->requests + d->rows / kStepPage) * ((d->Hkv + a.heads - 1) / a.heads), grid = pages + (d->rows + per - 1) / per;
   if (grid > 0x7fffffff) return PIE_EINVAL_SHAPE;
   a.page_ctas = (int)pages;
   count_launch();

@@ -264,6 +264,7 @@ def attention_workspace(units: int, nbytes: int, device) -> torch.Tensor:
 class _NoHost:
     """Where csrc/pie_host.cpp's module was not built, or for another torch or interpreter: None to every call."""
     mlp_rows = attend_rows = step_plan = rope_kv_slots = chunk_attention = verify_draft = staticmethod(lambda *args: None)
+    rope_kv_fp8 = chunk_attention_fp8 = int8_rows = int8_matmul = int8_linear = staticmethod(lambda *args: None)
 
 
 @functools.cache
@@ -280,6 +281,7 @@ def native_fused_rows():
         spec.loader.exec_module(host)
         host.bind({name: C.cast(getattr(L, name), C.c_void_p).value for name in host.functions})
         host.fused_rows, host.mlp_rows, host.attend_rows, host.step_plan, host.rope_kv_slots, host.chunk_attention, host.verify_draft
+        host.rope_kv_fp8, host.chunk_attention_fp8, host.int8_rows, host.int8_matmul, host.int8_linear
     except (ImportError, OSError, AttributeError, KeyError, TypeError) as e:   # (one of an earlier build has other functions, or another bind)
         warnings.warn(f"{path} does not load ({e}): build it again with make -C {_lib.CSRC}.  Calls of few rows take the Python form meanwhile.")
         return lambda *args: None
@@ -287,7 +289,7 @@ def native_fused_rows():
 
 
 def native_host():
-    """The module native_fused_rows() is of: several launches of few rows (mlp_rows, attend_rows) and the operators of a ragged step, with the same None."""
+    """The module native_fused_rows() is of: several launches of few rows (mlp_rows, attend_rows), the operators of a ragged step and products in 8-bit integers, with the same None."""
     return getattr(native_fused_rows(), "__self__", _NoHost)
 
 
@@ -773,6 +775,9 @@ def rope_kv_fp8(queries, keys, values, freqs, plan, k_pool, k_scales, v_pool, v_
     page anew, and a row that needs a larger scale has what the page holds in front of it brought to that, by a power of two and so without another rounding, but below e4m3's lowest.  A
     page and head that an infinity or a NaN was written to has scale NaN.  No two requests of a plan may write to the same page.  Returns the rotated queries, [T, Hq, D]; rows that
     belong to nobody as rope_kv_slots has them."""
+    got = native_host().rope_kv_fp8(queries, keys, values, freqs, plan.words, plan.dims, k_pool, k_scales, v_pool, v_scales, out)
+    if got is not None:
+        return got
     what = "rope_kv_fp8"
     if queries.dim() != 3 or keys.dim() != 3 or values.shape != keys.shape or keys.shape[0] != queries.shape[0] or keys.shape[2] != queries.shape[2]:
         raise ValueError(f"[{what}] queries [T, Hq, D], keys and values [T, Hkv, D] expected, but they are {tuple(queries.shape)}, {tuple(keys.shape)} and "
@@ -801,6 +806,9 @@ def chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan, scale: floa
     pages' scales.  Returns [T, Hq * D].  Softmax weights are rounded for their product with the values: to fp16, 2^-12 of one, where a request's rows, its new tokens x Hq / Hkv, are at
     most 64 (and for the last ones of longer requests), otherwise to bfloat16; the pages of those are first brought to bfloat16 in a workspace of twice the pools' bytes, which all layers
     share.  A page of scale NaN may make all of its request's new tokens NaN.  Rows that belong to nobody are zero, or with ``out`` given what that held."""
+    got = native_host().chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan.words, plan.dims, float(scale), out, workspaces.get)
+    if got is not None:
+        return got
     what = "chunk_attention_fp8"
     if q.dim() != 3 or q.dtype != _BF16:
         raise ValueError(f"[{what}] queries must be bfloat16 [T, Hq, D], but are {q.dtype} {tuple(q.shape)}")
@@ -906,9 +914,12 @@ def _int8_features(what: str, x, norm_weight) -> int:
 
 
 def int8_rows(x, *, norm_weight=None, eps: float = 1e-5):
-    """Rows of 8-bit integers with a scale each: of x bfloat16 [..., K] (K a multiple of 16) the codes int8 [..., K] and scales f32 [...], with s = max |x| / 127 and codes
+    """Rows of 8-bit integers with a scale each: of x bfloat16 [..., K] (K a multiple of 16) the codes int8 [..., K] and scales f32 [...], with s = max |x| / 127 (times the 32-bit 1 / 127) and codes
     x / s rounded to the nearest, of two the even one, so that x is about codes * s.  With norm_weight (bfloat16 [K]) of rms_norm(x, norm_weight, eps).  A row of zeros has scale
     0; a row with an infinity or a NaN has scale NaN, so that its products are NaN.  A weight [N, K] becomes integers with a scale for each output channel the same way."""
+    got = native_host().int8_rows(x, norm_weight, float(eps))
+    if got is not None:
+        return got
     what = "int8_rows"
     K = _int8_features(what, x, norm_weight)
     with _one_device(what, x, *(() if norm_weight is None else (norm_weight,))):
@@ -935,6 +946,9 @@ def int8_matmul(codes, scales, weight, weight_scales, *, residual=None):
     """Product of 8-bit integers with a scale for each token and each channel: y[..., n] = bf16((sum_k codes[..., k] weight[n, k]) scales[...] weight_scales[n]), and
     bf16(residual + y) with a residual (bfloat16 [..., N]).  codes int8 [..., K] and scales f32 [...] as int8_rows gives them, weight int8 [N, K] and weight_scales f32 [N] (int8_rows
     of a weight).  K: a multiple of 16 below 131072.  The sum is exact, and a row's result does not depend on the rows beside it."""
+    got = native_host().int8_matmul(codes, scales, weight, weight_scales, residual, workspaces.get)
+    if got is not None:
+        return got
     what = "int8_matmul"
     if codes.dim() < 1 or codes.dtype != torch.int8 or codes.shape[-1] == 0 or codes.shape[-1] % 16:
         raise ValueError(f"[{what}] codes must be int8 [..., K] with K a multiple of 16, but are {codes.dtype} {tuple(codes.shape)}")
@@ -964,6 +978,9 @@ def int8_matmul(codes, scales, weight, weight_scales, *, residual=None):
 def int8_linear(x, weight, weight_scales, *, norm_weight=None, eps: float = 1e-5, residual=None):
     """A linear layer of 8-bit integers: int8_rows of x (bfloat16 [..., K], through the layer's norm with norm_weight), int8_matmul of those with weight int8 [N, K] and
     weight_scales f32 [N], and the residual added.  Returns bfloat16 [..., N]."""
+    got = native_host().int8_linear(x, weight, weight_scales, norm_weight, float(eps), residual, workspaces.get)
+    if got is not None:
+        return got
     what = "int8_linear"
     K = _int8_features(what, x, norm_weight)
     N = _int8_weight(what, weight, weight_scales, K)

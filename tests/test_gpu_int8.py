@@ -27,7 +27,7 @@ def integers(g, *shape, lo=-127):
 def plain_rows(x):
     """The definition, in 32 bits, on the CPU (whose division is exact to the last place)."""
     x = x.float().cpu()
-    scales = x.abs().amax(-1) / 127
+    scales = x.abs().amax(-1) * torch.tensor(1 / 127, dtype=F32)
     ok = torch.isfinite(x).all(-1)
     codes = torch.where((scales > 0)[..., None] & ok[..., None], (x / scales[..., None]).round().clamp(-127, 127), 0.0)
     return torch.nan_to_num(codes).to(I8), torch.where(ok, scales, float("nan"))
