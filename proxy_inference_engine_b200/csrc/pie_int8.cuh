@@ -13,22 +13,25 @@
 namespace pie {
 
 // ---------------------------------------------------------------------------------------------------- rows
-// the code of x, in the lowest byte of the sum's bits: 1.5 2^23 + n
-__device__ __forceinline__ float int8_sum(float x, float s, float inv) {
-  const float t = x * inv, u = t + 12582912.f, d = fabsf(t - (u - 12582912.f));
-  // t is off by less than 2e-5: near a half, the quotient itself tells which side it is on
-  if (fabsf(d - 0.5f) < 1e-4f) return rintf(fminf(fmaxf(__fdiv_rn(x, s), -127.f), 127.f)) + 12582912.f;
-  return u;
-}
+// Eight codes: the quotients rounded by adding 1.5 2^23, whose sum has the code in its lowest byte.  A quotient by 1 / s is off by less than 2e-5: where one of the eight is as near to a half,
+// all are taken by division.  (Asked of each by itself, 8191 rows of 14336 115 us.)  s < 1e-30: by division too, since 1 / s may not be a number.
 __device__ __forceinline__ uint2 int8_codes(const uint4& v, float s, float inv) {
   const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+  float u[8], near = s < 1e-30f ? 0.f : 1.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = (e & 1 ? bf16hi(q[e >> 1]) : bf16lo(q[e >> 1])) * inv;
+    u[e] = t + 12582912.f;
+    near = fminf(near, fabsf(fabsf(t - (u[e] - 12582912.f)) - 0.5f));
+  }
+  if (near < 1e-4f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = rintf(fminf(fmaxf(__fdiv_rn(e & 1 ? bf16hi(q[e >> 1]) : bf16lo(q[e >> 1]), s), -127.f), 127.f)) + 12582912.f;
+  }
   uint32_t w[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t a = __float_as_uint(int8_sum(bf16lo(q[2 * h]), s, inv)), b = __float_as_uint(int8_sum(bf16hi(q[2 * h]), s, inv)),
-                   c = __float_as_uint(int8_sum(bf16lo(q[2 * h + 1]), s, inv)), d = __float_as_uint(int8_sum(bf16hi(q[2 * h + 1]), s, inv));
-    w[h] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-  }
+  for (int h = 0; h < 2; ++h)
+    w[h] = __byte_perm(__byte_perm(__float_as_uint(u[4 * h]), __float_as_uint(u[4 * h + 1]), 0x0040), __byte_perm(__float_as_uint(u[4 * h + 2]), __float_as_uint(u[4 * h + 3]), 0x0040), 0x5410);
   return make_uint2(w[0], w[1]);
 }
 // eight features through the norm, rounded as pie_rms_norm rounds
@@ -53,11 +56,12 @@ __device__ __forceinline__ uint32_t int8_most(const uint4& v, uint32_t m) {   //
   return __vmaxu2(__vmaxu2(__vmaxu2(m, v.x & ABS), __vmaxu2(v.y & ABS, v.z & ABS)), v.w & ABS);
 }
 
-// A CTA a row.  NV 16-byte pieces a thread are held in registers, so that a row is read once; NV 0: rows of any length, read again for each of the passes.
-template <int NV>
-__global__ void __launch_bounds__(256) int8_rows_kernel(int8_t* codes, float* scales, const uint16_t* x, long long x_ld, const uint16_t* norm, float eps, int nvec) {
-  __shared__ float sums[8];
-  __shared__ uint32_t most[8];
+// A CTA of THREADS a row.  NV 16-byte pieces a thread are held in registers, so that a row is read once; NV 0: rows of any length, read again for each of the passes.
+template <int NV, int THREADS, bool NORM>
+__global__ void __launch_bounds__(THREADS) int8_rows_kernel(int8_t* codes, float* scales, const uint16_t* x, long long x_ld, const uint16_t* norm, float eps, int nvec) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ float sums[WARPS];
+  __shared__ uint32_t most[WARPS];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -68,88 +72,81 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(int8_t* codes, float* sc
   if (NV) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int i = tid + 256 * j;
+      const int i = tid + THREADS * j;
       v[j] = i < nvec ? xr[i] : make_uint4(0, 0, 0, 0);
-      if (norm) g[j] = i < nvec ? __ldg(wr + i) : make_uint4(0, 0, 0, 0);
+      if (NORM) g[j] = i < nvec ? __ldg(wr + i) : make_uint4(0, 0, 0, 0);
     }
   }
   float inv_rms = 0.f;
-  if (norm) {
+  if (NORM) {
     float ss = 0.f;
     if (NV) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) ss = int8_squares(v[j], ss);
     } else {
-      for (int i = tid; i < nvec; i += 256) ss = int8_squares(xr[i], ss);
+      for (int i = tid; i < nvec; i += THREADS) ss = int8_squares(xr[i], ss);
     }
     ss = warp_sum(ss);
     if (lane == 0) sums[warp] = ss;
     __syncthreads();
     float total = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) total += sums[w];
+    for (int w = 0; w < WARPS; ++w) total += sums[w];
     inv_rms = 1.0f / sqrtf(total / (float)(nvec * 8) + eps);
   }
   uint32_t m = 0;
   if (NV) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (norm) v[j] = int8_norm(v[j], g[j], inv_rms);
+      if (NORM) v[j] = int8_norm(v[j], g[j], inv_rms);
       m = int8_most(v[j], m);   // (a piece behind the row's end is zeros, or 0 * inv_rms: where that is not 0, the row has no finite norm)
     }
   } else {
-    for (int i = tid; i < nvec; i += 256) {
+    for (int i = tid; i < nvec; i += THREADS) {
       const uint4 a = xr[i];
-      m = int8_most(norm ? int8_norm(a, __ldg(wr + i), inv_rms) : a, m);
+      m = int8_most(NORM ? int8_norm(a, __ldg(wr + i), inv_rms) : a, m);
     }
   }
   m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
   if (lane == 0) most[warp] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) m = max(m, most[w]);
+  for (int w = 0; w < WARPS; ++w) m = max(m, most[w]);
   // an infinity or a NaN: nothing of the row has a value, and its products are NaN
   const float amax = __uint_as_float(m << 16), s = m < 0x7f80u ? amax * (1.f / 127.f) : __uint_as_float(0x7fc00000u);
   if (tid == 0) scales[blockIdx.x] = s;
   const bool some = s > 0.f;
-  // (scales below 1e-30: every quotient is taken by division, since 1 / s may not be a number.  t = 0.5 takes it there.)
-  const bool tiny = s < 1e-30f;
-  const float inv = some ? (tiny ? 0.f : __fdiv_rn(1.f, s)) : 0.f;
+  const float inv = some && s >= 1e-30f ? __fdiv_rn(1.f, s) : 0.f;
   auto put = [&](int i, const uint4& a) {
     if (i >= nvec) return;
-    uint2 c = make_uint2(0, 0);
-    if (some) {
-      if (!tiny) {
-        c = int8_codes(a, s, inv);
-      } else {
-        const uint32_t q[4] = {a.x, a.y, a.z, a.w};
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float f = e & 1 ? bf16hi(q[e >> 1]) : bf16lo(q[e >> 1]);
-          w[e >> 2] |= (uint32_t)((int)rintf(fminf(fmaxf(__fdiv_rn(f, s), -127.f), 127.f)) & 255) << (8 * (e & 3));
-        }
-        c = make_uint2(w[0], w[1]);
-      }
-    }
-    out[i] = c;
+    out[i] = some ? int8_codes(a, s, inv) : make_uint2(0, 0);
   };
   if (NV) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) put(tid + 256 * j, v[j]);
+    for (int j = 0; j < NV; ++j) put(tid + THREADS * j, v[j]);
   } else {
-    for (int i = tid; i < nvec; i += 256) {
+    for (int i = tid; i < nvec; i += THREADS) {
       const uint4 a = xr[i];
-      put(i, norm ? int8_norm(a, __ldg(wr + i), inv_rms) : a);
+      put(i, NORM ? int8_norm(a, __ldg(wr + i), inv_rms) : a);
     }
   }
 }
 
+template <int THREADS, bool NORM>
+static cudaError_t launch_int8_rows_by(int8_t* codes, float* scales, const uint16_t* x, long long x_ld, int rows, int nvec, const uint16_t* norm, float eps, cudaStream_t st) {
+  const int per = (nvec + THREADS - 1) / THREADS;
+  auto kern = per <= 1 ? int8_rows_kernel<1, THREADS, NORM> : per <= 2 ? int8_rows_kernel<2, THREADS, NORM> : per <= 4 ? int8_rows_kernel<4, THREADS, NORM>
+              : per <= 8 && THREADS < 1024 ? int8_rows_kernel<THREADS < 1024 ? 8 : 4, THREADS, NORM> : int8_rows_kernel<0, THREADS, NORM>;
+  count_launch();
+  return launch_pdl(kern, dim3((unsigned)rows), dim3(THREADS), 0, st, codes, scales, x, x_ld, norm, eps, nvec);
+}
+// Few rows are a chain (loads, largest, division, codes) that the product waits for: as many threads as a row has pieces, up to 1024 (a row of 14336 as 256 threads 6.6 us); many rows are bound by
+// HBM (8191 of 14336 81.8 us at 127 registers, of which the norm's weights were 32).
 cudaError_t launch_int8_rows(int8_t* codes, float* scales, const uint16_t* x, long long x_ld, int rows, int K, const uint16_t* norm, float eps, cudaStream_t st) {
   const int nvec = K / 8;
-  auto kern = nvec <= 256 ? int8_rows_kernel<1> : nvec <= 512 ? int8_rows_kernel<2> : nvec <= 1024 ? int8_rows_kernel<4> : nvec <= 2048 ? int8_rows_kernel<8> : int8_rows_kernel<0>;
-  count_launch();
-  return launch_pdl(kern, dim3((unsigned)rows), dim3(256), 0, st, codes, scales, x, x_ld, norm, eps, nvec);
+  if (rows <= num_sms() && nvec > 512)
+    return norm ? launch_int8_rows_by<1024, true>(codes, scales, x, x_ld, rows, nvec, norm, eps, st) : launch_int8_rows_by<1024, false>(codes, scales, x, x_ld, rows, nvec, norm, eps, st);
+  return norm ? launch_int8_rows_by<256, true>(codes, scales, x, x_ld, rows, nvec, norm, eps, st) : launch_int8_rows_by<256, false>(codes, scales, x, x_ld, rows, nvec, norm, eps, st);
 }
 
 // ---------------------------------------------------------------------------------------------------- many rows
@@ -237,6 +234,7 @@ static cudaError_t launch_int8_core(const Int8Store& epi, const int8_t* codes, c
 //   * a tile that lies in several shares is added up in 32-bit integers: every CTA adds its part to the tile's sums in the workspace, and the last one to come takes them
 //     and leaves zeros.  (Integers: the same sum in any order.)
 constexpr int kInt8Few = 64;   // rows, at most
+constexpr int kInt8Ahead = 26; // K steps of 16 KB a CTA asks L2 for
 template <int NB>
 struct Int8Few {
   static constexpr int A_STAGE = 128 * 128, B_STAGE = NB * 128;
@@ -285,8 +283,9 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   if (warp == T::W_TMA && lane == 0) {
     tma_prefetch_desc(&map_w);
     tma_prefetch_desc(&map_x);
-    // the first weights on their way to L2 while the launch before this one drains (nothing is read ahead of the wait: it may have written them)
-    for (int i = 0; i < min(S, total); ++i) {
+    // The first weights on their way to L2 while the launch before this one, which makes the codes, goes on (nothing is read ahead of the wait: it may have written them): as much as
+    // half of L2 holds.
+    for (int i = 0; i < min(kInt8Ahead, total); ++i) {
       const int kb = (k_first + i) % a.nk, t = tile0 + (k_first + i) / a.nk;
       gemm_prefetch_3d(&map_w, kb * 64, t * 128, 0);
     }

@@ -78,10 +78,11 @@ __device__ __forceinline__ float e4m3_scale(uint32_t bits) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(256) rope_kv_fp8_kernel(const __grid_constant__ Fp8Args a) {
+__global__ void __launch_bounds__(256, 3) rope_kv_fp8_kernel(const __grid_constant__ Fp8Args a) {
   constexpr int half = D / 2, PB = half / 8, VC = D / 8;     // pieces of eight: pairs of a head, features of a head
   constexpr int KN = 64 * PB / 256, VN = 64 * VC / 256;      // of a page, a thread
   __shared__ uint32_t most[2][2][8];
+  __shared__ float4 angles[KN][4][256];                      // a thread's own: cosines, sines of its pairs
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -139,14 +140,33 @@ __global__ void __launch_bounds__(256) rope_kv_fp8_kernel(const __grid_constant_
   row0 += skipped;
   const int slot = __ldg(a.slots + row0);
   if (slot < 0 || slot >= a.pages * kStepPage) return;
-  float sn[KN][8], cs[KN][8];
+  {
+    float inv[8];
 #pragma unroll
-  for (int i = 0; i < KN; ++i) {
-    const int t = (tid + 256 * i) / PB;
-    if (t < count)
+    for (int e = 0; e < 8; ++e) inv[e] = 1.0f / __ldg(a.freqs + tid % PB * 8 + e);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sincos_of((float)(page * kStepPage + lies + t) * (1.0f / __ldg(a.freqs + tid % PB * 8 + e)), sn[i][e], cs[i][e]);
+    for (int i = 0; i < KN; ++i) {
+      const int t = (tid + 256 * i) / PB;
+      if (t >= count) break;
+      float sn[8], cs[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sincos_of((float)(page * kStepPage + lies + t) * inv[e], sn[e], cs[e]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        angles[i][h][tid] = make_float4(cs[4 * h], cs[4 * h + 1], cs[4 * h + 2], cs[4 * h + 3]);
+        angles[i][2 + h][tid] = make_float4(sn[4 * h], sn[4 * h + 1], sn[4 * h + 2], sn[4 * h + 3]);
+      }
+    }
   }
+  auto turned = [&](int i, const uint4& k1, const uint4& k2, float (&o1)[8], float (&o2)[8]) {
+    float cs[8], sn[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      *reinterpret_cast<float4*>(cs + 4 * h) = angles[i][h][tid];
+      *reinterpret_cast<float4*>(sn + 4 * h) = angles[i][2 + h][tid];
+    }
+    turn8(k1, k2, cs, sn, o1, o2);
+  };
 #pragma unroll 1
   for (int head = head0; head < min(head0 + a.heads, a.Hkv); ++head) {
     const size_t block = (size_t)(slot / kStepPage) * a.Hkv + head;
@@ -171,14 +191,14 @@ __global__ void __launch_bounds__(256) rope_kv_fp8_kernel(const __grid_constant_
       v[i] = make_uint4(0, 0, 0, 0);
       if (t < count) v[i] = *reinterpret_cast<const uint4*>(a.r.v + (row0 + t) * a.r.vs.sl + head * a.r.vs.sh + c * 8);
     }
-    float o1[KN][8], o2[KN][8];
     uint32_t mk = 0, mv = 0;   // magnitudes in the order of their bits
 #pragma unroll
     for (int i = 0; i < KN; ++i)
       if ((tid + 256 * i) / PB < count) {
-        turn8(k1[i], k2[i], cs[i], sn[i], o1[i], o2[i]);
+        float o1[8], o2[8];
+        turned(i, k1[i], k2[i], o1, o2);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mk = max(mk, max(__float_as_uint(o1[i][e]) & 0x7fffffffu, __float_as_uint(o2[i][e]) & 0x7fffffffu));
+        for (int e = 0; e < 8; ++e) mk = max(mk, max(__float_as_uint(o1[e]) & 0x7fffffffu, __float_as_uint(o2[e]) & 0x7fffffffu));
       }
 #pragma unroll
     for (int i = 0; i < VN; ++i) {
@@ -200,9 +220,11 @@ __global__ void __launch_bounds__(256) rope_kv_fp8_kernel(const __grid_constant_
     for (int i = 0; i < KN; ++i) {
       const int t = (tid + 256 * i) / PB, pb = tid % PB;
       if (t < count) {
+        float o1[8], o2[8];   // (once more: sooner done than held)
+        turned(i, k1[i], k2[i], o1, o2);
         uint8_t* const to = kp + (lies + t) * D + pb * 8;
-        *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(o1[i][0] * ik, o1[i][1] * ik, o1[i][2] * ik, o1[i][3] * ik), e4m3x4(o1[i][4] * ik, o1[i][5] * ik, o1[i][6] * ik, o1[i][7] * ik));
-        *reinterpret_cast<uint2*>(to + half) = make_uint2(e4m3x4(o2[i][0] * ik, o2[i][1] * ik, o2[i][2] * ik, o2[i][3] * ik), e4m3x4(o2[i][4] * ik, o2[i][5] * ik, o2[i][6] * ik, o2[i][7] * ik));
+        *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(o1[0] * ik, o1[1] * ik, o1[2] * ik, o1[3] * ik), e4m3x4(o1[4] * ik, o1[5] * ik, o1[6] * ik, o1[7] * ik));
+        *reinterpret_cast<uint2*>(to + half) = make_uint2(e4m3x4(o2[0] * ik, o2[1] * ik, o2[2] * ik, o2[3] * ik), e4m3x4(o2[4] * ik, o2[5] * ik, o2[6] * ik, o2[7] * ik));
       }
     }
 #pragma unroll
@@ -256,8 +278,9 @@ extern "C" int pie_rope_kv_fp8(void* q_out, uint8_t* kpool, float* k_scales, uin
   const int lanes = 256 / (D / 16);
   a.HL = d->rows >= 1024 ? 4 : lanes;
   const int per = lanes / a.HL;
-  // Heads that share a row's angles: as many as leave each SM some CTAs of full pages (8191 rows of 8 heads: one a CTA 43 us, two 40, four 42).
-  a.heads = d->rows / kStepPage * (long long)d->Hkv >= 4LL * num_sms() ? 2 : 1;
+  // Heads that share a row's angles, as many as leave each SM a CTA of full pages (8191 rows of 8 heads: one a CTA 42.7 us, two 42.4, four 37.1).
+  const long long blocks = d->rows / kStepPage * (long long)d->Hkv;
+  a.heads = blocks >= 4LL * num_sms() ? 4 : blocks >= 2LL * num_sms() ? 2 : 1;
   const long long pages = (2LL * d->requests + d->rows / kStepPage) * ((d->Hkv + a.heads - 1) / a.heads), grid = pages + (d->rows + per - 1) / per;
   if (grid > 0x7fffffff) return PIE_EINVAL_SHAPE;
   a.page_ctas = (int)pages;
