@@ -1407,21 +1407,26 @@ __global__ void __launch_bounds__(256) chunk_widen_kernel(const uint8_t* k8, con
       for (int u = ((int)blockIdx.x + (int)gridDim.x - done % (int)gridDim.x) % (int)gridDim.x; u < units; u += gridDim.x) {
         const size_t block = (size_t)__ldg(table + (size_t)r * blocks + u / Hkv) * Hkv + u % Hkv;
         const float fk = __ldg(ks + block), fv = __ldg(vs + block);
-        for (int e = tid; e < 2 * pieces; e += 256) {
-          const bool v = e >= pieces;
-          const size_t at = block * pieces + (v ? e - pieces : e);
-          const uint4 w = __ldg(reinterpret_cast<const uint4*>(v ? v8 : k8) + at);
-          const float f = v ? fv : fk;
-          const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+        uint4 w[4];   // all of a thread's on their way together: at most two of K, two of V
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int e = tid + 256 * (q & 1);
+          if (e < pieces) w[q] = __ldg(reinterpret_cast<const uint4*>(q >> 1 ? v8 : k8) + block * pieces + e);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int e = tid + 256 * (q & 1);
+          if (e >= pieces) continue;
+          const float f = q >> 1 ? fv : fk;
+          const uint32_t in[4] = {w[q].x, w[q].y, w[q].z, w[q].w};
           uint32_t out[8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const uint32_t two = chunk_f16(in[q >> 1] >> (16 * (q & 1)));
+          for (int i = 0; i < 8; ++i) {
             float lo, hi;
-            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(lo), "=f"(hi) : "r"(two));
-            out[q] = pack_bf16(lo * f, hi * f);   // (exact: the scale is a power of two)
+            chunk_f32(chunk_f16(in[i >> 1] >> (16 * (i & 1))), lo, hi);
+            out[i] = pack_bf16(lo * f, hi * f);   // (exact: the scale is a power of two)
           }
-          uint4* const to = reinterpret_cast<uint4*>(v ? v16 : k16) + 2 * at;
+          uint4* const to = reinterpret_cast<uint4*>(q >> 1 ? v16 : k16) + 2 * (block * pieces + e);
           to[0] = make_uint4(out[0], out[1], out[2], out[3]);
           to[1] = make_uint4(out[4], out[5], out[6], out[7]);
         }
@@ -1435,7 +1440,7 @@ __global__ void __launch_bounds__(256) chunk_widen_kernel(const uint8_t* k8, con
 static bool chunk_wide8(const pie_step_dims& d) { return d.rows > ChunkTile<128, true>::FEW / (d.Hq / d.Hkv); }
 static cudaError_t launch_chunk_widen(const ChunkArgs& a, const pie_step_dims& d, int D, const uint8_t* k8, const uint8_t* v8, uint16_t* k16, uint16_t* v16, cudaStream_t st) {
   count_launch();
-  return launch_pdl(chunk_widen_kernel, dim3((unsigned)(num_sms() * 4)), dim3(256), 0, st, k8, v8, a.k_scales, a.v_scales, k16, v16, a.row_starts, a.contexts, a.table, d.requests, d.blocks,
+  return launch_pdl(chunk_widen_kernel, dim3((unsigned)(num_sms() * 8)), dim3(256), 0, st, k8, v8, a.k_scales, a.v_scales, k16, v16, a.row_starts, a.contexts, a.table, d.requests, d.blocks,
                     d.Hkv, D, a.few_tokens);
 }
 static size_t chunk_workspace_bytes(int D) { return kStepMaxCtas * 4 + (size_t)2 * kStepMaxCtas * (D == 128 ? kChunkRecord<128> : kChunkRecord<64>) * 4; }

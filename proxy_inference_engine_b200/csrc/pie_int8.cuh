@@ -228,20 +228,21 @@ static cudaError_t launch_int8_core(const Int8Store& epi, const int8_t* codes, c
 
 // ---------------------------------------------------------------------------------------------------- few rows
 // What bounds it is the stream of weights, so the shape follows from keeping that going on every SM:
-//   * the weights are the MMA's A operand, 128 channels a tile, and the rows, padded to NB, its N: tcgen05.mma kind::i8, M128 N{16, 32, 64} K32.
+//   * the weights are the MMA's A operand, 128 channels a tile, and the rows, padded to 16, its N: tcgen05.mma kind::i8, M128 N16 K32.
 //   * the tiles' K steps of 128 bytes lie one behind the other on a line and every CTA has the same length of it, so that no SM waits for others' tiles.  A CTA's TMA ring
 //     goes on from one tile to the next; two accumulators, so that a tile's end is under the next one's start.
 //   * a tile that lies in several shares is added up in 32-bit integers: every CTA adds its part to the tile's sums in the workspace, and the last one to come takes them
 //     and leaves zeros.  (Integers: the same sum in any order.)
-constexpr int kInt8Few = 64;   // rows, at most
+// us, codes given, weights not in L2; this and the core: 1 row 6144 x 4096 9.0, 11; 4096 x 14336 14.2, 17.0; 28672 x 4096 22.7, 25.5 (5.2 TB/s).  16 rows 10.6, 15.7, 24.7.  What does not
+// shrink with the weights, some 5 us, is the start, sums and counter in L2, and their way back.  32 rows (as wider MMAs) 14.0, 18.4, 28.6: that many sums are sooner added up in the
+// shared memory of the core's clusters (11.0, 17.0, 25.6).
+constexpr int kInt8Few = 16;   // rows, at most
 constexpr int kInt8Ahead = 26; // K steps of 16 KB a CTA asks L2 for
-template <int NB>
 struct Int8Few {
-  static constexpr int A_STAGE = 128 * 128, B_STAGE = NB * 128;
-  static constexpr int S = NB == 16 ? 11 : NB == 32 ? 10 : 8;
+  static constexpr int A_STAGE = 128 * 128, B_STAGE = kInt8Few * 128, S = 11;
   static constexpr int SMEM = 1024 + S * (A_STAGE + B_STAGE);
   static constexpr int THREADS = 192, W_TMA = 4, W_MMA = 5;
-  static constexpr int TMEM_COLS = NB == 16 ? 32 : 2 * NB;
+  static constexpr int TMEM_COLS = 2 * kInt8Few;
   static_assert(SMEM <= 226 * 1024, "shared memory");
 };
 struct Int8FewArgs {
@@ -250,15 +251,14 @@ struct Int8FewArgs {
   const float *sx, *sw;
   int M, N, nk, ctas;        // nk: K steps of a tile
   long long steps;           // of all tiles
-  int* sums;                 // [tiles][NB][128], zero between launches
+  int* sums;                 // [tiles][16][128], zero between launches
   unsigned int* count;       // [tiles], zero between launches
 };
 
-template <int NB>
-__global__ void __launch_bounds__(Int8Few<NB>::THREADS, 1)
+__global__ void __launch_bounds__(Int8Few::THREADS, 1)
 int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Int8FewArgs a) {
-  using T = Int8Few<NB>;
-  constexpr int S = T::S;
+  using T = Int8Few;
+  constexpr int S = T::S, NB = kInt8Few;
   constexpr uint32_t IDESC = umma_idesc_i8<128, NB>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], tfull_bar[2], tempty_bar[2];
@@ -316,18 +316,15 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         const uint16_t o = f2bf((float)sum * __ldg(a.sx + m) * tw);
         a.y[p] = a.residual ? f2bf(bf16lo(o) + bf16lo(a.residual[p])) : o;
       };
-#pragma unroll 1
-      for (int c = 0; c < NB && c < a.M; c += 16) {
-        uint32_t v[16];
-        tmem_ld16(tmem + (uint32_t)(b * NB + c) + ((uint32_t)(warp * 32) << 16), v);
-        tmem_ld_wait();
+      uint32_t v[16];
+      tmem_ld16(tmem + (uint32_t)(b * NB) + ((uint32_t)(warp * 32) << 16), v);
+      tmem_ld_wait();
 #pragma unroll
-        for (int q = 0; q < 16; ++q)
-          if (c + q < a.M && there) {
-            if (whole) put(c + q, (int)v[q]);
-            else atomicAdd(sums + (c + q) * 128, (int)v[q]);
-          }
-      }
+      for (int q = 0; q < 16; ++q)
+        if (q < a.M && there) {
+          if (whole) put(q, (int)v[q]);
+          else atomicAdd(sums + q * 128, (int)v[q]);
+        }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty_bar[b]);
@@ -401,27 +398,25 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   if (warp == T::W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(T::TMEM_COLS) : "memory");
 }
 
-template <int NB>
 static cudaError_t launch_int8_few(Int8FewArgs a, const int8_t* codes, const int8_t* w, int K, cudaStream_t st) {
-  using T = Int8Few<NB>;
+  using T = Int8Few;
   static std::atomic<unsigned long long> served{0};
-  const cudaError_t set = once_per_device(served, [] { return cudaFuncSetAttribute(int8_few_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM); });
+  const cudaError_t set = once_per_device(served, [] { return cudaFuncSetAttribute(int8_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM); });
   if (set != cudaSuccess) return set;
   CUtensorMap mw, mx;
-  if (!gemm_map(&mw, w, 2, K / 2, a.N, K, 1, 0, 128) || !gemm_map(&mx, codes, 2, K / 2, a.M, K, 1, 0, NB)) return cudaErrorNotSupported;
+  if (!gemm_map(&mw, w, 2, K / 2, a.N, K, 1, 0, 128) || !gemm_map(&mx, codes, 2, K / 2, a.M, K, 1, 0, kInt8Few)) return cudaErrorNotSupported;
   const int tiles = (a.N + 127) / 128, sms = num_sms();
   a.nk = (K + 127) / 128;
   a.steps = (long long)tiles * a.nk;
   a.ctas = (int)(a.steps < sms ? a.steps : sms);
   count_launch();
-  return launch_pdl(int8_few_kernel<NB>, dim3((unsigned)a.ctas), dim3(T::THREADS), T::SMEM, st, mw, mx, a);
+  return launch_pdl(int8_few_kernel, dim3((unsigned)a.ctas), dim3(T::THREADS), T::SMEM, st, mw, mx, a);
 }
-static int int8_few_columns(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : 64; }
 
 size_t int8_workspace_bytes(int M, int N) {
   if (M > kInt8Few) return 0;
   const size_t tiles = ((size_t)N + 127) / 128;
-  return (tiles * 4 + 255) / 256 * 256 + tiles * 128 * int8_few_columns(M) * 4;
+  return (tiles * 4 + 255) / 256 * 256 + tiles * 128 * kInt8Few * 4;
 }
 
 cudaError_t launch_int8_matmul(uint16_t* y, const int8_t* codes, const float* sx, const int8_t* w, const float* sw, const uint16_t* residual, int M, int N, int K, void* ws,
@@ -432,7 +427,7 @@ cudaError_t launch_int8_matmul(uint16_t* y, const int8_t* codes, const float* sx
   a.y = y; a.residual = residual; a.sx = sx; a.sw = sw; a.M = M; a.N = N;
   a.count = (unsigned int*)ws;
   a.sums = (int*)((uint8_t*)ws + (tiles * 4 + 255) / 256 * 256);
-  return M <= 16 ? launch_int8_few<16>(a, codes, w, K, st) : M <= 32 ? launch_int8_few<32>(a, codes, w, K, st) : launch_int8_few<64>(a, codes, w, K, st);
+  return launch_int8_few(a, codes, w, K, st);
 }
 
 }  // namespace pie

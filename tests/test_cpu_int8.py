@@ -55,5 +55,5 @@ def test_c_calls():
     mul = lambda y=fake, w=fake, M=3, N=5, K=32, ws=fake, nb=1 << 20: L.pie_int8_matmul(y, fake, fake, w, fake, None, M, N, K, ws, nb, None)
     assert mul(y=None) == 5 and mul(w=odd) == 6 and mul(ws=odd) == 6 and mul(M=-1) == 1 and mul(N=0) == 1 and mul(K=40) == 1 and mul(K=131072) == 1
     assert mul(ws=None) == 7 and mul(nb=100) == 7 and mul(M=0) == 0 and mul(M=1 << 24, N=1 << 24) == 1
-    assert L.pie_int8_workspace_bytes(64, 1000) > 64 * 1000 * 4 and L.pie_int8_workspace_bytes(200, 1000) == 0 and L.pie_int8_workspace_bytes(0, 1000) == 0
+    assert L.pie_int8_workspace_bytes(16, 1000) > 16 * 1000 * 4 and L.pie_int8_workspace_bytes(200, 1000) == 0 and L.pie_int8_workspace_bytes(0, 1000) == 0
     assert L.pie_launch_count() == n0
