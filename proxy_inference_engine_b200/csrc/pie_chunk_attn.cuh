@@ -1446,12 +1446,12 @@ static cudaError_t launch_chunk_widen(const ChunkArgs& a, const pie_step_dims& d
 static size_t chunk_workspace_bytes(int D) { return kStepMaxCtas * 4 + (size_t)2 * kStepMaxCtas * (D == 128 ? kChunkRecord<128> : kChunkRecord<64>) * 4; }
 // the common part: q's maps, the plan's arrays
 template <bool F8>
-static int chunk_common(ChunkArgs& a, CUtensorMap* maps, void* out, const pie_head_rows* q, const int32_t* plan, const pie_step_dims* d, int D, float scale, int rest,
+static int chunk_common(ChunkArgs& a, CUtensorMap* maps, void* out, const pie_head_rows* q, const void* kpool, const void* vpool, const int32_t* plan, const pie_step_dims* d, int D, float scale, int rest,
                         void* workspace, size_t workspace_bytes) {
   if ((D != 64 && D != 128) || !(scale > 0.f) || scale > 3.4028234e38f / 1.5f || q->stride_h % 8 || q->stride_l % 8 || (d->rows > 1 && q->stride_l <= 0) ||
       (d->Hq > 1 && q->stride_h <= 0))
     return PIE_EINVAL_SHAPE;
-  for (const void* p : {(const void*)out, q->p, (const void*)plan, (const void*)workspace})
+  for (const void* p : {(const void*)out, q->p, kpool, vpool, (const void*)plan, (const void*)workspace})
     if (reinterpret_cast<uintptr_t>(p) & 15) return PIE_EALIGN;
   if (!workspace || workspace_bytes < chunk_workspace_bytes(D)) return PIE_EWORKSPACE;
   const StepLayout l = step_layout(*d);
@@ -1497,9 +1497,7 @@ int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const v
   if (kv->tok_stride <= 0 || kv->tok_stride % 8 || kv->head_stride % 8 || (d->Hkv > 1 && kv->head_stride <= 0)) return PIE_EINVAL_SHAPE;
   ChunkArgs a;
   CUtensorMap maps[4];
-  if (int s = chunk_common<false>(a, maps, out, q, plan, d, D, scale, rest, workspace, workspace_bytes)) return s;
-  for (const void* p : {kpool, vpool})
-    if (reinterpret_cast<uintptr_t>(p) & 15) return PIE_EALIGN;
+  if (int s = chunk_common<false>(a, maps, out, q, kpool, vpool, plan, d, D, scale, rest, workspace, workspace_bytes)) return s;
   const GemmEncodeFn fn = gemm_encode_fn();
   const cuuint32_t one[4] = {1, 1, 1, 1};
   for (int i = 0; i < 2; ++i) {   // a page of one head: 64 features of its 64 slots
@@ -1527,10 +1525,9 @@ int pie_chunk_attn_fp8(void* out, const pie_head_rows* q, const uint8_t* kpool, 
   if (!out || !q || !q->p || !kpool || !k_scales || !vpool || !v_scales || !plan) return PIE_ENULL;
   ChunkArgs a;
   CUtensorMap maps[4];
-  if (int s = chunk_common<true>(a, maps, out, q, plan, d, D, scale, rest, workspace, workspace_bytes)) return s;
-  for (const void* p : {(const void*)kpool, (const void*)vpool})
-    if (reinterpret_cast<uintptr_t>(p) & 15) return PIE_EALIGN;
-  if (workspace_bytes < pie_chunk_attn_fp8_workspace_bytes(d, D)) return PIE_EWORKSPACE;
+  if (D == 64 || D == 128)
+    if (!workspace || workspace_bytes < pie_chunk_attn_fp8_workspace_bytes(d, D)) return PIE_EWORKSPACE;
+  if (int s = chunk_common<true>(a, maps, out, q, kpool, vpool, plan, d, D, scale, rest, workspace, workspace_bytes)) return s;
   a.k_scales = k_scales; a.v_scales = v_scales;
   a.q = (const uint16_t*)q->p; a.q_row = d->rows > 1 ? q->stride_l : 0; a.q_head = d->Hq > 1 ? q->stride_h : 0;
   const GemmEncodeFn fn = gemm_encode_fn();

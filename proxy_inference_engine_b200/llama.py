@@ -211,6 +211,9 @@ class MLP(nn.Module):
 
     def activations(self, x):
         """silu(gate) * up of a prompt's rows."""
+        both = nn.int8_beside(x, (self.gate_proj, self.up_proj))
+        if both is not None:
+            return ops.silu_mul(*both)
         act = nn.fused_swiglu(x, self.gate_proj, self.up_proj)
         return ops.silu_mul(self.gate_proj(x), self.up_proj(x)) if act is None else act
 
@@ -334,6 +337,17 @@ class Model(nn.Module):
         w, s, b = self.head_slices()
         logits = ops.quantized_matmul(out, w, s, b, transpose=True, group_size=q["group_size"], bits=q["bits"])
         return all_gather_last(logits, getattr(self, "tp", None))
+
+    def to_int8(self):
+        """The layers' linears as nn.Int8Linear -- integers with a scale for each channel, and in the calls for each token -- made of what their weights stand for; embedding and
+        head stay as they are.  Takes the place of the weights (a call with a decode engine comes before it, or not at all: those read the quantised ones)."""
+        for ly in self.model.layers:
+            for part, names in ((ly.self_attn, ("q_proj", "k_proj", "v_proj", "o_proj")), (ly.mlp, ("gate_proj", "up_proj", "down_proj"))):
+                for name in names:
+                    lin = getattr(part, name)
+                    if type(lin) is nn.QuantizedLinear:
+                        setattr(part, name, nn.Int8Linear.from_quantized(lin))
+        return self
 
     def sanitize(self, weights: dict) -> dict:
         """language.py:212-219."""

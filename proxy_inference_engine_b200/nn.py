@@ -92,6 +92,53 @@ class QuantizedLinear(Module):
         return ql
 
 
+class Int8Linear(Module):
+    """A linear layer of 8-bit integers: ``weight`` int8 [output_dims, input_dims] and ``scales`` f32 [output_dims], a scale for each channel; its inputs become integers with
+    a scale for each token in the call (ops.int8_linear).  input_dims: a multiple of 16.  Made of a bfloat16 weight (from_linear) or of another layer (from_quantized)."""
+
+    def __init__(self, input_dims: int, output_dims: int, bias: bool = False, device="cuda"):
+        scale = math.sqrt(1.0 / input_dims)
+        w = (torch.rand((output_dims, input_dims), device=device) * 2 - 1) * scale
+        self.weight, self.scales = ops.int8_rows(w.to(torch.bfloat16))
+        if bias:
+            self.bias = torch.zeros((output_dims,), dtype=torch.bfloat16, device=device)
+
+    def __call__(self, x, norm=None, residual=None):
+        """norm: an RMSNorm in front; residual (as the output): added to it."""
+        bias = self.__dict__.get("bias")
+        y = ops.int8_linear(x, self.weight, self.scales, norm_weight=None if norm is None else norm.weight, eps=1e-5 if norm is None else norm.eps,
+                            residual=None if bias is not None else residual)
+        if bias is not None:
+            y = y + bias
+            if residual is not None:
+                y = residual + y
+        return y
+
+    @classmethod
+    def from_linear(cls, weight: torch.Tensor, bias=None):
+        lin = cls.__new__(cls)
+        lin.weight, lin.scales = ops.int8_rows(weight)
+        if bias is not None:
+            lin.bias = bias
+        return lin
+
+    @classmethod
+    def from_quantized(cls, lin: QuantizedLinear):
+        return cls.from_linear(ops.dequantize(lin.weight, lin.scales, lin.biases, lin.group_size, lin.bits), lin.__dict__.get("bias"))
+
+
+def int8_beside(x, linears, norm=None):
+    """Several Int8Linears of one x, which becomes integers once (behind the norm, where one is given): their outputs.  None where they are not all that."""
+    if any(type(lin) is not Int8Linear for lin in linears) or (norm is not None and type(norm) is not RMSNorm):
+        return None
+    codes, scales = ops.int8_rows(x, norm_weight=None if norm is None else norm.weight, eps=1e-5 if norm is None else norm.eps)
+    out = []
+    for lin in linears:
+        y = ops.int8_matmul(codes, scales, lin.weight, lin.scales)
+        out.append(y + lin.bias if "bias" in lin.__dict__ else y)
+    return out
+
+
 class QuantizedEmbedding(Module):
     """nn.QuantizedEmbedding(num_embeddings, dims, group_size, bits) (quantized.py:60-132)."""
 

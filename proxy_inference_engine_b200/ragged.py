@@ -17,7 +17,8 @@ it yet (its scheduler is a skeleton); here ``ragged_step`` runs it:
 Same arithmetic as the per-sequence path (Model.__call__ over a PagedKVCache); tests/test_gpu_ragged.py compares the two.
 
 ``StepPlan`` is the descriptor built on the device from lengths that live there: rows, slots and block table in one launch, one attention launch a layer that
-reads a request's keys once for all its new tokens, and drafted tokens among them (``speculative_step``).
+reads a request's keys once for all its new tokens, and drafted tokens among them (``speculative_step``).  Its cache may be of 8 bits (``fp8_pools``), and the model's
+linears of 8-bit integers (``llama.Model.to_int8``).
 """
 from __future__ import annotations
 
@@ -28,7 +29,7 @@ from dataclasses import dataclass, field
 
 import torch
 
-from . import _lib, ops
+from . import _lib, nn, ops
 from .ops import _p, _stream
 
 PAGE_TOKENS = 64
@@ -246,24 +247,49 @@ def _planned_step(model, plan: StepPlan, pools, all_logits: bool) -> torch.Tenso
     d = plan.dims   # (all of it before the first layer writes to its pools: slots of another plan's pools are other requests' places)
     for kp, vp in pools:
         if isinstance(kp, (tuple, list)):
-            raise ValueError("[ragged_step] a StepPlan's attention reads bfloat16 pools; 8-bit pools are for BatchDetails")
+            if len(kp) != 2 or not isinstance(vp, (tuple, list)) or len(vp) != 2:
+                raise ValueError("[ragged_step] a StepPlan's attention reads bfloat16 pools, or fp8_pools; other 8-bit pools are for BatchDetails")
+            if (d.Hq, d.Hkv) != (Hq, Hkv):
+                raise ValueError(f"[ragged_step] the plan is for {d.Hq} heads on {d.Hkv}, but the model has {Hq} on {Hkv}")
+            ops._fp8_pools("ragged_step", *kp, *vp, d, D)
+            continue
         ops._slot_pools("ragged_step", kp, vp)
         if (d.Hq, d.Hkv, d.pages) != (Hq, Hkv, kp.shape[0]) or kp.shape[2:] != (Hkv, D):
             raise ValueError(f"[ragged_step] the plan is for {d.Hq} heads over {d.pages} pages of {d.Hkv} heads, but the model has {Hq} over {Hkv} of {D} features and a pool is "
                              f"{tuple(kp.shape)}")
     h = model.model.embed_tokens(plan.token_ids[None])
     for ly, (kp, vp) in zip(model.layers, pools):
-        at = ly.self_attn
-        x = ly.input_layernorm(h)
-        q = ops.rope_kv_slots(at.q_proj(x).view(T, Hq, D), at.k_proj(x).view(T, Hkv, D), at.v_proj(x).view(T, Hkv, D), at.rope._freqs, plan.positions, plan.slots, kp, vp)
-        o = ops.chunk_attention(q, kp, vp, plan, at.scale)
-        h = ops.add(h, at.o_proj(o[None]))
-        h = ops.add(h, ly.mlp(ly.post_attention_layernorm(h)))
+        at, mlp = ly.self_attn, ly.mlp
+        qkv = nn.int8_beside(h, (at.q_proj, at.k_proj, at.v_proj), norm=ly.input_layernorm)
+        if qkv is None:
+            x = ly.input_layernorm(h)
+            qkv = at.q_proj(x), at.k_proj(x), at.v_proj(x)
+        q, k, v = qkv[0].view(T, Hq, D), qkv[1].view(T, Hkv, D), qkv[2].view(T, Hkv, D)
+        if isinstance(kp, (tuple, list)):
+            q = ops.rope_kv_fp8(q, k, v, at.rope._freqs, plan, *kp, *vp)
+            o = ops.chunk_attention_fp8(q, *kp, *vp, plan, at.scale)
+        else:
+            q = ops.rope_kv_slots(q, k, v, at.rope._freqs, plan.positions, plan.slots, kp, vp)
+            o = ops.chunk_attention(q, kp, vp, plan, at.scale)
+        h = at.o_proj(o[None], residual=h) if type(at.o_proj) is nn.Int8Linear else ops.add(h, at.o_proj(o[None]))
+        both = nn.int8_beside(h, (mlp.gate_proj, mlp.up_proj), norm=ly.post_attention_layernorm) if type(getattr(mlp, "down_proj", None)) is nn.Int8Linear else None
+        if both is not None:
+            h = mlp.down_proj(ops.silu_mul(*both), residual=h)
+        else:
+            h = ops.add(h, mlp(ly.post_attention_layernorm(h)))
     if not all_logits:
         h = h.index_select(1, plan.logit_rows)
     w, s, b = model.head_slices()
     qz = a.quantization
     return ops.quantized_matmul(model.model.norm(h), w, s, b, transpose=True, group_size=qz["group_size"], bits=qz["bits"])[0]
+
+
+def fp8_pools(model, num_pages: int, device="cuda") -> list:
+    """Pools of a cache of 8 bits for the steps of a StepPlan, per layer ((k_codes, k_scales), (v_codes, v_scales)): float8_e4m3fn [num_pages, n_kv, 64, D] and a float32 scale for each
+    page and head (ops.rope_kv_fp8).  Half the bytes of bfloat16 pools, and a two-thousandth."""
+    pair = lambda at: (torch.zeros((num_pages, at.n_kv_heads, PAGE_TOKENS, at.head_dim), dtype=torch.float8_e4m3fn, device=device),
+                       torch.zeros((num_pages, at.n_kv_heads), dtype=torch.float32, device=device))
+    return [(pair(ly.self_attn), pair(ly.self_attn)) for ly in model.layers]
 
 
 def speculative_step(model, plan: StepPlan, pools, *, max_draft: int, temp: float = 0.0, uniforms=None, noise=None, draft_logits=None):
@@ -279,7 +305,7 @@ def ragged_step(model, batch: BatchDetails, pools, all_logits: bool = False) -> 
     the pools the block table's page ids index -- or, for the 8-bit KV cache of cache.PagedQuantizedKVCache, per layer
     ((k_quants, k_scales, k_biases), (v_quants, v_scales, v_biases)) [n_pages, n_kv, 64, .].
     Returns logits [num_sequences, vocab] of each sequence's last token (all_logits: [total_tokens, vocab]).
-    ``batch`` may be a StepPlan (bfloat16 pools): logits [num_logits, vocab] of its logit rows."""
+    ``batch`` may be a StepPlan (bfloat16 pools, or fp8_pools): logits [num_logits, vocab] of its logit rows."""
     if isinstance(batch, StepPlan):
         return _planned_step(model, batch, pools, all_logits)
     batch.validate()
