@@ -60,12 +60,13 @@ template <int D, bool F8 = false>
 struct ChunkTile {
   static constexpr int CH = D / 64, TILE = 128 * D * 2;          // 64-feature chunks of a row, bytes of 128 rows
   static constexpr int RING = D == 64 ? 4 : 2;                   // tiles of K, and of V: 64 KB of each
-  static constexpr int FEW = F8 || D == 64 ? 64 : 48;            // rows of an item of the turned kind, at most: as shared memory has room for their weights
+  static constexpr int FEW = F8 ? 32 : D == 64 ? 64 : 48;        // rows of an item of the turned kind, at most: as shared memory has room for their weights (8-bit pages: as tensor memory has for four tiles' scores)
   static constexpr int PCHUNK = 2 * FEW * 128;                   // bytes of 64 keys of a group's P of the turned kind: eight rows' first halves, their second halves, ...
-  static constexpr int P = 2 * PCHUNK;
-  static constexpr int Q1 = F8 || TILE > 2 * P ? TILE : 2 * P;   // the second query tile; the turned kind's P (8-bit pages: its warps' results)
+  static constexpr int P = F8 ? 3 * FEW * 128 : 2 * PCHUNK;      // (8-bit pages: three numbers a weight, a byte each)
+  static constexpr int Q1 = TILE > 2 * P ? TILE : 2 * P;         // the second query tile; the turned kind's P
   static constexpr int PLACES = 2 * RING;                        // 8-bit pages, turned kind: a key tile's codes of K and of V take one tile's place
-  static constexpr int SMEM = 1024 + TILE + Q1 + 2 * RING * TILE;
+  static constexpr int QF = 2 * FEW * D;                         // and the queries of a piece, as two codes a feature; two pieces' are held
+  static constexpr int SMEM = 1024 + TILE + Q1 + 2 * RING * TILE + (F8 ? 2 * QF : 0);
   static constexpr int THREADS = 384;
 };
 constexpr int kChunkScales = 8;               // 8-bit pages: key tiles whose scales are held
@@ -218,9 +219,6 @@ __device__ __forceinline__ void chunk_merge(uint16_t* out, const float* part, in
 
 struct ChunkMaps8 { CUtensorMap k, v; };   // of the codes, a page of a head
 struct ChunkNone {};
-// what the turned kind over 8-bit pages keeps of its rows: a warp's maxima and sums
-struct ChunkFew8 { float2 ml[8][16]; };
-struct ChunkFew8Bars { uint64_t *f_full, *f_empty, *sc_full, *sc_empty; const float4* sc; };
 // two codes as fp16, exactly; numbers to codes
 __device__ __forceinline__ uint32_t chunk_f16(uint32_t two) {
   uint32_t d;
@@ -236,356 +234,46 @@ __device__ __forceinline__ uint32_t chunk_codes4(float a, float b, float c, floa
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
   return lo | ((uint32_t)hi << 16);
 }
-__device__ __forceinline__ void chunk_mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// D[128 x N] (+)= A B of 8-bit numbers, both from shared memory
+__device__ __forceinline__ void chunk_mma_f8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accum) : "memory");
 }
-__device__ __forceinline__ void chunk_mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void chunk_ld8(uint32_t taddr, float* v) {   // not waited for
+  uint32_t* const u = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+               : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void chunk_st8(uint32_t taddr, const float* v) {
+  const uint32_t* const u = reinterpret_cast<const uint32_t*>(v);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(taddr)
+               : "memory");
 }
 __device__ __forceinline__ uint32_t chunk_pack_f16(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-__device__ __forceinline__ uint32_t chunk_turn8x8(uint32_t x) {   // an 8 x 8 matrix of 16-bit numbers, two of a row a lane, turned around
-  uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
-  return d;
+// Two fp16 as three pairs of e5m2 numbers, each in a half's upper byte, whose sums they are: of eleven bits the first takes three, and what it leaves, which has a sign, each of the others
+// four.  (Below 2^-5 the lowest bits lie below e5m2's lowest, 2^-16.)  e5m2 is fp16 without its lowest eight bits, so that a rounding is an addition; no half is near the largest.
+__device__ __forceinline__ void chunk_thirds(uint32_t x, uint32_t (&to)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    to[i] = (x + 0x00800080u) & 0xff00ff00u;
+    if (i < 2) asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(x) : "r"(x), "r"(to[i]));
+  }
+}
+// whether a round is over; all of a warp's lanes are told the same
+__device__ __forceinline__ bool chunk_ready(const uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, ok);
 }
 // where 16 bytes of a row of a page lie in its place in shared memory
 template <int D>
 __device__ __forceinline__ uint32_t chunk_code_at(int row, int c16) {
   return D == 128 ? row * 128 + ((c16 ^ (row & 7)) << 4) : row * 64 + ((c16 ^ ((row >> 1) & 3)) << 4);
-}
-
-// A piece of few rows over 8-bit pages, by the eight softmax warps, whose A operand is made of the codes in registers: what bounds it is the stream of pages, and a detour of widened codes
-// through shared memory (store, fence, barrier, tcgen05) took 2.9 us a key tile where the stream takes 0.75.
-// S^T = K Q^T of 16 keys at a time: codes are an e4m3 MMA's operand as they lie.  A query, brought to 2^7 .. 2^8 by a power of two for each row, is the sum of two e4m3 numbers -- its first
-// four and its last four bits, nothing else is lost but what is 2^-17 of the row's largest -- and the products of both are added up.  (That MMA has four times fp16's rate: 1.1 cycles of an SM
-// for 16 x 8 x 32, fp16's 2.0 for 16 x 8 x 16.)  O^T = V^T P^T in fp16, the codes widened (exactly), weights rounded to 2^-12 of one; sums are fp32.
-// A lane (g, t = lane / 4, lane % 4) has rows g and g + 8 of A and the columns 2 t, 2 t + 1 of the results.  Which features make up a step and which rows are V's features is free, so that a
-// lane's codes are whole pieces: of K the features D / 4 t .. of its two keys; of V the features D / 8 g .. of its four keys, two to a tile, neighbouring keys' codes put together by a byte
-// permutation.  A page's scale of K is applied to the scores; that of V to the weights, relative to the largest so far, which the results are in units of, or where it is below
-// 2^-16 of that, whose weights fp16 might not hold, to the page's product.
-// A group of four warps takes every other tile, 16 rows a warp: up to 16 rows of an item are four slices of 32 keys, 32 two sets of two slices, 64 four sets of one.  U times 16 keys are
-// worked on side by side.  Every warp has its own running maximum; the warps' results meet at the end in shared memory, eight rows of each set at a time.
-template <int D, int NT, int U>
-__device__ __forceinline__ bool chunk_few8(const ChunkArgs& a, const ChunkPiece& p, ChunkFew8& few, uint32_t smP, uint32_t smO, const ChunkFew8Bars& bars, volatile int* abortp, int cf,
-                                           bool alive, int rows, bool whole, float* rec) {
-  using T = ChunkTile<D, true>;
-  constexpr int KC = D / 64, VW = D / 32;          // 16-byte pieces of K of a key, 32-bit words of V of a key, a lane
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int group = warp >> 2, quad = warp & 3, sets_log = rows <= 16 ? 0 : rows <= 32 ? 1 : 2, slices = 4 >> sets_log, slice = quad & (slices - 1), set = quad >> (2 - sets_log);
-  const int row_first = 16 * set, keys = 32 << sets_log, key0 = slice * keys;
-  const int parts = 2 * slices, part = set * parts + group * slices + slice;   // a set's, of the groups and slices; this warp's among all
-  // queries: the rows 8 n + g, as two codes a feature
-  uint32_t qh[NT][D / 16], ql[NT][D / 16];
-  float scale[NT][2];                               // of the columns' rows
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int row = row_first + 8 * n + g, tok = row / a.G;
-    uint4 x[D / 32];
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      x[i] = make_uint4(0, 0, 0, 0);
-      if (row < rows)
-        x[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (p.row0 + tok) * a.q_row + (p.head * a.G + row - tok * a.G) * a.q_head + t * (D / 4)) + i);
-    }
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      constexpr uint32_t ABS = 0x7fff7fffu;
-      m = __vmaxu2(__vmaxu2(__vmaxu2(m, x[i].x & ABS), __vmaxu2(x[i].y & ABS, x[i].z & ABS)), x[i].w & ABS);
-    }
-    m = max(m & 0xffffu, m >> 16);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    // (rows of less than 2^-95, whose scores are 0, as they are; an infinity or a NaN makes the row's scores NaN)
-    const int e = m < 0x1000u ? 127 + 7 : min((int)(m >> 7), 254);
-    const float up = __uint_as_float((uint32_t)(127 + 7 + 127 - e) << 23), down = m >= 0x7f80u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(e - 7) << 23);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float v0 = bf16lo(w[2 * h]) * up, v1 = bf16hi(w[2 * h]) * up, v2 = bf16lo(w[2 * h + 1]) * up, v3 = bf16hi(w[2 * h + 1]) * up;
-        const uint32_t c = chunk_codes4(v0, v1, v2, v3);
-        float c0, c1, c2, c3;
-        chunk_f32(chunk_f16(c), c0, c1);
-        chunk_f32(chunk_f16(c >> 16), c2, c3);
-        qh[n][2 * i + h] = c;
-        ql[n][2 * i + h] = chunk_codes4(v0 - c0, v1 - c1, v2 - c2, v3 - c3);
-      }
-    }
-    scale[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
-    scale[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
-  }
-  float o[NT][D / 16][4], m[NT][2], l[NT][2], unit = 0.f;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.f;
-  }
-  // (by the tile's number among all, so that a place, and its rounds, are always the same group's)
-  for (int j = (group - cf) & 1; j < p.n; j += 2) {
-    const int tile = cf + j, place = tile % T::PLACES, is = tile % kChunkScales;
-    alive = alive && gemm_wait_warp(smem_u32(&bars.sc_full[is]), (tile / kChunkScales) & 1, abortp);
-    const float4 of = bars.sc[is];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars.sc_empty[is]);
-    alive = alive && gemm_wait_warp(smem_u32(&bars.f_full[place]), (tile / T::PLACES) & 1, abortp);
-    if (!alive) break;   // (and on through the barriers)
-#pragma unroll 1
-    for (int key = key0; key < key0 + keys; key += 16 * U) {
-      const int page = key >> 6, k_row = key & 63;
-      const float to_log2 = page ? of.y : of.x, value = page ? of.w : of.z;
-      const uint32_t sk = smP + place * T::TILE + page * (64 * D), sv = sk + 2 * (64 * D);
-      const int beyond = (p.k0 + j) * 128 + key - p.pos0;   // the first key, from the first row's own on
-      float ratio = 1.f;
-      if (value != unit) {
-        if (value > unit) {
-          const float f = unit / value;
-          unit = value;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[n][i][e] *= f;
-        }
-        ratio = value / unit;
-      }
-      const bool near = ratio >= 0x1p-16f;
-      const float weight = near ? 16.f * ratio : 16.f;   // (results are 16 times what they are: the weights' lowest are 2^-29 of one)
-      float s[U][NT][4];
-      float s2[U][NT][4];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = s2[u][n][0] = s2[u][n][1] = s2[u][n][2] = s2[u][n][3] = 0.f;
-#pragma unroll
-      for (int h = 0; h < KC; ++h) {
-        uint4 x[U], y[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          x[u] = lds128(sk + chunk_code_at<D>(k_row + 16 * u + g, KC * t + h));
-          y[u] = lds128(sk + chunk_code_at<D>(k_row + 16 * u + g + 8, KC * t + h));
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            chunk_mma_e4m3(s[u][n], x[u].x, y[u].x, x[u].y, y[u].y, qh[n][4 * h], qh[n][4 * h + 1]);
-            chunk_mma_e4m3(s2[u][n], x[u].x, y[u].x, x[u].y, y[u].y, ql[n][4 * h], ql[n][4 * h + 1]);
-          }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            chunk_mma_e4m3(s[u][n], x[u].z, y[u].z, x[u].w, y[u].w, qh[n][4 * h + 2], qh[n][4 * h + 3]);
-            chunk_mma_e4m3(s2[u][n], x[u].z, y[u].z, x[u].w, y[u].w, ql[n][4 * h + 2], ql[n][4 * h + 3]);
-          }
-      }
-      // scores in log2 units
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float f = to_log2 * scale[n][e & 1];
-#pragma unroll
-          for (int u = 0; u < U; ++u) s[u][n][e] = (s[u][n][e] + s2[u][n][e]) * f;
-        }
-      if (beyond + 16 * U - 1 > 0) {   // keys beyond a row's own
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int of_lane = beyond + 16 * u + g;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int own = (row_first + 8 * n + 2 * t + e) / a.G;
-              if (of_lane > own) s[u][n][e] = -INFINITY;
-              if (of_lane + 8 > own) s[u][n][2 + e] = -INFINITY;
-            }
-        }
-      }
-      float top[NT][2];
-      bool over = false;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          top[n][e] = fmaxf(s[0][n][e], s[0][n][2 + e]);
-#pragma unroll
-          for (int u = 1; u < U; ++u) top[n][e] = fmaxf(top[n][e], fmaxf(s[u][n][e], s[u][n][2 + e]));
-          over = over || top[n][e] > m[n][e] + 8.f;
-        }
-      // the reference of a row moves where a score exceeds it by 8
-      if (__any_sync(0xffffffffu, over)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = top[n][e];
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            if (x > m[n][e] + 8.f) {
-              const float f = m[n][e] == -INFINITY ? 0.f : fap_exp2(m[n][e] - x);
-              m[n][e] = x;
-              l[n][e] *= f;
-#pragma unroll
-              for (int i = 0; i < D / 16; ++i) { o[n][i][e] *= f; o[n][i][2 + e] *= f; }
-            }
-          }
-      }
-      uint32_t b[U][NT][2];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-          const float e0 = fap_exp2(s[u][n][0] - m0), e1 = fap_exp2(s[u][n][1] - m1), e2 = fap_exp2(s[u][n][2] - m0), e3 = fap_exp2(s[u][n][3] - m1);
-          l[n][0] += e0 + e2;
-          l[n][1] += e1 + e3;
-          b[u][n][0] = chunk_turn8x8(chunk_pack_f16(e0 * weight, e1 * weight));
-          b[u][n][1] = chunk_turn8x8(chunk_pack_f16(e2 * weight, e3 * weight));
-        }
-      uint32_t w[U][4][VW];   // values of the keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = k_row + 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
-          if (D == 128) {
-            const uint4 x = lds128(sv + chunk_code_at<D>(r, g));
-            w[u][i][0] = x.x; w[u][i][1] = x.y; w[u][i][VW - 2] = x.z; w[u][i][VW - 1] = x.w;
-          } else {
-            const uint2 x = lds64(sv + chunk_code_at<D>(r, g >> 1) + 8 * (g & 1));
-            w[u][i][0] = x.x; w[u][i][1] = x.y;
-          }
-        }
-      if (beyond + 16 * U > p.tokens) {   // behind the item's last key there may be anything: 0 * NaN is not 0
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (beyond + 16 * u + 2 * t + (i & 1) + 8 * (i >> 1) >= p.tokens)
-#pragma unroll
-              for (int h = 0; h < VW; ++h) w[u][i][h] = 0;
-      }
-      auto values = [&](int u, int i, uint32_t (&v)[4]) {
-        const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
-        const uint32_t lo = __byte_perm(w[u][0][i >> 1], w[u][1][i >> 1], sel), hi = __byte_perm(w[u][2][i >> 1], w[u][3][i >> 1], sel);
-        v[0] = chunk_f16(lo); v[1] = chunk_f16(lo >> 16); v[2] = chunk_f16(hi); v[3] = chunk_f16(hi >> 16);
-      };
-      if (near) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t v[4];
-            values(u, i, v);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) chunk_mma_f16(o[n][i], v[0], v[1], v[2], v[3], b[u][n][0], b[u][n][1]);
-          }
-      } else {
-#pragma unroll 1
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t v[4];
-            values(0, i, v);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
-              chunk_mma_f16(d, v[0], v[1], v[2], v[3], b[0][n][0], b[0][n][1]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[n][i][e] = fmaf(d[e], ratio, o[n][i][e]);
-            }
-            if (i == D / 16 - 1 && U > 1) {   // (the other keys in the same registers)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int h = 0; h < VW; ++h) w[0][k][h] = w[U - 1][k][h];
-#pragma unroll
-              for (int n = 0; n < NT; ++n) { b[0][n][0] = b[U - 1][n][0]; b[0][n][1] = b[U - 1][n][1]; }
-            }
-          }
-      }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars.f_empty[place]);
-  }
-  // sums over the lanes of a column, then the slices' maxima and sums
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float x = l[n][e];
-      x += __shfl_xor_sync(0xffffffffu, x, 4);
-      x += __shfl_xor_sync(0xffffffffu, x, 8);
-      x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (g == 0) few.ml[part][8 * n + 2 * t + e] = make_float2(m[n][e], x);
-    }
-  chunk_sync();
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int col = 8 * n + 2 * t + e, row = row_first + col;
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll 1
-      for (int w = 0; w < parts; ++w) top = fmaxf(top, few.ml[set * parts + w][col].x);
-#pragma unroll 1
-      for (int w = 0; w < parts; ++w) {
-        const float2 x = few.ml[set * parts + w][col];
-        sum += x.x == -INFINITY ? 0.f : x.y * fap_exp2(x.x - top);
-      }
-      float f = m[n][e] == -INFINITY ? 0.f : fap_exp2(m[n][e] - top) * (unit * 0.0625f);
-      if (whole) f /= sum;
-      else if (part == set * parts && g == 0 && row < rows) __stcg(reinterpret_cast<float2*>(rec + 256 * D + 2 * row), make_float2(top, sum));
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) { o[n][i][e] *= f; o[n][i][2 + e] *= f; }
-    }
-  // eight rows of each set at a time: [warp][row][D] fp32, the 16-byte pieces of a row in another order for every other row
-  constexpr int LANES = D / 4;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    if (n > 0) chunk_sync();
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const uint32_t to = smO + (part * 8 + 2 * t + e) * D * 4;
-#pragma unroll
-      for (int i = 0; i < D / 16; i += 2)   // features D / 8 g + 2 i ..
-        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((g * (D / 32) + (i >> 1)) ^ t) << 4)), "f"(o[n][i][e]), "f"(o[n][i][2 + e]), "f"(o[n][i + 1][e]),
-                     "f"(o[n][i + 1][2 + e]) : "memory");
-    }
-    chunk_sync();
-#pragma unroll 1
-    for (int x = tid; x < (8 << sets_log) * LANES; x += 256) {
-      const int c4 = x % LANES, r8 = x / LANES % 8, of_set = x / (8 * LANES), row = 16 * of_set + 8 * n + r8;
-      if (row >= rows) continue;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int w = 0; w < parts; ++w) {
-        const uint4 u = lds128(smO + ((of_set * parts + w) * 8 + r8) * D * 4 + ((c4 ^ (r8 >> 1)) << 4));
-        sum.x += __uint_as_float(u.x); sum.y += __uint_as_float(u.y); sum.z += __uint_as_float(u.z); sum.w += __uint_as_float(u.w);
-      }
-      const int tok = row / a.G;
-      if (whole)
-        *reinterpret_cast<uint2*>(a.out + ((size_t)(p.row0 + tok) * a.Hq + p.head * a.G + row - tok * a.G) * D + 4 * c4) = make_uint2(pack_bf16(sum.x, sum.y), pack_bf16(sum.z, sum.w));
-      else
-        __stcg(reinterpret_cast<float4*>(rec + row * D + 4 * c4), sum);
-    }
-  }
-  fence_proxy_async();   // (what lies there is read: a query tile may be copied there)
-  chunk_sync();
-  return alive;
 }
 
 template <int D, bool F8>
@@ -602,10 +290,12 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full[2], q_empty[2], k_full[RING], k_empty[RING], v_full[RING], v_empty[RING], s_full[2], p_full[2], o_full[2];
   __shared__ __align__(16) int4 list[3 * kChunkList];
-  // 8-bit pages: places of the turned kind's tiles, scales of its tiles, and whether a piece's results have left the place of the second query tile (in turn)
-  __shared__ __align__(8) uint64_t f_full[F8 ? T::PLACES : 1], f_empty[F8 ? T::PLACES : 1], sc_full[F8 ? kChunkScales : 1], sc_empty[F8 ? kChunkScales : 1], turn_free[2];
-  __shared__ __align__(16) float4 sc[F8 ? kChunkScales : 1];   // of the two pages: scores to log2 units, the values' scale
-  __shared__ __align__(16) typename std::conditional<F8, ChunkFew8, ChunkFew>::type few;
+  // 8-bit pages, turned kind: places of its key tiles, their scales, the queries of a piece (two in turn), its last product (in turn), behind which P's place is free, four tiles' scores, and weights and
+  // products of either group, whose tiles are every other one
+  __shared__ __align__(8) uint64_t f_full[F8 ? T::PLACES : 1], f_empty[F8 ? T::PLACES : 1], sc_full[F8 ? kChunkScales : 1], sc_empty[F8 ? kChunkScales : 1], qf_full[2], qf_empty[2], turn_free[2], fs_full[4], fp_full[2], fo_full[2];
+  __shared__ __align__(16) float4 sc[F8 ? kChunkScales : 1][2];   // of either page of a tile: scores to log2 units, log2 of the values' scale, its reciprocal
+  __shared__ __align__(16) float q_scale[2][F8 ? T::FEW : 4];
+  __shared__ __align__(16) ChunkFew few;
   __shared__ float2 ml[2][128];           // a row's maximum and sum: of the two groups of a tile, of the rows of a cut item
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag, last_flag;
@@ -613,7 +303,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   // (The turned kind's P lies where Q1 does.  Its V^T has 128 rows whatever the head size: at 64 the upper ones are what lies 16 KB behind, so V does not lie last.)
-  const uint32_t smV = base, smK = smV + RING * T::TILE, smQ = smK + RING * T::TILE, smQ1 = smQ + T::TILE;
+  const uint32_t smV = base, smK = smV + RING * T::TILE, smQ = smK + RING * T::TILE, smQ1 = smQ + T::TILE, smF = smQ1 + T::Q1;
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -625,9 +315,10 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
     }
     if (F8) {
-      for (int i = 0; i < T::PLACES; ++i) { mbar_init(&f_full[i], 1); mbar_init(&f_empty[i], 4); }
+      for (int i = 0; i < T::PLACES; ++i) { mbar_init(&f_full[i], 1); mbar_init(&f_empty[i], 1); }
       for (int i = 0; i < kChunkScales; ++i) { mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 4); }
-      for (int i = 0; i < 2; ++i) mbar_init(&turn_free[i], 1);
+      for (int i = 0; i < 2; ++i) { mbar_init(&qf_full[i], 1); mbar_init(&qf_empty[i], 9); mbar_init(&turn_free[i], 1); mbar_init(&fp_full[i], 4); mbar_init(&fo_full[i], 1); }
+      for (int i = 0; i < 4; ++i) mbar_init(&fs_full[i], 1);
     }
     abort_flag = 0;
     fence_mbar_init();
@@ -684,18 +375,205 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     while (chunk_piece(a, list, begin, at, end, p)) {
       const int keys = p.pos0 + p.tokens, tail = keys & 127, tail_step = tail ? (keys - 1) / 128 - p.k0 : -1, cnt = p.cnt(g);
       if (F8 && p.kind == CHUNK_FEW) {
-        // ---------------------------------------------------------------------------------- 8-bit pages, few rows: every warp its keys
+        // ---------------------------------------------------------------------------------- 8-bit pages: a key a lane, a row a column
+        // As below, with other operands, and bound by the stream of pages, half as long.  The codes of K and V are the MMAs' as they lie, and all else is made to suit them: a query, brought to
+        // 2^7 .. 2^8 by a power of two for each row, is the sum of two e4m3 numbers (its first four and its last four bits; what is 2^-17 of the row's largest is lost), a weight, as fp16, of
+        // three e5m2 numbers, each with columns of its own, that are added up as fp32.  The MMA with its 128 keys or features by 16 to 96 columns is a hundred cycles or two; what it costs
+        // to widen the codes instead was 2.9 us a key tile by way of shared memory and 2.2 in registers (mma.sync, 24 rows), where the stream takes 0.75.
+        // A row's reference is that of its weights times their pages' scale of V, so that its results are in the units of the largest of those, whatever scales the pages have; its sum is rid of
+        // the scale again.  The CTA's key tiles of this kind go to the groups in turn, and four tiles' scores are under way at a time, of the next piece too, so that a group never waits for
+        // the products of its last tile (40 answers with up to five drafts over 6000 keys: two tiles' scores, rows in fours 184 us; four tiles', rows in eights without a branch 143).
         if constexpr (F8) {
-          const int rows = p.tokens * a.G;
+          const int rows = p.tokens * a.G, which = few_pieces & 1, half = quad >> 1, own = (g ^ cf) & 1;   // the group's first tile
+          const int cnt_own = (p.n + 1 - own) / 2, cnt_other = p.n - cnt_own;
+          const int beyond = p.k0 * 128 + r - p.pos0, edge_step = (p.pos0 + 1) / 128 - p.k0;   // the first key tile with a key that some row must not see
+          const uint32_t sp = smQ1 + g * T::P + (r & 15);
+          const int chunk16 = r >> 4;
+          alive = alive && gemm_wait_warp(smem_u32(&qf_full[which]), (few_pieces >> 1) & 1, abortp);   // (for the queries' scales)
+          auto weights = [&](auto blocks) {
+            constexpr int N = 8 * decltype(blocks)::value;
+            float l[32];
+#pragma unroll
+            for (int n = 0; n < 32; ++n) l[n] = 0.f;
+            for (int i = 0; i < cnt_own; ++i) {
+              const int step = 2 * i + own, tile = cf + step, is = tile % kChunkScales;
+              alive = alive && gemm_wait_warp(smem_u32(&sc_full[is]), (tile / kChunkScales) & 1, abortp);
+              const float4 of = sc[is][half];
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sc_empty[is]);
+              alive = alive && gemm_wait_warp(smem_u32(&fs_full[tile & 3]), (tile >> 2) & 1, abortp);
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              float v[2 * N], s[N];
+#pragma unroll
+              for (int b = 0; b < N / 8; ++b) chunk_ld16(tS + 32 * (tile & 2) + 16 * b, v + 16 * b);
+              tmem_ld_wait();
+#pragma unroll
+              for (int n = 0; n < N; n += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(&q_scale[which][n]);
+                const float f[4] = {q.x * of.x, q.y * of.x, q.z * of.x, q.w * of.x};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[n + k] = fmaf(v[2 * n - n % 8 + k] + v[2 * n - n % 8 + 8 + k], f[k], of.y);
+              }
+              if (step >= edge_step) {
+                const int cut = (beyond + step * 128) * a.G;
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                  if (n < cut) s[n] = -INFINITY;
+              }
+              bool over = i == 0;
+              if (i > 0) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < N; n += 4) {
+                  const float4 less = *reinterpret_cast<const float4*>(&few.less[g][n]);
+                  s[n] += less.x; s[n + 1] += less.y; s[n + 2] += less.z; s[n + 3] += less.w;
+                  mx = fmaxf(fmaxf(mx, fmaxf(s[n], s[n + 1])), fmaxf(s[n + 2], s[n + 3]));
+                }
+                over = mx > 15.f;
+                // behind the product before this one P's place is free, and O holds the tiles so far
+                alive = alive && gemm_wait_warp(smem_u32(&fo_full[g]), ((tile >> 1) - 1) & 1, abortp);
+              }
+              // the reference of a row moves where a weight exceeds it 16 times
+              if (chunk_group_any(g, over)) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                int mine = 0;
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                  if (i > 0) s[n] -= few.less[g][n];
+                  const int x = __reduce_max_sync(0xffffffffu, chunk_order(s[n]));
+                  if (lane == n) mine = x;
+                }
+                few.best[g][quad][lane] = mine;
+                chunk_group_sync(g);
+                if (quad == 0 && lane < N) {
+                  const float was = i == 0 ? -INFINITY : few.m[g][lane];
+                  const float now = chunk_unorder(max(max(few.best[g][0][lane], few.best[g][1][lane]), max(few.best[g][2][lane], few.best[g][3][lane])));
+                  const bool move = i == 0 || now > was + 4.f;
+                  const float m = move ? now : was;
+                  few.factor[g][lane] = !move ? 1.f : was == -INFINITY ? 0.f : fap_exp2(was - m);
+                  few.m[g][lane] = m;
+                  few.less[g][lane] = m == -INFINITY ? 0.f : 11.f - m;   // weights of up to 2^15
+                }
+                chunk_group_sync(g);
+#pragma unroll
+                for (int n = 0; n < N; ++n) s[n] += few.less[g][n];
+                if (i > 0) {
+#pragma unroll
+                  for (int b = 0; b < N / 8; ++b) {
+                    float f[8];
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                      f[n] = few.factor[g][8 * b + n];
+                      l[8 * b + n] *= f[n];
+                    }
+#pragma unroll 1
+                    for (int k = 0; k < 3; ++k) {
+                      float o[8];
+                      chunk_ld8(tO + g * OST + 24 * b + 8 * k, o);
+                      tmem_ld_wait();
+#pragma unroll
+                      for (int n = 0; n < 8; ++n) o[n] *= f[n];
+                      chunk_st8(tO + g * OST + 24 * b + 8 * k, o);
+                    }
+                  }
+                  tmem_st_wait();
+                }
+              }
+#pragma unroll
+              for (int n = 0; n < N; n += 2) {
+                const float e0 = fap_exp2(s[n]), e1 = fap_exp2(s[n + 1]);
+                l[n] = fmaf(e0, of.z, l[n]);
+                l[n + 1] = fmaf(e1, of.z, l[n + 1]);
+                uint32_t c3[3];
+                chunk_thirds(chunk_pack_f16(e0, e1), c3);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  const uint32_t to = sp + ((chunk16 ^ (n % 8 + j)) << 4);
+#pragma unroll
+                  for (int q = 0; q < 3; ++q)
+                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(to + (24 * (n / 8) + n % 8 + j + 8 * q) * 128), "r"(c3[q] >> (j ? 24 : 8)) : "memory");
+                }
+              }
+              if (step == tail_step) {   // values behind the item's last key
+                alive = alive && gemm_wait_warp(smem_u32(&f_full[tile % T::PLACES]), (tile / T::PLACES) & 1, abortp);
+                if (alive && r >= tail)
+#pragma unroll
+                  for (int q = 0; q < D / 16; ++q)
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(smV + tile % T::PLACES * T::TILE + (128 + r) * D + 16 * q), "r"(0) : "memory");
+              }
+              fence_proxy_async();
+              asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&fp_full[g]);
+            }
+            // a row's sum over the warp's lanes: half of the columns a step, until a lane has one
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+              for (int k = 0; k < o; ++k) {
+                const float give = lane & o ? l[k] : l[k + o], keep = lane & o ? l[k + o] : l[k];
+                l[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+              }
+            few.sum[g][quad][lane] = l[0];
+          };
+          switch ((rows - 1) / 8) {   // (rows behind the last are worked on with those beside them: their scores are 0)
+            case 0: weights(std::integral_constant<int, 1>()); break;
+            case 1: weights(std::integral_constant<int, 2>()); break;
+            case 2: weights(std::integral_constant<int, 3>()); break;
+            default: weights(std::integral_constant<int, 4>());
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&qf_empty[which]);
+          const int cnt0 = g ? cnt_other : cnt_own, cnt1 = g ? cnt_own : cnt_other;
+          read_again();
           const bool whole = p.pieces == 1;
           float* const rec = a.part + (size_t)(2 * blockIdx.x + ((int)blockIdx.x == p.first)) * kChunkRecord<D>;
-          const ChunkFew8Bars bars = {f_full, f_empty, sc_full, sc_empty, sc};
-          if (rows > 8) alive = chunk_few8<D, 2, 2>(a, p, few, smV, smQ1, bars, abortp, cf, alive, rows, whole, rec);
-          else alive = chunk_few8<D, 1, 2>(a, p, few, smV, smQ1, bars, abortp, cf, alive, rows, whole, rec);
-          cf += p.n;
-          read_again();
-          if (tid == 0) mbar_arrive(&turn_free[few_pieces & 1]);   // (behind a barrier of the eight warps)
-          ++few_pieces;
+          if (cnt_own > 0) alive = alive && gemm_wait_warp(smem_u32(&fo_full[g]), ((cf + 2 * cnt_own - 2 + own) >> 1) & 1, abortp);
+          cf += p.n; ++few_pieces;
+          chunk_sync();     // (the other group has waited for its own)
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (tid < rows) {
+            const float m0 = cnt0 > 0 ? few.m[0][tid] : -INFINITY, m1 = cnt1 > 0 ? few.m[1][tid] : -INFINITY, m = fmaxf(m0, m1);
+            const float f0 = m0 == -INFINITY ? 0.f : fap_exp2(m0 - m), f1 = m1 == -INFINITY ? 0.f : fap_exp2(m1 - m);
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              if (cnt0 > 0) sum = fmaf(few.sum[0][w][tid], f0, sum);
+              if (cnt1 > 0) sum = fmaf(few.sum[1][w][tid], f1, sum);
+            }
+            const float inv = whole ? 1.f / sum : 1.f;   // (weights and sums are 2^11 times too large)
+            few.share[tid] = make_float2(f0 * inv, f1 * inv);
+            const int t = tid / a.G;
+            few.row[tid] = (p.row0 + t) * a.Hq + p.head * a.G + tid - t * a.G;
+            if (!whole) __stcg(reinterpret_cast<float2*>(rec + 256 * D + 2 * tid), make_float2(m, sum));
+          }
+          chunk_sync();
+          if (alive && (D == 128 || quad < 2)) {   // (head size 64: nothing in the upper lanes)
+#pragma unroll 1
+            for (int n0 = 8 * g; n0 < rows; n0 += 16) {
+              float v[8];
+#pragma unroll
+              for (int n = 0; n < 8; ++n) v[n] = 0.f;
+#pragma unroll 1
+              for (int h = cnt0 > 0 ? 0 : 1; h < (cnt1 > 0 ? 2 : 1); ++h) {
+                float o[24];
+#pragma unroll
+                for (int k = 0; k < 3; ++k) chunk_ld8(tO + h * OST + 3 * n0 + 8 * k, o + 8 * k);
+                tmem_ld_wait();
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                  const float2 f = few.share[n0 + n];
+                  v[n] = fmaf(o[n] + o[8 + n] + o[16 + n], h ? f.y : f.x, v[n]);
+                }
+              }
+#pragma unroll
+              for (int n = 0; n < 8; ++n)
+                if (n0 + n < rows) {
+                  if (whole) a.out[(size_t)few.row[n0 + n] * D + r] = f2bf(v[n]);
+                  else __stcg(rec + (n0 + n) * D + r, v[n]);
+                }
+            }
+          }
         }
       } else if (!F8 && p.kind == CHUNK_FEW) {
         if constexpr (!F8) {
@@ -1055,7 +933,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         chunk_sync();
         if (last_flag) chunk_merge<D>(a.out, a.part, p.first, p.pieces, p.tokens, p.row0, p.head, a.Hq, a.G, p.kind == CHUNK_FEW);
-      } else if (p.kind != CHUNK_PAIR && !(F8 && p.kind == CHUNK_FEW)) {
+      } else if (p.kind != CHUNK_PAIR) {
         chunk_sync();     // both groups have read both accumulators
       }
     }
@@ -1090,7 +968,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const int lead0 = z.y, lead1 = z.z;   // the pages of its first key tile
         ChunkPiece p;
         if (!chunk_read(a, e[0], e[1], z, p)) continue;
-        // 8-bit pages: pieces of the turned kind leave their results where Q1 is.  Those before the last two are known here to be done, so that the two barriers tell them apart.
+        // 8-bit pages: the last products of pieces of the turned kind before the last two are known here to be done, so that the two barriers tell the rounds apart.
         if (F8 && p.kind == CHUNK_FEW && few_pieces > 1 && !(alive = gemm_wait_warp(smem_u32(&turn_free[few_pieces & 1]), ((few_pieces >> 1) - 1) & 1, abortp))) break;
         const int32_t* const pages = a.table + (size_t)p.request * a.blocks;
         const int last_page = (p.pos0 + p.tokens - 1) / kStepPage;
@@ -1199,18 +1077,32 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         fap_commit(&o_full[g]);
       };
+      // 8-bit pages, turned kind: S^T = K Q^T, O^T += V^T P^T of the codes in a place; blocks: eights of rows
+      auto qk8 = [&](int tile, int which, int blocks) {
+        constexpr uint64_t UP = D == 128 ? UPPER : ((uint64_t)(512 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)4 << 61);   // (rows of 128 bytes, of 64)
+        uint32_t dk = ((smV + tile % T::PLACES * T::TILE) & 0x3FFFF) >> 4, dq = ((smF + which * T::QF) & 0x3FFFF) >> 4;
+        asm volatile("" : "+r"(dq), "+r"(dk));
+        const uint32_t id = (1u << 4) | ((uint32_t)(2 * blocks) << 17) | ((128u >> 4) << 24);
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) chunk_mma_f8(tm + COL_S + (tile & 1) * 128 + 32 * (tile & 2), UP | (dk + 2 * k), UP | (dq + 2 * k), id, k > 0 ? 1u : 0u);
+        fap_commit(&fs_full[tile & 3]);
+      };
+      auto pv8 = [&](int tile, bool first, int blocks) {
+        // V with its rows (keys) for K: eight of them D bytes each an atom; behind the first D features of 128 rows of A there are none at head size 64 (what lies 8 KB on)
+        constexpr uint64_t UP = ((uint64_t)(8 * D >> 4) << 32) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)1 << 46) | ((uint64_t)(D == 128 ? 2 : 4) << 61);
+        uint32_t dv = ((smV + tile % T::PLACES * T::TILE + 128 * D) & 0x3FFFF) >> 4, dp = dq1 + (tile & 1) * (T::P >> 4);
+        asm volatile("" : "+r"(dv), "+r"(dp));
+        const uint32_t id = (1u << 4) | (1u << 10) | (1u << 15) | ((uint32_t)((3 * blocks + 1) / 2 * 2) << 17) | ((128u >> 4) << 24);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) chunk_mma_f8(tm + COL_O + (tile & 1) * OST, UP | (dv + k * (32 * D >> 4)), UPPER | (dp + 2 * k), id, (!first || k > 0) ? 1u : 0u);
+        fap_commit(&fo_full[tile & 1]);
+        fap_commit(&f_empty[tile % T::PLACES]);
+      };
       auto wide_of = [&](const ChunkPiece& p) { return p.kind == CHUNK_FEW ? (uint32_t)((p.tokens * a.G + 15) / 16 * 2) << 17 : 0u; };
-      bool apart = false;                          // 8-bit pages: pieces of few rows lie in front of the next one
+      int cf = 0, few_pieces = 0, scored = 0;      // 8-bit pages: key tiles and pieces of the turned kind before this piece, which ck leaves out; tiles whose scores were asked for
       // the next piece; warp-uniform, and known to be
       auto fetch = [&](int& at, ChunkPiece& p) {
-        bool more = chunk_piece(a, list, begin, at, end, p);
-        if constexpr (F8) {   // (those are the softmax warps' own, and what comes behind one is not begun before it: its operands wait for it)
-          apart = false;
-          while (more && p.kind == CHUNK_FEW) {
-            apart = true;
-            more = chunk_piece(a, list, begin, at, end, p);
-          }
-        }
+        const bool more = chunk_piece(a, list, begin, at, end, p);
         at = __shfl_sync(0xffffffffu, at, 0);
         p.n = __shfl_sync(0xffffffffu, p.n, 0);
         p.kind = __shfl_sync(0xffffffffu, p.kind, 0);
@@ -1241,8 +1133,50 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       while (more) {
         p = next;
         more = fetch(at, next);
-        const int tn = ck + p.n;                   // the next piece's first key tile
         const bool pair = p.kind == CHUNK_PAIR;
+        if constexpr (F8) {
+          if (p.kind == CHUNK_FEW) {
+            // Scores as soon as their tile is there and one of the four places for them is free (which the weights of the tile four before say), products as soon as their weights are.
+            const int end_own = cf + p.n, end_all = more && next.kind == CHUNK_FEW ? end_own + next.n : end_own;
+            int tile = cf, idle = 0;
+            alive = __all_sync(0xffffffffu, alive);
+            while (alive && tile < end_own) {
+              bool moved = false;
+              if (scored < min(tile + 4, end_all)) {
+                const bool own = scored < end_own;
+                const int which = (few_pieces + !own) & 1, place = scored % T::PLACES;
+                if (chunk_ready(&qf_full[which], ((few_pieces + !own) >> 1) & 1) && chunk_ready(&f_full[place], (scored / T::PLACES) & 1)) {
+                  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                  if (elect_one()) {
+                    qk8(scored, which, ((own ? p.tokens : next.tokens) * a.G + 7) / 8);
+                    if (scored + 1 == (own ? end_own : end_all)) fap_commit(&qf_empty[which]);
+                  }
+                  ++scored;
+                  moved = true;
+                }
+              }
+              if (tile < scored && chunk_ready(&fp_full[tile & 1], (tile >> 1) & 1)) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elect_one()) {
+                  pv8(tile, tile < cf + 2, (p.tokens * a.G + 7) / 8);
+                  if (tile + 1 == end_own) fap_commit(&turn_free[few_pieces & 1]);
+                }
+                ++tile;
+                moved = true;
+              }
+              idle = moved ? 0 : idle + 1;
+              if (__any_sync(0xffffffffu, idle > (int)kGemmWaitLimit || *abortp)) {
+                *abortp = 1;
+                if (lane == 0) atomicExch(&g_gemm_error, 1u);
+                alive = false;
+              }
+            }
+            if (!alive) break;
+            cf = end_own; ++few_pieces;
+            continue;
+          }
+        }
+        const int tn = ck + p.n;                   // the next piece's first key tile
         const int nq0 = cq[0] + (pair ? p.cnt0 > 0 : 1), nq1 = cq[1] + (pair && p.cnt1 > 0);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
@@ -1250,9 +1184,9 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           ahead[g] = false;
         }
         // the next piece's scores, while this one's last tiles and its O are worked on
-        // (The second key tile's scores come behind the first's: the last ones give Q's place up.)
+        // (The second key tile's scores come behind the first's: the last ones give Q's place up.  8-bit pages: a piece of the turned kind uses the places that this one holds.)
         auto go_on = [&](int g) {
-          if (more && !apart && next.cnt(g) > 0 && (next.kind == CHUNK_PAIR || g == 0 || ahead[0])) {
+          if (more && !(F8 && next.kind == CHUNK_FEW) && next.cnt(g) > 0 && (next.kind == CHUNK_PAIR || g == 0 || ahead[0])) {
             open(next, g, tn, nq0, nq1);
             ahead[g] = true;
           }
@@ -1338,13 +1272,71 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           }
           const int i = cf % kChunkScales, at0 = 2 * (p.k0 + j) - first;
           if (!(alive = gemm_wait_warp(smem_u32(&sc_empty[i]), ((cf / kChunkScales) & 1) ^ 1, abortp))) break;
-          const float4 of = make_float4(__shfl_sync(0xffffffffu, to_log2, at0), __shfl_sync(0xffffffffu, to_log2, at0 + 1), __shfl_sync(0xffffffffu, value, at0),
-                                        __shfl_sync(0xffffffffu, value, at0 + 1));
+          if (lane == at0 || lane == at0 + 1) sc[i][lane - at0] = make_float4(to_log2, log2f(value), 1.f / value, 0.f);
+          __syncwarp();
           if (lane == 0) {
-            sc[i] = of;
             mbar_arrive(&sc_full[i]);
           }
         }
+      }
+    }
+    // ------------------------------------------------------------------------------------------------ queries of few rows as codes
+    if (F8 && warp == 11) {
+      bool alive = true;
+      int at = begin, n = 0;
+      ChunkPiece p;
+      while (alive && chunk_piece(a, list, begin, at, end, p)) {
+        if (p.kind != CHUNK_FEW) continue;
+        const int rows = p.tokens * a.G, which = n & 1;
+        const uint32_t smq = smF + which * T::QF;
+        bool waited = n < 2;   // (rows come from memory meanwhile)
+        // D / 16 lanes a row, 16 features each
+        for (int x = lane; x < (rows + 7) / 8 * 8 * (D / 16); x += 32) {
+          const int row = x / (D / 16), c16 = x % (D / 16), tok = row / a.G;
+          uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+          if (row < rows) {
+            const uint4* const from = reinterpret_cast<const uint4*>(a.q + (p.row0 + tok) * a.q_row + (p.head * a.G + row - tok * a.G) * a.q_head) + 2 * c16;
+            v[0] = __ldg(from);
+            v[1] = __ldg(from + 1);
+          }
+          uint32_t m = 0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            constexpr uint32_t ABS = 0x7fff7fffu;
+            m = __vmaxu2(__vmaxu2(__vmaxu2(m, v[i].x & ABS), __vmaxu2(v[i].y & ABS, v[i].z & ABS)), v[i].w & ABS);
+          }
+          m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+          for (int k = 1; k < D / 16; k <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));   // (whole warps come here: eight rows are 64 or 32 pieces)
+          if (!waited) {
+            waited = true;
+            if (!(alive = gemm_wait_warp(smem_u32(&qf_empty[which]), ((n >> 1) - 1) & 1, abortp))) break;
+          }
+          // The largest becomes 2^7 and a little (rows of less than 2^-95, whose scores are 0, as they are; an infinity or a NaN makes the row's scores NaN).
+          const int e = m < 0x1000u ? 127 + 7 : min((int)(m >> 7), 254);
+          const float up = __uint_as_float((uint32_t)(127 + 7 + 127 - e) << 23);
+          if (c16 == 0) q_scale[which][row] = m >= 0x7f80u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(e - 7) << 23);
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4& u = v[i >> 1];
+            const uint32_t w0 = i & 1 ? u.z : u.x, w1 = i & 1 ? u.w : u.y;
+            const float v0 = bf16lo(w0) * up, v1 = bf16hi(w0) * up, v2 = bf16lo(w1) * up, v3 = bf16hi(w1) * up;
+            float c0, c1, c2, c3;
+            hi[i] = chunk_codes4(v0, v1, v2, v3);
+            chunk_f32(chunk_f16(hi[i]), c0, c1);
+            chunk_f32(chunk_f16(hi[i] >> 16), c2, c3);
+            lo[i] = chunk_codes4(v0 - c0, v1 - c1, v2 - c2, v3 - c3);
+          }
+          const uint32_t to = smq + (row >> 3) * (16 * D) + chunk_code_at<D>(row & 7, c16);   // eight rows' first numbers, their second ones, ...
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + 8 * D), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+        }
+        if (!alive) break;
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&qf_full[which]);
+        ++n;
       }
     }
     // ------------------------------------------------------------------------------------------------ rows behind the last request's
@@ -1379,8 +1371,7 @@ static cudaError_t launch_chunk(const CUtensorMap (&m)[4], const Codes& codes, c
 }
 
 // 8-bit pages of the requests that have more rows than the turned kind takes, as bf16 where they will be read as those are: the tensor cores' operands of that kind come from shared memory
-// alone, and every query tile would turn the same codes around again.  (Done so, by four warps beside the softmax's: 2048 tokens behind 15000 1024 us, with products of the operands as they
-// lay 970.)  A block (page, head) a CTA at a time.
+// alone, and every query tile would turn the same codes around again.  (Four warps beside the softmax's that widened them tile by tile: 2048 tokens behind 15000 812 us and more; so 499; pages of 16 bits 478.)  A block (page, head) a CTA at a time.
 __global__ void __launch_bounds__(256) chunk_widen_kernel(const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs, uint16_t* k16, uint16_t* v16, const int32_t* row_starts,
                                                           const int32_t* contexts, const int32_t* table, int requests, int blocks, int Hkv, int D, int few_tokens) {
   __shared__ int list[256];   // requests of this round that have so many

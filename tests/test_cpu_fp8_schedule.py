@@ -32,20 +32,22 @@ class Bar:
 
 
 class Walk:
-    def __init__(self, pieces, D, seed, results_wait=True, keep_apart=True):
+    def __init__(self, pieces, D, seed, weights_wait=True):
         self.rng, self.pieces = random.Random(seed), pieces
         self.R, self.SC = constants(D)
-        self.PLACES, self.results_wait, self.keep_apart = 2 * self.R, results_wait, keep_apart
+        self.PLACES, self.weights_wait = 2 * self.R, weights_wait
         bars = lambda n, count: [Bar(count) for _ in range(n)]
         self.q_full, self.q_empty = bars(2, 1), bars(2, 1)
         self.k_full, self.k_empty, self.v_full, self.v_empty = (bars(self.R, 1) for _ in range(4))
         self.s_full, self.p_full, self.o_full = bars(2, 1), bars(2, 4), bars(2, 1)
-        self.f_full, self.f_empty = bars(self.PLACES, 1), bars(self.PLACES, 4)
+        self.f_full, self.f_empty = bars(self.PLACES, 1), bars(self.PLACES, 1)
         self.sc_full, self.sc_empty = bars(self.SC, 1), bars(self.SC, 4)
-        self.turn_free = bars(2, 1)
-        self.pipe, self.copies, self.at_sync = [], [], 0
+        self.fs_full, self.fp_full, self.fo_full = bars(4, 1), bars(2, 4), bars(2, 1)
+        self.turn_free, self.qf_full, self.qf_empty = bars(2, 1), bars(2, 1), bars(2, 9)
+        self.pipe, self.copies, self.at_sync, self.moves = [], [], 0, 0
         self.sync_round = 0
-        self.place_in, self.q_in = [None] * self.PLACES, [None, None]   # places: those of V, then those of K
+        self.place_in, self.q_in = [None] * self.PLACES, [None, None]   # places: those of V, then those of K; the two query tiles, the second of which is P's place too
+        self.qf_in, self.scale_in, self.scores_in = [None, None], [None] * self.SC, [None] * 4
 
     # ---- waits: a generator yields what it waits for
     def wait(self, bar, round_, own=True):
@@ -61,6 +63,12 @@ class Walk:
         else:
             assert bar.done == 0
             yield
+
+    @staticmethod
+    def ready(bar, round_):
+        done = (bar.done & 1) != (round_ & 1)
+        assert not done or bar.done == round_ + 1, f"round {round_} was asked for, {bar.done} are done"
+        return done
 
     def sync(self):
         round_ = self.sync_round
@@ -94,7 +102,7 @@ class Walk:
                     return
                 yield from self.wait_free(self.q_empty[g], cq[g])
                 cq[g] += 1
-                if g and few > 0 and self.results_wait:
+                if g and few > 0 and self.weights_wait:
                     yield from self.wait(self.turn_free[(few - 1) & 1], (few - 1) >> 1)
                 copy(self.q_full[g], self.q_in, g, n)
             yield from fetch_q(0)
@@ -120,17 +128,27 @@ class Walk:
 
     def scales(self):
         cf = 0
-        for kind, tiles, *_ in self.pieces:
+        for n, (kind, tiles, *_) in enumerate(self.pieces):
             for j in range(tiles if kind == FEW else 0):
                 i = cf % self.SC
                 yield from self.wait_free(self.sc_empty[i], cf // self.SC)
                 cf += 1
+                self.scale_in[i] = (n, j)
                 yield
                 self.sc_full[i].arrive()
 
+    def queries(self):
+        k = 0
+        for n, (kind, *_) in enumerate(self.pieces):
+            if kind == FEW:
+                yield from self.wait_free(self.qf_empty[k & 1], k >> 1)
+                self.qf_in[k & 1] = n
+                yield
+                self.qf_full[k & 1].arrive()
+                k += 1
+
     def mma(self):
-        todo = [(n, p) for n, p in enumerate(self.pieces) if p[0] != FEW]
-        c, cq, ck = [0, 0], [0, 0], 0
+        c, cq, ck, cf, few, scored = [0, 0], [0, 0], 0, 0, 0, 0
         ahead = [False, False]
 
         def commit(bar):
@@ -148,6 +166,21 @@ class Walk:
             self.pipe.append(run)
             commit(self.o_full[g])
 
+        def scores8(n, tile, which, step):
+            def run():
+                assert self.place_in[tile % self.PLACES] == (n, step) and self.qf_in[which] == n, "scores of other operands"
+                assert self.scores_in[tile & 3] is None, "scores written over"
+                self.scores_in[tile & 3] = (n, step)
+            self.pipe.append(run)
+            commit(self.fs_full[tile & 3])
+
+        def product8(n, tile, step):
+            def run():
+                assert self.place_in[tile % self.PLACES] == (n, step) and self.q_in[1][tile & 1] == (n, step), "a product of other operands"
+            self.pipe.append(run)
+            commit(self.fo_full[tile & 1])
+            commit(self.f_empty[tile % self.PLACES])
+
         def open_(n, p, g, t, q):
             kind, tiles, cnt = p[:3]
             pair = kind == PAIR
@@ -159,12 +192,33 @@ class Walk:
                 commit(self.k_empty[(t + step) % self.R])
             if (cnt[g] == 1) if pair else step == tiles - 1:
                 commit(self.q_empty[tile])
-        for at, (n, p) in enumerate(todo):
+        for n, p in enumerate(self.pieces):
             kind, tiles, cnt = p[:3]
-            more = at + 1 < len(todo)
-            nn, following = todo[at + 1] if more else (None, (None, 0, (0, 0)))
-            apart = more and nn != n + 1 and self.keep_apart
-            tn, pair = ck + tiles, kind == PAIR
+            more = n + 1 < len(self.pieces)
+            following = self.pieces[n + 1] if more else (None, 0, (0, 0))
+            pair = kind == PAIR
+            if kind == FEW:
+                end_own = cf + tiles
+                end_all = end_own + (following[1] if following[0] == FEW else 0)
+                tile = cf
+                while tile < end_own:
+                    if scored < min(tile + 4, end_all):
+                        own = scored < end_own
+                        f, place = few + (not own), scored % self.PLACES
+                        if self.ready(self.qf_full[f & 1], f >> 1) and self.ready(self.f_full[place], scored // self.PLACES):
+                            scores8(n if own else n + 1, scored, f & 1, scored - (cf if own else end_own))
+                            if scored + 1 == (end_own if own else end_all):
+                                commit(self.qf_empty[f & 1])
+                            scored += 1
+                    if tile < scored and self.ready(self.fp_full[tile & 1], tile >> 1):
+                        product8(n, tile, tile - cf)
+                        if tile + 1 == end_own:
+                            commit(self.turn_free[few & 1])
+                        tile += 1
+                    yield
+                cf, few = end_own, few + 1
+                continue
+            tn = ck + tiles
             nq = [cq[0] + (cnt[0] > 0 if pair else 1), cq[1] + (pair and cnt[1] > 0)]
             for g in range(2):
                 if cnt[g] > 0 and not ahead[g]:
@@ -172,8 +226,8 @@ class Walk:
                 ahead[g] = False
 
             def go_on(g):
-                if more and not apart and following[2][g] > 0 and (following[0] == PAIR or g == 0 or ahead[0]):
-                    yield from open_(nn, following, g, tn, nq)
+                if more and following[0] != FEW and following[2][g] > 0 and (following[0] == PAIR or g == 0 or ahead[0]):
+                    yield from open_(n + 1, following, g, tn, nq)
                     ahead[g] = True
             if pair:
                 commit(self.k_empty[ck % self.R])
@@ -214,31 +268,33 @@ class Walk:
             ck, cq = tn, nq
 
     def softmax(self, warp):
-        g = warp >> 2
+        g, quad = warp >> 2, warp & 3
         c, cf, few = [0, 0], 0, 0
         for n, (kind, tiles, cnt, cut) in enumerate(self.pieces):
             if kind == FEW:
-                for j in range(tiles):
-                    if (cf + j) % 2 != g:   # (the other group's)
-                        continue
-                    tile = cf + j
-                    place, i = tile % self.PLACES, tile % self.SC
-                    yield from self.wait(self.sc_full[i], tile // self.SC)
-                    self.sc_empty[i].arrive()
-                    yield from self.wait(self.f_full[place], tile // self.PLACES)
-                    assert self.place_in[place] == (n, j), "another tile"
+                yield from self.wait(self.qf_full[few & 1], few >> 1)
+                own = (g ^ cf) & 1
+                cnt = [(tiles + 1 - (h ^ cf & 1)) // 2 for h in range(2)]
+                for i in range(cnt[g]):
+                    step = 2 * i + own
+                    tile = cf + step
+                    yield from self.wait(self.sc_full[tile % self.SC], tile // self.SC)
+                    assert self.scale_in[tile % self.SC] == (n, step), "another tile's scales"
+                    self.sc_empty[tile % self.SC].arrive()
+                    yield from self.wait(self.fs_full[tile & 3], tile >> 2)
+                    assert self.scores_in[tile & 3] == (n, step) and self.qf_in[few & 1] == n
+                    if i > 0 and self.weights_wait:
+                        yield from self.wait(self.fo_full[g], (tile >> 1) - 1)
+                    self.q_in[1] = {**(self.q_in[1] if isinstance(self.q_in[1], dict) else {}), g: (n, step)}
+                    if step == tiles - 1:   # values behind the last key
+                        yield from self.wait(self.f_full[tile % self.PLACES], tile // self.PLACES)
+                        assert self.place_in[tile % self.PLACES] == (n, step)
                     yield
-                    assert self.place_in[place] == (n, j), "another tile"
-                    self.f_empty[place].arrive()
-                cf += tiles
-                yield from self.sync()
-                self.q_in[1] = ("results", n)
-                yield from self.sync()
-                assert self.q_in[1] == ("results", n), "results written over"
-                yield from self.sync()
-                if warp == 0:
-                    self.turn_free[few & 1].arrive()
-                few += 1
+                    if self.fp_full[g].left == 1:
+                        self.scores_in[tile & 3] = None
+                    self.fp_full[g].arrive()
+                self.qf_empty[few & 1].arrive()
+                few, cf = few + 1, cf + tiles
             else:
                 for i in range(cnt[g]):
                     yield from self.wait(self.s_full[g], c[g] + i)
@@ -246,6 +302,13 @@ class Walk:
                         yield from self.wait(self.o_full[g], c[g] + i - 1)
                     yield
                     self.p_full[g].arrive()
+            if kind == FEW:
+                if cnt[g]:
+                    yield from self.wait(self.fo_full[g], (cf - tiles + 2 * cnt[g] - 2 + own) >> 1)
+                yield from self.sync()
+                assert all(self.fo_full[last & 1].done == (last >> 1) + 1 for last in range(cf - min(tiles, 2), cf))
+                yield from self.sync()
+            else:
                 c = [c[0] + cnt[0], c[1] + cnt[1]]
                 for h in (g,) if kind == PAIR else (0, 1):
                     if cnt[h] > 0:   # (the other group's: its own warps see to it, and all meet behind that)
@@ -256,11 +319,11 @@ class Walk:
             if cut:
                 yield from self.sync()
                 yield from self.sync()
-            elif kind == ONE:
+            elif kind != PAIR:
                 yield from self.sync()
 
     def go(self):
-        roles = [self.tma(), self.scales(), self.mma()] + [self.softmax(w) for w in range(8)]
+        roles = [self.tma(), self.scales(), self.queries(), self.mma()] + [self.softmax(w) for w in range(8)]
         pace = [self.rng.choice([1, 1, 1, 8, 40]) for _ in roles]
         pipe_pace, copy_pace = self.rng.choice([1, 3, 20]), self.rng.choice([1, 3, 20])
         idle = 0
@@ -285,7 +348,7 @@ class Walk:
             assert idle < 400 * 40 * 20, "nothing moves"
 
     def mark(self):
-        return self.at_sync, self.sync_round, sum(b.done * 16 + b.left for bars in (self.p_full, self.f_empty, self.sc_full, self.sc_empty, self.turn_free) for b in bars)
+        return self.at_sync, self.sync_round, sum(b.done * 16 + b.left for bars in (self.p_full, self.fp_full, self.qf_full, self.qf_empty, self.sc_full, self.sc_empty) for b in bars)
 
 
 def pieces_of(rng, count, most=6):
@@ -305,13 +368,11 @@ def test_every_wait_ends_with_its_own_round(D, seed):
 
 
 def test_the_walk_finds_what_would_break():
-    """A query tile copied to where a piece's results still lie, and a piece begun while pieces of few rows lie in front of it."""
-    def broken(**kw):
-        for seed in range(30):
-            rng = random.Random(seed)
-            try:
-                Walk(pieces_of(rng, 12), 128, seed, **kw).go()
-            except (AssertionError, IndexError):
-                return True
-        return False
-    assert broken(results_wait=False) and broken(keep_apart=False)
+    """A query tile copied to where weights still lie, and weights written over that a product still reads."""
+    for seed in range(30):
+        rng = random.Random(seed)
+        try:
+            Walk(pieces_of(rng, 12), 128, seed, weights_wait=False).go()
+        except (AssertionError, IndexError, TypeError):
+            return
+    assert False

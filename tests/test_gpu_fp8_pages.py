@@ -1,7 +1,7 @@
 """A ragged step over a cache of 8 bits against plain arithmetic in 64 bits.
 
 Tolerances.  Codes: a feature's code is the nearest of e4m3, half a step off: 2^-4 of it, or 2^-10 of the scale; values (and keys at angle 0) are coded from the numbers as they are,
-so their codes and scales are equal.  Attention, as over 16-bit pages: the result's rounding 2^-8, the weights' 2^-8 (fp16's 2^-11 where a request has up to 64 rows), and 2^-12 of the weights
+so their codes and scales are equal.  Attention, as over 16-bit pages: the result's rounding 2^-8, the weights' 2^-8 (fp16's 2^-11 where a request has up to 32 rows), and 2^-12 of the weights
 for the scores' sums in fp32, the exponentials and the row's sum."""
 import random
 
@@ -208,7 +208,7 @@ def attention_holds(got, q, pools, new, cached, tables, scale, slack=2.0 ** -12)
     Hkv = pools[0].shape[1]
     k, v = (values(*p).transpose(1, 2) for p in (pools[:2], pools[2:]))
     want, weight = O.attention(q[:sum(new)], k, v, new, cached, tables, scale)
-    few = torch.tensor([n * (Hq // Hkv) <= 64 // (Hq // Hkv) * (Hq // Hkv) for n in new for _ in range(n)])[:, None, None]
+    few = torch.tensor([n * (Hq // Hkv) <= 32 for n in new for _ in range(n)])[:, None, None]
     off = (got[:sum(new)].view(want.shape).cpu().double() - want).abs()
     bound = 2.0 ** -8 * want.abs() + (torch.where(few, 2.0 ** -11, 2.0 ** -8).double() + slack) * weight + 1e-37
     assert bool((off <= bound).all()), float((off - bound).max())
