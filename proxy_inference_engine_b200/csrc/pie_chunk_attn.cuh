@@ -382,13 +382,19 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         // to widen the codes instead was 2.9 us a key tile by way of shared memory and 2.2 in registers (mma.sync, 24 rows), where the stream takes 0.75.
         // A row's reference is that of its weights times their pages' scale of V, so that its results are in the units of the largest of those, whatever scales the pages have; its sum is rid of
         // the scale again.  The CTA's key tiles of this kind go to the groups in turn, and four tiles' scores are under way at a time, of the next piece too, so that a group never waits for
-        // the products of its last tile (40 answers with up to five drafts over 6000 keys: two tiles' scores, rows in fours 184 us; four tiles', rows in eights without a branch 143).
+        // the products of its last tile (40 answers with up to five drafts over 6000 keys: two tiles' scores, rows in fours 184 us; four tiles', rows in eights
+        // without a branch 143; two numbers an instruction, and P in words, turned around among four lanes, in place of bytes 125).
         if constexpr (F8) {
           const int rows = p.tokens * a.G, which = few_pieces & 1, half = quad >> 1, own = (g ^ cf) & 1;   // the group's first tile
           const int cnt_own = (p.n + 1 - own) / 2, cnt_other = p.n - cnt_own;
           const int beyond = p.k0 * 128 + r - p.pos0, edge_step = (p.pos0 + 1) / 128 - p.k0;   // the first key tile with a key that some row must not see
-          const uint32_t sp = smQ1 + g * T::P + (r & 15);
-          const int chunk16 = r >> 4;
+          const uint32_t turn1 = lane & 1 ? 0x3715 : 0x6240, turn2 = lane & 2 ? 0x3276 : 0x5410;
+          uint32_t sp[2];   // this lane's four keys in P's rows lane % 4, and four on
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int row = 4 * k + (lane & 3);
+            sp[k] = smQ1 + g * T::P + row * 128 + (((r >> 4) ^ row) << 4) + (r & 12);
+          }
           alive = alive && gemm_wait_warp(smem_u32(&qf_full[which]), (few_pieces >> 1) & 1, abortp);   // (for the queries' scales)
           auto weights = [&](auto blocks) {
             constexpr int N = 8 * decltype(blocks)::value;
@@ -403,16 +409,17 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
               if (lane == 0) mbar_arrive(&sc_empty[is]);
               alive = alive && gemm_wait_warp(smem_u32(&fs_full[tile & 3]), (tile >> 2) & 1, abortp);
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              float v[2 * N], s[N];
+              float v[2 * N], s[N];   // (two at a time where that is one instruction)
 #pragma unroll
               for (int b = 0; b < N / 8; ++b) chunk_ld16(tS + 32 * (tile & 2) + 16 * b, v + 16 * b);
               tmem_ld_wait();
 #pragma unroll
               for (int n = 0; n < N; n += 4) {
                 const float4 q = *reinterpret_cast<const float4*>(&q_scale[which][n]);
-                const float f[4] = {q.x * of.x, q.y * of.x, q.z * of.x, q.w * of.x};
+                const float f[4] = {q.x, q.y, q.z, q.w}, *const hi = v + 2 * n - n % 8;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s[n + k] = fmaf(v[2 * n - n % 8 + k] + v[2 * n - n % 8 + 8 + k], f[k], of.y);
+                for (int k = 0; k < 4; k += 2)
+                  f2_unpack(f2_fma(f2_add(f2_pack(hi[k], hi[k + 1]), f2_pack(hi[8 + k], hi[9 + k])), f2_mul(f2_pack(f[k], f[k + 1]), f2_pack(of.x, of.x)), f2_pack(of.y, of.y)), s[n + k], s[n + k + 1]);
               }
               if (step >= edge_step) {
                 const int cut = (beyond + step * 128) * a.G;
@@ -426,14 +433,16 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll
                 for (int n = 0; n < N; n += 4) {
                   const float4 less = *reinterpret_cast<const float4*>(&few.less[g][n]);
-                  s[n] += less.x; s[n + 1] += less.y; s[n + 2] += less.z; s[n + 3] += less.w;
+                  f2_unpack(f2_add(f2_pack(s[n], s[n + 1]), f2_pack(less.x, less.y)), s[n], s[n + 1]);
+                  f2_unpack(f2_add(f2_pack(s[n + 2], s[n + 3]), f2_pack(less.z, less.w)), s[n + 2], s[n + 3]);
                   mx = fmaxf(fmaxf(mx, fmaxf(s[n], s[n + 1])), fmaxf(s[n + 2], s[n + 3]));
                 }
                 over = mx > 15.f;
                 // behind the product before this one P's place is free, and O holds the tiles so far
                 alive = alive && gemm_wait_warp(smem_u32(&fo_full[g]), ((tile >> 1) - 1) & 1, abortp);
               }
-              // the reference of a row moves where a weight exceeds it 16 times
+              // The reference of a row, four times the largest weight that it was made from, moves where a weight exceeds it 16 times.  (At once the largest: scores of 2.9 log2 units' deviation
+              // move some of 24 rows' in every fifth tile; so in one of twenty.)
               if (chunk_group_any(g, over)) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 int mine = 0;
@@ -449,7 +458,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                   const float was = i == 0 ? -INFINITY : few.m[g][lane];
                   const float now = chunk_unorder(max(max(few.best[g][0][lane], few.best[g][1][lane]), max(few.best[g][2][lane], few.best[g][3][lane])));
                   const bool move = i == 0 || now > was + 4.f;
-                  const float m = move ? now : was;
+                  const float m = move ? now + 2.f : was;
                   few.factor[g][lane] = !move ? 1.f : was == -INFINITY ? 0.f : fap_exp2(was - m);
                   few.m[g][lane] = m;
                   few.less[g][lane] = m == -INFINITY ? 0.f : 11.f - m;   // weights of up to 2^15
@@ -480,18 +489,22 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 }
               }
 #pragma unroll
-              for (int n = 0; n < N; n += 2) {
-                const float e0 = fap_exp2(s[n]), e1 = fap_exp2(s[n + 1]);
-                l[n] = fmaf(e0, of.z, l[n]);
-                l[n + 1] = fmaf(e1, of.z, l[n + 1]);
-                uint32_t c3[3];
-                chunk_thirds(chunk_pack_f16(e0, e1), c3);
+              for (int n = 0; n < N; n += 4) {
+                uint32_t c3[2][3];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                  const uint32_t to = sp + ((chunk16 ^ (n % 8 + j)) << 4);
+                for (int k = 0; k < 2; ++k) {
+                  float* const ln = l + n + 2 * k;
+                  const float e0 = fap_exp2(s[n + 2 * k]), e1 = fap_exp2(s[n + 2 * k + 1]);
+                  f2_unpack(f2_fma(f2_pack(e0, e1), f2_pack(of.z, of.z), f2_pack(ln[0], ln[1])), ln[0], ln[1]);
+                  chunk_thirds(chunk_pack_f16(e0, e1), c3[k]);
+                }
+                // four rows of a key turned into four keys of a row, among four lanes
 #pragma unroll
-                  for (int q = 0; q < 3; ++q)
-                    asm volatile("st.shared.u8 [%0], %1;" ::"r"(to + (24 * (n / 8) + n % 8 + j + 8 * q) * 128), "r"(c3[q] >> (j ? 24 : 8)) : "memory");
+                for (int q = 0; q < 3; ++q) {
+                  uint32_t x = __byte_perm(c3[0][q], c3[1][q], 0x7531);
+                  x = __byte_perm(x, __shfl_xor_sync(0xffffffffu, x, 1), turn1);
+                  x = __byte_perm(x, __shfl_xor_sync(0xffffffffu, x, 2), turn2);
+                  asm volatile("st.shared.u32 [%0], %1;" ::"r"(sp[n / 4 & 1] + (24 * (n / 8) + 8 * q) * 128), "r"(x) : "memory");
                 }
               }
               if (step == tail_step) {   // values behind the item's last key

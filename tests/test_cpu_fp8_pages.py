@@ -70,6 +70,6 @@ def test_room_for_pages_in_16_bits():
     """Where every request is of few rows, there is none; otherwise twice the pools."""
     L = _lib.load()
     of = lambda **kw: L.pie_chunk_attn_fp8_workspace_bytes(C.byref(_lib.StepDims(*{**DIMS, **kw}.values())), 128)
-    few = of(rows=16)
-    assert few == L.pie_chunk_attn_workspace_bytes(C.byref(_lib.StepDims(*DIMS.values())), 128) and of(rows=17) == few + 2 * 2 * 5 * 2 * 64 * 128
+    few = of(rows=8)
+    assert few == L.pie_chunk_attn_workspace_bytes(C.byref(_lib.StepDims(*DIMS.values())), 128) and of(rows=9) == few + 2 * 2 * 5 * 2 * 64 * 128
     assert of(requests=0) == 0 and L.pie_chunk_attn_fp8_workspace_bytes(C.byref(_lib.StepDims(*DIMS.values())), 96) == 0
