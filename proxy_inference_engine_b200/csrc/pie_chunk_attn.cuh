@@ -1276,6 +1276,7 @@ chunk_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           const size_t e = (size_t)__ldg(pages + min(first + lane, last_page)) * a.Hkv + p.head;
           to_log2 = __ldg(a.k_scales + e) * a.scale_log2e;
           value = __ldg(a.v_scales + e);
+          value = value < 0x1p-60f ? 0x1p-60f : value;   // (0, as pools begin, with codes of 0)
         };
         read();
         for (int j = 0; j < p.n; ++j, ++cf) {

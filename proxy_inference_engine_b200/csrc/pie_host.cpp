@@ -535,7 +535,7 @@ PyObject* rope_kv_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan's words, plan's dims, scale, out or None, workspace) -> [T, Hq D], or None.  workspace(key, bytes, device)
+// chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan's words, plan's dims, scale, out or None, workspace) -> [T, Hq D], or None.  workspace(key, bytes, device, zeroed)
 PyObject* chunk_attention_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 10 || !bound || !on_gpu(args[0]) || !PyFloat_CheckExact(args[7])) Py_RETURN_NONE;
@@ -553,7 +553,8 @@ PyObject* chunk_attention_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   THPObjectPtr dev(PyObject_GetAttr(args[0], s_device));
   if (!dev) return nullptr;
   at::Tensor ws, out;
-  if (const Answer a = buffer(Py_BuildValue("(snO)", "chunk8", (Py_ssize_t)need, dev.get()), args[9], ws)) {
+  const Py_ssize_t zeroed = (Py_ssize_t)lib.pie_chunk_attn_workspace_bytes(&d, (int)D);   // (the rest, twice the pools' bytes, need not be: each replay of a captured step would see to it)
+  if (const Answer a = buffer(Py_BuildValue("(snOn)", "chunk8", (Py_ssize_t)need, dev.get(), zeroed), args[9], ws)) {
     if (a == FAILED) return nullptr;
     Py_RETURN_NONE;
   }

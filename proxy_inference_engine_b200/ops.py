@@ -104,7 +104,8 @@ class _Workspaces:
     def __init__(self):
         self.mine = _Mine()
 
-    def get(self, key, nbytes, device):
+    def get(self, key, nbytes, device, zeroed=None):
+        """zeroed: bytes at the buffer's beginning that a launch may count on; all of them."""
         mine, index = self.mine, device.index
         stream = _raw_stream(index)
         bufs = mine.eager
@@ -119,7 +120,12 @@ class _Workspaces:
         buf = bufs.get(key)
         if buf is None or buf.numel() < nbytes:
             bufs.pop(key, None)
-            buf = bufs[key] = torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+            if zeroed is None:
+                buf = torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+            else:
+                buf = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+                buf[:zeroed].zero_()
+            bufs[key] = buf
             if len(bufs) > self.KEEP:
                 del bufs[next(iter(bufs))]   # the oldest; its memory is used again in its stream's order
         return buf
@@ -823,7 +829,7 @@ def chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan, scale: floa
         L = _lib.load()
         out, rest = _fresh(out, (T, Hq * D), q.device)
         held, rows = _head_rows(q)
-        ws = workspaces.get("chunk8", L.pie_chunk_attn_fp8_workspace_bytes(C.byref(d), D), q.device)
+        ws = workspaces.get("chunk8", L.pie_chunk_attn_fp8_workspace_bytes(C.byref(d), D), q.device, L.pie_chunk_attn_workspace_bytes(C.byref(d), D))
         _lib.check(L.pie_chunk_attn_fp8(_p(out), C.byref(rows), _p(k_pool), _p(k_scales), _p(v_pool), _p(v_scales), _p(plan.words), C.byref(d), D, float(scale), rest, _p(ws),
                                         ws.numel(), _stream()), what)
     return out

@@ -315,6 +315,21 @@ def test_pages_of_very_different_scales(new):
     assert bool(((got - mean).abs() <= 2.0 ** -8 * mean.abs() + (2.0 ** -8 + 2.0 ** -12) * values(pools[2], pools[3])[tables[0][one]].abs().mean(1)[None, :, None]).all())
 
 
+@pytest.mark.parametrize("new", [[1], [8], [30]])
+def test_pages_that_nothing_was_written_to(new):
+    """Codes of 0 and scale 0, as pools begin: keys and values of 0, alone and among others."""
+    from proxy_inference_engine_b200 import ops
+    cached, D, Hq, Hkv = [700], 128, 8, 2
+    plan, q, pools, tables = attention_case(new, cached, Hq, Hkv, D, seed=5)
+    for page in tables[0][2:5]:
+        for pool in pools:
+            raw(pool)[page] = 0
+    attention_holds(ops.chunk_attention_fp8(q, *pools, plan, D ** -0.5), q, pools, new, cached, tables, D ** -0.5)
+    for pool in pools:
+        raw(pool)[:] = 0
+    assert not ops.chunk_attention_fp8(q, *pools, plan, D ** -0.5).any()
+
+
 @pytest.mark.parametrize("std", [0.0, 30.0])
 def test_flat_and_steep_scores(std):
     from proxy_inference_engine_b200 import ops
