@@ -26,6 +26,8 @@
 // busy for 54 % of it, as in the prompt's kernel one tile's softmax is covered by the other's products in part); 16 answers with up to five drafted tokens over 4000 keys 51.6 (4.4 TB/s),
 // 40 over 12000 309 (6.4 TB/s), one with four over 9000 26.3; D 64, three portions of 700 tokens beside 29 answers over 1500 keys 83.9, 40 answers over 12000 220 (4.5 TB/s).  Short
 // steps pay 4 us from the launch to the first scores, some 3 at each turn from one piece to the next and 5 at the end: results, one counter, the last CTA's sums.
+// Pages of 8 bits (F8): the turned kind's operands are the codes as they lie (below); of requests of more rows the pages are brought to 16 bits by a launch in front (chunk_widen_kernel).
+// 40 answers with up to five drafts over 6000 keys 124 us (4.1 TB/s; 16-bit pages 214), without drafts 98 (5.2 TB/s), one with four over 9000 28; 2048 tokens behind 15000 507.
 #include <type_traits>
 
 #include "pie_step_plan.h"

@@ -344,6 +344,26 @@ def test_flat_and_steep_scores(std):
     attention_holds(ops.chunk_attention_fp8(big, *same, plan, 128 ** -0.5), big, same, new, cached, tables, 128 ** -0.5, slack=0.044)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_queries_of_all_sizes(D):
+    """Down to bfloat16's lowest, each row with a power of two of its own; what is not finite makes its own row NaN and no other."""
+    from proxy_inference_engine_b200 import ops
+    new, cached, Hq, Hkv = [7, 1, 40, 8], [700, 3000, 100, 0], 8, 2
+    plan, q, pools, tables = attention_case(new, cached, Hq, Hkv, D, seed=21)
+    powers = torch.randint(-135, 1, (sum(new), Hq, 1), generator=gen(2), device="cuda").double()
+    q = (q.double() * torch.exp2(powers)).to(BF)
+    want = ops.chunk_attention_fp8(q, *pools, plan, D ** -0.5)
+    attention_holds(want, q, pools, new, cached, tables, D ** -0.5)
+    bad = q.clone()
+    bad[2, 3, 5], bad[7, 0, D - 1], bad[50, 7, 0] = torch.nan, torch.inf, -torch.inf
+    got = ops.chunk_attention_fp8(bad, *pools, plan, D ** -0.5).view(-1, Hq, D)
+    for row, head in ((2, 3), (7, 0), (50, 7)):
+        assert bool(got[row, head].isnan().all())
+        got[row, head] = want.view(-1, Hq, D)[row, head]
+    assert torch.equal(got.view(want.shape), want)
+    ops.check_pipeline()
+
+
 def test_two_streams_and_captured_graphs_at_once():
     from proxy_inference_engine_b200 import ops
     cases = [attention_case([4, 1, 70], [6000, 3000, 100], 8, 2, 128, seed=s) for s in (1, 2)]
