@@ -300,12 +300,14 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 
   if (warp < 4) {
     // ---------------------------------------------------------------- a channel a thread
+    // A warp whose wait ran out has no sums to give, but walks on: its CTA's barriers count it, and each part of a tile is counted and each tile's sums are cleared all the same, so that
+    // the workspace is left at zero.
+    bool alive = true;
     int done = 0;
     for (int t = tile0, k0 = k_first, i = 0; done < total; ++t, k0 = 0, ++i) {
       const int n = min(a.nk - k0, total - done), b = i & 1;
       done += n;
-      if (!gemm_wait_warp(smem_u32(&tfull_bar[b]), (i >> 1) & 1, abortp)) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      alive = alive && gemm_wait_warp(smem_u32(&tfull_bar[b]), (i >> 1) & 1, abortp);
       const bool whole = n == a.nk;
       const int channel = t * 128 + tid;
       const bool there = channel < a.N;
@@ -316,18 +318,21 @@ int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         const uint16_t o = f2bf((float)sum * __ldg(a.sx + m) * tw);
         a.y[p] = a.residual ? f2bf(bf16lo(o) + bf16lo(a.residual[p])) : o;
       };
-      uint32_t v[16];
-      tmem_ld16(tmem + (uint32_t)(b * NB) + ((uint32_t)(warp * 32) << 16), v);
-      tmem_ld_wait();
+      if (alive) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        uint32_t v[16];
+        tmem_ld16(tmem + (uint32_t)(b * NB) + ((uint32_t)(warp * 32) << 16), v);
+        tmem_ld_wait();
 #pragma unroll
-      for (int q = 0; q < 16; ++q)
-        if (q < a.M && there) {
-          if (whole) put(q, (int)v[q]);
-          else atomicAdd(sums + q * 128, (int)v[q]);
-        }
+        for (int q = 0; q < 16; ++q)
+          if (q < a.M && there) {
+            if (whole) put(q, (int)v[q]);
+            else atomicAdd(sums + q * 128, (int)v[q]);
+          }
+      }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty_bar[b]);
+      if (alive && lane == 0) mbar_arrive(&tempty_bar[b]);
       if (!whole) {
         // the CTAs whose shares the tile lies in: that of its first step, to that of its last
         const long long s0 = (long long)t * a.nk, s1 = s0 + a.nk - 1;
