@@ -30,6 +30,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _lib, nn, ops
+from .llama import MLP
 from .ops import _p, _stream
 
 PAGE_TOKENS = 64
@@ -272,7 +273,9 @@ def _planned_step(model, plan: StepPlan, pools, all_logits: bool) -> torch.Tenso
             q = ops.rope_kv_slots(q, k, v, at.rope._freqs, plan.positions, plan.slots, kp, vp)
             o = ops.chunk_attention(q, kp, vp, plan, at.scale)
         h = at.o_proj(o[None], residual=h) if type(at.o_proj) is nn.Int8Linear else ops.add(h, at.o_proj(o[None]))
-        both = nn.int8_beside(h, (mlp.gate_proj, mlp.up_proj), norm=ly.post_attention_layernorm) if type(getattr(mlp, "down_proj", None)) is nn.Int8Linear else None
+        both = None
+        if type(mlp) is MLP and type(mlp.down_proj) is nn.Int8Linear:   # (a class made from it may put something else between the matrices)
+            both = nn.int8_beside(h, (mlp.gate_proj, mlp.up_proj), norm=ly.post_attention_layernorm)
         if both is not None:
             h = mlp.down_proj(ops.silu_mul(*both), residual=h)
         else:

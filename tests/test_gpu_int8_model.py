@@ -1,0 +1,47 @@
+"""A model whose linears are of 8-bit integers, beside what a plain call of its parts makes."""
+import pytest
+import torch
+
+import step_oracle as O
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def small(head_dim=64, **kw):
+    from parity_util import tiny_args
+    from proxy_inference_engine_b200.checkpoint import build_model, random_weights
+    args = tiny_args(bits=8, head_dim=head_dim, **kw)
+    return args, build_model(args, random_weights(args, seed=5, device="cuda", gen_device="cpu"))
+
+
+def step(args, model, ids, n_pages=4):
+    """A planned step of one prompt, over fresh pools."""
+    from proxy_inference_engine_b200.ragged import StepPlan, fp8_pools, ragged_step
+    need = O.need(len(ids), 0)
+    plan = StepPlan.build(ints(ids), ints([len(ids)]), ints([0]), ints(list(range(need))), num_pages=n_pages, max_blocks=need, num_heads=args.num_attention_heads,
+                          num_kv_heads=args.num_key_value_heads)
+    plan.check()
+    return ragged_step(model, plan, fp8_pools(model, n_pages), all_logits=True)
+
+
+def test_a_planned_step_calls_a_feed_forward_of_another_class():
+    """One that gives nothing: the same bits as a feed-forward whose last matrix is zeros, not those of silu(gate) * up."""
+    from proxy_inference_engine_b200.llama import MLP
+
+    class Nothing(MLP):
+        def __call__(self, x):
+            return torch.zeros_like(x)
+
+    args, model = small()
+    model.to_int8()
+    ids = [(37 * i + 5) % args.vocab_size for i in range(70)]
+    usual = step(args, model, ids)
+    for ly in model.layers:
+        ly.mlp.__class__ = Nothing
+    got = step(args, model, ids)
+    for ly in model.layers:
+        ly.mlp.__class__ = MLP
+        ly.mlp.down_proj.scales.zero_()
+    assert torch.equal(got, step(args, model, ids)) and not torch.equal(got, usual)
