@@ -104,7 +104,9 @@ class Int8Linear(Module):
             self.bias = torch.zeros((output_dims,), dtype=torch.bfloat16, device=device)
 
     def __call__(self, x, norm=None, residual=None):
-        """norm: an RMSNorm in front; residual (as the output): added to it."""
+        """norm: a layer's norm in front (an RMSNorm within the call, another one before it); residual (as the output): added to it."""
+        if norm is not None and type(norm) is not RMSNorm:
+            x, norm = norm(x), None
         bias = self.__dict__.get("bias")
         y = ops.int8_linear(x, self.weight, self.scales, norm_weight=None if norm is None else norm.weight, eps=1e-5 if norm is None else norm.eps,
                             residual=None if bias is not None else residual)

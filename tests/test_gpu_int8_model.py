@@ -45,3 +45,20 @@ def test_a_planned_step_calls_a_feed_forward_of_another_class():
         ly.mlp.__class__ = MLP
         ly.mlp.down_proj.scales.zero_()
     assert torch.equal(got, step(args, model, ids)) and not torch.equal(got, usual)
+
+
+def test_a_layer_calls_a_norm_of_another_class():
+    """One made from RMSNorm whose weights are offsets from one: what the norm gives, through the layer."""
+    from proxy_inference_engine_b200 import nn, ops
+
+    class Offset(nn.RMSNorm):
+        def __call__(self, x):
+            return ops.rms_norm(x, 1 + self.weight, self.eps)
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = (torch.randn(s, generator=g, device="cuda").to(BF) for s in ((3, 256), (40, 256)))
+    lin, norm, offset = nn.Int8Linear.from_linear(w), nn.RMSNorm(256, eps=1e-6), Offset(256, eps=1e-6)
+    norm.weight = (1 + 0.1 * torch.randn(256, generator=g, device="cuda")).to(BF)
+    offset.weight = norm.weight - 1
+    assert torch.equal(lin(x, norm=offset), lin(ops.rms_norm(x, 1 + offset.weight, 1e-6)))
+    assert torch.equal(lin(x, norm=norm), ops.int8_linear(x, lin.weight, lin.scales, norm_weight=norm.weight, eps=1e-6))
