@@ -130,7 +130,7 @@ int pie_qmm_rows(void* y, int y_ld, const void* x, const pie_qmv_seg* segs_host,
 /* ---- products in 8-bit integers with a scale for each token and each channel (no counterpart in the reference, whose integers are affine weights) -----------------
  * pie_int8_rows: x bf16 [rows, K], x_ld elements between rows (a multiple of 8; x 16-byte aligned) -> scales f32 [rows], s = max |x| / 127 (times the 32-bit 1 / 127), and codes int8 [rows, K],
  * x / s rounded to the nearest integer, of two the even one.  A row of zeros has scale 0; one with an infinity or a NaN has scale NaN and codes 0.  norm_weight (bf16 [K], or
- * NULL): the rows are pie_rms_norm's of x (the squares may be added up in another order).  Weights take the same form: a row a channel.
+ * NULL): the rows are pie_rms_norm's of x (the squares may be added up in another order, which the rows beside one do not change).  Weights take the same form: a row a channel.
  * pie_int8_matmul: y bf16 [M, N] = bf16((sum_k codes[m, k] w[n, k]) scales[m] w_scales[n]), the sum exact, each product of fp32 rounded; residual (bf16 [M, N] or NULL; may be
  * y): added to that, rounded again.  The same bits whatever M the row comes with.
  * K: a multiple of 16 below 131072 (of pie_int8_rows: any multiple of 16); all pointers 16-byte aligned.  Workspace: pie_int8_workspace_bytes() bytes (0: none), ZEROED ONCE

@@ -921,8 +921,8 @@ def _int8_features(what: str, x, norm_weight) -> int:
 
 def int8_rows(x, *, norm_weight=None, eps: float = 1e-5):
     """Rows of 8-bit integers with a scale each: of x bfloat16 [..., K] (K a multiple of 16) the codes int8 [..., K] and scales f32 [...], with s = max |x| / 127 (times the 32-bit 1 / 127) and codes
-    x / s rounded to the nearest, of two the even one, so that x is about codes * s.  With norm_weight (bfloat16 [K]) of rms_norm(x, norm_weight, eps).  A row of zeros has scale
-    0; a row with an infinity or a NaN has scale NaN, so that its products are NaN.  A weight [N, K] becomes integers with a scale for each output channel the same way."""
+    x / s rounded to the nearest, of two the even one, so that x is about codes * s.  With norm_weight (bfloat16 [K]) of rms_norm(x, norm_weight, eps), whose sum
+    of squares may be taken in another order.  A row of zeros has scale 0; a row with an infinity or a NaN has scale NaN, so that its products are NaN.  A row's result does not depend on the rows beside it.  A weight [N, K] becomes integers with a scale for each output channel the same way."""
     got = native_host().int8_rows(x, norm_weight, float(eps))
     if got is not None:
         return got
@@ -983,7 +983,7 @@ def int8_matmul(codes, scales, weight, weight_scales, *, residual=None):
 
 def int8_linear(x, weight, weight_scales, *, norm_weight=None, eps: float = 1e-5, residual=None):
     """A linear layer of 8-bit integers: int8_rows of x (bfloat16 [..., K], through the layer's norm with norm_weight), int8_matmul of those with weight int8 [N, K] and
-    weight_scales f32 [N], and the residual added.  Returns bfloat16 [..., N]."""
+    weight_scales f32 [N], and the residual added.  Returns bfloat16 [..., N]; a row's result does not depend on the rows beside it."""
     got = native_host().int8_linear(x, weight, weight_scales, norm_weight, float(eps), residual, workspaces.get)
     if got is not None:
         return got

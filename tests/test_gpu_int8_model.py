@@ -62,3 +62,15 @@ def test_a_layer_calls_a_norm_of_another_class():
     offset.weight = norm.weight - 1
     assert torch.equal(lin(x, norm=offset), lin(ops.rms_norm(x, 1 + offset.weight, 1e-6)))
     assert torch.equal(lin(x, norm=norm), ops.int8_linear(x, lin.weight, lin.scales, norm_weight=norm.weight, eps=1e-6))
+
+
+@pytest.mark.parametrize("features", [2048, 4096, 4112, 8192, 14336, 16400, 40000])
+def test_a_row_behind_a_norm_does_not_depend_on_the_rows_beside_it(features):
+    """Fewer rows than a GPU has SMs, and more."""
+    from proxy_inference_engine_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(features)
+    x, w = torch.randn((600, features), generator=g, device="cuda").to(BF), (1 + 0.1 * torch.randn(features, generator=g, device="cuda")).to(BF)
+    codes, scales = ops.int8_rows(x, norm_weight=w)
+    for lo in range(0, 600, 100):
+        part, of = ops.int8_rows(x[lo:lo + 100], norm_weight=w)
+        assert torch.equal(part, codes[lo:lo + 100]) and torch.equal(of, scales[lo:lo + 100])
