@@ -22,7 +22,7 @@ import os
 import torch
 import torch.distributed as dist
 
-from . import _lib, ops
+from . import _lib, nn, ops
 from ._lib import EPI_RESADD, EPI_SILUMUL, EPI_STORE, KvLayout, QmvSeg, StepIO, StepLayer, StepModel
 from .cache import KVCache, PagedKVCache, PagedQuantizedKVCache, QuantizedKVCache
 from .llama import Model
@@ -48,6 +48,10 @@ class DecodeEngine:
         plus `seed`; None or temp == 0 is greedy.  With temp > 0 every step ends in pie_sample instead of pie_argmax, inside
         the captured graph (the Philox draw counter lives in device memory), and token ids still never leave the GPU."""
         a = model.args
+        linears = [(ly.self_attn.q_proj, ly.self_attn.k_proj, ly.self_attn.v_proj, ly.self_attn.o_proj, ly.mlp.gate_proj, ly.mlp.up_proj, ly.mlp.down_proj)
+                   for ly in model.layers]
+        if any(isinstance(lin, nn.Int8Linear) for ly in linears for lin in ly):
+            raise ValueError("[DecodeEngine] layers of 8-bit integers (Model.to_int8) are not built here: its steps read quantised weights")
         sp = dict(sampling or {})
         self.sampling = None
         if sp.get("temp", 0.0) > 0:
@@ -186,12 +190,13 @@ class DecodeEngine:
         # per-layer segment tables (host structs must outlive the captured graph: keep references)
         self.seg_qkv, self.seg_o, self.seg_gu, self.seg_down = [], [], [], []
         nb = 0
-        for ly in model.layers:
-            at, mlp = ly.self_attn, ly.mlp
-            self.seg_qkv.append(_segs(at.q_proj, at.k_proj, at.v_proj))
-            self.seg_o.append(_segs(at.o_proj))
-            self.seg_gu.append(_segs(mlp.gate_proj, mlp.up_proj))
-            self.seg_down.append(_segs(mlp.down_proj))
+        # (and the arrays they point to: another may be put in a layer's place, and the steps go on with these)
+        self._weights_keep = [(lin.weight, lin.scales, lin.biases) for ly in linears for lin in ly]
+        for q, k, v, o, gate, up, down in linears:
+            self.seg_qkv.append(_segs(q, k, v))
+            self.seg_o.append(_segs(o))
+            self.seg_gu.append(_segs(gate, up))
+            self.seg_down.append(_segs(down))
         hw, hs, hb = model.head_slices()
         self._head_keep = (hw, hs, hb)
         self.seg_head = (QmvSeg * 1)()

@@ -340,7 +340,8 @@ class Model(nn.Module):
 
     def to_int8(self):
         """The layers' linears as nn.Int8Linear -- integers with a scale for each channel, and in the calls for each token -- made of what their weights stand for; embedding and
-        head stay as they are.  Takes the place of the weights (a call with a decode engine comes before it, or not at all: those read the quantised ones)."""
+        head stay as they are.  Takes the place of the quantised weights, which are rounded a second time (from 4 bits it doubles their bytes).  The layers' calls and planned steps take such
+        layers; a decode engine does not: one made before goes on with the quantised weights in its steps, and keeps them, and one made after is refused."""
         for ly in self.model.layers:
             for part, names in ((ly.self_attn, ("q_proj", "k_proj", "v_proj", "o_proj")), (ly.mlp, ("gate_proj", "up_proj", "down_proj"))):
                 for name in names:

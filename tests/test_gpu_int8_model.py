@@ -74,3 +74,31 @@ def test_a_row_behind_a_norm_does_not_depend_on_the_rows_beside_it(features):
     for lo in range(0, 600, 100):
         part, of = ops.int8_rows(x[lo:lo + 100], norm_weight=w)
         assert torch.equal(part, codes[lo:lo + 100]) and torch.equal(of, scales[lo:lo + 100])
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_a_decode_engine_keeps_the_weights_it_was_made_with(use_graph):
+    """Layers of integers take the place of quantised ones whose addresses an engine's tables hold."""
+    import gc
+    import weakref
+    from proxy_inference_engine_b200.checkpoint import build_model, random_weights
+    from proxy_inference_engine_b200.decode import DecodeEngine
+    from parity_util import tiny_args
+    args = tiny_args(bits=4)
+    model = build_model(args, random_weights(args, seed=3, device="cuda", gen_device="cpu"))
+    prompt = torch.tensor([[(11 * i + 2) % args.vocab_size for i in range(20)]], dtype=torch.int32, device="cuda")
+    engine = DecodeEngine(model, 1, 64, use_graph=use_graph)
+    engine.prefill(prompt)
+    engine.step(10)
+    want = engine.generated()
+    engine.prefill(prompt)
+    arrays = lambda lin: (lin.weight, lin.scales, lin.biases)
+    held = [weakref.ref(t) for ly in model.layers for part, names in ((ly.self_attn, "qkvo"), (ly.mlp, ("gate", "up", "down"))) for n in names for t in arrays(getattr(part, n + "_proj"))]
+    model.to_int8()
+    gc.collect()
+    assert all(t() is not None for t in held)
+    spoil = [torch.full((1 << 20,), -1, dtype=torch.int32, device="cuda") for _ in range(8)]   # (what was given back would be these)
+    engine.step(10)
+    assert torch.equal(engine.generated(), want) and spoil
+    with pytest.raises(ValueError, match="8-bit integers"):
+        DecodeEngine(model, 1, 64)
