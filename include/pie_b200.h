@@ -340,9 +340,11 @@ int pie_chunk_attn(void* out, const pie_head_rows* q, const void* kpool, const v
  * pie_rope_kv_fp8 is pie_rope_kv_slots into such pools (keys are not rounded between rotation and code).  A row at a page's first place begins the page anew; where a row needs a
  * larger scale than the page has, what the page holds in front of it is brought to that.  Rows of one request go to a page together: no two requests of a plan may write to the same page.
  * A block with an infinity or a NaN has scale NaN, and stays so until it begins anew.
- * pie_chunk_attn_fp8 is pie_chunk_attn over such pools (scales > 0).  Requests of up to 32 rows (new tokens x Hq / Hkv; the last ones of longer requests too) have weights of fp16, off by
- * 2^-12 of one and 2^-27 of the row's largest (times its page's scale of V), and scales of V up to 2^100 apart; the pages of the others are brought to bf16 in the workspace, and then it is what pie_chunk_attn makes of those.  Workspace:
- * pie_chunk_attn_fp8_workspace_bytes(): pie_chunk_attn's, ZEROED ONCE as there, and where a request may have more rows, behind it, twice the bytes of the two pools. */
+ * pie_chunk_attn_fp8 is pie_chunk_attn over such pools (scale 0, as a pool of zeros begins: a page of zeros).  Requests of up to 32 rows (new tokens x Hq / Hkv; the last ones of longer
+ * requests too) have weights of fp16, off by 2^-11 of one and by 2^-26 of the row's largest (times its page's scale of V), and scales of V up to 2^100 apart; of their queries what is 2^-17 of
+ * the row's largest is lost.  The pages of the others are brought to bf16 in the workspace, and then it is what pie_chunk_attn makes of those.
+ * Workspace: pie_chunk_attn_fp8_workspace_bytes(): pie_chunk_attn's, ZEROED ONCE as there, and behind it, where the whole step may have more than 32 rows, however few each of its requests
+ * has, twice the bytes of the two pools. */
 size_t pie_chunk_attn_fp8_workspace_bytes(const pie_step_dims* dims, int D);
 int pie_rope_kv_fp8(void* q_out, uint8_t* kpool, float* k_scales, uint8_t* vpool, float* v_scales, const pie_head_rows* q, const pie_head_rows* k, const pie_head_rows* v,
                     const int32_t* plan, const pie_step_dims* dims, const float* freqs, int D, int rest, void* stream);

@@ -809,9 +809,10 @@ def rope_kv_fp8(queries, keys, values, freqs, plan, k_pool, k_scales, v_pool, v_
 
 def chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan, scale: float, out=None):
     """chunk_attention over a cache of 8 bits (rope_kv_fp8): row t of q [T, Hq, D] attends to the keys 0 .. position of its own request, a key and a value being their codes times their
-    pages' scales.  Returns [T, Hq * D].  Softmax weights are rounded for their product with the values: to fp16, off by 2^-12 of one and 2^-27 of the row's largest, where a request's
-    rows, its new tokens x Hq / Hkv, are at most 32 (and for the last ones of longer requests), otherwise to bfloat16; the pages of those are first brought to bfloat16 in a workspace of twice the pools' bytes, which all layers
-    share.  A page of scale NaN may make all of its request's new tokens NaN.  Rows that belong to nobody are zero, or with ``out`` given what that held."""
+    pages' scales.  Returns [T, Hq * D].  Softmax weights are rounded for their product with the values: to fp16, off by 2^-11 of one and by 2^-26 of the row's largest, where a request's
+    rows, its new tokens x Hq / Hkv, are at most 32 (and for the last ones of longer requests; of the queries what is 2^-17 of the row's largest is lost there), otherwise to bfloat16; the
+    pages of those are first brought to bfloat16 in a workspace of twice the pools' bytes, which all layers share.  (It is held, a thread, stream and captured graph, for every plan of more
+    than 32 such rows in all, since lengths are known on the device alone.)  A page of scale NaN may make all of its request's new tokens NaN.  Rows that belong to nobody are zero, or with ``out`` given what that held."""
     got = native_host().chunk_attention_fp8(q, k_pool, k_scales, v_pool, v_scales, plan.words, plan.dims, float(scale), out, workspaces.get)
     if got is not None:
         return got
