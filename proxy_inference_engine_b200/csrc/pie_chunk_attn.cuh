@@ -22,12 +22,14 @@
 // workspace, and the last CTA of the item to arrive adds all pieces up in their order: the same bits whichever that is.
 // Keys that a row must not see get weight 0; values behind the item's last key are cleared in shared memory, since 0 * NaN is not 0.
 // Every wait is bounded (pie_gemm.cuh); a warp whose wait ran out does nothing more, but walks on through the barriers of the softmax warps.
-// Device time in a row of such calls, inputs not in L2, 32 query / 8 kv heads: D 128, 2048 tokens behind 15000 460 us (1170 TFLOP/s, of cuBLAS's 1638 in a burst; the tensor pipe is
+// Device time in a row of such calls, inputs not in L2, 32 query / 8 kv heads: D 128, 2048 tokens behind 15000 468 us (1150 TFLOP/s, of cuBLAS's 1638 in a burst; 490 to 508 in a long run, at a lower clock; the tensor pipe is
 // busy for 54 % of it, as in the prompt's kernel one tile's softmax is covered by the other's products in part); 16 answers with up to five drafted tokens over 4000 keys 51.6 (4.4 TB/s),
 // 40 over 12000 309 (6.4 TB/s), one with four over 9000 26.3; D 64, three portions of 700 tokens beside 29 answers over 1500 keys 83.9, 40 answers over 12000 220 (4.5 TB/s).  Short
 // steps pay 4 us from the launch to the first scores, some 3 at each turn from one piece to the next and 5 at the end: results, one counter, the last CTA's sums.
 // Pages of 8 bits (F8): the turned kind's operands are the codes as they lie (below); of requests of more rows the pages are brought to 16 bits by a launch in front (chunk_widen_kernel).
-// 40 answers with up to five drafts over 6000 keys 124 us (4.1 TB/s; 16-bit pages 214), without drafts 98 (5.2 TB/s), one with four over 9000 28; 2048 tokens behind 15000 507.
+// us, and over 16-bit pages in the same run: 40 answers with up to five drafts over 6000 keys 122 (4.2 TB/s), 175; without drafts 107 (4.7 TB/s), 166; over 12000 keys 197, 314; one with four over
+// 9000 25.8, 26.3; D 64, 40 over 12000 181, 222.  Where prompts take part nothing is won: three portions beside 29 answers over 1500 keys 99.5, 92 (D 64: 119, 111), 2048 tokens behind 15000 502, 469
+// (557 to 568 in a long run).
 #include <type_traits>
 
 #include "pie_step_plan.h"
@@ -1387,7 +1389,7 @@ static cudaError_t launch_chunk(const CUtensorMap (&m)[4], const Codes& codes, c
 }
 
 // 8-bit pages of the requests that have more rows than the turned kind takes, as bf16 where they will be read as those are: the tensor cores' operands of that kind come from shared memory
-// alone, and every query tile would turn the same codes around again.  (Four warps beside the softmax's that widened them tile by tile: 2048 tokens behind 15000 812 us and more; so 499; pages of 16 bits 478.)  A block (page, head) a CTA at a time.
+// alone, and every query tile would turn the same codes around again.  (Four warps beside the softmax's that widened them tile by tile: 2048 tokens behind 15000 812 us and more; so 502; pages of 16 bits 469.)  A block (page, head) a CTA at a time.
 __global__ void __launch_bounds__(256) chunk_widen_kernel(const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs, uint16_t* k16, uint16_t* v16, const int32_t* row_starts,
                                                           const int32_t* contexts, const int32_t* table, int requests, int blocks, int Hkv, int D, int few_tokens) {
   __shared__ int list[256];   // requests of this round that have so many
