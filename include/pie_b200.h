@@ -133,7 +133,7 @@ int pie_qmm_rows(void* y, int y_ld, const void* x, const pie_qmv_seg* segs_host,
  * NULL): the rows are pie_rms_norm's of x (the squares may be added up in another order, which the rows beside one do not change).  Weights take the same form: a row a channel.
  * pie_int8_matmul: y bf16 [M, N] = bf16((sum_k codes[m, k] w[n, k]) scales[m] w_scales[n]), the sum exact, each product of fp32 rounded; residual (bf16 [M, N] or NULL; may be
  * y): added to that, rounded again.  The same bits whatever M the row comes with.
- * K: a multiple of 16 below 131072 (of pie_int8_rows: any multiple of 16); all pointers 16-byte aligned.  Workspace: pie_int8_workspace_bytes() bytes (0: none), ZEROED ONCE
+ * K: a multiple of 16 below 131072 (of pie_int8_rows: any multiple of 16); M and N at most 2^31 - 257; all pointers 16-byte aligned.  Workspace: pie_int8_workspace_bytes() bytes (0: none), ZEROED ONCE
  * at allocation and left at zero, for launches that come one after the other. */
 int pie_int8_rows(int8_t* codes, float* scales, const void* x, long long x_ld, int rows, int K, const void* norm_weight, float eps, void* stream);
 size_t pie_int8_workspace_bytes(int M, int N);

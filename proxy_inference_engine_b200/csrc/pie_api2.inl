@@ -242,8 +242,8 @@ int pie_int8_matmul(void* y, const int8_t* codes, const float* scales, const int
                     void* workspace, size_t workspace_bytes, void* stream) {
   if (M == 0) return PIE_OK;
   if (!y || !codes || !scales || !w || !w_scales) return PIE_ENULL;
-  // (products of two -128 are 2^14: below 2^17 of them fit 32 bits)
-  if (M < 0 || N <= 0 || K <= 0 || K % 16 || K >= 131072 || ((M + 127LL) / 128) * ((N + 127LL) / 128) > (1 << 30)) return PIE_EINVAL_SHAPE;
+  // (products of two -128 are 2^14: below 2^17 of them fit 32 bits; the rows and columns of the last tile, of up to 256, are counted in 31)
+  if (M < 0 || N <= 0 || M > 0x7fffffff - 256 || N > 0x7fffffff - 256 || K <= 0 || K % 16 || K >= 131072 || ((M + 127LL) / 128) * ((N + 127LL) / 128) > (1 << 30)) return PIE_EINVAL_SHAPE;
   if (!aligned16(y) || !aligned16(codes) || !aligned16(scales) || !aligned16(w) || !aligned16(w_scales) || !aligned16(residual) || !aligned16(workspace)) return PIE_EALIGN;
   const size_t need = int8_workspace_bytes(M, N);
   if (need && (!workspace || workspace_bytes < need)) return PIE_EWORKSPACE;

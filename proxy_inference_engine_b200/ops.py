@@ -913,8 +913,8 @@ def _int8_features(what: str, x, norm_weight) -> int:
     if x.dim() < 1 or x.dtype != _BF16:
         raise ValueError(f"[{what}] x must be bfloat16 [..., K], but is {x.dtype} {tuple(x.shape)}")
     K = x.shape[-1]
-    if K == 0 or K % 16:
-        raise ValueError(f"[{what}] rows of {K} features are not built here (a multiple of 16)")
+    if K == 0 or K % 16 or x.numel() // K > _INT8_MOST:
+        raise ValueError(f"[{what}] {x.numel() // max(K, 1)} rows of {K} features are not built here (a multiple of 16; at most {_INT8_MOST} rows)")
     if norm_weight is not None and (norm_weight.dtype != _BF16 or tuple(norm_weight.shape) != (K,)):
         raise ValueError(f"[{what}] norm_weight must be bfloat16 [{K}], but is {norm_weight.dtype} {list(norm_weight.shape)}")
     return K
@@ -946,7 +946,12 @@ def _int8_weight(what: str, weight, weight_scales, K: int) -> int:
         raise ValueError(f"[{what}] weight_scales must be contiguous float32 [{N}], but is {weight_scales.dtype} {list(weight_scales.shape)}")
     if K >= 131072:
         raise ValueError(f"[{what}] sums of {K} products are not built here (below 131072)")
+    if N > _INT8_MOST:
+        raise ValueError(f"[{what}] {N} output channels are not built here (at most {_INT8_MOST})")
     return N
+
+
+_INT8_MOST = 2 ** 31 - 257   # rows, channels: tiles of 256 are counted in 31 bits (and ctypes would take a number modulo 2^32)
 
 
 def int8_matmul(codes, scales, weight, weight_scales, *, residual=None):
@@ -962,6 +967,8 @@ def int8_matmul(codes, scales, weight, weight_scales, *, residual=None):
     K = codes.shape[-1]
     if scales.dtype != torch.float32 or scales.shape != codes.shape[:-1]:
         raise ValueError(f"[{what}] scales must be float32 {list(codes.shape[:-1])}, but are {scales.dtype} {list(scales.shape)}")
+    if scales.numel() > _INT8_MOST:
+        raise ValueError(f"[{what}] {scales.numel()} rows are not built here (at most {_INT8_MOST})")
     N = _int8_weight(what, weight, weight_scales, K)
     shape = codes.shape[:-1] + (N,)
     if residual is not None and (residual.dtype != _BF16 or residual.shape != shape):
